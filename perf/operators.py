@@ -8,8 +8,8 @@ Five kinds of work, in the order a step meets them:
   attend     one decode step's attention of a batch over the 4-bit cache                                                   FP4KVCache.attention
   sample     one token per row from its logits: temperature, top-k, top-p, min-p, with given random numbers                sample
 
-The cache holds MXFP4: 32 consecutive channels of one token and head share a power of two 2^E, the smallest (E >= -125) with max |x| < 7 * 2^E, and an
-element is the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6 times 2^E (ties to the even code), with its sign; a block that is not finite reads as NaN.
+The cache holds MXFP4: 32 consecutive channels of one token and head share a power of two 2^E, the smallest with max |x| < 7 * 2^E, from -125 to 125,
+and an element is the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6 times 2^E (ties to the even code; 6 beyond it), with its sign; a block that is not finite reads as NaN.
 
 K and V are Gaussian per (kv head, channel) with channel scales log-uniform in 2^[-2, 2], and queries are standard normal: a softmax that spreads over many
 tokens.  Logits are a wide Gaussian with a few dozen likely tokens above it, as a trained model's."""
@@ -159,7 +159,7 @@ def _quantise(x):
     """x [..., D] -> codes uint8 [..., D/2] (an even channel in the low half of its byte), exponent bytes uint8 [..., D/32]."""
     b = x.float().unflatten(-1, (-1, BLOCK))
     top = b.abs().amax(-1)
-    E = (((top.view(torch.int32) + 0x200000) >> 23) - 129).clamp(min=-125)
+    E = (((top.view(torch.int32) + 0x200000) >> 23) - 129).clamp(min=-125, max=125)
     y = b.abs() * ((127 - E) << 23).view(torch.float32).unsqueeze(-1)
     code = (y > 0.25).to(torch.uint8) + (y >= 0.75) + (y > 1.25) + (y >= 1.75) + (y > 2.5) + (y >= 3.5) + (y > 5.0) + 8 * (b < 0)
     code = code.to(torch.uint8).flatten(-2)
@@ -323,7 +323,7 @@ def _stored64(x):
     E = torch.floor(torch.log2(top.clamp(min=1e-300))) - 3      # at or below the smallest power that will do
     for _ in range(4):
         E = torch.where(top >= 7 * torch.exp2(E), E + 1, E)
-    s = torch.exp2(E.clamp(min=-125))
+    s = torch.exp2(E.clamp(min=-125, max=125))
     grid = torch.tensor(_GRID, dtype=torch.float64, device=x.device)
     y = b.abs() / s
     best, value = torch.full_like(y, math.inf), torch.zeros_like(y)
