@@ -2,7 +2,7 @@
 is the library for ctypes, which takes the calls where there is no binding for the installed torch.  There is no other fallback: if the library is
 missing, or a call is made without a GPU, the call raises."""
 from __future__ import annotations
-import ctypes, os, warnings
+import contextlib, ctypes, os, warnings
 import torch
 
 _LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libgaac_hip.so")
@@ -40,6 +40,12 @@ _SIGNATURES = {
     "gaac_static_init": [],
     "gaac_static_reset": [P],
     "gaac_static_flags": [P, P],
+    "gaac_fp4_store": [P, P] + [c_long] * 4 + [c_int] * 3 + [P] * 3,
+    "gaac_fp4_load": [P] + [c_int] * 3 + [P, P] + [c_long] * 4 + [P],
+    "gaac_fp4_append": [P] + [c_int] * 3 + [P, P] + [c_long] * 4 + [P, c_int, c_int, P, P, P],
+    "gaac_fp4_attn": [P, P, P, c_int, c_int, c_int, P, c_int, c_int, c_int, c_float, c_int, P, P, P],
+    "gaac_qk_norm_rope": [c_int, P, P] + [c_long] * 5 + [c_int] * 4 + [P, P, c_long, c_long, c_float, P, c_int, P, P, c_int, c_int, P, P, P],
+    "gaac_sample": [c_int, P, c_long, c_int, c_int, P, P, c_float, P, c_int, P, c_float, P, c_float, P, P],
     "gaac_attn_launch": [P] * 16 + [P, P, c_int, c_int, c_int, P, c_int, c_float, c_int, c_int, P, P, P, c_int, P, P, P, P, P],
 }
 
@@ -127,3 +133,18 @@ def stream() -> int:
 
 def call(name: str, *args):
     getattr(_calls or calls(), name)(*args)
+
+
+def on_device(*tensors):
+    """A context in which the device of the given tensors (None among them is left out) is the current one, so that `stream` is a stream of theirs.  Raises
+    for host tensors and for tensors of several devices."""
+    dev = None
+    for t in tensors:
+        if t is None: continue
+        if not t.is_cuda: raise RuntimeError("gaac_amd kernels need device tensors (got a CPU tensor): there is no CPU path")
+        if dev is None: dev = t.device
+        elif t.device != dev: raise RuntimeError(f"tensors on {dev} and on {t.device} in one call")
+    return _HERE if dev.index == torch._C._cuda_getDevice() else torch.cuda.device(dev)
+
+
+_HERE = contextlib.nullcontext()

@@ -1,0 +1,446 @@
+// The 4-bit cache: its tiles, their encoder (prompt, appended token), decoder, and decode attention over them.
+//
+// Format (OCP MXFP4): 32 consecutive channels of one token and head are a block.  A block has one power of two 2^E, E the smallest integer with
+// amax < 7 * 2^E, from -125 to 125, held as the byte E + 127 (255: the block held a NaN or an infinity and reads as NaN), and 4-bit codes: sign, and the nearest of
+// 0 .5 1 1.5 2 3 4 6 to |x| * 2^-E, ties to the even code, at most 6.  With amax < 7 * 2^E no element is off by more than half of the grid's last step, and
+// the exponent needs one addition to amax's bits.  Rounding is by a power of two, so a code is exact whatever type it is computed in; every value is a
+// normal number of bf16 (2^-126 to 6 * 2^125) or zero, so expanding a code rounds nothing.  gfx950 converts both ways in one instruction for two elements, scale included.
+//
+// A tile is 32 tokens of one cache head, K and V, 4352 bytes in a row.  Its unit is a dword: 8 consecutive channels of one token, so that appending a
+// token writes whole dwords.  They lie in the order of the operands of the 16x16x32 matrix instruction, a lane's 16 bytes next to each other:
+//   lane l = 16 g + m.  K: token 16 s + m, channels 32 c + 8 g ..: byte 1024 s + 16 l + 4 c.      (scores: A = K, 32 channels at a time)
+//                       V: token 16 s + 4 g + i, channels 8 m ..:  byte 2048 + 1024 s + 16 l + 4 i.      (output: A = V^T, all 32 tokens at once)
+//   K's exponent byte of token 16 s + m, block c: 4096 + 8 m + 4 s + c.  V's of token 16 s + 4 g + i, block b: 4224 + 32 b + 8 g + 4 s + i.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+#include "gaac_capi.h"
+#include "../../include/gaac_hip.h"
+
+namespace {
+
+constexpr int DIM = 128, TT = 32, TILE = 4352, V_AT = 2048, KS_AT = 4096, VS_AT = 4224;
+constexpr int NW = 8;      // waves of an attention block
+
+typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef unsigned u2 __attribute__((ext_vector_type(2)));
+typedef unsigned u4 __attribute__((ext_vector_type(4)));
+typedef unsigned short us2 __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ unsigned pk_max(unsigned a, unsigned b) {
+  return __builtin_bit_cast(unsigned, __builtin_elementwise_max(__builtin_bit_cast(us2, a), __builtin_bit_cast(us2, b)));
+}
+// Largest magnitude (bf16 bits) of a unit's 8 elements, two candidates packed.
+__device__ __forceinline__ unsigned unit_max(u4 x) {
+  return pk_max(pk_max(x[0] & 0x7fff7fffu, x[1] & 0x7fff7fffu), pk_max(x[2] & 0x7fff7fffu, x[3] & 0x7fff7fffu));
+}
+// Exponent byte from the packed magnitudes of a block.  amax = m 2^e < 7 * 2^E = 1.75 * 2^(E+2): one more where the mantissa is 1.75 or above.
+__device__ __forceinline__ unsigned exponent_byte(unsigned packed) {
+  const unsigned a = max(packed & 0xffffu, packed >> 16);
+  return a >= 0x7f80u ? 255u : (unsigned)min(max((int)((a + 0x20u) >> 7) - 2, 2), 252);
+}
+__device__ __forceinline__ float scale_of(unsigned byte) { return __builtin_bit_cast(float, byte << 23); }
+__device__ __forceinline__ bf2 pair(unsigned x) { return __builtin_bit_cast(bf2, x); }      // (a bit cast of a vector's element takes the first one)
+__device__ __forceinline__ unsigned encode_unit(u4 x, float scale) {
+  unsigned w = 0;
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, pair(x[0]), scale, 0);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, pair(x[1]), scale, 1);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, pair(x[2]), scale, 2);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, pair(x[3]), scale, 3);
+  return w;
+}
+__device__ __forceinline__ u4 decode_unit(unsigned w, float scale) {
+  u4 x;
+  x[0] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 0));
+  x[1] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 1));
+  x[2] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 2));
+  x[3] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 3));
+  return x;
+}
+
+// ---------------------------------------------------------------------------------------------------- prompt
+// A wave encodes K (blockIdx.z = 0) or V of one tile; four tiles a block.  Bound by HBM: 8 KB read and 2.1 KB written per tile and kind.  A load
+// instruction takes 64 bytes of 16 token rows (K) or whole 256-byte rows (V), a store 1 KB in a row.  Rows of the last tile behind the prompt become zero bytes.
+__global__ __launch_bounds__(256) void k_fp4_store(const uint16_t* k, const uint16_t* v, long k_hs, long k_rs, long v_hs, long v_rs, int L, int tiles, uint8_t* cache, int* len) {
+  if (len != nullptr && blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0 && threadIdx.x == 0) *len = L;
+  const int tile = blockIdx.x * 4 + (threadIdx.x >> 6), l = threadIdx.x & 63, m = l & 15, g = l >> 4, head = blockIdx.y;
+  if (tile * TT >= L) return;
+  uint8_t* out = cache + ((long)head * tiles + tile) * TILE;
+  if (blockIdx.z == 0) {
+    const uint16_t* src = k + head * k_hs + 8 * g;
+    u4 x[2][4];
+    for (int s = 0; s < 2; ++s) {
+      const int t = tile * TT + 16 * s + m;
+      for (int c = 0; c < 4; ++c) x[s][c] = t < L ? *reinterpret_cast<const u4*>(src + t * k_rs + 32 * c) : u4{0, 0, 0, 0};
+    }
+    u2 exps = {0, 0};
+    for (int s = 0; s < 2; ++s) {
+      u4 w;
+      for (int c = 0; c < 4; ++c) {      // a block of K is spread over the four lanes 16 g + m
+        unsigned a = unit_max(x[s][c]);
+        a = pk_max(a, __shfl_xor(a, 16));
+        a = pk_max(a, __shfl_xor(a, 32));
+        const unsigned e = exponent_byte(a);
+        w[c] = encode_unit(x[s][c], scale_of(e));
+        if (tile * TT + 16 * s + m < L) exps[s] |= e << 8 * c;
+      }
+      *reinterpret_cast<u4*>(out + 1024 * s + 16 * l) = w;
+    }
+    if (g == 0) *reinterpret_cast<u2*>(out + KS_AT + 8 * m) = exps;
+  } else {
+    const uint16_t* src = v + head * v_hs + 8 * m;
+    u4 x[2][4];
+    for (int s = 0; s < 2; ++s)
+      for (int i = 0; i < 4; ++i) {
+        const int t = tile * TT + 16 * s + 4 * g + i;
+        x[s][i] = t < L ? *reinterpret_cast<const u4*>(src + t * v_rs) : u4{0, 0, 0, 0};
+      }
+    u2 exps = {0, 0};
+    for (int s = 0; s < 2; ++s) {
+      u4 w;
+      for (int i = 0; i < 4; ++i) {      // a block of V is four lanes next to each other
+        unsigned a = unit_max(x[s][i]);
+        a = pk_max(a, __shfl_xor(a, 1));
+        a = pk_max(a, __shfl_xor(a, 2));
+        const unsigned e = exponent_byte(a);
+        w[i] = encode_unit(x[s][i], scale_of(e));
+        if (tile * TT + 16 * s + 4 * g + i < L) exps[s] |= e << 8 * i;
+      }
+      *reinterpret_cast<u4*>(out + V_AT + 1024 * s + 16 * l) = w;
+    }
+    if ((m & 3) == 0) *reinterpret_cast<u2*>(out + VS_AT + 8 * m + 8 * g) = exps;      // block m / 4
+  }
+}
+
+__global__ __launch_bounds__(256) void k_fp4_load(const uint8_t* cache, int L, int tiles, uint16_t* k, uint16_t* v, long k_hs, long k_rs, long v_hs, long v_rs) {
+  const int tile = blockIdx.x * 4 + (threadIdx.x >> 6), l = threadIdx.x & 63, m = l & 15, g = l >> 4, head = blockIdx.y;
+  if (tile * TT >= L) return;
+  const uint8_t* in = cache + ((long)head * tiles + tile) * TILE;
+  if (blockIdx.z == 0) {
+    const u2 exps = *reinterpret_cast<const u2*>(in + KS_AT + 8 * m);
+    for (int s = 0; s < 2; ++s) {
+      const u4 w = *reinterpret_cast<const u4*>(in + 1024 * s + 16 * l);
+      const int t = tile * TT + 16 * s + m;
+      if (t < L)
+        for (int c = 0; c < 4; ++c) *reinterpret_cast<u4*>(k + head * k_hs + t * k_rs + 32 * c + 8 * g) = decode_unit(w[c], scale_of(exps[s] >> 8 * c & 255));
+    }
+  } else {
+    const u2 exps = *reinterpret_cast<const u2*>(in + VS_AT + 32 * (m >> 2) + 8 * g);
+    for (int s = 0; s < 2; ++s) {
+      const u4 w = *reinterpret_cast<const u4*>(in + V_AT + 1024 * s + 16 * l);
+      for (int i = 0; i < 4; ++i) {
+        const int t = tile * TT + 16 * s + 4 * g + i;
+        if (t < L) *reinterpret_cast<u4*>(v + head * v_hs + t * v_rs + 8 * m) = decode_unit(w[i], scale_of(exps[s] >> 8 * i & 255));
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------- one token
+// A block per batch row, a thread per unit (K or V, head, 8 channels); a block of channels is four threads next to each other.  The row's length is
+// raised once all of the block have read it.
+__global__ __launch_bounds__(256) void k_fp4_append(const int* slots, int n_slots, int n_kv, const uint16_t* k, const uint16_t* v, long k_bs, long k_hs, long v_bs, long v_hs, int* lens,
+                                                    int tiles, int cap, uint8_t* cache, int* errors) {
+  const int b = blockIdx.x, slot = slots[b];
+  if (slot < 0) return;
+  bool again = false;      // a slot that an earlier row of the batch names: two tokens for one place
+  for (int i = threadIdx.x; i < b; i += 256) again |= slots[i] == slot;
+  const int len = slot < n_slots ? lens[slot] : 0;
+  if (__syncthreads_or(again) || slot >= n_slots || len >= cap) {
+    if (threadIdx.x == 0) atomicOr(errors, slot >= n_slots ? 4 : len >= cap ? 1 : 2);
+    return;
+  }
+  const int t = len & (TT - 1), s = t >> 4, m = t & 15, g = (t >> 2) & 3, i = t & 3;
+  for (int at = threadIdx.x; at < n_kv * 32; at += 256) {
+    const int u = at & 15, kind = at >> 4 & 1, head = at >> 5;
+    const u4 x = *reinterpret_cast<const u4*>((kind ? v + b * v_bs + head * v_hs : k + b * k_bs + head * k_hs) + 8 * u);
+    unsigned a = unit_max(x);
+    a = pk_max(a, __shfl_xor(a, 1));
+    a = pk_max(a, __shfl_xor(a, 2));
+    const unsigned e = exponent_byte(a), w = encode_unit(x, scale_of(e));
+    uint8_t* tile = cache + (((long)slot * n_kv + head) * tiles + len / TT) * TILE;
+    *reinterpret_cast<unsigned*>(tile + 1024 * s + (kind ? V_AT + 16 * (16 * g + u) + 4 * i : 16 * (16 * (u & 3) + m) + 4 * (u >> 2))) = w;
+    if ((u & 3) == 0) tile[kind ? VS_AT + 32 * (u >> 2) + 8 * g + 4 * s + i : KS_AT + 8 * m + 4 * s + (u >> 2)] = (uint8_t)e;
+  }
+  if (threadIdx.x == 0) lens[slot] = len + 1;
+}
+
+// ---------------------------------------------------------------------------------------------------- attention
+// How the rows' tiles are shared out: split p of a kv head takes tiles [first, end) of row `row`.  Every row is cut into splits of `size` tiles, size being
+// the smallest that needs no more than P splits in all, so that long rows get many splits and short ones a single one.  All of it is computed by each wave
+// from the lengths on the device.
+struct Share { int row, len, slot, first, end, index, count; };      // row < 0: nothing for this split
+
+__device__ __forceinline__ int row_slot(const int* slots, int b) { return slots[b]; }
+__device__ __forceinline__ int row_len(const int* lens, int n_slots, int cap, int slot) { return slot >= 0 && slot < n_slots ? min(lens[slot], cap) : 0; }
+__device__ __forceinline__ int wave_sum(int x) {
+  for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o);
+  return x;
+}
+__device__ __forceinline__ int splits_of(int tiles, int size) { return (tiles + size - 1) / size; }
+
+__device__ __forceinline__ int split_size(const int* slots, const int* lens, int n_slots, int cap, int B, int P) {
+  const int l = threadIdx.x & 63;
+  int total = 0, mine = 0;
+  for (int b = l; b < B; b += 64) total += mine = (row_len(lens, n_slots, cap, slots[b]) + TT - 1) / TT;
+  total = wave_sum(total);
+  int lo = max((total + P - 1) / P, 1), hi = P > B ? max((total + P - B - 1) / (P - B), lo) : max(total, 1);
+  if (B == 1) return lo;
+  if (B > 64) return hi;      // sum of ceil(t / hi) < total / hi + B <= P
+  while (lo < hi) {
+    const int mid = (lo + hi) / 2;
+    if (wave_sum(splits_of(mine, mid)) <= P) hi = mid; else lo = mid + 1;
+  }
+  return hi;
+}
+
+__device__ __forceinline__ Share share_of(const int* slots, const int* lens, int n_slots, int cap, int B, int size, int p) {
+  const int l = threadIdx.x & 63;
+  int before = 0;
+  for (int b0 = 0; b0 < B; b0 += 64) {
+    const int b = b0 + l, slot = b < B ? slots[b] : -1, len = row_len(lens, n_slots, cap, slot), n = splits_of((len + TT - 1) / TT, size);
+    int run = n;
+    for (int o = 1; o < 64; o <<= 1) { const int x = __shfl_up(run, o); if (l >= o) run += x; }
+    const unsigned long long here = __ballot(n > 0 && p >= before + run - n && p < before + run);
+    if (here) {
+      const int src = __builtin_ctzll(here);
+      Share s;
+      s.row = b0 + src; s.len = __shfl(len, src); s.slot = __shfl(slot, src); s.count = __shfl(n, src); s.index = p - (before + __shfl(run, src) - s.count);
+      s.first = s.index * size; s.end = min(s.first + size, (s.len + TT - 1) / TT);
+      return s;
+    }
+    before += __shfl(run, 63);
+  }
+  return Share{-1, 0, 0, 0, 0, 0, 0};
+}
+
+struct Tile { u4 k[2], v[2]; u2 ks, vs; };
+
+__device__ __forceinline__ Tile load_tile(const uint8_t* t, int l) {
+  const int m = l & 15, g = l >> 4;
+  Tile x;
+  x.ks = __builtin_nontemporal_load(reinterpret_cast<const u2*>(t + KS_AT + 8 * m));
+  x.vs = __builtin_nontemporal_load(reinterpret_cast<const u2*>(t + VS_AT + 32 * (m >> 2) + 8 * g));
+  for (int s = 0; s < 2; ++s) x.k[s] = __builtin_nontemporal_load(reinterpret_cast<const u4*>(t + 1024 * s + 16 * l));
+  for (int s = 0; s < 2; ++s) x.v[s] = __builtin_nontemporal_load(reinterpret_cast<const u4*>(t + V_AT + 1024 * s + 16 * l));
+  return x;
+}
+
+// Online softmax of a wave: lane 16 g + n holds query head n.  max2 is in units of log2 and common to the four lanes of a head; sum is the lane's own tokens'.
+struct Running { float max2, sum; f4 o[8]; };      // o[j][r]: channel 32 g + 8 r + j
+
+// Scores: C = K Q^T, 16 tokens x 16 heads, 4 x 32 channels.  Its rows 4 g + r are the lane's tokens, which is the order that V's units have along the
+// contraction of C = V^T P^T: the weights go from one product into the other in registers.  Weights are rounded to bf16 (half a unit, 2^-9, of random sign, on
+// each), their sum and the output are not.  The maximum is only raised where a score exceeds it by 2^8, so that the 32 accumulators are rarely scaled.
+__device__ __forceinline__ void attend_tile(Running& r, const Tile& t, const bf8 (&q)[4], float scale2, int valid, int g) {
+  f4 s[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    s[h] = f4{0, 0, 0, 0};
+#pragma unroll
+    for (int c = 0; c < 4; ++c) s[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8, decode_unit(t.k[h][c], scale_of(t.ks[h] >> 8 * c & 255))), q[c], s[h], 0, 0, 0);
+  }
+  float d[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) d[i] = __builtin_fmaf(s[i >> 2][i & 3], scale2, -r.max2);
+  u4 v[2] = {t.v[0], t.v[1]};
+  u2 vs = t.vs;
+  unsigned dead = 0;
+  if (valid < TT) {      // tokens behind the end: no weight, and nothing that an earlier sequence left in their place (it may be NaN)
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (16 * (i >> 2) + 4 * g + (i & 3) >= valid) {
+        d[i] = -__builtin_inff(); dead |= 1u << i;
+        v[i >> 2][i & 3] = 0; vs[i >> 2] &= ~(255u << 8 * (i & 3));
+      }
+  }
+  float top = d[0];
+#pragma unroll
+  for (int i = 1; i < 8; ++i) top = fmaxf(top, d[i]);
+  if (__ballot(top > 8.f)) {
+    float x = -__builtin_inff();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x = fmaxf(x, dead >> i & 1 ? -__builtin_inff() : s[i >> 2][i & 3] * scale2);
+    x = fmaxf(x, __shfl_xor(x, 16));
+    x = fmaxf(fmaxf(x, __shfl_xor(x, 32)), r.max2);
+    const float a = __builtin_amdgcn_exp2f(r.max2 - x);
+    r.max2 = x; r.sum *= a;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) r.o[j] *= a;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) d[i] = dead >> i & 1 ? -__builtin_inff() : __builtin_fmaf(s[i >> 2][i & 3], scale2, -x);
+  }
+  bf8 p;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float w = __builtin_amdgcn_exp2f(d[i]);
+    r.sum += w; p[i] = (__bf16)w;
+  }
+  u4 x[8];      // token i of the lane's 8, channels 8 m .. 8 m + 7 in pairs
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = decode_unit(v[i >> 2][i & 3], scale_of(vs[i >> 2] >> 8 * (i & 3) & 255));
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {      // channel 8 m + j of all eight tokens
+    u4 a;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a[i] = __builtin_amdgcn_perm(x[2 * i + 1][j >> 1], x[2 * i][j >> 1], j & 1 ? 0x07060302u : 0x05040100u);
+    r.o[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8, a), p, r.o[j], 0, 0, 0);
+  }
+}
+
+constexpr int OROW = DIM + 4;      // LDS row of a head's accumulators
+
+// One block = eight waves = one split of one (row, kv head).  One split a row (P == B): the output is written here; otherwise a row with several splits leaves
+// partials [p][kv head][head]: DIM accumulators, then maximum and sum.
+__global__ __launch_bounds__(64 * NW) void k_fp4_attn(const uint8_t* cache, const int* lens, const int* slots, int n_slots, int tiles, int cap, const uint16_t* q, int B, int n_kv, int G,
+                                                      float scale, int P, float* part, uint16_t* out) {
+  extern __shared__ __attribute__((aligned(16))) float lds[];      // [NW][G][OROW] accumulators, [NW][16] maxima, [NW][16] sums
+  const int l = threadIdx.x & 63, w = threadIdx.x >> 6, n = l & 15, g = l >> 4, kvh = blockIdx.x % n_kv, p = blockIdx.x / n_kv;
+  Share sh;
+  if (P == B) {
+    sh.row = p; sh.slot = slots[p]; sh.len = row_len(lens, n_slots, cap, sh.slot); sh.first = 0; sh.end = (sh.len + TT - 1) / TT; sh.index = 0; sh.count = 1;
+    if (sh.len == 0) {      // no tokens: 0; a slot that the cache does not have: NaN
+      for (int i = threadIdx.x; i < G * DIM; i += 64 * NW) out[((long)p * n_kv + kvh) * G * DIM + i] = sh.slot >= n_slots ? 0x7fc0 : 0;
+      return;
+    }
+  } else {
+    sh = share_of(slots, lens, n_slots, cap, B, split_size(slots, lens, n_slots, cap, B, P), p);
+    if (sh.row < 0) return;
+  }
+  const int row = __builtin_amdgcn_readfirstlane(sh.row), slot = __builtin_amdgcn_readfirstlane(sh.slot), len = __builtin_amdgcn_readfirstlane(sh.len);
+  const int end = __builtin_amdgcn_readfirstlane(sh.end), count = __builtin_amdgcn_readfirstlane(sh.count);
+  const uint8_t* base = cache + ((long)slot * n_kv + kvh) * tiles * TILE;
+  const long q0 = ((long)row * n_kv + kvh) * G * DIM;
+  bf8 qf[4];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    u4 x = n < G ? *reinterpret_cast<const u4*>(q + q0 + n * DIM + 32 * c + 8 * g) : u4{0, 0, 0, 0};
+    if (scale < 0) x ^= 0x80008000u;
+    qf[c] = __builtin_bit_cast(bf8, x);
+  }
+  const float scale2 = fabsf(scale) * 1.44269504f;
+  Running r;
+  r.max2 = -__builtin_inff(); r.sum = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) r.o[j] = f4{0, 0, 0, 0};
+  for (int t = __builtin_amdgcn_readfirstlane(sh.first) + w; t < end; t += NW) {
+    const Tile x = load_tile(base + (long)t * TILE, l);
+    attend_tile(r, x, qf, scale2, len - t * TT, g);
+  }
+  r.sum += __shfl_xor(r.sum, 16);
+  r.sum += __shfl_xor(r.sum, 32);
+  float *acc = lds, *mx = lds + NW * G * OROW, *sm = mx + NW * 16;
+  if (n < G) {
+#pragma unroll
+    for (int rr = 0; rr < 4; ++rr)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        *reinterpret_cast<f4*>(acc + (w * G + n) * OROW + 32 * g + 8 * rr + 4 * h) = f4{r.o[4 * h][rr], r.o[4 * h + 1][rr], r.o[4 * h + 2][rr], r.o[4 * h + 3][rr]};
+    if (g == 0) { mx[w * 16 + n] = r.max2; sm[w * 16 + n] = r.sum; }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < G * DIM; i += 64 * NW) {
+    const int h = i / DIM, ch = i % DIM;
+    float top = mx[h];
+    for (int k = 1; k < NW; ++k) top = fmaxf(top, mx[k * 16 + h]);
+    float o = 0, sum = 0;
+    for (int k = 0; k < NW; ++k) {
+      const float f = __builtin_amdgcn_exp2f(mx[k * 16 + h] - top);
+      o += f * acc[(k * G + h) * OROW + ch]; sum += f * sm[k * 16 + h];
+    }
+    if (count == 1) out[q0 + i] = __builtin_bit_cast(uint16_t, (__bf16)(o / sum));
+    else {
+      float* dst = part + (((long)p * n_kv + kvh) * G + h) * (DIM + 2);
+      dst[ch] = o;
+      if (ch == 0) { dst[DIM] = top; dst[DIM + 1] = sum; }
+    }
+  }
+}
+
+// Adds up the splits of a row's query head, in their order.  A block per (row, query head); rows of a single split are done already.
+__global__ __launch_bounds__(256) void k_fp4_merge(const float* part, const int* lens, const int* slots, int n_slots, int cap, int B, int n_kv, int G, int P, uint16_t* out) {
+  __shared__ float acc[2][DIM], wsum[2];
+  const int row = blockIdx.x / (n_kv * G), head = blockIdx.x % (n_kv * G), l = threadIdx.x & 63;
+  const int slot = slots[row], len = row_len(lens, n_slots, cap, slot);
+  uint16_t* dst = out + (long)blockIdx.x * DIM;
+  if (len == 0) {
+    if (threadIdx.x < DIM) dst[threadIdx.x] = slot >= n_slots ? 0x7fc0 : 0;
+    return;
+  }
+  const int size = split_size(slots, lens, n_slots, cap, B, P), count = splits_of((len + TT - 1) / TT, size);
+  if (count == 1) return;
+  int first = 0;
+  for (int b = l; b < row; b += 64) first += splits_of((row_len(lens, n_slots, cap, slots[b]) + TT - 1) / TT, size);
+  first = wave_sum(first);
+  const long stride = (long)n_kv * G * (DIM + 2);
+  const float* src = part + (long)first * stride + head * (DIM + 2);
+  float top = -__builtin_inff();
+  for (int i = l; i < count; i += 64) top = fmaxf(top, src[i * stride + DIM]);
+  for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+  const int ch = threadIdx.x % DIM, half = threadIdx.x / DIM;
+  float o = 0, sum = 0;
+  for (int i = half; i < count; i += 2) {
+    const float f = __builtin_amdgcn_exp2f(src[i * stride + DIM] - top);
+    o += f * src[i * stride + ch]; sum += f * src[i * stride + DIM + 1];
+  }
+  acc[half][ch] = o;
+  if (ch == 0) wsum[half] = sum;
+  __syncthreads();
+  if (half == 0) dst[ch] = __builtin_bit_cast(uint16_t, (__bf16)((acc[0][ch] + acc[1][ch]) / (wsum[0] + wsum[1])));
+}
+
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+}  // namespace
+
+extern "C" {
+
+int gaac_fp4_store(const void* k, const void* v, long k_head_stride, long k_row_stride, long v_head_stride, long v_row_stride, int L, int n_kv, int tiles, uint8_t* cache, int* len, void* stream) {
+  GAAC_REQUIRE(cache != nullptr && len != nullptr && (L == 0 || (k != nullptr && v != nullptr)), "gaac_fp4_store: null pointer");
+  GAAC_REQUIRE(n_kv > 0 && n_kv <= 65535 && tiles > 0 && L >= 0 && L <= (long)tiles * TT, "gaac_fp4_store: bad sizes (n_kv %d, %d tokens, %d tiles of %d)", n_kv, L, tiles, TT);
+  GAAC_REQUIRE(aligned16(k) && aligned16(v) && aligned16(cache) && (k_head_stride | k_row_stride | v_head_stride | v_row_stride) % 8 == 0, "gaac_fp4_store: rows must be 16-byte aligned");
+  k_fp4_store<<<dim3(L > 0 ? (L + 4 * TT - 1) / (4 * TT) : 1, n_kv, 2), 256, 0, (hipStream_t)stream>>>((const uint16_t*)k, (const uint16_t*)v, k_head_stride, k_row_stride, v_head_stride, v_row_stride, L, tiles,
+                                                                                                    cache, len);
+  return gaac::launch_status("gaac_fp4_store");
+}
+
+int gaac_fp4_load(const uint8_t* cache, int L, int n_kv, int tiles, void* k, void* v, long k_head_stride, long k_row_stride, long v_head_stride, long v_row_stride, void* stream) {
+  GAAC_REQUIRE(cache != nullptr && k != nullptr && v != nullptr, "gaac_fp4_load: null pointer");
+  GAAC_REQUIRE(n_kv > 0 && n_kv <= 65535 && tiles > 0 && L > 0 && L <= (long)tiles * TT, "gaac_fp4_load: bad sizes (n_kv %d, %d tokens, %d tiles of %d)", n_kv, L, tiles, TT);
+  GAAC_REQUIRE(aligned16(k) && aligned16(v) && aligned16(cache) && (k_head_stride | k_row_stride | v_head_stride | v_row_stride) % 8 == 0, "gaac_fp4_load: rows must be 16-byte aligned");
+  k_fp4_load<<<dim3((L + 4 * TT - 1) / (4 * TT), n_kv, 2), 256, 0, (hipStream_t)stream>>>(cache, L, tiles, (uint16_t*)k, (uint16_t*)v, k_head_stride, k_row_stride, v_head_stride, v_row_stride);
+  return gaac::launch_status("gaac_fp4_load");
+}
+
+int gaac_fp4_append(const int* slots, int B, int n_slots, int n_kv, const void* k, const void* v, long k_batch_stride, long k_head_stride, long v_batch_stride, long v_head_stride, int* lens, int tiles, int cap,
+                    uint8_t* cache, int* errors, void* stream) {
+  GAAC_REQUIRE(slots != nullptr && k != nullptr && v != nullptr && lens != nullptr && cache != nullptr && errors != nullptr, "gaac_fp4_append: null pointer");
+  GAAC_REQUIRE(B > 0 && n_slots > 0 && n_kv > 0 && n_kv < 1 << 24 && tiles > 0 && cap > 0 && cap <= (long)tiles * TT, "gaac_fp4_append: bad sizes (B %d, n_slots %d, n_kv %d, capacity %d in %d tiles)", B, n_slots,
+               n_kv, cap, tiles);
+  GAAC_REQUIRE(aligned16(k) && aligned16(v) && aligned16(cache) && (k_batch_stride | k_head_stride | v_batch_stride | v_head_stride) % 8 == 0, "gaac_fp4_append: rows must be 16-byte aligned");
+  k_fp4_append<<<B, 256, 0, (hipStream_t)stream>>>(slots, n_slots, n_kv, (const uint16_t*)k, (const uint16_t*)v, k_batch_stride, k_head_stride, v_batch_stride, v_head_stride, lens, tiles, cap, cache, errors);
+  return gaac::launch_status("gaac_fp4_append");
+}
+
+int gaac_fp4_attn(const uint8_t* cache, const int* lens, const int* slots, int n_slots, int tiles, int cap, const void* q, int B, int n_q, int n_kv, float scale, int nsplit, float* partials, void* out,
+                  void* stream) {
+  GAAC_REQUIRE(cache != nullptr && lens != nullptr && slots != nullptr && q != nullptr && out != nullptr, "gaac_fp4_attn: null pointer");
+  GAAC_REQUIRE(B > 0 && n_slots > 0 && n_kv > 0 && n_q >= n_kv && n_q % n_kv == 0 && n_q / n_kv <= 16, "gaac_fp4_attn: GQA group size must be 1..16 (n_q %d, n_kv %d)", n_q, n_kv);
+  GAAC_REQUIRE(tiles > 0 && cap > 0 && cap <= (long)tiles * TT && nsplit > 0 && (long)B * nsplit * n_kv < 1l << 31 && (long)B * n_q < 1l << 31, "gaac_fp4_attn: bad sizes (B %d, capacity %d in %d tiles, %d splits)", B,
+               cap, tiles, nsplit);
+  GAAC_REQUIRE(nsplit == 1 || partials != nullptr, "gaac_fp4_attn: more than one split needs partials");
+  GAAC_REQUIRE(aligned16(q) && aligned16(cache), "gaac_fp4_attn: q must be 16-byte aligned");
+  const int G = n_q / n_kv, P = B * nsplit, lds = 4 * (NW * G * OROW + 2 * NW * 16);
+  if (lds > 64 * 1024) {
+    const hipError_t e = hipFuncSetAttribute((const void*)k_fp4_attn, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    if (e != hipSuccess) { gaac::fail("gaac_fp4_attn: %s", hipGetErrorString(e)); return (int)e; }
+  }
+  k_fp4_attn<<<P * n_kv, 64 * NW, lds, (hipStream_t)stream>>>(cache, lens, slots, n_slots, tiles, cap, (const uint16_t*)q, B, n_kv, G, scale, P, partials, (uint16_t*)out);
+  const int rc = gaac::launch_status("gaac_fp4_attn");
+  if (rc != 0 || P == B) return rc;
+  k_fp4_merge<<<B * n_q, 256, 0, (hipStream_t)stream>>>(partials, lens, slots, n_slots, cap, B, n_kv, G, P, (uint16_t*)out);
+  return gaac::launch_status("gaac_fp4_attn (merge)");
+}
+
+}  // extern "C"

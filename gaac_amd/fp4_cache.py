@@ -1,0 +1,130 @@
+"""Slot cache of one attention layer in 4 bits, with the methods of CompressedKVCache (kv_cache.py): 3.76 times smaller than bf16 where that one is lossless
+and 1.4 times smaller.
+
+32 consecutive channels of a token and head share a power of two 2^E, the smallest with max |x| < 7 * 2^E, from -125 to 125; an element is held as its sign and the
+nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6 times 2^E, ties to the even code (OCP MXFP4, 4.25 bits an element).  A block with a NaN or an infinity reads as NaN.  A
+token is quantised as it is written and by itself: what the cache holds of it does not depend on whether it came in a prompt or as a decode step's token.  The
+values are numbers of bf16, so reading them back rounds nothing.
+
+Slot s owns cache heads [s*n_kv, (s+1)*n_kv); a head is a row of tiles of 32 tokens, K and V of a tile in 4352 bytes next to each other (csrc/fp4.hip).
+append and attention take the batch's slot map and the slots' lengths from device memory and never return to the host, so a decode step can be captured in a
+HIP graph.  Calls on one cache must be ordered on one stream where one of them writes; attention keeps nothing between calls (its scratch is the call's own),
+so that readers may overlap."""
+from __future__ import annotations
+import torch
+from . import _lib
+from .codec import D
+from .kernel import GMAX
+
+T = 32                          # tokens per tile
+ROW_BYTES = D // 2 + D // 32    # bytes of a token and head of K or of V: codes and exponents
+TILE_BYTES = 2 * T * ROW_BYTES
+
+
+def choose_nsplit(B: int, n_kv: int, S: int) -> int:
+    """Splits per row of a launch, of which rows get theirs by length: S tokens in the longest."""
+    return max(1, min(-(-256 // (B * n_kv)), S // 256))
+
+
+def _rows(x: torch.Tensor) -> torch.Tensor:
+    """x [., heads, 128] as the kernels read it: channels next to each other, heads and tokens any multiple of 16 bytes apart; other layouts are copied."""
+    (rs, hs, one), shape = x.stride(), x.shape
+    if one == 1 and (shape[1] == 1 or hs % 8 == 0) and (shape[0] == 1 or rs % 8 == 0) and x.data_ptr() % 16 == 0: return x
+    return x.clone(memory_format=torch.contiguous_format)
+
+
+def _strides(x: torch.Tensor) -> tuple[int, int]:
+    """(head stride, row stride)."""
+    return x.stride(1) if x.shape[1] > 1 else 0, x.stride(0) if x.shape[0] > 1 else 0
+
+
+class FP4KVCache:
+    def __init__(self, n_slots: int, n_kv: int, capacity: int, device="cuda"):
+        """n_slots sequences of up to `capacity` tokens (rounded up to whole tiles), n_kv cache heads each."""
+        _lib.load()      # fail here, not at the first decode step, if the native library is missing
+        if n_slots < 1 or n_kv < 1 or capacity < 1: raise RuntimeError(f"FP4KVCache expects slots, kv heads and capacity of at least 1, got {n_slots}, {n_kv}, {capacity}")
+        self.n_slots, self.n_kv = n_slots, n_kv
+        self.tiles = -(-capacity // T)
+        self.cap = self.tiles * T
+        self.H = n_slots * n_kv
+        self.data = torch.zeros(self.H, self.tiles, TILE_BYTES, dtype=torch.uint8, device=device)
+        self.lens = torch.zeros(n_slots, dtype=torch.int32, device=device)          # tokens per slot
+        # set by append instead of writing: bit 0 = a slot was full, bit 1 = a slot twice in a batch, bit 2 = no such slot
+        self.overflow = torch.zeros(1, dtype=torch.int32, device=device)
+
+    @staticmethod
+    def bytes_per_slot(n_kv: int, capacity: int) -> int:
+        """Device bytes one slot occupies: its tiles and its length."""
+        return n_kv * -(-capacity // T) * TILE_BYTES + 4
+
+    def _check(self, what: str, k: torch.Tensor, v: torch.Tensor):
+        if k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16 or k.shape != v.shape or k.dim() != 3 or tuple(k.shape[1:]) != (self.n_kv, D):
+            raise RuntimeError(f"{what} expects k, v bf16 [., {self.n_kv}, {D}], got {k.dtype} {list(k.shape)} and {v.dtype} {list(v.shape)}")
+
+    # ------------------------------------------------------------------ prefill
+    def prefill(self, slot: int, k: torch.Tensor, v: torch.Tensor):
+        """Put a whole prompt into `slot`, replacing what the slot held: k, v bf16 [L, n_kv, D] in the model's token-major layout, through any strides of whole
+        16 bytes.  One launch, no wait."""
+        self._check("prefill", k, v)
+        L = k.shape[0]
+        if not 0 <= slot < self.n_slots: raise RuntimeError(f"prefill expects a slot in 0..{self.n_slots - 1}, got {slot}")
+        if L > self.cap: raise RuntimeError(f"prompt has {L} tokens, a slot holds {self.cap}")
+        with _lib.on_device(self.data, k, v):
+            k, v = _rows(k), _rows(v)
+            (k_hs, k_rs), (v_hs, v_rs) = _strides(k), _strides(v)
+            _lib.call("gaac_fp4_store", k, v, k_hs, k_rs, v_hs, v_rs, L, self.n_kv, self.tiles, self.data[slot * self.n_kv], self.lens[slot:], _lib.stream)
+
+    # ------------------------------------------------------------------ decode step
+    def append(self, slots: torch.Tensor, k: torch.Tensor, v: torch.Tensor):
+        """Decode-step write: batch row b adds the token k[b], v[b] (bf16 [B, n_kv, D], through any strides of whole 16 bytes) to slot slots[b] (int32 [B]; -1 leaves the
+        row out).  One launch, no wait.  A row whose slot is full, stands earlier in the batch already or does not exist is left out, and check_capacity raises."""
+        self._check("append", k, v)
+        if slots.dtype != torch.int32 or slots.dim() != 1 or slots.shape[0] != k.shape[0]: raise RuntimeError("append expects slots int32 [B]")
+        if k.shape[0] == 0: return
+        with _lib.on_device(self.data, slots, k, v):
+            k, v = _rows(k), _rows(v)
+            (k_hs, k_bs), (v_hs, v_bs) = _strides(k), _strides(v)
+            _lib.call("gaac_fp4_append", slots.contiguous(), slots.shape[0], self.n_slots, self.n_kv, k, v, k_bs, k_hs, v_bs, v_hs, self.lens, self.tiles, self.cap,
+                      self.data, self.overflow, _lib.stream)
+
+    def attention(self, q: torch.Tensor, slots: torch.Tensor, scale: float, max_len: int | None = None, nsplit: int | None = None) -> torch.Tensor:
+        """Decode-step read: bf16 [B, n_q, D] queries, row b over everything slot slots[b] holds; returns bf16 [B, n_q, D].  A row whose slot is -1 or empty is 0, one
+        whose slot does not exist NaN.  max_len, the longest row if the caller knows it, only picks the split count when nsplit is not given."""
+        if q.dtype != torch.bfloat16 or q.dim() != 3 or q.shape[2] != D: raise RuntimeError(f"attention expects q bf16 [B, n_q, {D}], got {q.dtype} {list(q.shape)}")
+        B, n_q, _ = q.shape
+        if n_q % self.n_kv or not 1 <= n_q // self.n_kv <= GMAX: raise RuntimeError(f"GQA group size must be 1..{GMAX}")
+        if slots.dtype != torch.int32 or slots.dim() != 1 or slots.shape[0] != B: raise RuntimeError("attention expects slots int32 [B]")
+        if nsplit is None: nsplit = choose_nsplit(max(B, 1), self.n_kv, min(int(max_len or self.cap), self.cap))
+        if nsplit < 1: raise RuntimeError(f"attention expects at least one split, got {nsplit}")
+        with _lib.on_device(self.data, q, slots):
+            out = torch.empty(B, n_q, D, dtype=q.dtype, device=q.device)
+            if B == 0: return out
+            partials = torch.empty(B * nsplit * n_q * (D + 2), dtype=torch.float32, device=q.device) if nsplit > 1 else None
+            q = q if q.is_contiguous() and q.data_ptr() % 16 == 0 else q.clone(memory_format=torch.contiguous_format)
+            _lib.call("gaac_fp4_attn", self.data, self.lens, slots.contiguous(), self.n_slots, self.tiles, self.cap, q, B, n_q, self.n_kv, float(scale), nsplit, partials, out, _lib.stream)
+            return out
+
+    # ------------------------------------------------------------------ housekeeping
+    def check_capacity(self, used: int | None = None):
+        """Raises if append had to leave a row out since the cache was made (waits for the stream).  used: the word, if the caller fetched it already."""
+        hit = int(self.overflow) if used is None else used
+        if hit:
+            raise RuntimeError("4-bit KV cache lost data:" + (" a sequence grew past the slot's token capacity;" if hit & 1 else "") +
+                               (" a slot stood twice in a batch;" if hit & 2 else "") + (" a batch named a slot that does not exist" if hit & 4 else ""))
+
+    def decompress(self, slot: int) -> tuple[torch.Tensor, torch.Tensor]:
+        """The K and V that `slot` holds, bf16 [L, n_kv, D] each (waits for the stream, to read the slot's length)."""
+        if not 0 <= slot < self.n_slots: raise RuntimeError(f"decompress expects a slot in 0..{self.n_slots - 1}, got {slot}")
+        L = int(self.lens[slot])
+        k = torch.empty(L, self.n_kv, D, dtype=torch.bfloat16, device=self.data.device)
+        v = torch.empty_like(k)
+        if L:
+            with _lib.on_device(self.data):
+                _lib.call("gaac_fp4_load", self.data[slot * self.n_kv], L, self.n_kv, self.tiles, k, v, D, self.n_kv * D, D, self.n_kv * D, _lib.stream)
+        return k, v
+
+    def stats(self) -> dict:
+        """Occupancy (the keys of CompressedKVCache.stats): bytes_used counts codes and exponents of the tokens held."""
+        tokens = int(self.lens.sum())
+        used, bf16 = tokens * self.n_kv * 2 * ROW_BYTES, tokens * self.n_kv * 2 * D * 2
+        return dict(tokens=tokens, bytes_used=used, bf16_bytes=bf16, ratio=bf16 / max(1, used))

@@ -234,6 +234,41 @@ int gaac_bf16_attn(const void* k, const void* v, int S, const int* seq_lens, lon
                    int n_kv, float scale, int nsplit, unsigned long long* pm, unsigned long long* pl, unsigned long long* pa,
                    unsigned int* epoch, void* out, void* stream);
 
+/* A slot cache in 4 bits (OCP MXFP4, 32 channels of a token and head share an exponent; the tile format is stated in gaac_amd/csrc/fp4.hip): cache heads of
+ * `tiles` tiles of 32 tokens, 4352 bytes a tile (K and V), slot s owning heads s*n_kv .. ; lens int32 [n_slots] tokens per slot.
+ * gaac_fp4_store: a prompt of L tokens becomes what a slot holds.  cache: the slot's first tile; len: its word of lens.  k, v: bf16, element (token t, head h,
+ * channel c) at x[t*row_stride + h*head_stride + c], rows 16-byte aligned. */
+int gaac_fp4_store(const void* k, const void* v, long k_head_stride, long k_row_stride, long v_head_stride, long v_row_stride, int L, int n_kv, int tiles,
+                   uint8_t* cache, int* len, void* stream);
+/* gaac_fp4_load: the values of a slot's first L tokens, bf16; cache: the slot's first tile. */
+int gaac_fp4_load(const uint8_t* cache, int L, int n_kv, int tiles, void* k, void* v, long k_head_stride, long k_row_stride, long v_head_stride,
+                  long v_row_stride, void* stream);
+/* gaac_fp4_append: batch row b adds a token, k, v bf16 element (row b, head h, channel c) at x[b*batch_stride + h*head_stride + c], to slot slots[b] (below 0:
+ * none).  A row that cannot be added is left out and sets a bit in errors: 1 = the slot holds cap tokens already, 2 = an earlier row of the batch names the
+ * same slot, 4 = there is no such slot. */
+int gaac_fp4_append(const int* slots, int B, int n_slots, int n_kv, const void* k, const void* v, long k_batch_stride, long k_head_stride, long v_batch_stride,
+                    long v_head_stride, int* lens, int tiles, int cap, uint8_t* cache, int* errors, void* stream);
+/* gaac_fp4_attn: decode attention, q bf16 [B, n_q, 128], row b over what slot slots[b] holds (below 0 or without tokens: 0; n_slots or above: NaN); out bf16
+ * [B, n_q, 128].  The rows' tiles are shared out over B * nsplit splits a kv head by the lengths found on the device.  partials: scratch of this launch, fp32
+ * [B*nsplit*n_q*130], need not be set to anything (NULL where nsplit is 1). */
+int gaac_fp4_attn(const uint8_t* cache, const int* lens, const int* slots, int n_slots, int tiles, int cap, const void* q, int B, int n_q, int n_kv, float scale,
+                  int nsplit, float* partials, void* out, void* stream);
+
+/* Norms of queries and keys for each head and their rotation (the model's steps before /root/reference/nanovllm/layers/attention.py:43-96).  type: 0 bf16,
+ * 1 fp16, 2 fp32, of q, k, the weights and the outputs.  q [N, n_q, D], k [N, n_k, D] through strides in elements (channels next to each other, rows
+ * 16-byte aligned); weights [D], or [heads, D] with a stride, or both NULL: no norm.  cos, sin fp32 [max_pos, R/2]: of the first R channels the pairs
+ * (p, p + R/2), or (2p, 2p + 1) if interleaved, are rotated by row positions[token] (int64 if positions64, else int32); a position outside makes NaN.
+ * q_out [N, n_q, D], k_out [N, n_k, D]: contiguous, not over the inputs. */
+int gaac_qk_norm_rope(int type, const void* q, const void* k, long q_token_stride, long q_head_stride, long k_token_stride, long k_head_stride, long N, int n_q,
+                      int n_k, int D, int R, const void* q_weight, const void* k_weight, long q_weight_stride, long k_weight_stride, float eps,
+                      const void* positions, int positions64, const float* cos, const float* sin, int max_pos, int interleaved, void* q_out, void* k_out,
+                      void* stream);
+
+/* One token per row of logits [B, V] (type as above, rows row_stride elements apart): out int64 [B].  Each setting comes per row (device, [B]) or, where
+ * that is NULL, as one number.  u in [0, 1).  The definition is stated in gaac_amd/csrc/sample.hip. */
+int gaac_sample(int type, const void* logits, long row_stride, int B, int V, const float* u, const float* temperature_rows, float temperature, const int* top_k_rows,
+                int top_k, const float* top_p_rows, float top_p, const float* min_p_rows, float min_p, int64_t* out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
