@@ -14,8 +14,9 @@
 
 namespace {
 
-constexpr int NT = 1024, BINS = 2048, CHUNK = 512, MAX_V = 1 << 20, MAX_CHUNKS = MAX_V / CHUNK;
-static_assert(MAX_CHUNKS <= BINS);
+constexpr int NT = 512, SEG = NT * 8, BINS = 2048, MAX_V = 1 << 20, MAX_SEGS = MAX_V / SEG;      // a segment is a block's: 8 elements a thread
+constexpr int ROOM = 8192;      // elements of a row that are looked at one by one, at most
+static_assert(MAX_SEGS <= NT);
 typedef unsigned long long u64;
 typedef unsigned u4 __attribute__((ext_vector_type(4)));
 
@@ -31,21 +32,26 @@ template <typename T> __device__ __forceinline__ float number(T v) {
   return x != x ? -__builtin_inff() : x + 0.f;      // -0 + 0 = +0: equal numbers have equal keys
 }
 
-// The row as chunks of 512 elements from the 16-byte boundary at or below its start; a lane has 8 in a row.  Elements before and behind the row are -inf.
+// The row as segments from the 16-byte boundary at or below its start; a thread has 8 elements in a row.  Elements before and behind the row are -inf.
 template <typename T> struct Row {
   const T* base;      // aligned
   int shift, V;       // row element i is base[shift + i]
-  __device__ __forceinline__ int chunks() const { return (shift + V + CHUNK - 1) / CHUNK; }
-  __device__ __forceinline__ void load(int chunk, int l, float (&x)[8]) const {
+  __device__ __forceinline__ Row(const T* start, int V_) : shift((int)(reinterpret_cast<uintptr_t>(start) % 16 / sizeof(T))), V(V_) { base = start - shift; }
+  __device__ __forceinline__ int segs() const { return (shift + V + SEG - 1) / SEG; }
+  __device__ __forceinline__ int index(int seg, int i) const { return seg * SEG + threadIdx.x * 8 + i; }      // of element i of the thread, counted from base
+  __device__ __forceinline__ void load(int seg, float (&x)[8]) const {
     constexpr int G = 16 / sizeof(T);      // elements of a 16-byte load
+#pragma unroll
     for (int part = 0; part < 8 / G; ++part) {
-      const int at = chunk * CHUNK + l * 8 + part * G;
+      const int at = index(seg, part * G);
       if (at >= shift && at + G <= shift + V) {
         const u4 raw = *reinterpret_cast<const u4*>(base + at);
         T v[G];
         __builtin_memcpy(v, &raw, 16);
+#pragma unroll
         for (int i = 0; i < G; ++i) x[part * G + i] = number(v[i]);
       } else {
+#pragma unroll
         for (int i = 0; i < G; ++i) x[part * G + i] = at + i >= shift && at + i < shift + V ? number(base[at + i]) : -__builtin_inff();
       }
     }
@@ -87,61 +93,90 @@ __device__ __forceinline__ u64 wave_scan(u64 x, int l) {      // inclusive
   for (int o = 1; o < 64; o <<= 1) { const u64 y = __shfl_up(x, o); if (l >= o) x += y; }
   return x;
 }
+__device__ __forceinline__ unsigned wave_scan(unsigned x, int l) {
+  for (int o = 1; o < 64; o <<= 1) { const unsigned y = __shfl_up(x, o); if (l >= o) x += y; }
+  return x;
+}
 
+constexpr int WAVES = NT / 64;
 struct Shared {
-  u64 mass[BINS];           // of bins; of chunks
+  u64 mass[BINS];           // of bins; candidates in order
   unsigned count[BINS];
-  u64 wave_mass[16];
-  unsigned wave_count[16];
-  u64 best[16];
-  u64 total;
-  u64 before_mass;
-  unsigned before_count;
-  int found;
+  u64 seg_mass[MAX_SEGS];
+  unsigned seg_ties[MAX_SEGS];
+  u64 wave_mass[WAVES];
+  unsigned wave_count[WAVES];
+  u64 total, before_mass;
+  unsigned total_count, before_count, base, key, ties;
+  int found, last;
 };
 
-// Inclusive prefix sums over the block of each thread's (count, mass); afterwards sh.total and the last thread's count are complete.
+// Inclusive prefix sums over the block of each thread's (count, mass); sh.total_count and sh.total are those of all.
 __device__ __forceinline__ void block_scan(Shared& sh, unsigned& count, u64& mass) {
   const int l = threadIdx.x & 63, w = threadIdx.x >> 6;
   mass = wave_scan(mass, l);
-  count = (unsigned)wave_scan(count, l);
+  count = wave_scan(count, l);
   if (l == 63) { sh.wave_mass[w] = mass; sh.wave_count[w] = count; }
   __syncthreads();
   for (int i = 0; i < w; ++i) { mass += sh.wave_mass[i]; count += sh.wave_count[i]; }
+  if (threadIdx.x == NT - 1) { sh.total = mass; sh.total_count = count; }
   __syncthreads();
 }
 
-// Where a limit falls: the key of the last element kept, how many of its equals are, and count and sum of what stands before that key.
-struct Limit { unsigned key, ties; };
+struct Limit { unsigned key, ties; };      // the key of the last element kept, and how many of its equals are kept; key 0: all
 
-// The first element in the order at which the running count reaches `count` (BY_MASS false) or the running sum of weights reaches `mass` (true), among the
-// elements with key above `from.key` and from.ties of its equals.
-template <bool BY_MASS, typename T>
-__device__ Limit find_limit(Shared& sh, const Row<T>& row, const Weights& weight, float bin_scale, Limit from, unsigned want_count, u64 want_mass) {
-  const int l = threadIdx.x & 63, w = threadIdx.x >> 6, chunks = row.chunks();
+struct Bins {      // of max - x, 1/32 of the temperature (or of 1, if that is less) wide, 64 of it in all; never ascends with x
+  float top, scale;
+  __device__ __forceinline__ Bins(float top_, float t) : top(top_), scale(fmaxf(32.f / t, 32.f)) {}
+  __device__ __forceinline__ int operator()(float x) const { return x == top ? 0 : (int)fminf((top - x) * scale, (float)(BINS - 1)); }
+};
+
+// Zero the bins / find the first of them at which the running count or sum reaches what is wanted: into sh.found (-1: none), before_count, before_mass.
+__device__ __forceinline__ void clear_bins(Shared& sh) {
+  for (int i = threadIdx.x; i < BINS; i += NT) { sh.mass[i] = 0; sh.count[i] = 0; }
+  __syncthreads();
+}
+template <bool BY_MASS> __device__ void find_bin(Shared& sh, unsigned before_count, u64 before_mass, unsigned want_count, u64 want_mass) {
+  constexpr int PER = BINS / NT;
+  unsigned count = 0;
+  u64 mass = 0;
+  const int b0 = threadIdx.x * PER;
+  for (int i = 0; i < PER; ++i) { count += sh.count[b0 + i]; mass += sh.mass[b0 + i]; }
+  const unsigned own_count = count;
+  const u64 own_mass = mass;
+  if (threadIdx.x == 0) sh.found = -1;
+  block_scan(sh, count, mass);
+  count += before_count - own_count; mass += before_mass - own_mass;      // before this thread's bins
+  for (int i = 0; i < PER; ++i) {
+    const unsigned c = count + sh.count[b0 + i];
+    const u64 m = mass + sh.mass[b0 + i];
+    if (BY_MASS ? mass < want_mass && m >= want_mass : count < want_count && c >= want_count) { sh.found = b0 + i; sh.before_count = count; sh.before_mass = mass; }
+    count = c; mass = m;
+  }
+  __syncthreads();
+}
+
+// The first element in the order at which the running count reaches want_count (BY_MASS false) or the running sum of weights reaches want_mass (true), among
+// the elements with key above `from.key` and from.ties of its equals.  each(f) calls f(x) for the thread's share of the elements.
+template <bool BY_MASS, typename Each>
+__device__ Limit find_limit(Shared& sh, Each each, const Weights& weight, const Bins& bin_of, Limit from, unsigned want_count, u64 want_mass) {
   unsigned lo = 0, hi = 0xffffffffu, before_count = 0;
   u64 before_mass = 0;
   int bin0 = -1;
   const float top = weight.top;
-  const auto bin_of = [&](float x) { return x == top ? 0 : (int)fminf((top - x) * bin_scale, (float)(BINS - 1)); };      // never ascends with x
   for (int level = 0;; ++level) {
     // level 0: bins of top - x; then bins of 2^s keys in [lo, hi]
     const int s = level == 0 ? 0 : max(0, 32 - __builtin_clz((hi - lo) | 1) - 11);
-    for (int i = threadIdx.x; i < BINS; i += NT) { sh.mass[i] = 0; sh.count[i] = 0; }
-    __syncthreads();
-    for (int c = w; c < chunks; c += NT / 64) {
-      float x[8];
-      row.load(c, l, x);
-      for (int i = 0; i < 8; ++i) {
-        const unsigned k = key_of(x[i]);
-        if (x[i] == -__builtin_inff() || k < from.key || k < lo || k > hi) continue;
-        const int b0 = bin_of(x[i]);
-        if (level > 0 && b0 != bin0) continue;
-        const int b = level == 0 ? b0 : (int)((hi - k) >> s);
-        atomicAdd(&sh.count[b], 1u);
-        if constexpr (BY_MASS) if (k != from.key) { const u64 m = fixed(weight(x[i])); if (m) atomicAdd(&sh.mass[b], m); }
-      }
-    }
+    clear_bins(sh);
+    each([&](float x) {
+      const unsigned k = key_of(x);
+      if (x == -__builtin_inff() || k < from.key || k < lo || k > hi) return;
+      const int b0 = bin_of(x);
+      if (level > 0 && b0 != bin0) return;
+      const int b = level == 0 ? b0 : (int)((hi - k) >> s);
+      atomicAdd(&sh.count[b], 1u);
+      if constexpr (BY_MASS) if (k != from.key) { const u64 m = fixed(weight(x)); if (m) atomicAdd(&sh.mass[b], m); }
+    });
     __syncthreads();
     if constexpr (BY_MASS) {      // the equals of the limit that is there already: only the first of them are kept
       if (threadIdx.x == 0 && from.key != 0 && from.key >= lo && from.key <= hi) {
@@ -151,32 +186,17 @@ __device__ Limit find_limit(Shared& sh, const Row<T>& row, const Weights& weight
       }
       __syncthreads();
     }
-    unsigned count = 0;
-    u64 mass = 0;
-    const int b0 = threadIdx.x * (BINS / NT);
-    for (int i = 0; i < BINS / NT; ++i) { count += sh.count[b0 + i]; mass += sh.mass[b0 + i]; }
-    const unsigned own_count = count;
-    const u64 own_mass = mass;
-    if (threadIdx.x == 0) sh.found = -1;
-    block_scan(sh, count, mass);
-    count += before_count - own_count; mass += before_mass - own_mass;      // before this thread's bins
-    for (int i = 0; i < BINS / NT; ++i) {
-      const bool reached = BY_MASS ? mass < want_mass && mass + sh.mass[b0 + i] >= want_mass : count < want_count && count + sh.count[b0 + i] >= want_count;
-      if (reached) { sh.found = b0 + i; sh.before_count = count; sh.before_mass = mass; }
-      count += sh.count[b0 + i]; mass += sh.mass[b0 + i];
-    }
-    __syncthreads();
+    find_bin<BY_MASS>(sh, before_count, before_mass, want_count, want_mass);
     const int f = sh.found;
-    if (f < 0) return from.key ? from : Limit{0, 0};      // not reached: all of them
+    if (f < 0) { __syncthreads(); return from; }      // not reached: all of them
     before_count = sh.before_count; before_mass = sh.before_mass;
     if (level == 0) {
       bin0 = f;
+      lo = 0; hi = key_of(top);
       if (__builtin_isfinite(top) && f < BINS - 1) {      // bounds of the bin's keys, with room for the roundings of its index
-        const double a = (double)top - (f + 1) / (double)bin_scale * (1 + 1e-6), b = (double)top - f / (double)bin_scale * (1 - 1e-6);
-        lo = key_of((float)a + 0.f) - 2; hi = min(key_of((float)b + 0.f) + 2, key_of(top));
-        if (!(a > -3e38)) lo = 0;
-      } else {
-        lo = 0; hi = key_of(top);
+        const double a = (double)top - (f + 1) / (double)bin_of.scale * (1 + 1e-6), b = (double)top - f / (double)bin_of.scale * (1 - 1e-6);
+        if (a > -3e38) lo = key_of((float)a + 0.f) - 2;
+        if (b > -3e38) hi = min(key_of((float)b + 0.f) + 2, hi);
       }
       lo = max(lo, from.key); hi = max(hi, lo);
     } else {
@@ -198,148 +218,383 @@ __device__ Limit find_limit(Shared& sh, const Row<T>& row, const Weights& weight
   return r;
 }
 
+__device__ __forceinline__ u64 share_of(float p, u64 total) {      // the least whole number that is at least p * total, and at least 1
+  const double want = (double)p * (double)total;
+  u64 m = want > 0 ? (u64)want : 0;
+  if ((double)m < want) ++m;
+  return m > 0 ? m : 1;
+}
+
 struct Setting { const float* rows; float all; __device__ float operator()(int b) const { return rows ? rows[b] : all; } };
 struct Args {
   const void* logits;
   long stride;
-  int V;
+  int V, segs;      // segments of a row, at most
   const float* u;
   Setting temperature, top_p, min_p;
   const int* top_k_rows;
   int top_k;
   long* out;
+  uint8_t* work;
 };
 
-template <typename T> __global__ __launch_bounds__(NT) void k_sample(Args a) {
-  __shared__ Shared sh;
-  const int b = blockIdx.x, l = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const T* start = static_cast<const T*>(a.logits) + b * a.stride;
-  const int shift = (int)(reinterpret_cast<uintptr_t>(start) % 16 / sizeof(T));
-  const Row<T> row{start - shift, shift, a.V};
-  const int chunks = row.chunks();
-  // the maximum, and the first place that has it
-  u64 best = 0;
-  for (int c = w; c < chunks; c += NT / 64) {
-    float x[8];
-    row.load(c, l, x);
-    for (int i = 0; i < 8; ++i) {
-      const u64 e = (u64)key_of(x[i]) << 32 | (unsigned)~(c * CHUNK + l * 8 + i);
-      best = best > e ? best : e;
-    }
+// What a row's blocks leave for each other (in a.work, set up by the first launch).
+struct Work {
+  u64 *best, *seg_mass, *mass, *candidates;
+  unsigned *count, *ticket, *n;
+  static __host__ __device__ long bytes(int segs) { return 16l * segs + 12l * BINS + 8l * ROOM + 16; }
+  __device__ Work(const Args& a, int b) {
+    uint8_t* p = a.work + b * bytes(a.segs);
+    best = reinterpret_cast<u64*>(p); seg_mass = best + a.segs; mass = seg_mass + a.segs; candidates = mass + BINS;
+    count = reinterpret_cast<unsigned*>(candidates + ROOM); ticket = count + BINS; n = ticket + 1;
   }
+};
+
+struct Settings {
+  float t, p, min_p;
+  int k;      // 0: none
+  __device__ __forceinline__ Settings(const Args& a, int b) : t(a.temperature(b)), p(a.top_p(b)) {
+    const float m = a.min_p(b);
+    min_p = m > 1 ? 1 : m;
+    k = a.top_k_rows ? a.top_k_rows[b] : a.top_k;
+    if (k <= 0 || k >= a.V) k = 0;
+  }
+  __device__ __forceinline__ bool greedy() const { return !(t > 0); }
+  __device__ __forceinline__ bool cut() const { return k > 0 || p < 1; }
+};
+
+// max of key << 32 | ~index over the block
+__device__ __forceinline__ u64 block_best(Shared& sh, u64 best) {
   for (int o = 32; o > 0; o >>= 1) { const u64 y = __shfl_xor(best, o); best = best > y ? best : y; }
-  if (l == 0) sh.best[w] = best;
+  if ((threadIdx.x & 63) == 0) sh.wave_mass[threadIdx.x >> 6] = best;
   __syncthreads();
-  for (int i = 0; i < NT / 64; ++i) best = best > sh.best[i] ? best : sh.best[i];
-  const float top = value_of((unsigned)(best >> 32)), t = a.temperature(b);
-  if (top == -__builtin_inff()) { if (threadIdx.x == 0) a.out[b] = -1; return; }
-  if (!(t > 0)) { if (threadIdx.x == 0) a.out[b] = (long)(unsigned)~(unsigned)best - shift; return; }
-  const Weights weight{top, 1.0 / (double)t};
-  const float bin_scale = fmaxf(32.f / t, 32.f), p = a.top_p(b), m = a.min_p(b), min_p = m > 1 ? 1 : m;
-  const int k = a.top_k_rows ? a.top_k_rows[b] : a.top_k;
-  Limit limit{0, 0};      // key 0: none
-  if (k > 0 && k < a.V) limit = find_limit<false>(sh, row, weight, bin_scale, limit, (unsigned)k, 0);
-  if (p < 1) {
-    // the sum that p is a share of
+  best = 0;
+  for (int i = 0; i < WAVES; ++i) best = best > sh.wave_mass[i] ? best : sh.wave_mass[i];
+  __syncthreads();
+  return best;
+}
+template <typename T> __device__ __forceinline__ u64 segment_best(const Row<T>& row, int seg, const float (&x)[8]) {
+  u64 best = 0;
+  for (int i = 0; i < 8; ++i) {
+    const u64 e = (u64)key_of(x[i]) << 32 | (unsigned)~row.index(seg, i);
+    best = best > e ? best : e;
+  }
+  return best;
+}
+// The rows that need no weights: true if it is done.
+template <typename T> __device__ __forceinline__ bool easy(const Args& a, int b, const Row<T>& row, const Settings& set, u64 best, bool writes) {
+  const bool none = value_of((unsigned)(best >> 32)) == -__builtin_inff();
+  if (!none && !set.greedy()) return false;
+  if (writes && threadIdx.x == 0) a.out[b] = none ? -1 : (long)(unsigned)~(unsigned)best - row.shift;
+  return true;
+}
+
+// The limit by looking at every element, as often as it takes.
+template <typename Each> __device__ Limit full_limit(Shared& sh, Each each, const Settings& set, const Weights& weight, const Bins& bins) {
+  Limit limit{0, 0};
+  if (set.k > 0) limit = find_limit<false>(sh, each, weight, bins, limit, (unsigned)set.k, 0);
+  if (set.p < 1) {
     u64 mass = 0;
-    for (int c = w; c < chunks; c += NT / 64) {
-      float x[8];
-      row.load(c, l, x);
-      for (int i = 0; i < 8; ++i) if (key_of(x[i]) > limit.key) mass += fixed(weight(x[i]));
-    }
     unsigned count = 0;
+    each([&](float x) { if (key_of(x) > limit.key) mass += fixed(weight(x)); });
     block_scan(sh, count, mass);
-    if (threadIdx.x == NT - 1) sh.total = mass;
+    const u64 total = sh.total + (limit.key ? limit.ties * fixed(weight(value_of(limit.key))) : 0);
     __syncthreads();
-    u64 total = sh.total;
-    if (limit.key) total += limit.ties * fixed(weight(value_of(limit.key)));
-    const double want = (double)p * (double)total;
-    u64 target = want > 0 ? (u64)want : 0;
-    if ((double)target < want) ++target;
-    limit = find_limit<true>(sh, row, weight, bin_scale, limit, 0, target > 0 ? target : 1);
+    limit = find_limit<true>(sh, each, weight, bins, limit, 0, share_of(set.p, total));
   }
-  // sums of what is kept, by chunks
-  for (int c = w; c < chunks; c += NT / 64) {
-    float x[8];
-    row.load(c, l, x);
-    u64 mass = 0;
-    unsigned ties = 0;
-    for (int i = 0; i < 8; ++i) {
-      const unsigned key = key_of(x[i]);
-      if (key < limit.key) continue;
-      if (key == limit.key) { ++ties; continue; }
-      const double e = weight(x[i]);
-      if (!(e < min_p)) mass += fixed(e);
-    }
-    for (int o = 32; o > 0; o >>= 1) { mass += __shfl_xor(mass, o); ties += __shfl_xor(ties, o); }
-    if (l == 0) { sh.mass[c] = mass; sh.count[c] = ties; }
-  }
-  __syncthreads();
-  const double tie_weight = limit.key ? weight(value_of(limit.key)) : 0.0;
-  const u64 tie_mass = tie_weight < min_p ? 0 : fixed(tie_weight);
-  constexpr int PER = (MAX_CHUNKS + NT - 1) / NT;
-  unsigned ties = 0;
+  return limit;
+}
+template <typename T> __device__ __forceinline__ u64 kept_mass(const float (&x)[8], const Weights& weight, const Settings& set, unsigned above, unsigned& ties) {
   u64 mass = 0;
-  for (int i = 0; i < PER; ++i) { const int c = threadIdx.x * PER + i; if (c < chunks) ties += sh.count[c]; }
-  const unsigned own_ties = ties;
+  for (int i = 0; i < 8; ++i) {
+    const unsigned key = key_of(x[i]);
+    ties += key == above;
+    if (key <= above) continue;
+    const double e = weight(x[i]);
+    if (!(e < set.min_p)) mass += fixed(e);
+  }
+  return mass;
+}
+
+// The limit among n candidates (key << 32 | index): all elements of the order up to the limit but those of `certain` weight, of which none is a candidate.
+__device__ Limit candidate_limit(Shared& sh, const u64* cand, int n, const Settings& set, const Weights& weight, const Bins& bins, u64 want) {
+  if (n <= NT) {      // by rank: a thread counts what comes before its candidate, which puts it in its place in the order
+    const u64 e = threadIdx.x < n ? cand[threadIdx.x] ^ 0xffffffffu : 0;      // descends in the order
+    sh.mass[threadIdx.x] = e;
+    __syncthreads();
+    int rank = 0;
+    for (int i = 0; i < n; ++i) rank += sh.mass[i] > e;
+    __syncthreads();
+    if (threadIdx.x < n) sh.mass[rank] = e;
+    __syncthreads();
+    const unsigned key = threadIdx.x < n ? (unsigned)(sh.mass[threadIdx.x] >> 32) : 0;
+    const int k = set.k > 0 ? min(set.k, n) : n;
+    u64 mass = 0;
+    int keep = k;
+    if (set.p < 1) {
+      if (threadIdx.x < k) mass = fixed(weight(value_of(key)));
+      const u64 own = mass;
+      unsigned none = 0;
+      block_scan(sh, none, mass);
+      const u64 target = set.k > 0 ? share_of(set.p, sh.total) : want;
+      if (threadIdx.x == 0) sh.found = k;
+      __syncthreads();
+      if (threadIdx.x < k && mass - own < target && mass >= target) sh.found = threadIdx.x + 1;
+      __syncthreads();
+      keep = sh.found;
+    }
+    const unsigned last = (unsigned)(sh.mass[keep - 1] >> 32);
+    const unsigned ties = __syncthreads_count(threadIdx.x < keep && key == last);
+    return Limit{last, ties};
+  }
+  const auto each = [&](auto f) { for (int i = threadIdx.x; i < n; i += NT) f(value_of((unsigned)(cand[i] >> 32))); };
+  return set.k > 0 ? full_limit(sh, each, set, weight, bins) : find_limit<true>(sh, each, weight, bins, Limit{0, 0}, 0, want);
+}
+
+// The token: sh.seg_mass and sh.seg_ties hold, by segments, the kept sums above limit.key and the number of its equals.
+template <typename T> __device__ void draw(Shared& sh, const Args& a, int b, const Row<T>& row, const Settings& set, const Weights& weight, Limit limit) {
+  const int segs = row.segs(), s = threadIdx.x;
+  const double tie_weight = limit.key ? weight(value_of(limit.key)) : 0.0;
+  const u64 tie_mass = tie_weight < set.min_p ? 0 : fixed(tie_weight);
+  const unsigned own_ties = s < segs ? sh.seg_ties[s] : 0;
+  unsigned ties = own_ties, none = 0;
+  u64 mass = 0;
   block_scan(sh, ties, mass);
-  ties -= own_ties;
-  const unsigned first_ties = ties;
-  const auto kept_mass = [&](int c, unsigned before) { return sh.mass[c] + tie_mass * (before >= limit.ties ? 0u : min(sh.count[c], limit.ties - before)); };
-  mass = 0;
-  for (int i = 0; i < PER; ++i) { const int c = threadIdx.x * PER + i; if (c < chunks) { mass += kept_mass(c, ties); ties += sh.count[c]; } }
-  const u64 own_mass = mass;
-  unsigned none = 0;
+  const unsigned before = ties - own_ties;
+  const u64 own = s < segs ? sh.seg_mass[s] + tie_mass * (before >= limit.ties ? 0u : min(own_ties, limit.ties - before)) : 0;
+  mass = own;
   block_scan(sh, none, mass);
-  if (threadIdx.x == NT - 1) sh.total = mass;
-  __syncthreads();
   const u64 total = sh.total;
   const double want = (double)a.u[b] * (double)total;
-  u64 target = want > 0 ? (want < (double)total ? (u64)want : total - 1) : 0;      // the first running sum above it
-  target = min(target, total - 1);
-  u64 at = mass - own_mass;
-  ties = first_ties;
-  for (int i = 0; i < PER; ++i) {
-    const int c = threadIdx.x * PER + i;
-    if (c >= chunks) break;
-    const u64 m = kept_mass(c, ties);
-    if (at <= target && target < at + m) { sh.found = c; sh.before_mass = at; sh.before_count = ties; }
-    at += m; ties += sh.count[c];
-  }
+  const u64 target = want > 0 ? (want < (double)total ? min((u64)want, total - 1) : total - 1) : 0;      // the first running sum above it
+  if (mass - own <= target && target < mass) { sh.found = s; sh.before_mass = mass - own; sh.before_count = before; }
   __syncthreads();
-  if (w != 0) return;
-  const int c = sh.found;
+  const int seg = sh.found;
+  const u64 before_mass = sh.before_mass;
+  const unsigned before_ties = sh.before_count;
   float x[8];
-  row.load(c, l, x);
-  unsigned lane_ties = 0;
-  for (int i = 0; i < 8; ++i) lane_ties += key_of(x[i]) == limit.key;
-  unsigned seen = sh.before_count + (unsigned)wave_scan(lane_ties, l) - lane_ties;
+  row.load(seg, x);
+  unsigned t = 0;
+  for (int i = 0; i < 8; ++i) t += key_of(x[i]) == limit.key;
+  const unsigned own_t = t;
+  mass = 0;
+  block_scan(sh, t, mass);
+  unsigned seen = before_ties + t - own_t;
   u64 e[8], sum = 0;
   for (int i = 0; i < 8; ++i) {
     const unsigned key = key_of(x[i]);
     e[i] = 0;
     if (key == limit.key) { if (seen++ < limit.ties) e[i] = tie_mass; }
-    else if (key > limit.key) { const double y = weight(x[i]); if (!(y < min_p)) e[i] = fixed(y); }
+    else if (key > limit.key) { const double y = weight(x[i]); if (!(y < set.min_p)) e[i] = fixed(y); }
     sum += e[i];
   }
-  u64 run = sh.before_mass + wave_scan(sum, l) - sum;
+  mass = sum;
+  block_scan(sh, none, mass);
+  u64 run = before_mass + mass - sum;
   for (int i = 0; i < 8; ++i) {
-    if (run <= target && target < run + e[i]) a.out[b] = (long)c * CHUNK + l * 8 + i - shift;
+    if (run <= target && target < run + e[i]) a.out[b] = row.index(seg, i) - row.shift;
     run += e[i];
   }
 }
 
+// Whether this block is the last of its row to come here; what the others wrote before is then to be seen.  (One thread's release and acquire stand for the
+// block's, between two barriers: each of them writes back or empties a cache.)
+__device__ __forceinline__ bool last_of_row(Shared& sh, const Work& work) {
+  __syncthreads();
+  if (threadIdx.x == 0) sh.last = __hip_atomic_fetch_add(work.ticket, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
+  __syncthreads();
+  return sh.last;
+}
+
+// First launch: the maximum of each segment; the row's bins and counters are zeroed.
+template <typename T> __global__ __launch_bounds__(NT) void k_sample_max(Args a) {
+  __shared__ Shared sh;
+  const int seg = blockIdx.x, b = blockIdx.y;
+  const Row<T> row(static_cast<const T*>(a.logits) + b * a.stride, a.V);
+  const Work work(a, b);
+  float x[8];
+  row.load(seg, x);
+  for (int i = seg * NT + threadIdx.x; i < BINS; i += gridDim.x * NT) { work.mass[i] = 0; work.count[i] = 0; }
+  const u64 best = block_best(sh, segment_best(row, seg, x));
+  if (threadIdx.x == 0) {
+    work.best[seg] = best;
+    if (seg == 0) *work.ticket = *work.n = 0;
+  }
+}
+
+// Second: rows that are cut get their bins (counts; sums only where there is no k, which leaves few), the others their token.
+template <typename T> __global__ __launch_bounds__(NT) void k_sample_bins(Args a) {
+  __shared__ Shared sh;
+  const int seg = blockIdx.x, b = blockIdx.y;
+  const Row<T> row(static_cast<const T*>(a.logits) + b * a.stride, a.V);
+  const Work work(a, b);
+  const Settings set(a, b);
+  float x[8];
+  row.load(seg, x);
+  const u64 best = block_best(sh, threadIdx.x < gridDim.x ? work.best[threadIdx.x] : 0);
+  if (easy(a, b, row, set, best, seg == 0)) return;
+  const Weights weight{value_of((unsigned)(best >> 32)), 1.0 / (double)set.t};
+  if (set.cut()) {
+    const Bins bins(weight.top, set.t);
+    clear_bins(sh);
+    for (int i = 0; i < 8; ++i) {
+      if (x[i] == -__builtin_inff()) continue;
+      const int bin = bins(x[i]);
+      atomicAdd(&sh.count[bin], 1u);
+      if (set.k == 0) { const u64 m = fixed(weight(x[i])); if (m) atomicAdd(&sh.mass[bin], m); }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < BINS; i += NT) {
+      if (sh.count[i]) atomicAdd(&work.count[i], sh.count[i]);
+      if (sh.mass[i]) atomicAdd(&work.mass[i], sh.mass[i]);
+    }
+    return;
+  }
+  unsigned ties = 0;
+  u64 mass = kept_mass<T>(x, weight, set, 0, ties);
+  block_scan(sh, ties, mass);
+  if (threadIdx.x == 0) work.seg_mass[seg] = sh.total;
+  if (!last_of_row(sh, work)) return;
+  if (threadIdx.x < row.segs()) { sh.seg_mass[threadIdx.x] = work.seg_mass[threadIdx.x]; sh.seg_ties[threadIdx.x] = 0; }
+  __syncthreads();
+  draw(sh, a, b, row, set, weight, Limit{0, 0});
+}
+
+// Third: the bin where the limit falls; its elements (with k: all up to it) become candidates, of what stands before it the segments' sums are taken.  The
+// row's last block finds the limit among the candidates and draws.
+template <typename T> __global__ __launch_bounds__(NT) void k_sample_draw(Args a) {
+  __shared__ Shared sh;
+  const int seg = blockIdx.x, b = blockIdx.y;
+  const Row<T> row(static_cast<const T*>(a.logits) + b * a.stride, a.V);
+  const Settings set(a, b);
+  if (!set.cut() || set.greedy()) return;
+  const Work work(a, b);
+  float x[8];
+  row.load(seg, x);
+  for (int i = threadIdx.x; i < BINS; i += NT) { sh.count[i] = work.count[i]; sh.mass[i] = work.mass[i]; }
+  const u64 best = block_best(sh, threadIdx.x < gridDim.x ? work.best[threadIdx.x] : 0);
+  if (easy(a, b, row, set, best, false)) return;
+  const Weights weight{value_of((unsigned)(best >> 32)), 1.0 / (double)set.t};
+  const Bins bins(weight.top, set.t);
+  u64 want = 0;
+  if (set.k > 0) {
+    find_bin<false>(sh, 0, 0, (unsigned)set.k, 0);
+  } else {
+    u64 m = 0;
+    unsigned c = 0;
+    for (int i = threadIdx.x; i < BINS; i += NT) m += sh.mass[i];
+    block_scan(sh, c, m);
+    want = share_of(set.p, sh.total);
+    __syncthreads();
+    find_bin<true>(sh, 0, 0, 0, want);
+  }
+  const int f = sh.found < 0 ? BINS - 1 : sh.found;      // fewer than k: all of them
+  const unsigned n = set.k > 0 ? (sh.found < 0 ? sh.total_count : sh.before_count + sh.count[f]) : sh.count[f];
+  if (set.k == 0) want -= sh.before_mass;
+  const bool room = n <= ROOM;
+  u64 mass = 0;
+  unsigned mine = 0, take = 0;
+  for (int i = 0; i < 8; ++i) {
+    if (x[i] == -__builtin_inff()) continue;
+    const int bin = bins(x[i]);
+    if (set.k > 0 ? bin <= f : bin == f) { take |= 1u << i; ++mine; }
+    else if (set.k == 0 && bin < f && room) { const double e = weight(x[i]); if (!(e < set.min_p)) mass += fixed(e); }
+  }
+  if (room) {
+    unsigned at = mine;
+    block_scan(sh, at, mass);
+    if (threadIdx.x == 0) {
+      work.seg_mass[seg] = sh.total;
+      sh.base = sh.total_count ? atomicAdd(work.n, sh.total_count) : 0;
+    }
+    __syncthreads();
+    at += sh.base - mine;
+    for (int i = 0; i < 8; ++i) if (take >> i & 1) work.candidates[at++] = (u64)key_of(x[i]) << 32 | (unsigned)row.index(seg, i);
+  }
+  if (!last_of_row(sh, work)) return;
+  const int segs = row.segs();
+  Limit limit;
+  if (room) {
+    limit = candidate_limit(sh, work.candidates, (int)n, set, weight, bins, want);
+    if (threadIdx.x < segs) { sh.seg_mass[threadIdx.x] = work.seg_mass[threadIdx.x]; sh.seg_ties[threadIdx.x] = 0; }
+    __syncthreads();
+    for (int i = threadIdx.x; i < (int)n; i += NT) {
+      const u64 c = work.candidates[i];
+      const unsigned key = (unsigned)(c >> 32);
+      if (key < limit.key) continue;
+      const int s = (unsigned)c / SEG;
+      if (key == limit.key) { atomicAdd(&sh.seg_ties[s], 1u); continue; }
+      const double e = weight(value_of(key));
+      if (!(e < set.min_p)) atomicAdd(&sh.seg_mass[s], fixed(e));
+    }
+  } else {
+    limit = full_limit(sh, [&](auto f) {
+      for (int s = 0; s < segs; ++s) {
+        float y[8];
+        row.load(s, y);
+        for (int i = 0; i < 8; ++i) f(y[i]);
+      }
+    }, set, weight, bins);
+    for (int s = 0; s < segs; ++s) {
+      row.load(s, x);
+      unsigned ties = 0;
+      u64 sum = kept_mass<T>(x, weight, set, limit.key, ties);
+      block_scan(sh, ties, sum);
+      if (threadIdx.x == 0) { sh.seg_mass[s] = sh.total; sh.seg_ties[s] = sh.total_count; }
+      __syncthreads();
+    }
+  }
+  __syncthreads();
+  draw(sh, a, b, row, set, weight, limit);
+}
+
+// Rows of one segment, in one launch.
+template <typename T> __global__ __launch_bounds__(NT) void k_sample_short(Args a) {
+  __shared__ Shared sh;
+  const int b = blockIdx.y;
+  const Row<T> row(static_cast<const T*>(a.logits) + b * a.stride, a.V);
+  const Settings set(a, b);
+  float x[8];
+  row.load(0, x);
+  const u64 best = block_best(sh, segment_best(row, 0, x));
+  if (easy(a, b, row, set, best, true)) return;
+  const Weights weight{value_of((unsigned)(best >> 32)), 1.0 / (double)set.t};
+  const Limit limit = full_limit(sh, [&](auto f) { for (int i = 0; i < 8; ++i) f(x[i]); }, set, weight, Bins(weight.top, set.t));
+  unsigned ties = 0;
+  u64 mass = kept_mass<T>(x, weight, set, limit.key, ties);
+  block_scan(sh, ties, mass);
+  if (threadIdx.x == 0) { sh.seg_mass[0] = sh.total; sh.seg_ties[0] = sh.total_count; }
+  __syncthreads();
+  draw(sh, a, b, row, set, weight, limit);
+}
+
+template <typename T> int launch(const Args& a, int B, bool cut, hipStream_t stream) {
+  const dim3 grid(a.segs, B);
+  if (a.segs == 1) {
+    k_sample_short<T><<<grid, NT, 0, stream>>>(a);
+    return gaac::launch_status("gaac_sample");
+  }
+  k_sample_max<T><<<grid, NT, 0, stream>>>(a);
+  k_sample_bins<T><<<grid, NT, 0, stream>>>(a);
+  if (cut) k_sample_draw<T><<<grid, NT, 0, stream>>>(a);
+  return gaac::launch_status("gaac_sample");
+}
+
+int segments(int V) { return (V + 7 + SEG - 1) / SEG; }      // whatever the rows' alignment
+
 }  // namespace
 
 extern "C" int gaac_sample(int type, const void* logits, long row_stride, int B, int V, const float* u, const float* temperature_rows, float temperature, const int* top_k_rows, int top_k,
-                           const float* top_p_rows, float top_p, const float* min_p_rows, float min_p, int64_t* out, void* stream) {
-  GAAC_REQUIRE(logits != nullptr && u != nullptr && out != nullptr, "gaac_sample: null pointer");
+                           const float* top_p_rows, float top_p, const float* min_p_rows, float min_p, void* work, long work_bytes, int64_t* out, void* stream) {
+  GAAC_REQUIRE(logits != nullptr && u != nullptr && out != nullptr && work != nullptr, "gaac_sample: null pointer");
   GAAC_REQUIRE(type >= 0 && type <= 2, "gaac_sample: type must be 0 (bf16), 1 (fp16) or 2 (fp32)");
-  GAAC_REQUIRE(B > 0 && V > 0 && V <= MAX_V - 16 && row_stride >= 0, "gaac_sample: bad sizes (%d rows of %d logits, at most %d)", B, V, MAX_V - 16);
+  GAAC_REQUIRE(B > 0 && B <= 65535 && V > 0 && V <= MAX_V - 16 && row_stride >= 0, "gaac_sample: bad sizes (%d rows of %d logits, at most 65535 of %d)", B, V, MAX_V - 16);
   GAAC_REQUIRE(reinterpret_cast<uintptr_t>(logits) % (type == 2 ? 4 : 2) == 0, "gaac_sample: logits are not aligned to their type");
-  const Args a{logits, row_stride, V, u, {temperature_rows, temperature}, {top_p_rows, top_p}, {min_p_rows, min_p}, top_k_rows, top_k, (long*)out};
-  if (type == 0) k_sample<__bf16><<<B, NT, 0, (hipStream_t)stream>>>(a);
-  else if (type == 1) k_sample<_Float16><<<B, NT, 0, (hipStream_t)stream>>>(a);
-  else k_sample<float><<<B, NT, 0, (hipStream_t)stream>>>(a);
-  return gaac::launch_status("gaac_sample");
+  const int segs = segments(V);
+  GAAC_REQUIRE(reinterpret_cast<uintptr_t>(work) % 8 == 0 && work_bytes >= B * Work::bytes(segs), "gaac_sample: %ld bytes of work memory, aligned to 8, are too few", work_bytes);
+  const Args a{logits, row_stride, V, segs, u, {temperature_rows, temperature}, {top_p_rows, top_p}, {min_p_rows, min_p}, top_k_rows, top_k, (long*)out, (uint8_t*)work};
+  const bool cut = top_k_rows != nullptr || top_p_rows != nullptr || (top_k > 0 && top_k < V) || top_p < 1;
+  if (type == 0) return launch<__bf16>(a, B, cut, (hipStream_t)stream);
+  if (type == 1) return launch<_Float16>(a, B, cut, (hipStream_t)stream);
+  return launch<float>(a, B, cut, (hipStream_t)stream);
 }

@@ -8,8 +8,9 @@ values are numbers of bf16, so reading them back rounds nothing.
 
 Slot s owns cache heads [s*n_kv, (s+1)*n_kv); a head is a row of tiles of 32 tokens, K and V of a tile in 4352 bytes next to each other (csrc/fp4.hip).
 append and attention take the batch's slot map and the slots' lengths from device memory and never return to the host, so a decode step can be captured in a
-HIP graph.  Calls on one cache must be ordered on one stream where one of them writes; attention keeps nothing between calls (its scratch is the call's own),
-so that readers may overlap."""
+HIP graph.  Calls on one cache must be ordered on one stream where one of them writes; attention may run on several streams at
+once, and in several graphs: its scratch is the call's own, and the counters by which the splits of a row find the last of them are one set for each stream and one
+for each captured call (CAPTURES of them; calls captured after these, or of more rows than the cache has slots, take a launch more instead)."""
 from __future__ import annotations
 import torch
 from . import _lib
@@ -19,11 +20,21 @@ from .kernel import GMAX
 T = 32                          # tokens per tile
 ROW_BYTES = D // 2 + D // 32    # bytes of a token and head of K or of V: codes and exponents
 TILE_BYTES = 2 * T * ROW_BYTES
+LINE = 32                       # words from one counter of attention to the next
+CAPTURES = 64                   # captured calls of attention that get counters of their own
 
 
 def choose_nsplit(B: int, n_kv: int, S: int) -> int:
-    """Splits per row of a launch, of which rows get theirs by length: S tokens in the longest."""
-    return max(1, min(-(-256 // (B * n_kv)), S // 256))
+    """Splits for each of B rows, S tokens in the longest, which the launch then shares out by length (csrc/fp4.hip).  Measured, 8 kv heads, 4 query heads each, us:
+      * up to 1500 tokens none (1000 tokens: 7.3, against 8.0 with 8 splits and 9.1 with 32; 1500: 8.4, with 16 the same);
+      * one block per CU (64K tokens: 18.3 with 32 splits, 20.7 with 16, 21.6 with 64; 8 rows of 7000..8192: 17.7 with 4, 21.6 with 2, 19.0 with 8; 16 rows of
+        4096..65536: 101 with 2, 185 with 1), of at least 128 tokens (2000: 8.6 with 16, 9.2 with 32; 16000: 10.6 with 32);
+      * heads that fill half of the chip by themselves: none, since a split's start and merge cost more than even shares save (32 rows of 300..6000: 24.4, against
+        26.8 with 2; 24 of 2000..16000: 52.6 and 52.6; 64 of 2000..16000: 107 and 114), but not where a single row may take as long as all (from 32768 tokens)."""
+    H = B * n_kv
+    if S <= 1500: return 1
+    if H <= 128: return max(1, min(256 // H, S // 128))
+    return 1 if S < 32768 else 2
 
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
@@ -51,6 +62,20 @@ class FP4KVCache:
         self.lens = torch.zeros(n_slots, dtype=torch.int32, device=device)          # tokens per slot
         # set by append instead of writing: bit 0 = a slot was full, bit 1 = a slot twice in a batch, bit 2 = no such slot
         self.overflow = torch.zeros(1, dtype=torch.int32, device=device)
+        self._tickets = {}      # stream -> counters, zero between launches
+        self._spare = torch.zeros(CAPTURES, self.H * LINE, dtype=torch.int32, device=device)      # of captured calls: one row each
+        self._captured = 0
+
+    def _counters(self, n: int) -> torch.Tensor | None:
+        """Counters of an attention launch, n of them: launches on one stream are in order and share theirs; a captured call may be replayed beside any other."""
+        if torch._C._cuda_isCurrentStreamCapturing():
+            if n > self.H or self._captured == CAPTURES: return None
+            self._captured += 1
+            return self._spare[self._captured - 1]
+        stream = _lib.stream()
+        have = self._tickets.get(stream)
+        if have is None or have.numel() < n * LINE: have = self._tickets[stream] = torch.zeros(max(n, self.H) * LINE, dtype=torch.int32, device=self.data.device)
+        return have
 
     @staticmethod
     def bytes_per_slot(n_kv: int, capacity: int) -> int:
@@ -99,9 +124,10 @@ class FP4KVCache:
         with _lib.on_device(self.data, q, slots):
             out = torch.empty(B, n_q, D, dtype=q.dtype, device=q.device)
             if B == 0: return out
-            partials = torch.empty(B * nsplit * n_q * (D + 2), dtype=torch.float32, device=q.device) if nsplit > 1 else None
+            partials, tickets = (torch.empty(B * nsplit * n_q * (D + 2), dtype=torch.float32, device=q.device), self._counters(B * self.n_kv)) if nsplit > 1 else (None, None)
             q = q if q.is_contiguous() and q.data_ptr() % 16 == 0 else q.clone(memory_format=torch.contiguous_format)
-            _lib.call("gaac_fp4_attn", self.data, self.lens, slots.contiguous(), self.n_slots, self.tiles, self.cap, q, B, n_q, self.n_kv, float(scale), nsplit, partials, out, _lib.stream)
+            _lib.call("gaac_fp4_attn", self.data, self.lens, slots.contiguous(), self.n_slots, self.tiles, self.cap, q, B, n_q, self.n_kv, float(scale), nsplit, partials,
+                      tickets, out, _lib.stream)
             return out
 
     # ------------------------------------------------------------------ housekeeping

@@ -4,7 +4,12 @@ import torch
 from . import _lib
 from .rope import TYPES
 
-MAX_VOCAB = (1 << 20) - 16
+MAX_VOCAB, MAX_ROWS = (1 << 20) - 16, 65535
+
+
+def work_bytes(B: int, V: int) -> int:
+    """Scratch of a call: per row two words for each segment of 4096 logits, 2048 bins of 12 bytes, 8192 candidates, two counters."""
+    return B * (16 * -(-(V + 7) // 4096) + 12 * 2048 + 8 * 8192 + 16)
 
 
 def _setting(name: str, x, B: int, dtype, like: torch.Tensor):
@@ -24,16 +29,18 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_
 
     A temperature that is not positive: the first maximum.  A token whose logit is -inf or NaN never comes; -1 for a row that has nothing else.  An infinite
     maximum: evenly among the tokens that have it.  u outside [0, 1) counts as the nearest number inside, NaN as 0.  Sums are exact to 2^-43 of the largest
-    weight and do not depend on their order.  One launch, no wait."""
+    weight and do not depend on their order.  At most three launches, no wait."""
     if logits.dim() != 2 or logits.dtype not in TYPES or not 1 <= logits.shape[1] <= MAX_VOCAB:
         raise RuntimeError(f"sample expects logits bf16, fp16 or fp32 [B, V], V up to {MAX_VOCAB}, got {logits.dtype} {list(logits.shape)}")
     B, V = logits.shape
+    if B > MAX_ROWS: raise RuntimeError(f"sample takes {MAX_ROWS} rows at a time, got {B}")
     if u.dtype != torch.float32 or tuple(u.shape) != (B,): raise RuntimeError(f"sample expects u fp32 [{B}], got {u.dtype} {list(u.shape)}")
     (t_rows, t), (k_rows, k), (p_rows, p), (m_rows, m) = (_setting(name, x, B, dtype, logits) for name, x, dtype in (
         ("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)))
     with _lib.on_device(logits, u, t_rows, k_rows, p_rows, m_rows):
         out = torch.empty(B, dtype=torch.int64, device=logits.device)
         if B == 0: return out
+        work = torch.empty(work_bytes(B, V), dtype=torch.uint8, device=logits.device)
         if V > 1 and logits.stride(1) != 1 or B > 1 and logits.stride(0) < 0: logits = logits.contiguous()
-        _lib.call("gaac_sample", TYPES[logits.dtype], logits, logits.stride(0) if B > 1 else 0, B, V, u.contiguous(), t_rows, float(t), k_rows, max(0, min(int(k), V)), p_rows, float(p), m_rows, float(m), out, _lib.stream)
+        _lib.call("gaac_sample", TYPES[logits.dtype], logits, logits.stride(0) if B > 1 else 0, B, V, u.contiguous(), t_rows, float(t), k_rows, max(0, min(int(k), V)), p_rows, float(p), m_rows, float(m), work, work.numel(), out, _lib.stream)
         return out

@@ -250,9 +250,10 @@ int gaac_fp4_append(const int* slots, int B, int n_slots, int n_kv, const void* 
                     long v_head_stride, int* lens, int tiles, int cap, uint8_t* cache, int* errors, void* stream);
 /* gaac_fp4_attn: decode attention, q bf16 [B, n_q, 128], row b over what slot slots[b] holds (below 0 or without tokens: 0; n_slots or above: NaN); out bf16
  * [B, n_q, 128].  The rows' tiles are shared out over B * nsplit splits a kv head by the lengths found on the device.  partials: scratch of this launch, fp32
- * [B*nsplit*n_q*130], need not be set to anything (NULL where nsplit is 1). */
+ * [B*nsplit*n_q*130], need not be set to anything (NULL where nsplit is 1).  8-byte aligned.  tickets: uint32 [B*n_kv*32], zeroed once, zero again after each launch, for launches
+ * that are ordered on one stream; or NULL: the splits are then added up by a second launch. */
 int gaac_fp4_attn(const uint8_t* cache, const int* lens, const int* slots, int n_slots, int tiles, int cap, const void* q, int B, int n_q, int n_kv, float scale,
-                  int nsplit, float* partials, void* out, void* stream);
+                  int nsplit, float* partials, unsigned* tickets, void* out, void* stream);
 
 /* Norms of queries and keys for each head and their rotation (the model's steps before /root/reference/nanovllm/layers/attention.py:43-96).  type: 0 bf16,
  * 1 fp16, 2 fp32, of q, k, the weights and the outputs.  q [N, n_q, D], k [N, n_k, D] through strides in elements (channels next to each other, rows
@@ -265,9 +266,10 @@ int gaac_qk_norm_rope(int type, const void* q, const void* k, long q_token_strid
                       void* stream);
 
 /* One token per row of logits [B, V] (type as above, rows row_stride elements apart): out int64 [B].  Each setting comes per row (device, [B]) or, where
- * that is NULL, as one number.  u in [0, 1).  The definition is stated in gaac_amd/csrc/sample.hip. */
+ * that is NULL, as one number.  u in [0, 1).  The definition is stated in gaac_amd/csrc/sample.hip.  work: scratch of this call, 8-byte aligned, need not be set to
+ * anything: B * (16 * ceil((V + 7) / 4096) + 90128) bytes. */
 int gaac_sample(int type, const void* logits, long row_stride, int B, int V, const float* u, const float* temperature_rows, float temperature, const int* top_k_rows,
-                int top_k, const float* top_p_rows, float top_p, const float* min_p_rows, float min_p, int64_t* out, void* stream);
+                int top_k, const float* top_p_rows, float top_p, const float* min_p_rows, float min_p, void* work, long work_bytes, int64_t* out, void* stream);
 
 #ifdef __cplusplus
 }

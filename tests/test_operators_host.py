@@ -11,7 +11,7 @@ BF = torch.bfloat16
 
 def test_sizes_of_the_cache():
     assert FP4KVCache.bytes_per_slot(8, 65536) == 8 * 2048 * 4352 + 4 and FP4KVCache.bytes_per_slot(1, 1) == 4352 + 4
-    assert choose_nsplit(1, 8, 65536) == 32 and choose_nsplit(1, 8, 100) == 1 and choose_nsplit(300, 8, 65536) == 1
+    assert [choose_nsplit(*x) for x in ((1, 8, 65536), (1, 8, 100), (1, 8, 2000), (16, 8, 65536), (32, 8, 6000), (300, 8, 65536), (1, 1, 10 ** 6))] == [32, 1, 15, 2, 1, 2, 256]
     for bad in ((0, 8, 64), (1, 0, 64), (1, 8, 0)):
         with pytest.raises(RuntimeError, match="at least 1"): FP4KVCache(*bad, device="cpu")
 
@@ -68,6 +68,7 @@ def test_samples_that_are_refused():
     x, u = torch.zeros(4, 100), torch.zeros(4)
     for bad in (x.double(), x[0], x[:, :0], torch.zeros(1).expand(2, 1 << 20)):
         with pytest.raises(RuntimeError, match="sample expects logits"): sample(bad, u)
+    with pytest.raises(RuntimeError, match="65535 rows at a time"): sample(torch.zeros(1, 2).expand(65536, 2), torch.zeros(65536))
     for bad in (u.double(), u[:3], u[:, None]):
         with pytest.raises(RuntimeError, match="sample expects u"): sample(x, bad)
     for name, bad in (("temperature", u.double()), ("temperature", u[:3]), ("top_k", u), ("top_k", torch.zeros(4, dtype=torch.int64)), ("top_p", u[:, None]), ("min_p", u.half())):
@@ -83,20 +84,22 @@ def test_samples_that_are_refused():
     ("gaac_fp4_load", [16, 64, 8, 2, 16, 16, 128, 1020, 128, 1024, None], "16-byte aligned"),
     ("gaac_fp4_append", [16, 4, 2, 8, 16, 16, 1024, 128, 1024, 128, 16, 2, 65, 16, 16, None], "bad sizes"),
     ("gaac_fp4_append", [16, 4, 2, 8, 16, 17, 1024, 128, 1024, 128, 16, 2, 64, 16, 16, None], "16-byte aligned"),
-    ("gaac_fp4_attn", [16, 16, 16, 2, 2, 64, 16, 1, 9, 8, 1.0, 1, None, 16, None], "GQA group"),
-    ("gaac_fp4_attn", [16, 16, 16, 2, 2, 64, 16, 1, 136, 8, 1.0, 1, None, 16, None], "GQA group"),
-    ("gaac_fp4_attn", [16, 16, 16, 2, 2, 64, 16, 1, 8, 8, 1.0, 2, None, 16, None], "needs partials"),
-    ("gaac_fp4_attn", [16, 16, 16, 2, 2, 64, 16, 1, 8, 8, 1.0, 0, None, 16, None], "bad sizes"),
-    ("gaac_fp4_attn", [16, 16, 16, 2, 2, 64, 24, 1, 8, 8, 1.0, 1, None, 16, None], "16-byte aligned"),
+    ("gaac_fp4_attn", [16, 16, 16, 2, 2, 64, 16, 1, 9, 8, 1.0, 1, None, None, 16, None], "GQA group"),
+    ("gaac_fp4_attn", [16, 16, 16, 2, 2, 64, 16, 1, 136, 8, 1.0, 1, None, None, 16, None], "GQA group"),
+    ("gaac_fp4_attn", [16, 16, 16, 2, 2, 64, 16, 1, 8, 8, 1.0, 2, None, None, 16, None], "needs partials"),
+    ("gaac_fp4_attn", [16, 16, 16, 2, 2, 64, 16, 1, 8, 8, 1.0, 0, None, None, 16, None], "bad sizes"),
+    ("gaac_fp4_attn", [16, 16, 16, 2, 2, 64, 24, 1, 8, 8, 1.0, 1, None, None, 16, None], "16-byte aligned"),
     ("gaac_qk_norm_rope", [3, 16, 16, 1, 1, 1, 1, 1, 1, 1, 128, 128, None, None, 0, 0, 1e-6, 16, 1, 16, 16, 1, 0, 16, 16, None], "type must be"),
     ("gaac_qk_norm_rope", [0, 16, 16, 8, 8, 8, 8, 1, 1, 1, 96, 96, None, None, 0, 0, 1e-6, 16, 1, 16, 16, 1, 0, 16, 16, None], "head_dim must be"),
     ("gaac_qk_norm_rope", [0, 16, 16, 8, 8, 8, 8, 1, 1, 1, 128, 136, None, None, 0, 0, 1e-6, 16, 1, 16, 16, 1, 0, 16, 16, None], "head_dim must be"),
     ("gaac_qk_norm_rope", [0, 16, 16, 8, 8, 8, 8, 0, 1, 1, 128, 128, None, None, 0, 0, 1e-6, 16, 1, 16, 16, 1, 0, 16, 16, None], "bad sizes"),
     ("gaac_qk_norm_rope", [0, 16, 16, 8, 8, 8, 8, 1, 1, 1, 128, 128, 16, None, 0, 0, 1e-6, 16, 1, 16, 16, 1, 0, 16, 16, None], "for both"),
     ("gaac_qk_norm_rope", [0, 16, 16, 8, 4, 8, 8, 1, 1, 1, 128, 128, None, None, 0, 0, 1e-6, 16, 1, 16, 16, 1, 0, 16, 16, None], "16-byte aligned"),
-    ("gaac_sample", [0, 16, 100, 0, 100, 16, None, 1.0, None, 0, None, 1.0, None, 0.0, 16, None], "bad sizes"),
-    ("gaac_sample", [0, 16, 100, 1, 1 << 20, 16, None, 1.0, None, 0, None, 1.0, None, 0.0, 16, None], "bad sizes"),
-    ("gaac_sample", [0, 17, 100, 1, 100, 16, None, 1.0, None, 0, None, 1.0, None, 0.0, 16, None], "not aligned"),
+    ("gaac_sample", [0, 16, 100, 0, 100, 16, None, 1.0, None, 0, None, 1.0, None, 0.0, 16, 1 << 30, 16, None], "bad sizes"),
+    ("gaac_sample", [0, 16, 100, 1, 1 << 20, 16, None, 1.0, None, 0, None, 1.0, None, 0.0, 16, 1 << 30, 16, None], "bad sizes"),
+    ("gaac_sample", [0, 17, 100, 1, 100, 16, None, 1.0, None, 0, None, 1.0, None, 0.0, 16, 1 << 30, 16, None], "not aligned"),
+    ("gaac_sample", [0, 16, 100, 2, 100, 16, None, 1.0, None, 0, None, 1.0, None, 0.0, 16, 2 * (16 + 90128) - 1, 16, None], "work memory"),
+    ("gaac_sample", [0, 16, 100, 1, 100, 16, None, 1.0, None, 0, None, 1.0, None, 0.0, 20, 1 << 20, 16, None], "work memory"),
 ])
 def test_the_library_refuses_before_it_launches(name, args, message):
     with pytest.raises(RuntimeError, match=f"{name} failed .*{message}"): _lib.call(name, *args)
