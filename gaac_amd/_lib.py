@@ -77,7 +77,7 @@ def load():
 class _CtypesCalls:
     """calls() through ctypes, for any torch: 14 us for an attention() where the binding takes 9.0, or 7.2 as a whole call (binding.cpp).  These are left to Python."""
     def attend(self, *args): return None
-    token_append = prompt_store = page_encode = page_decode = attend
+    token_append = prompt_store = page_encode = page_decode = fp4_prefill = fp4_append = fp4_attend = fp4_read = norm_rope = draw = attend
     def __getattr__(self, name):
         fn, n, error = getattr(load(), name), len(_SIGNATURES[name]), load().gaac_last_error
         def entry(*args):
@@ -94,7 +94,7 @@ def calls():
     """The entry points as functions, in the order of arguments of include/gaac_hip.h: tensors on the device, addresses or None for pointers,
     numbers, last the stream (its handle, or the function `stream`).  They raise RuntimeError with the library's message.  The binding reads
     tensors by the layout of the torch that it was built with, and is left alone where another one is installed.  attend, token_append, prompt_store,
-    page_encode and page_decode make a public call as a whole, or return None and leave it to Python."""
+    page_encode, page_decode, fp4_prefill, fp4_append, fp4_attend, fp4_read, norm_rope and draw make a public call as a whole, or return None and leave it to Python."""
     global _calls
     if _calls is None:
         load()

@@ -9,6 +9,7 @@
 #include <dlfcn.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/ops/empty.h>
+#include <c10/core/impl/DeviceGuardImplInterface.h>
 #include <algorithm>
 #include <exception>
 #include <tuple>
@@ -125,7 +126,8 @@ struct Refs {             // objects that are held until the call has been made 
 };
 #define GAAC_NAMES(X)                                                                                                                        \
   X(k) X(v) X(sm) X(codes) X(flags) X(tile_off) X(ovf) X(head_start) X(ovf_head_start) X(base3) X(base4) X(tail) X(ovf_used) X(ovf_cap)     \
-  X(n_kv) X(cap) X(S) X(H) X(kind) X(tail_len) X(overflow) X(n_slots) X(per_sequence_bases) X(_scan) X(pm) X(pl) X(pa) X(epoch) X(rows) X(nslot)
+  X(n_kv) X(cap) X(S) X(H) X(kind) X(tail_len) X(overflow) X(n_slots) X(per_sequence_bases) X(_scan) X(pm) X(pl) X(pa) X(epoch) X(rows) X(nslot)                            \
+  X(data) X(lens) X(tiles)
 #define X(name) PyObject* n_##name = nullptr;
 GAAC_NAMES(X)
 #undef X
@@ -363,7 +365,198 @@ PyObject* page_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return THPVariable_Wrap(out);
   });
 }
-#define GAAC_WHOLE_CALLS(X) X(attend) X(token_append) X(prompt_store) X(page_encode) X(page_decode)
+// The calls of the 4-bit cache, of qk_norm_rope and of sample, the same way.  Their tensors have to be on the current device.  Host us a call, Python / here: append
+// 7.8 / 4.6, attention 11.0 / 6.0, qk_norm_rope 15.9 / 5.4, sample 26 / 14 (three launches).
+const at::Tensor& here(PyObject* o) {
+  const at::Tensor& t = tensor(o);
+  if (t.device() != c10::impl::getDeviceGuardImpl(c10::DeviceType::CUDA)->getDevice()) throw Otherwise{};
+  return t;
+}
+// rows [n, heads, d] that a kernel reads through strides of whole 16 bytes
+void strides_of(const at::Tensor& t, long& row, long& head) {
+  const long per = 16 / t.itemsize();
+  row = t.size(0) > 1 ? t.stride(0) : 0;
+  head = t.size(1) > 1 ? t.stride(1) : 0;
+  if (t.stride(2) != 1 || row % per != 0 || head % per != 0 || reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 != 0) throw Otherwise{};
+}
+bool is_slots(const at::Tensor& t, long B) { return t.dim() == 1 && t.size(0) == B && t.scalar_type() == at::kInt && t.is_contiguous(); }
+struct Fp4Cache {
+  uint8_t* data;
+  int* lens;
+  long n_slots, n_kv, tiles;
+  Fp4Cache(Refs& get, PyObject* o) : data(static_cast<uint8_t*>(here(get(o, n_data)).data_ptr())), lens(address<int>(get(o, n_lens))), n_slots(number(get(o, n_n_slots))), n_kv(number(get(o, n_n_kv))),
+                                     tiles(number(get(o, n_tiles))) {}
+  uint8_t* slot(long i) const { return data + i * n_kv * tiles * 4352; }
+};
+
+// fp4_prefill(cache, slot, k, v, stream) -> True
+PyObject* fp4_prefill(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return whole_call(n, 5, [&]() -> PyObject* {
+    Refs get;
+    const Fp4Cache c(get, a[0]);
+    const long slot = number(a[1]);
+    const at::Tensor &k = here(a[2]), &v = here(a[3]);
+    if (!is_rows(k, 3) || !is_rows(v, 3) || k.sizes() != v.sizes() || k.size(1) != c.n_kv || k.size(0) == 0 || k.size(0) > c.tiles * 32 || slot < 0 || slot >= c.n_slots) throw Otherwise{};
+    long k_rs, k_hs, v_rs, v_hs;
+    strides_of(k, k_rs, k_hs);
+    strides_of(v, v_rs, v_hs);
+    void* stream = stream_of(a[4]);
+    must("gaac_fp4_store", without_gil([&] {
+      return p_gaac_fp4_store(k.data_ptr(), v.data_ptr(), k_hs, k_rs, v_hs, v_rs, static_cast<int>(k.size(0)), static_cast<int>(c.n_kv), static_cast<int>(c.tiles), c.slot(slot), c.lens + slot, stream);
+    }));
+    Py_RETURN_TRUE;
+  });
+}
+
+// fp4_append(cache, slots, k, v, stream) -> True
+PyObject* fp4_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return whole_call(n, 5, [&]() -> PyObject* {
+    Refs get;
+    const Fp4Cache c(get, a[0]);
+    const at::Tensor &slots = here(a[1]), &k = here(a[2]), &v = here(a[3]);
+    if (!is_rows(k, 3) || !is_rows(v, 3) || k.sizes() != v.sizes() || k.size(1) != c.n_kv || k.size(0) == 0 || !is_slots(slots, k.size(0))) throw Otherwise{};
+    long k_rs, k_hs, v_rs, v_hs;
+    strides_of(k, k_rs, k_hs);
+    strides_of(v, v_rs, v_hs);
+    int* overflow = address<int>(get(a[0], n_overflow));
+    const long cap = number(get(a[0], n_cap));
+    void* stream = stream_of(a[4]);
+    must("gaac_fp4_append", without_gil([&] {
+      return p_gaac_fp4_append(static_cast<int*>(slots.data_ptr()), static_cast<int>(k.size(0)), static_cast<int>(c.n_slots), static_cast<int>(c.n_kv), k.data_ptr(), v.data_ptr(), k_rs, k_hs, v_rs, v_hs, c.lens,
+                               static_cast<int>(c.tiles), static_cast<int>(cap), c.data, overflow, stream);
+    }));
+    Py_RETURN_TRUE;
+  });
+}
+
+// fp4_attend(cache, q, slots, scale, nsplit, tickets or None, stream) -> out like q [B, n_q, 128]
+PyObject* fp4_attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return whole_call(n, 7, [&]() -> PyObject* {
+    Refs get;
+    const Fp4Cache c(get, a[0]);
+    const at::Tensor &q = here(a[1]), &slots = here(a[2]);
+    const long nsplit = number(a[4]), cap = number(get(a[0], n_cap));
+    if (!is_rows(q, 3) || !q.is_contiguous() || reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 != 0 || q.size(0) == 0 || !is_slots(slots, q.size(0)) || nsplit < 1 || nsplit > 1 << 20) throw Otherwise{};
+    const long B = q.size(0), n_q = q.size(1);
+    if (n_q < c.n_kv || n_q % c.n_kv != 0 || n_q / c.n_kv > 16 || !PyFloat_CheckExact(a[3])) throw Otherwise{};
+    unsigned* tickets = a[5] == Py_None ? nullptr : address<unsigned>(a[5]);
+    const float scale = static_cast<float>(PyFloat_AS_DOUBLE(a[3]));
+    void* stream = stream_of(a[6]);
+    at::Tensor out = bytes(q, {B, n_q, DIM}, at::kBFloat16), partials;
+    if (nsplit > 1) partials = bytes(q, {B * nsplit * n_q * (DIM + 2)}, at::kFloat);
+    float* part = nsplit > 1 ? static_cast<float*>(partials.data_ptr()) : nullptr;
+    must("gaac_fp4_attn", without_gil([&] {
+      return p_gaac_fp4_attn(c.data, c.lens, static_cast<int*>(slots.data_ptr()), static_cast<int>(c.n_slots), static_cast<int>(c.tiles), static_cast<int>(cap), q.data_ptr(), static_cast<int>(B), static_cast<int>(n_q),
+                             static_cast<int>(c.n_kv), scale, static_cast<int>(nsplit), part, tickets, out.data_ptr(), stream);
+    }));
+    return THPVariable_Wrap(out);
+  });
+}
+
+// fp4_read(cache, slot, stream) -> (K, V) bf16 [tokens, n_kv, 128]; waits for the slot's length
+PyObject* fp4_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return whole_call(n, 3, [&]() -> PyObject* {
+    Refs get;
+    const Fp4Cache c(get, a[0]);
+    const long slot = number(a[1]);
+    if (slot < 0 || slot >= c.n_slots) throw Otherwise{};
+    void* stream = stream_of(a[2]);
+    at::Tensor word = host_words(1);
+    int* len = static_cast<int*>(word.data_ptr());
+    must("gaac_cache_check", without_gil([&] { return p_gaac_cache_check(nullptr, 0, c.lens + slot, nullptr, nullptr, 0, len, stream); }));
+    must("gaac_wait_words", without_gil([&] { return p_gaac_wait_words(len, 1, stream); }));
+    const long L = *len, row = c.n_kv * DIM;
+    const at::Tensor& like = tensor(get(a[0], n_data));
+    at::Tensor k = bytes(like, {L, c.n_kv, DIM}, at::kBFloat16), v = bytes(like, {L, c.n_kv, DIM}, at::kBFloat16);
+    if (L > 0)
+      must("gaac_fp4_load", without_gil([&] {
+        return p_gaac_fp4_load(c.slot(slot), static_cast<int>(L), static_cast<int>(c.n_kv), static_cast<int>(c.tiles), k.data_ptr(), v.data_ptr(), DIM, row, DIM, row, stream);
+      }));
+    return Py_BuildValue("(NN)", THPVariable_Wrap(k), THPVariable_Wrap(v));
+  });
+}
+
+int float_type(const at::Tensor& t) {      // the number of the type in the C interface
+  switch (t.scalar_type()) {
+    case at::kBFloat16: return 0;
+    case at::kHalf: return 1;
+    case at::kFloat: return 2;
+    default: throw Otherwise{};
+  }
+}
+
+// norm_rope(q, k, positions, cos, sin, q_weight or None, k_weight or None, eps, interleaved, stream) -> (q, k)
+PyObject* norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return whole_call(n, 10, [&]() -> PyObject* {
+    const at::Tensor &q = here(a[0]), &k = here(a[1]), &pos = here(a[2]), &cos = here(a[3]), &sin = here(a[4]);
+    const int type = float_type(q);
+    if (q.dim() != 3 || k.dim() != 3 || q.scalar_type() != k.scalar_type() || q.size(0) != k.size(0) || q.size(2) != k.size(2) || q.size(0) == 0 || q.size(1) == 0 || k.size(1) == 0) throw Otherwise{};
+    const long N = q.size(0), n_q = q.size(1), n_k = k.size(1), D = q.size(2);
+    if ((D != 64 && D != 128 && D != 256) || N >= 1l << 28 || n_q >= 1 << 20 || n_k >= 1 << 20) throw Otherwise{};
+    if (pos.dim() != 1 || pos.size(0) != N || !pos.is_contiguous() || (pos.scalar_type() != at::kLong && pos.scalar_type() != at::kInt)) throw Otherwise{};
+    if (cos.scalar_type() != at::kFloat || sin.scalar_type() != at::kFloat || cos.dim() != 2 || cos.sizes() != sin.sizes() || cos.size(0) < 1 || cos.size(0) >= 1l << 31 || !cos.is_contiguous() || !sin.is_contiguous()) throw Otherwise{};
+    const long R = 2 * cos.size(1);
+    if (R < 16 || R > D || R % 16 != 0 || !PyFloat_CheckExact(a[7])) throw Otherwise{};
+    long q_ts, q_hs, k_ts, k_hs, w_hs[2] = {0, 0};
+    strides_of(q, q_ts, q_hs);
+    strides_of(k, k_ts, k_hs);
+    void* w[2] = {nullptr, nullptr};
+    uintptr_t all = reinterpret_cast<uintptr_t>(cos.data_ptr()) | reinterpret_cast<uintptr_t>(sin.data_ptr());
+    if ((a[5] == Py_None) != (a[6] == Py_None)) throw Otherwise{};
+    for (int i = 0; i < 2 && a[5] != Py_None; ++i) {
+      const at::Tensor& t = here(a[5 + i]);
+      const long heads = i == 0 ? n_q : n_k;
+      if (t.scalar_type() != q.scalar_type() || !t.is_contiguous() || !((t.dim() == 1 && t.size(0) == D) || (t.dim() == 2 && t.size(0) == heads && t.size(1) == D))) throw Otherwise{};
+      w[i] = t.data_ptr(); w_hs[i] = t.dim() == 2 ? D : 0;
+      all |= reinterpret_cast<uintptr_t>(w[i]);
+    }
+    const int interleaved = PyObject_IsTrue(a[8]);
+    if (all % 16 != 0 || interleaved < 0) throw Otherwise{};
+    void* stream = stream_of(a[9]);
+    at::Tensor qo = bytes(q, {N, n_q, D}, q.scalar_type()), ko = bytes(k, {N, n_k, D}, q.scalar_type());
+    must("gaac_qk_norm_rope", without_gil([&] {
+      return p_gaac_qk_norm_rope(type, q.data_ptr(), k.data_ptr(), q_ts, q_hs, k_ts, k_hs, N, static_cast<int>(n_q), static_cast<int>(n_k), static_cast<int>(D), static_cast<int>(R), w[0], w[1], w_hs[0], w_hs[1],
+                                 static_cast<float>(PyFloat_AS_DOUBLE(a[7])), pos.data_ptr(), pos.scalar_type() == at::kLong, static_cast<float*>(cos.data_ptr()), static_cast<float*>(sin.data_ptr()),
+                                 static_cast<int>(cos.size(0)), interleaved, qo.data_ptr(), ko.data_ptr(), stream);
+    }));
+    return Py_BuildValue("(NN)", THPVariable_Wrap(qo), THPVariable_Wrap(ko));
+  });
+}
+
+// draw(logits, u, temperature, top_k, top_p, min_p, stream) -> tokens int64 [B]; each setting a number or a tensor [B]
+PyObject* draw(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return whole_call(n, 7, [&]() -> PyObject* {
+    const at::Tensor &x = here(a[0]), &u = here(a[1]);
+    const int type = float_type(x);
+    if (x.dim() != 2 || x.size(0) == 0 || x.size(0) > 65535 || x.size(1) == 0 || x.size(1) > (1l << 20) - 16 || (x.size(1) > 1 && x.stride(1) != 1)) throw Otherwise{};
+    const long B = x.size(0), V = x.size(1);
+    if (u.dim() != 1 || u.size(0) != B || u.scalar_type() != at::kFloat || !u.is_contiguous()) throw Otherwise{};
+    const auto rows = [&](PyObject* o, at::ScalarType t) -> void* {
+      if (!THPVariable_CheckExact(o)) return nullptr;
+      const at::Tensor& r = here(o);
+      if (r.dim() != 1 || r.size(0) != B || r.scalar_type() != t || !r.is_contiguous()) throw Otherwise{};
+      return r.data_ptr();
+    };
+    const auto real = [&](PyObject* o) -> float {
+      if (PyFloat_CheckExact(o)) return static_cast<float>(PyFloat_AS_DOUBLE(o));
+      if (THPVariable_CheckExact(o)) return 0.f;
+      return static_cast<float>(number(o));
+    };
+    float *t = static_cast<float*>(rows(a[2], at::kFloat)), *p = static_cast<float*>(rows(a[4], at::kFloat)), *m = static_cast<float*>(rows(a[5], at::kFloat));
+    int* k = static_cast<int*>(rows(a[3], at::kInt));
+    const long top_k = THPVariable_CheckExact(a[3]) ? 0 : std::max(0l, std::min(number(a[3]), V));
+    const float temperature = real(a[2]), top_p = real(a[4]), min_p = real(a[5]);
+    void* stream = stream_of(a[6]);
+    const long work_bytes = B * (16 * ((V + 7 + 4095) / 4096) + 90128);      // work_bytes in sampling.py
+    at::Tensor out = bytes(x, {B}, at::kLong), work = bytes(x, {work_bytes});
+    must("gaac_sample", without_gil([&] {
+      return p_gaac_sample(type, x.data_ptr(), B > 1 ? x.stride(0) : 0, static_cast<int>(B), static_cast<int>(V), static_cast<float*>(u.data_ptr()), t, temperature, k, static_cast<int>(top_k), p, top_p, m, min_p,
+                           work.data_ptr(), work_bytes, static_cast<int64_t*>(out.data_ptr()), stream);
+    }));
+    return THPVariable_Wrap(out);
+  });
+}
+#define GAAC_WHOLE_CALLS(X) X(attend) X(token_append) X(prompt_store) X(page_encode) X(page_decode) X(fp4_prefill) X(fp4_append) X(fp4_attend) X(fp4_read) X(norm_rope) X(draw)
 
 // bind(path): the entry points of the library at path (the product or one of its measurement builds); AttributeError names a missing one
 PyObject* bind(PyObject*, PyObject* path) {

@@ -15,6 +15,9 @@
 namespace {
 
 constexpr int NT = 512, SEG = NT * 8, BINS = 2048, MAX_V = 1 << 20, MAX_SEGS = MAX_V / SEG;      // a segment is a block's: 8 elements a thread
+#ifndef BLOCKS
+#define BLOCKS 1024
+#endif
 constexpr int ROOM = 8192;      // elements of a row that are looked at one by one, at most
 static_assert(MAX_SEGS <= NT);
 typedef unsigned long long u64;
@@ -89,13 +92,18 @@ struct Weights {      // of a row
   }
 };
 
-__device__ __forceinline__ u64 wave_scan(u64 x, int l) {      // inclusive
-  for (int o = 1; o < 64; o <<= 1) { const u64 y = __shfl_up(x, o); if (l >= o) x += y; }
+// Inclusive sums over the wave in the vector unit: shifts within rows of 16 lanes, then the last lane of a row to the next ones.
+template <int CTRL, int ROWS> __device__ __forceinline__ unsigned moved(unsigned x) { return (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false); }
+template <int CTRL, int ROWS> __device__ __forceinline__ u64 moved(u64 x) { return (u64)moved<CTRL, ROWS>((unsigned)(x >> 32)) << 32 | moved<CTRL, ROWS>((unsigned)x); }
+template <typename U> __device__ __forceinline__ U wave_scan(U x) {
+  x += moved<0x111, 0xf>(x); x += moved<0x112, 0xf>(x); x += moved<0x114, 0xf>(x); x += moved<0x118, 0xf>(x);
+  x += moved<0x142, 0xa>(x); x += moved<0x143, 0xc>(x);
   return x;
 }
-__device__ __forceinline__ unsigned wave_scan(unsigned x, int l) {
-  for (int o = 1; o < 64; o <<= 1) { const unsigned y = __shfl_up(x, o); if (l >= o) x += y; }
-  return x;
+__device__ __forceinline__ u64 larger(u64 a, u64 b) { return a > b ? a : b; }
+__device__ __forceinline__ u64 wave_max(u64 x) {      // in lane 63
+  x = larger(x, moved<0x111, 0xf>(x)); x = larger(x, moved<0x112, 0xf>(x)); x = larger(x, moved<0x114, 0xf>(x)); x = larger(x, moved<0x118, 0xf>(x));
+  x = larger(x, moved<0x142, 0xa>(x)); return larger(x, moved<0x143, 0xc>(x));
 }
 
 constexpr int WAVES = NT / 64;
@@ -107,15 +115,15 @@ struct Shared {
   u64 wave_mass[WAVES];
   unsigned wave_count[WAVES];
   u64 total, before_mass;
-  unsigned total_count, before_count, base, key, ties;
+  unsigned total_count, before_count, found_count;
   int found, last;
 };
 
 // Inclusive prefix sums over the block of each thread's (count, mass); sh.total_count and sh.total are those of all.
 __device__ __forceinline__ void block_scan(Shared& sh, unsigned& count, u64& mass) {
   const int l = threadIdx.x & 63, w = threadIdx.x >> 6;
-  mass = wave_scan(mass, l);
-  count = wave_scan(count, l);
+  mass = wave_scan(mass);
+  count = wave_scan(count);
   if (l == 63) { sh.wave_mass[w] = mass; sh.wave_count[w] = count; }
   __syncthreads();
   for (int i = 0; i < w; ++i) { mass += sh.wave_mass[i]; count += sh.wave_count[i]; }
@@ -136,21 +144,22 @@ __device__ __forceinline__ void clear_bins(Shared& sh) {
   for (int i = threadIdx.x; i < BINS; i += NT) { sh.mass[i] = 0; sh.count[i] = 0; }
   __syncthreads();
 }
-template <bool BY_MASS> __device__ void find_bin(Shared& sh, unsigned before_count, u64 before_mass, unsigned want_count, u64 want_mass) {
-  constexpr int PER = BINS / NT;
+constexpr int PER = BINS / NT;      // bins of a thread
+template <bool BY_MASS> __device__ void find_bin(Shared& sh, const unsigned (&counts)[PER], const u64 (&masses)[PER], unsigned before_count, u64 before_mass, unsigned want_count, u64 want_mass) {
   unsigned count = 0;
   u64 mass = 0;
-  const int b0 = threadIdx.x * PER;
-  for (int i = 0; i < PER; ++i) { count += sh.count[b0 + i]; mass += sh.mass[b0 + i]; }
+  for (int i = 0; i < PER; ++i) { count += counts[i]; mass += masses[i]; }
   const unsigned own_count = count;
   const u64 own_mass = mass;
   if (threadIdx.x == 0) sh.found = -1;
   block_scan(sh, count, mass);
   count += before_count - own_count; mass += before_mass - own_mass;      // before this thread's bins
   for (int i = 0; i < PER; ++i) {
-    const unsigned c = count + sh.count[b0 + i];
-    const u64 m = mass + sh.mass[b0 + i];
-    if (BY_MASS ? mass < want_mass && m >= want_mass : count < want_count && c >= want_count) { sh.found = b0 + i; sh.before_count = count; sh.before_mass = mass; }
+    const unsigned c = count + counts[i];
+    const u64 m = mass + masses[i];
+    if (BY_MASS ? mass < want_mass && m >= want_mass : count < want_count && c >= want_count) {
+      sh.found = threadIdx.x * PER + i; sh.before_count = count; sh.before_mass = mass; sh.found_count = counts[i];
+    }
     count = c; mass = m;
   }
   __syncthreads();
@@ -186,7 +195,10 @@ __device__ Limit find_limit(Shared& sh, Each each, const Weights& weight, const 
       }
       __syncthreads();
     }
-    find_bin<BY_MASS>(sh, before_count, before_mass, want_count, want_mass);
+    unsigned counts[PER];
+    u64 masses[PER];
+    for (int i = 0; i < PER; ++i) { counts[i] = sh.count[threadIdx.x * PER + i]; masses[i] = sh.mass[threadIdx.x * PER + i]; }
+    find_bin<BY_MASS>(sh, counts, masses, before_count, before_mass, want_count, want_mass);
     const int f = sh.found;
     if (f < 0) { __syncthreads(); return from; }      // not reached: all of them
     before_count = sh.before_count; before_mass = sh.before_mass;
@@ -263,13 +275,17 @@ struct Settings {
   __device__ __forceinline__ bool cut() const { return k > 0 || p < 1; }
 };
 
+// To and from other blocks of the row, past the caches.
+template <typename U> __device__ __forceinline__ void put(U* p, U v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+template <typename U> __device__ __forceinline__ U get(const U* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+
 // max of key << 32 | ~index over the block
 __device__ __forceinline__ u64 block_best(Shared& sh, u64 best) {
-  for (int o = 32; o > 0; o >>= 1) { const u64 y = __shfl_xor(best, o); best = best > y ? best : y; }
-  if ((threadIdx.x & 63) == 0) sh.wave_mass[threadIdx.x >> 6] = best;
+  best = wave_max(best);
+  if ((threadIdx.x & 63) == 63) sh.wave_mass[threadIdx.x >> 6] = best;
   __syncthreads();
   best = 0;
-  for (int i = 0; i < WAVES; ++i) best = best > sh.wave_mass[i] ? best : sh.wave_mass[i];
+  for (int i = 0; i < WAVES; ++i) best = larger(best, sh.wave_mass[i]);
   __syncthreads();
   return best;
 }
@@ -319,7 +335,7 @@ template <typename T> __device__ __forceinline__ u64 kept_mass(const float (&x)[
 // The limit among n candidates (key << 32 | index): all elements of the order up to the limit but those of `certain` weight, of which none is a candidate.
 __device__ Limit candidate_limit(Shared& sh, const u64* cand, int n, const Settings& set, const Weights& weight, const Bins& bins, u64 want) {
   if (n <= NT) {      // by rank: a thread counts what comes before its candidate, which puts it in its place in the order
-    const u64 e = threadIdx.x < n ? cand[threadIdx.x] ^ 0xffffffffu : 0;      // descends in the order
+    const u64 e = threadIdx.x < n ? get(cand + threadIdx.x) ^ 0xffffffffu : 0;      // descends in the order
     sh.mass[threadIdx.x] = e;
     __syncthreads();
     int rank = 0;
@@ -347,7 +363,7 @@ __device__ Limit candidate_limit(Shared& sh, const u64* cand, int n, const Setti
     const unsigned ties = __syncthreads_count(threadIdx.x < keep && key == last);
     return Limit{last, ties};
   }
-  const auto each = [&](auto f) { for (int i = threadIdx.x; i < n; i += NT) f(value_of((unsigned)(cand[i] >> 32))); };
+  const auto each = [&](auto f) { for (int i = threadIdx.x; i < n; i += NT) f(value_of((unsigned)(get(cand + i) >> 32))); };
   return set.k > 0 ? full_limit(sh, each, set, weight, bins) : find_limit<true>(sh, each, weight, bins, Limit{0, 0}, 0, want);
 }
 
@@ -397,51 +413,61 @@ template <typename T> __device__ void draw(Shared& sh, const Args& a, int b, con
   }
 }
 
-// Whether this block is the last of its row to come here; what the others wrote before is then to be seen.  (One thread's release and acquire stand for the
-// block's, between two barriers: each of them writes back or empties a cache.)
+// Whether this block is the last of its row to come here.  What the blocks leave for it they store past the caches (put, or an atomic), which is waited for here, and it
+// reads them past the caches (get): a release and an acquire would write back and empty a whole L2 in each block.
 __device__ __forceinline__ bool last_of_row(Shared& sh, const Work& work) {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
-  if (threadIdx.x == 0) sh.last = __hip_atomic_fetch_add(work.ticket, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
+  if (threadIdx.x == 0) sh.last = __hip_atomic_fetch_add(work.ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
   __syncthreads();
   return sh.last;
 }
 
-// First launch: the maximum of each segment; the row's bins and counters are zeroed.
+// First launch: the maximum of each segment; what the row's blocks add to later is zeroed.  A block takes every gridDim.x-th segment, in all launches.
 template <typename T> __global__ __launch_bounds__(NT) void k_sample_max(Args a) {
   __shared__ Shared sh;
-  const int seg = blockIdx.x, b = blockIdx.y;
+  const int b = blockIdx.y;
   const Row<T> row(static_cast<const T*>(a.logits) + b * a.stride, a.V);
   const Work work(a, b);
-  float x[8];
-  row.load(seg, x);
-  for (int i = seg * NT + threadIdx.x; i < BINS; i += gridDim.x * NT) { work.mass[i] = 0; work.count[i] = 0; }
-  const u64 best = block_best(sh, segment_best(row, seg, x));
-  if (threadIdx.x == 0) {
-    work.best[seg] = best;
-    if (seg == 0) *work.ticket = *work.n = 0;
+  for (int i = blockIdx.x * NT + threadIdx.x; i < BINS; i += gridDim.x * NT) { work.mass[i] = 0; work.count[i] = 0; }
+  if (blockIdx.x == 0 && threadIdx.x == 0) *work.ticket = *work.n = 0;
+  for (int seg = blockIdx.x; seg < a.segs; seg += gridDim.x) {
+    float x[8];
+    row.load(seg, x);
+    const u64 best = block_best(sh, segment_best(row, seg, x));
+    if (threadIdx.x == 0) { work.best[seg] = best; work.seg_mass[seg] = 0; }
   }
+}
+
+template <typename T> __device__ __forceinline__ void draw_kept(Shared& sh, const Args& a, int b, const Row<T>& row, const Settings& set, const Weights& weight, const Work& work) {
+  if (threadIdx.x < row.segs()) { sh.seg_mass[threadIdx.x] = get(work.seg_mass + threadIdx.x); sh.seg_ties[threadIdx.x] = 0; }
+  __syncthreads();
+  draw(sh, a, b, row, set, weight, Limit{0, 0});
 }
 
 // Second: rows that are cut get their bins (counts; sums only where there is no k, which leaves few), the others their token.
 template <typename T> __global__ __launch_bounds__(NT) void k_sample_bins(Args a) {
   __shared__ Shared sh;
-  const int seg = blockIdx.x, b = blockIdx.y;
+  const int b = blockIdx.y, l = threadIdx.x & 63;
   const Row<T> row(static_cast<const T*>(a.logits) + b * a.stride, a.V);
   const Work work(a, b);
   const Settings set(a, b);
   float x[8];
-  row.load(seg, x);
-  const u64 best = block_best(sh, threadIdx.x < gridDim.x ? work.best[threadIdx.x] : 0);
-  if (easy(a, b, row, set, best, seg == 0)) return;
+  row.load(blockIdx.x, x);
+  const u64 best = block_best(sh, threadIdx.x < a.segs ? work.best[threadIdx.x] : 0);
+  if (easy(a, b, row, set, best, blockIdx.x == 0)) return;
   const Weights weight{value_of((unsigned)(best >> 32)), 1.0 / (double)set.t};
   if (set.cut()) {
     const Bins bins(weight.top, set.t);
     clear_bins(sh);
-    for (int i = 0; i < 8; ++i) {
-      if (x[i] == -__builtin_inff()) continue;
-      const int bin = bins(x[i]);
-      atomicAdd(&sh.count[bin], 1u);
-      if (set.k == 0) { const u64 m = fixed(weight(x[i])); if (m) atomicAdd(&sh.mass[bin], m); }
+    for (int seg = blockIdx.x; seg < a.segs; seg += gridDim.x) {
+      if (seg != (int)blockIdx.x) row.load(seg, x);
+      for (int i = 0; i < 8; ++i) {
+        if (x[i] == -__builtin_inff()) continue;
+        const int bin = bins(x[i]);
+        atomicAdd(&sh.count[bin], 1u);
+        if (set.k == 0) { const u64 m = fixed(weight(x[i])); if (m) atomicAdd(&sh.mass[bin], m); }
+      }
     }
     __syncthreads();
     for (int i = threadIdx.x; i < BINS; i += NT) {
@@ -450,76 +476,82 @@ template <typename T> __global__ __launch_bounds__(NT) void k_sample_bins(Args a
     }
     return;
   }
-  unsigned ties = 0;
-  u64 mass = kept_mass<T>(x, weight, set, 0, ties);
-  block_scan(sh, ties, mass);
-  if (threadIdx.x == 0) work.seg_mass[seg] = sh.total;
-  if (!last_of_row(sh, work)) return;
-  if (threadIdx.x < row.segs()) { sh.seg_mass[threadIdx.x] = work.seg_mass[threadIdx.x]; sh.seg_ties[threadIdx.x] = 0; }
-  __syncthreads();
-  draw(sh, a, b, row, set, weight, Limit{0, 0});
+  for (int seg = blockIdx.x; seg < a.segs; seg += gridDim.x) {
+    if (seg != (int)blockIdx.x) row.load(seg, x);
+    unsigned ties = 0;
+    const u64 mass = wave_scan(kept_mass<T>(x, weight, set, 0, ties));
+    if (l == 63 && mass) atomicAdd(&work.seg_mass[seg], mass);
+  }
+  if (last_of_row(sh, work)) draw_kept(sh, a, b, row, set, weight, work);
 }
 
 // Third: the bin where the limit falls; its elements (with k: all up to it) become candidates, of what stands before it the segments' sums are taken.  The
 // row's last block finds the limit among the candidates and draws.
 template <typename T> __global__ __launch_bounds__(NT) void k_sample_draw(Args a) {
   __shared__ Shared sh;
-  const int seg = blockIdx.x, b = blockIdx.y;
+  const int b = blockIdx.y, l = threadIdx.x & 63;
   const Row<T> row(static_cast<const T*>(a.logits) + b * a.stride, a.V);
   const Settings set(a, b);
   if (!set.cut() || set.greedy()) return;
   const Work work(a, b);
   float x[8];
-  row.load(seg, x);
-  for (int i = threadIdx.x; i < BINS; i += NT) { sh.count[i] = work.count[i]; sh.mass[i] = work.mass[i]; }
-  const u64 best = block_best(sh, threadIdx.x < gridDim.x ? work.best[threadIdx.x] : 0);
+  row.load(blockIdx.x, x);
+  unsigned counts[PER];
+  u64 masses[PER];
+  for (int i = 0; i < PER; ++i) {
+    counts[i] = work.count[threadIdx.x * PER + i];
+    masses[i] = set.k > 0 ? 0 : work.mass[threadIdx.x * PER + i];
+  }
+  const u64 best = block_best(sh, threadIdx.x < a.segs ? work.best[threadIdx.x] : 0);
   if (easy(a, b, row, set, best, false)) return;
   const Weights weight{value_of((unsigned)(best >> 32)), 1.0 / (double)set.t};
   const Bins bins(weight.top, set.t);
   u64 want = 0;
   if (set.k > 0) {
-    find_bin<false>(sh, 0, 0, (unsigned)set.k, 0);
+    find_bin<false>(sh, counts, masses, 0, 0, (unsigned)set.k, 0);
   } else {
     u64 m = 0;
     unsigned c = 0;
-    for (int i = threadIdx.x; i < BINS; i += NT) m += sh.mass[i];
+    for (int i = 0; i < PER; ++i) m += masses[i];
     block_scan(sh, c, m);
     want = share_of(set.p, sh.total);
     __syncthreads();
-    find_bin<true>(sh, 0, 0, 0, want);
+    find_bin<true>(sh, counts, masses, 0, 0, 0, want);
   }
   const int f = sh.found < 0 ? BINS - 1 : sh.found;      // fewer than k: all of them
-  const unsigned n = set.k > 0 ? (sh.found < 0 ? sh.total_count : sh.before_count + sh.count[f]) : sh.count[f];
+  const unsigned n = set.k > 0 ? (sh.found < 0 ? sh.total_count : sh.before_count + sh.found_count) : sh.found_count;
   if (set.k == 0) want -= sh.before_mass;
   const bool room = n <= ROOM;
-  u64 mass = 0;
-  unsigned mine = 0, take = 0;
-  for (int i = 0; i < 8; ++i) {
-    if (x[i] == -__builtin_inff()) continue;
-    const int bin = bins(x[i]);
-    if (set.k > 0 ? bin <= f : bin == f) { take |= 1u << i; ++mine; }
-    else if (set.k == 0 && bin < f && room) { const double e = weight(x[i]); if (!(e < set.min_p)) mass += fixed(e); }
-  }
-  if (room) {
-    unsigned at = mine;
-    block_scan(sh, at, mass);
-    if (threadIdx.x == 0) {
-      work.seg_mass[seg] = sh.total;
-      sh.base = sh.total_count ? atomicAdd(work.n, sh.total_count) : 0;
+  for (int seg = blockIdx.x; seg < a.segs && room; seg += gridDim.x) {
+    if (seg != (int)blockIdx.x) row.load(seg, x);
+    u64 mass = 0;
+    unsigned mine = 0, take = 0;
+    for (int i = 0; i < 8; ++i) {
+      if (x[i] == -__builtin_inff()) continue;
+      const int bin = bins(x[i]);
+      if (set.k > 0 ? bin <= f : bin == f) { take |= 1u << i; ++mine; }
+      else if (set.k == 0 && bin < f) { const double e = weight(x[i]); if (!(e < set.min_p)) mass += fixed(e); }
     }
-    __syncthreads();
-    at += sh.base - mine;
-    for (int i = 0; i < 8; ++i) if (take >> i & 1) work.candidates[at++] = (u64)key_of(x[i]) << 32 | (unsigned)row.index(seg, i);
+    if (set.k == 0) {
+      mass = wave_scan(mass);
+      if (l == 63 && mass) atomicAdd(&work.seg_mass[seg], mass);
+    }
+    if (__ballot(mine > 0) == 0) continue;
+    const unsigned run = wave_scan(mine);
+    unsigned at = 0;
+    if (l == 63) at = atomicAdd(work.n, run);
+    at = (unsigned)__builtin_amdgcn_readlane((int)at, 63) + run - mine;
+    for (int i = 0; i < 8; ++i) if (take >> i & 1) put(work.candidates + at++, (u64)key_of(x[i]) << 32 | (unsigned)row.index(seg, i));
   }
   if (!last_of_row(sh, work)) return;
   const int segs = row.segs();
   Limit limit;
   if (room) {
+    if (threadIdx.x < segs) { sh.seg_mass[threadIdx.x] = get(work.seg_mass + threadIdx.x); sh.seg_ties[threadIdx.x] = 0; }
     limit = candidate_limit(sh, work.candidates, (int)n, set, weight, bins, want);
-    if (threadIdx.x < segs) { sh.seg_mass[threadIdx.x] = work.seg_mass[threadIdx.x]; sh.seg_ties[threadIdx.x] = 0; }
     __syncthreads();
     for (int i = threadIdx.x; i < (int)n; i += NT) {
-      const u64 c = work.candidates[i];
+      const u64 c = get(work.candidates + i);
       const unsigned key = (unsigned)(c >> 32);
       if (key < limit.key) continue;
       const int s = (unsigned)c / SEG;
@@ -569,7 +601,8 @@ template <typename T> __global__ __launch_bounds__(NT) void k_sample_short(Args 
 }
 
 template <typename T> int launch(const Args& a, int B, bool cut, hipStream_t stream) {
-  const dim3 grid(a.segs, B);
+  // about four blocks a CU: each starts with the row's maxima or bins, which costs as much as several segments
+  const dim3 grid(min(a.segs, max(BLOCKS / B, 1)), B);
   if (a.segs == 1) {
     k_sample_short<T><<<grid, NT, 0, stream>>>(a);
     return gaac::launch_status("gaac_sample");

@@ -12,6 +12,7 @@ HIP graph.  Calls on one cache must be ordered on one stream where one of them w
 once, and in several graphs: its scratch is the call's own, and the counters by which the splits of a row find the last of them are one set for each stream and one
 for each captured call (CAPTURES of them; calls captured after these, or of more rows than the cache has slots, take a launch more instead)."""
 from __future__ import annotations
+import functools
 import torch
 from . import _lib
 from .codec import D
@@ -24,6 +25,7 @@ LINE = 32                       # words from one counter of attention to the nex
 CAPTURES = 64                   # captured calls of attention that get counters of their own
 
 
+@functools.lru_cache(maxsize=1024)
 def choose_nsplit(B: int, n_kv: int, S: int) -> int:
     """Splits for each of B rows, S tokens in the longest, which the launch then shares out by length (csrc/fp4.hip).  Measured, 8 kv heads, 4 query heads each, us:
       * up to 1500 tokens none (1000 tokens: 7.3, against 8.0 with 8 splits and 9.1 with 32; 1500: 8.4, with 16 the same);
@@ -90,6 +92,7 @@ class FP4KVCache:
     def prefill(self, slot: int, k: torch.Tensor, v: torch.Tensor):
         """Put a whole prompt into `slot`, replacing what the slot held: k, v bf16 [L, n_kv, D] in the model's token-major layout, through any strides of whole
         16 bytes.  One launch, no wait."""
+        if (_lib._calls or _lib.calls()).fp4_prefill(self, slot, k, v, _lib.stream): return
         self._check("prefill", k, v)
         L = k.shape[0]
         if not 0 <= slot < self.n_slots: raise RuntimeError(f"prefill expects a slot in 0..{self.n_slots - 1}, got {slot}")
@@ -103,6 +106,7 @@ class FP4KVCache:
     def append(self, slots: torch.Tensor, k: torch.Tensor, v: torch.Tensor):
         """Decode-step write: batch row b adds the token k[b], v[b] (bf16 [B, n_kv, D], through any strides of whole 16 bytes) to slot slots[b] (int32 [B]; -1 leaves the
         row out).  One launch, no wait.  A row whose slot is full, stands earlier in the batch already or does not exist is left out, and check_capacity raises."""
+        if (_lib._calls or _lib.calls()).fp4_append(self, slots, k, v, _lib.stream): return
         self._check("append", k, v)
         if slots.dtype != torch.int32 or slots.dim() != 1 or slots.shape[0] != k.shape[0]: raise RuntimeError("append expects slots int32 [B]")
         if k.shape[0] == 0: return
@@ -115,18 +119,23 @@ class FP4KVCache:
     def attention(self, q: torch.Tensor, slots: torch.Tensor, scale: float, max_len: int | None = None, nsplit: int | None = None) -> torch.Tensor:
         """Decode-step read: bf16 [B, n_q, D] queries, row b over everything slot slots[b] holds; returns bf16 [B, n_q, D].  A row whose slot is -1 or empty is 0, one
         whose slot does not exist NaN.  max_len, the longest row if the caller knows it, only picks the split count when nsplit is not given."""
+        if nsplit is None: nsplit = choose_nsplit(max(len(q), 1), self.n_kv, min(int(max_len), self.cap) if max_len else self.cap)
+        if nsplit == 1: out = (_lib._calls or _lib.calls()).fp4_attend(self, q, slots, scale, 1, None, _lib.stream)
+        elif nsplit > 1 and q.device == self.data.device and q.device.index == torch._C._cuda_getDevice():
+            out = (_lib._calls or _lib.calls()).fp4_attend(self, q, slots, scale, nsplit, self._counters(len(q) * self.n_kv), _lib.stream)
+        else: out = None
+        if out is not None: return out
         if q.dtype != torch.bfloat16 or q.dim() != 3 or q.shape[2] != D: raise RuntimeError(f"attention expects q bf16 [B, n_q, {D}], got {q.dtype} {list(q.shape)}")
         B, n_q, _ = q.shape
         if n_q % self.n_kv or not 1 <= n_q // self.n_kv <= GMAX: raise RuntimeError(f"GQA group size must be 1..{GMAX}")
         if slots.dtype != torch.int32 or slots.dim() != 1 or slots.shape[0] != B: raise RuntimeError("attention expects slots int32 [B]")
-        if nsplit is None: nsplit = choose_nsplit(max(B, 1), self.n_kv, min(int(max_len or self.cap), self.cap))
         if nsplit < 1: raise RuntimeError(f"attention expects at least one split, got {nsplit}")
         with _lib.on_device(self.data, q, slots):
             out = torch.empty(B, n_q, D, dtype=q.dtype, device=q.device)
             if B == 0: return out
             partials, tickets = (torch.empty(B * nsplit * n_q * (D + 2), dtype=torch.float32, device=q.device), self._counters(B * self.n_kv)) if nsplit > 1 else (None, None)
             q = q if q.is_contiguous() and q.data_ptr() % 16 == 0 else q.clone(memory_format=torch.contiguous_format)
-            _lib.call("gaac_fp4_attn", self.data, self.lens, slots.contiguous(), self.n_slots, self.tiles, self.cap, q, B, n_q, self.n_kv, float(scale), nsplit, partials,
+            _lib.call("gaac_fp4_attn", self.data, self.lens, slots.contiguous(), self.n_slots, self.tiles, self.cap, q, B, n_q, self.n_kv, float(scale), int(nsplit), partials,
                       tickets, out, _lib.stream)
             return out
 
@@ -140,6 +149,8 @@ class FP4KVCache:
 
     def decompress(self, slot: int) -> tuple[torch.Tensor, torch.Tensor]:
         """The K and V that `slot` holds, bf16 [L, n_kv, D] each (waits for the stream, to read the slot's length)."""
+        both = (_lib._calls or _lib.calls()).fp4_read(self, slot, _lib.stream)
+        if both is not None: return both
         if not 0 <= slot < self.n_slots: raise RuntimeError(f"decompress expects a slot in 0..{self.n_slots - 1}, got {slot}")
         L = int(self.lens[slot])
         k = torch.empty(L, self.n_kv, D, dtype=torch.bfloat16, device=self.data.device)

@@ -27,6 +27,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, cos:
 
     with row positions[token] (int64 or int32 [N]) of cos, sin (fp32 [max_pos, R/2], R a multiple of 16).  A token whose position the tables do not have becomes NaN.
     In 32 bits, rounded once.  One launch, no wait."""
+    out = (_lib._calls or _lib.calls()).norm_rope(q, k, positions, cos, sin, q_weight, k_weight, eps, interleaved, _lib.stream)
+    if out is not None: return out
     if q.dim() != 3 or k.dim() != 3 or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2] or q.dtype != k.dtype or q.dtype not in TYPES:
         raise RuntimeError(f"qk_norm_rope expects q [N, n_q, D] and k [N, n_kv, D] of one type, bf16, fp16 or fp32, got {q.dtype} {list(q.shape)} and {k.dtype} {list(k.shape)}")
     N, n_q, D = q.shape

@@ -30,6 +30,8 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_
     A temperature that is not positive: the first maximum.  A token whose logit is -inf or NaN never comes; -1 for a row that has nothing else.  An infinite
     maximum: evenly among the tokens that have it.  u outside [0, 1) counts as the nearest number inside, NaN as 0.  Sums are exact to 2^-43 of the largest
     weight and do not depend on their order.  At most three launches, no wait."""
+    out = (_lib._calls or _lib.calls()).draw(logits, u, temperature, top_k, top_p, min_p, _lib.stream)
+    if out is not None: return out
     if logits.dim() != 2 or logits.dtype not in TYPES or not 1 <= logits.shape[1] <= MAX_VOCAB:
         raise RuntimeError(f"sample expects logits bf16, fp16 or fp32 [B, V], V up to {MAX_VOCAB}, got {logits.dtype} {list(logits.shape)}")
     B, V = logits.shape
