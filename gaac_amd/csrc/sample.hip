@@ -15,9 +15,7 @@
 namespace {
 
 constexpr int NT = 512, SEG = NT * 8, BINS = 2048, MAX_V = 1 << 20, MAX_SEGS = MAX_V / SEG;      // a segment is a block's: 8 elements a thread
-#ifndef BLOCKS
-#define BLOCKS 1024
-#endif
+constexpr int BLOCKS = 512;
 constexpr int ROOM = 8192;      // elements of a row that are looked at one by one, at most
 static_assert(MAX_SEGS <= NT);
 typedef unsigned long long u64;
@@ -339,7 +337,10 @@ __device__ Limit candidate_limit(Shared& sh, const u64* cand, int n, const Setti
     sh.mass[threadIdx.x] = e;
     __syncthreads();
     int rank = 0;
-    for (int i = 0; i < n; ++i) rank += sh.mass[i] > e;
+    if (threadIdx.x < n) {
+#pragma unroll 8
+      for (int i = 0; i < n; ++i) rank += sh.mass[i] > e;
+    }
     __syncthreads();
     if (threadIdx.x < n) sh.mass[rank] = e;
     __syncthreads();
@@ -368,7 +369,7 @@ __device__ Limit candidate_limit(Shared& sh, const u64* cand, int n, const Setti
 }
 
 // The token: sh.seg_mass and sh.seg_ties hold, by segments, the kept sums above limit.key and the number of its equals.
-template <typename T> __device__ void draw(Shared& sh, const Args& a, int b, const Row<T>& row, const Settings& set, const Weights& weight, Limit limit) {
+template <typename T> __device__ void draw(Shared& sh, const Args& a, int b, float u, const Row<T>& row, const Settings& set, const Weights& weight, Limit limit) {
   const int segs = row.segs(), s = threadIdx.x;
   const double tie_weight = limit.key ? weight(value_of(limit.key)) : 0.0;
   const u64 tie_mass = tie_weight < set.min_p ? 0 : fixed(tie_weight);
@@ -381,7 +382,7 @@ template <typename T> __device__ void draw(Shared& sh, const Args& a, int b, con
   mass = own;
   block_scan(sh, none, mass);
   const u64 total = sh.total;
-  const double want = (double)a.u[b] * (double)total;
+  const double want = (double)u * (double)total;
   const u64 target = want > 0 ? (want < (double)total ? min((u64)want, total - 1) : total - 1) : 0;      // the first running sum above it
   if (mass - own <= target && target < mass) { sh.found = s; sh.before_mass = mass - own; sh.before_count = before; }
   __syncthreads();
@@ -423,6 +424,22 @@ __device__ __forceinline__ bool last_of_row(Shared& sh, const Work& work) {
   return sh.last;
 }
 
+// The bin where the limit falls, in sh.found (-1: there are fewer than k): by count where there is a k, otherwise by sum, and then what is wanted of that bin's.
+__device__ __forceinline__ u64 find_cut(Shared& sh, const Settings& set, const unsigned (&counts)[PER], const u64 (&masses)[PER]) {
+  if (set.k > 0) {
+    find_bin<false>(sh, counts, masses, 0, 0, (unsigned)set.k, 0);
+    return 0;
+  }
+  u64 m = 0;
+  unsigned c = 0;
+  for (int i = 0; i < PER; ++i) m += masses[i];
+  block_scan(sh, c, m);
+  const u64 want = share_of(set.p, sh.total);
+  __syncthreads();
+  find_bin<true>(sh, counts, masses, 0, 0, 0, want);
+  return want - sh.before_mass;
+}
+
 // First launch: the maximum of each segment; what the row's blocks add to later is zeroed.  A block takes every gridDim.x-th segment, in all launches.
 template <typename T> __global__ __launch_bounds__(NT) void k_sample_max(Args a) {
   __shared__ Shared sh;
@@ -439,19 +456,20 @@ template <typename T> __global__ __launch_bounds__(NT) void k_sample_max(Args a)
   }
 }
 
-template <typename T> __device__ __forceinline__ void draw_kept(Shared& sh, const Args& a, int b, const Row<T>& row, const Settings& set, const Weights& weight, const Work& work) {
+template <typename T> __device__ __forceinline__ void draw_kept(Shared& sh, const Args& a, int b, float u, const Row<T>& row, const Settings& set, const Weights& weight, const Work& work) {
   if (threadIdx.x < row.segs()) { sh.seg_mass[threadIdx.x] = get(work.seg_mass + threadIdx.x); sh.seg_ties[threadIdx.x] = 0; }
   __syncthreads();
-  draw(sh, a, b, row, set, weight, Limit{0, 0});
+  draw(sh, a, b, u, row, set, weight, Limit{0, 0});
 }
 
-// Second: rows that are cut get their bins (counts; sums only where there is no k, which leaves few), the others their token.
+// Second: rows that are cut get their bins (counts where there is a k, which leaves few elements to look at, otherwise sums), the others their token.
 template <typename T> __global__ __launch_bounds__(NT) void k_sample_bins(Args a) {
   __shared__ Shared sh;
   const int b = blockIdx.y, l = threadIdx.x & 63;
   const Row<T> row(static_cast<const T*>(a.logits) + b * a.stride, a.V);
   const Work work(a, b);
   const Settings set(a, b);
+  const float u = a.u[b];      // (fetched with the first loads)
   float x[8];
   row.load(blockIdx.x, x);
   const u64 best = block_best(sh, threadIdx.x < a.segs ? work.best[threadIdx.x] : 0);
@@ -465,8 +483,9 @@ template <typename T> __global__ __launch_bounds__(NT) void k_sample_bins(Args a
       for (int i = 0; i < 8; ++i) {
         if (x[i] == -__builtin_inff()) continue;
         const int bin = bins(x[i]);
-        atomicAdd(&sh.count[bin], 1u);
-        if (set.k == 0) { const u64 m = fixed(weight(x[i])); if (m) atomicAdd(&sh.mass[bin], m); }
+        if (set.k > 0) { atomicAdd(&sh.count[bin], 1u); continue; }
+        const u64 m = fixed(weight(x[i]));
+        if (m) atomicAdd(&sh.mass[bin], m);
       }
     }
     __syncthreads();
@@ -482,7 +501,7 @@ template <typename T> __global__ __launch_bounds__(NT) void k_sample_bins(Args a
     const u64 mass = wave_scan(kept_mass<T>(x, weight, set, 0, ties));
     if (l == 63 && mass) atomicAdd(&work.seg_mass[seg], mass);
   }
-  if (last_of_row(sh, work)) draw_kept(sh, a, b, row, set, weight, work);
+  if (last_of_row(sh, work)) draw_kept(sh, a, b, u, row, set, weight, work);
 }
 
 // Third: the bin where the limit falls; its elements (with k: all up to it) become candidates, of what stands before it the segments' sums are taken.  The
@@ -494,35 +513,24 @@ template <typename T> __global__ __launch_bounds__(NT) void k_sample_draw(Args a
   const Settings set(a, b);
   if (!set.cut() || set.greedy()) return;
   const Work work(a, b);
+  const float u = a.u[b];
   float x[8];
   row.load(blockIdx.x, x);
   unsigned counts[PER];
   u64 masses[PER];
   for (int i = 0; i < PER; ++i) {
-    counts[i] = work.count[threadIdx.x * PER + i];
+    counts[i] = set.k > 0 ? work.count[threadIdx.x * PER + i] : 0;
     masses[i] = set.k > 0 ? 0 : work.mass[threadIdx.x * PER + i];
   }
   const u64 best = block_best(sh, threadIdx.x < a.segs ? work.best[threadIdx.x] : 0);
   if (easy(a, b, row, set, best, false)) return;
   const Weights weight{value_of((unsigned)(best >> 32)), 1.0 / (double)set.t};
   const Bins bins(weight.top, set.t);
-  u64 want = 0;
-  if (set.k > 0) {
-    find_bin<false>(sh, counts, masses, 0, 0, (unsigned)set.k, 0);
-  } else {
-    u64 m = 0;
-    unsigned c = 0;
-    for (int i = 0; i < PER; ++i) m += masses[i];
-    block_scan(sh, c, m);
-    want = share_of(set.p, sh.total);
-    __syncthreads();
-    find_bin<true>(sh, counts, masses, 0, 0, 0, want);
-  }
+  const u64 want = find_cut(sh, set, counts, masses);
   const int f = sh.found < 0 ? BINS - 1 : sh.found;      // fewer than k: all of them
-  const unsigned n = set.k > 0 ? (sh.found < 0 ? sh.total_count : sh.before_count + sh.found_count) : sh.found_count;
-  if (set.k == 0) want -= sh.before_mass;
-  const bool room = n <= ROOM;
-  for (int seg = blockIdx.x; seg < a.segs && room; seg += gridDim.x) {
+  const unsigned up_to_k = set.k > 0 ? (sh.found < 0 ? sh.total_count : sh.before_count + sh.found_count) : 0;
+  const bool few = up_to_k <= ROOM;
+  for (int seg = blockIdx.x; seg < a.segs && few; seg += gridDim.x) {
     if (seg != (int)blockIdx.x) row.load(seg, x);
     u64 mass = 0;
     unsigned mine = 0, take = 0;
@@ -541,12 +549,14 @@ template <typename T> __global__ __launch_bounds__(NT) void k_sample_draw(Args a
     unsigned at = 0;
     if (l == 63) at = atomicAdd(work.n, run);
     at = (unsigned)__builtin_amdgcn_readlane((int)at, 63) + run - mine;
-    for (int i = 0; i < 8; ++i) if (take >> i & 1) put(work.candidates + at++, (u64)key_of(x[i]) << 32 | (unsigned)row.index(seg, i));
+    for (int i = 0; i < 8; ++i)
+      if (take >> i & 1) { if (at < ROOM) put(work.candidates + at, (u64)key_of(x[i]) << 32 | (unsigned)row.index(seg, i)); ++at; }
   }
   if (!last_of_row(sh, work)) return;
   const int segs = row.segs();
+  const unsigned n = few ? get(work.n) : up_to_k;
   Limit limit;
-  if (room) {
+  if (n <= ROOM) {
     if (threadIdx.x < segs) { sh.seg_mass[threadIdx.x] = get(work.seg_mass + threadIdx.x); sh.seg_ties[threadIdx.x] = 0; }
     limit = candidate_limit(sh, work.candidates, (int)n, set, weight, bins, want);
     __syncthreads();
@@ -577,31 +587,59 @@ template <typename T> __global__ __launch_bounds__(NT) void k_sample_draw(Args a
     }
   }
   __syncthreads();
-  draw(sh, a, b, row, set, weight, limit);
+  draw(sh, a, b, u, row, set, weight, limit);
 }
 
-// Rows of one segment, in one launch.
+// Rows of one segment, in one launch: the same steps by one block, with the bins and candidates in LDS.
 template <typename T> __global__ __launch_bounds__(NT) void k_sample_short(Args a) {
   __shared__ Shared sh;
+  __shared__ u64 cand[SEG];
+  __shared__ int n;
   const int b = blockIdx.y;
   const Row<T> row(static_cast<const T*>(a.logits) + b * a.stride, a.V);
   const Settings set(a, b);
+  const float u = a.u[b];      // (fetched with the first loads)
   float x[8];
   row.load(0, x);
+  if (threadIdx.x == 0) n = 0;
   const u64 best = block_best(sh, segment_best(row, 0, x));
   if (easy(a, b, row, set, best, true)) return;
   const Weights weight{value_of((unsigned)(best >> 32)), 1.0 / (double)set.t};
-  const Limit limit = full_limit(sh, [&](auto f) { for (int i = 0; i < 8; ++i) f(x[i]); }, set, weight, Bins(weight.top, set.t));
+  Limit limit{0, 0};
+  if (set.cut()) {
+    const Bins bins(weight.top, set.t);
+    clear_bins(sh);
+    for (int i = 0; i < 8; ++i) {
+      if (x[i] == -__builtin_inff()) continue;
+      const int bin = bins(x[i]);
+      if (set.k > 0) { atomicAdd(&sh.count[bin], 1u); continue; }
+      const u64 m = fixed(weight(x[i]));
+      if (m) atomicAdd(&sh.mass[bin], m);
+    }
+    __syncthreads();
+    unsigned counts[PER];
+    u64 masses[PER];
+    for (int i = 0; i < PER; ++i) { counts[i] = sh.count[threadIdx.x * PER + i]; masses[i] = sh.mass[threadIdx.x * PER + i]; }
+    const u64 want = find_cut(sh, set, counts, masses);
+    const int f = sh.found < 0 ? BINS - 1 : sh.found;
+    for (int i = 0; i < 8; ++i) {
+      if (x[i] == -__builtin_inff()) continue;
+      const int bin = bins(x[i]);
+      if (set.k > 0 ? bin <= f : bin == f) cand[atomicAdd(&n, 1)] = (u64)key_of(x[i]) << 32 | (unsigned)row.index(0, i);
+    }
+    __syncthreads();
+    limit = candidate_limit(sh, cand, n, set, weight, bins, want);
+  }
   unsigned ties = 0;
   u64 mass = kept_mass<T>(x, weight, set, limit.key, ties);
   block_scan(sh, ties, mass);
   if (threadIdx.x == 0) { sh.seg_mass[0] = sh.total; sh.seg_ties[0] = sh.total_count; }
   __syncthreads();
-  draw(sh, a, b, row, set, weight, limit);
+  draw(sh, a, b, u, row, set, weight, limit);
 }
 
 template <typename T> int launch(const Args& a, int B, bool cut, hipStream_t stream) {
-  // about four blocks a CU: each starts with the row's maxima or bins, which costs as much as several segments
+  // two blocks a CU: each starts with the row's maxima or bins, which costs as much as several segments (64 rows of 128256: 49.7 us, 60.7 with 256 blocks, 56.4 with 1024)
   const dim3 grid(min(a.segs, max(BLOCKS / B, 1)), B);
   if (a.segs == 1) {
     k_sample_short<T><<<grid, NT, 0, stream>>>(a);
