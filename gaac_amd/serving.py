@@ -12,16 +12,20 @@ built on it.
                                                          captured as a graph with padded rows at slot -1, the escape-capacity check
                                                          every 16 steps
 
-The model is a Llama-architecture stack (RMSNorm, rotary embedding, GQA, SwiGLU) on plain torch ops with random weights.  Where the
-reference calls flash-attn (prefill, and the uncompressed decode path) this module uses torch's scaled_dot_product_attention and the
-library's own BF16 decode kernel; the KV backend of a layer is either CompressedKVCache (`Attention.gaac`) or an uncompressed BF16
-cache (`Attention.bf16`), the baseline."""
+The model is a Llama-architecture stack (RMSNorm, rotary embedding, GQA, SwiGLU) on plain torch ops with random weights; queries and keys
+are rotated, and with ModelConfig.qk_norm normalised for each head before, by qk_norm_rope.  Where the reference calls flash-attn (prefill, and the uncompressed decode path) this module uses torch's scaled_dot_product_attention and the
+library's own BF16 decode kernel; the KV backend of a layer is CompressedKVCache (`Attention.gaac`), FP4KVCache
+(`Attention.fp4`: 4 bits, 3.76 times smaller than BF16, not lossless) or an uncompressed BF16 cache (`Attention.bf16`), the baseline.  A step takes the likeliest
+token or, with start_decode(sampling=...), one drawn by sample() from given random numbers."""
 from __future__ import annotations
 from dataclasses import dataclass
 import torch
 import torch.nn.functional as F
 from .kv_cache import CompressedKVCache
 from .kernel import bf16_attention, choose_nsplit, AttnWorkspace
+from .fp4_cache import FP4KVCache
+from .rope import qk_norm_rope
+from .sampling import sample
 
 D = 128
 
@@ -71,8 +75,8 @@ def _causal_varlen_attention(q, k, v, spans, scale):
 
 
 class Attention(torch.nn.Module):
-    """The attention layer of the engine (attention.py:43-96).  `gaac`: the layer's CompressedKVCache; `bf16`: an uncompressed cache
-    (the baseline); `observer`: callable(k, v) on every prefill step (exponent-base calibration).  `nsplit`: split count of the decode
+    """The attention layer of the engine (attention.py:43-96).  `gaac`: the layer's CompressedKVCache; `fp4`: its FP4KVCache instead, which is called the
+    same way; `bf16`: an uncompressed cache (the baseline); `observer`: callable(k, v) on every prefill step (exponent-base calibration).  `nsplit`: split count of the decode
     launch (None: chosen per call from context.max_seqlen_k, fixed by the runner when the step is captured as a graph)."""
     def __init__(self, num_heads, head_dim, scale, num_kv_heads):
         super().__init__()
@@ -80,6 +84,7 @@ class Attention(torch.nn.Module):
         self.num_heads, self.head_dim, self.scale, self.num_kv_heads = num_heads, head_dim, scale, num_kv_heads
         self.k_cache = self.v_cache = torch.tensor([])
         self.gaac = None
+        self.fp4 = None
         self.bf16 = None
         self.observer = None
         self.nsplit = None
@@ -88,10 +93,10 @@ class Attention(torch.nn.Module):
         context = get_context()
         if self.observer is not None and context.is_prefill:
             self.observer(k, v)
-        if self.gaac is not None:
+        if self.gaac is not None or self.fp4 is not None:
             return self.forward_gaac(q, k, v, context)
         if self.bf16 is None:
-            raise RuntimeError("Attention: no KV cache attached (set .gaac to a CompressedKVCache or .bf16 to an uncompressed cache)")
+            raise RuntimeError("Attention: no KV cache attached (set .gaac to a CompressedKVCache, .fp4 to an FP4KVCache or .bf16 to an uncompressed cache)")
         if context.is_prefill:
             o = _causal_varlen_attention(q, k, v, [(s, e) for _slot, s, e in context.prefill_spans or ()], self.scale)
             for slot, start, end in context.prefill_spans or ():
@@ -101,16 +106,17 @@ class Attention(torch.nn.Module):
         return self.bf16.attention(q, context.context_lens + 1, self.scale, self.nsplit or choose_nsplit(q.shape[0], self.num_kv_heads, context.max_seqlen_k))
 
     def forward_gaac(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, context: Context):
+        cache = self.gaac if self.gaac is not None else self.fp4
         if context.is_prefill:
             # the whole prompt is in this step: attend over its own K/V, then compress it into the sequence's slot
             assert context.block_tables is None, "GAAC mode: chunked prefill / prefix caching are not supported"
             o = _causal_varlen_attention(q, k, v, [(s, e) for _slot, s, e in context.prefill_spans or ()], self.scale)
             for slot, start, end in context.prefill_spans or ():
-                self.gaac.prefill(slot, k[start:end], v[start:end])
+                cache.prefill(slot, k[start:end], v[start:end])
             return o
         # decode: append the new token (compressing a tile when the tail fills), then fused attention over the compressed cache
-        self.gaac.append(context.kv_slots, k, v)
-        return self.gaac.attention(q, context.kv_slots, self.scale, max_len=context.max_seqlen_k, nsplit=self.nsplit)
+        cache.append(context.kv_slots, k, v)
+        return cache.attention(q, context.kv_slots, self.scale, max_len=context.max_seqlen_k, nsplit=self.nsplit)
 
 
 def allocate_gaac_cache(layers, budget: int, num_kv_heads: int, max_model_len: int, max_num_seqs: int, gaac_bases=None,
@@ -130,8 +136,21 @@ def allocate_gaac_cache(layers, budget: int, num_kv_heads: int, max_model_len: i
     return num_slots, caches
 
 
+def allocate_fp4_cache(layers, budget: int, num_kv_heads: int, max_model_len: int, max_num_seqs: int, device="cuda"):
+    """allocate_gaac_cache for 4-bit caches: one FP4KVCache per attention layer, attached as `layer.fp4`.  Returns (num_slots, caches)."""
+    layers = list(layers)
+    per_slot = len(layers) * FP4KVCache.bytes_per_slot(num_kv_heads, max_model_len)
+    num_slots = min(max_num_seqs, budget // per_slot)
+    assert num_slots > 0, f"4-bit cache: {per_slot / 2**30:.2f} GiB per sequence does not fit in {budget / 2**30:.2f} GiB"
+    caches = []
+    for layer in layers:
+        layer.fp4 = FP4KVCache(num_slots, num_kv_heads, max_model_len, device=device)
+        caches.append(layer.fp4)
+    return num_slots, caches
+
+
 def gaac_stats(caches, num_kv_slots: int) -> dict:
-    """model_runner.py:150-153."""
+    """model_runner.py:150-153.  caches: of either kind."""
     s = [c.stats() for c in caches]
     used, bf16 = sum(x["bytes_used"] for x in s), sum(x["bf16_bytes"] for x in s)
     return dict(num_kv_slots=num_kv_slots, bytes_used=used, bf16_bytes=bf16, ratio=bf16 / max(1, used))
@@ -148,6 +167,7 @@ class ModelConfig:
     rope_theta: float = 500000.0
     rms_eps: float = 1e-5
     max_len: int = 32768 + 256
+    qk_norm: bool = False       # RMSNorm of every query and key head before the rotation
 
 
 class Weights:
@@ -163,6 +183,8 @@ class Weights:
         self.layers = [dict(norm1=torch.ones(cfg.hidden, dtype=torch.bfloat16, device=device), qkv=w(qkv_out, cfg.hidden),
                             o=w(cfg.hidden, cfg.n_heads * D), norm2=torch.ones(cfg.hidden, dtype=torch.bfloat16, device=device),
                             gate_up=w(2 * cfg.ffn, cfg.hidden), down=w(cfg.hidden, cfg.ffn)) for _ in range(cfg.n_layers)]
+        if cfg.qk_norm:
+            for l in self.layers: l.update(q_norm=torch.ones(D, dtype=torch.bfloat16, device=device), k_norm=torch.ones(D, dtype=torch.bfloat16, device=device))
         half = torch.arange(0, D, 2, device=device, dtype=torch.float32) / D
         ang = torch.arange(cfg.max_len, device=device, dtype=torch.float32)[:, None] * (cfg.rope_theta ** -half)[None, :]
         self.cos, self.sin = ang.cos(), ang.sin()          # [max_len, 64]
@@ -170,13 +192,6 @@ class Weights:
     def nbytes(self) -> int:
         n = self.embed.numel() + self.lm_head.numel() + self.final_norm.numel()
         return 2 * (n + sum(t.numel() for l in self.layers for t in l.values()))
-
-
-def _rope(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.Tensor:
-    """x: [N, heads, D]; cos/sin: [N, D/2] (rotate-half convention)."""
-    x1, x2 = x[..., :D // 2].float(), x[..., D // 2:].float()
-    c, s = cos[:, None, :], sin[:, None, :]
-    return torch.cat([x1 * c - x2 * s, x2 * c + x1 * s], -1).to(x.dtype)
 
 
 class _Bf16Cache:
@@ -213,8 +228,9 @@ class DecodeRunner:
     """Prefill sequences into slots, then run greedy decode steps for slots 0..B-1, optionally as one captured HIP graph."""
     def __init__(self, weights: Weights, n_slots: int, kv: str = "gaac", bases: dict | None = None, ovf_bytes_per_tile: int = 128,
                  kv_budget: int | None = None):
-        """kv_budget: bytes for the compressed caches (None: exactly n_slots slots); with a budget the slot count is what fits, at most n_slots."""
-        assert kv in ("gaac", "bf16")
+        """kv: "gaac" (lossless), "fp4" (4 bits) or "bf16" (uncompressed).  kv_budget: bytes for the compressed or 4-bit caches (None: exactly n_slots slots); with a
+        budget the slot count is what fits, at most n_slots.  bases, ovf_bytes_per_tile: of "gaac"."""
+        assert kv in ("gaac", "fp4", "bf16")
         self.w, self.cfg, self.kv = weights, weights.cfg, kv
         cfg, dev = self.cfg, weights.embed.device
         self.scale = D ** -0.5
@@ -223,6 +239,9 @@ class DecodeRunner:
             if kv_budget is None:
                 kv_budget = n_slots * cfg.n_layers * CompressedKVCache.bytes_per_slot(cfg.n_kv_heads, cfg.max_len, ovf_bytes_per_tile, per_sequence_bases=bases is None)
             n_slots, self.caches = allocate_gaac_cache(self.attn, kv_budget, cfg.n_kv_heads, cfg.max_len, n_slots, bases, ovf_bytes_per_tile, dev)
+        elif kv == "fp4":
+            if kv_budget is None: kv_budget = n_slots * cfg.n_layers * FP4KVCache.bytes_per_slot(cfg.n_kv_heads, cfg.max_len)
+            n_slots, self.caches = allocate_fp4_cache(self.attn, kv_budget, cfg.n_kv_heads, cfg.max_len, n_slots, dev)
         else:
             self.caches = [_Bf16Cache(n_slots, cfg.n_kv_heads, cfg.max_len, dev) for _ in range(cfg.n_layers)]
             for a, c in zip(self.attn, self.caches): a.bf16 = c
@@ -230,6 +249,7 @@ class DecodeRunner:
         self.lens = torch.zeros(n_slots, dtype=torch.int32, device=dev)      # tokens held per slot
         self.steps = 0
         self.graph = None
+        self.sampling = None
 
     # ---------------------------------------------------------------- layers
     def _qkv(self, layer, x, pos):
@@ -237,8 +257,8 @@ class DecodeRunner:
         h = F.rms_norm(x, (cfg.hidden,), layer["norm1"], cfg.rms_eps)
         qkv = F.linear(h, layer["qkv"]).view(x.shape[0], cfg.n_heads + 2 * cfg.n_kv_heads, D)
         q, k, v = qkv[:, :cfg.n_heads], qkv[:, cfg.n_heads:cfg.n_heads + cfg.n_kv_heads], qkv[:, cfg.n_heads + cfg.n_kv_heads:]
-        cos, sin = self.w.cos.index_select(0, pos), self.w.sin.index_select(0, pos)
-        return _rope(q, cos, sin), _rope(k, cos, sin).contiguous(), v.contiguous()
+        q, k = qk_norm_rope(q, k, pos, self.w.cos, self.w.sin, layer.get("q_norm"), layer.get("k_norm"), cfg.rms_eps)
+        return q, k, v if self.kv == "fp4" else v.contiguous()      # (the 4-bit cache reads v where the projection left it)
 
     def _mlp(self, layer, x):
         cfg = self.cfg
@@ -285,15 +305,17 @@ class DecodeRunner:
         return F.linear(x, self.w.lm_head)
 
     @torch.no_grad()
-    def start_decode(self, first_tokens: torch.Tensor, use_graph: bool = True, nsplit: int | None = None):
+    def start_decode(self, first_tokens: torch.Tensor, use_graph: bool = True, nsplit: int | None = None, sampling: dict | None = None):
         """first_tokens int64 [B]: the token each of slots 0..B-1 decodes next.  With use_graph the step (all layers, cache appends,
-        attention, greedy sampling, feeding the token back) is captured once and replayed."""
+        attention, sampling, feeding the token back) is captured once and replayed.  sampling: arguments of sample() (temperature, top_k, top_p, min_p; numbers
+        or tensors [B]), decode() then takes the random numbers; None: the likeliest token."""
         B, dev = first_tokens.shape[0], first_tokens.device
         self.B = B
         self.tok = first_tokens.clone()
         self.slots = torch.arange(B, dtype=torch.int32, device=dev)
         self.dlens = self.lens[:B].clone()
-        self.nsplit = nsplit or choose_nsplit(B, self.cfg.n_kv_heads, self.cfg.max_len)
+        self.nsplit = nsplit or (None if self.kv == "fp4" else choose_nsplit(B, self.cfg.n_kv_heads, self.cfg.max_len))      # (the 4-bit cache chooses by itself)
+        self.sampling, self.u = sampling, torch.zeros(B, dtype=torch.float32, device=dev)
         self.logits = None
         self.graph = None
         if not use_graph: return
@@ -316,15 +338,18 @@ class DecodeRunner:
 
     def _one(self):
         self.logits = self._step(self.tok, self.slots, self.dlens, self.nsplit)
-        self.tok.copy_(self.logits.argmax(-1))
+        self.tok.copy_(self.logits.argmax(-1) if self.sampling is None else sample(self.logits, self.u, **self.sampling))
 
     @torch.no_grad()
-    def decode(self, n_steps: int, forced: torch.Tensor | None = None, keep_logits: bool = False):
-        """Runs n_steps greedy steps; returns the generated tokens [n_steps, B] (device).  forced int64 [n_steps, B]: teacher forcing: the
+    def decode(self, n_steps: int, forced: torch.Tensor | None = None, keep_logits: bool = False, u: torch.Tensor | None = None):
+        """Runs n_steps steps (with sampling: u fp32 [n_steps, B] in [0, 1), a random number for every token); returns the generated tokens [n_steps, B] (device).  forced int64 [n_steps, B]: teacher forcing: the
         token every row consumes at step i+1 is forced[i] instead of the one it generated (the returned tokens are still the model's
         own choices).  keep_logits: also returns the logits of every step [n_steps, B, vocab] (fp32)."""
+        if (u is None) != (self.sampling is None) or u is not None and tuple(u.shape) != (n_steps, self.B):
+            raise RuntimeError(f"decode expects u fp32 [{n_steps}, {self.B}] where start_decode was given sampling, and nothing otherwise")
         out, logits = [], []
         for i in range(n_steps):
+            if u is not None: self.u.copy_(u[i])
             if self.graph is not None: self.graph.replay()
             else: self._one()
             out.append(self.tok.clone())
@@ -333,7 +358,9 @@ class DecodeRunner:
             self.steps += 1
             if self.kv == "gaac" and self.steps % 16 == 0:      # every 16 steps a head finalizes at most one tile (model_runner.py:268-273)
                 used = torch.stack([c.max_escape_bytes() for c in self.caches]).tolist()
-                for c, u in zip(self.caches, used): c.check_capacity(u)
+                for c, n in zip(self.caches, used): c.check_capacity(n)
+            elif self.kv == "fp4" and self.steps % 16 == 0:
+                for c, n in zip(self.caches, torch.cat([c.overflow for c in self.caches]).tolist()): c.check_capacity(n)
         self.lens[:self.B] = self.dlens
         return (torch.stack(out), torch.stack(logits)) if keep_logits else torch.stack(out)
 
@@ -347,6 +374,9 @@ class DecodeRunner:
             s = [c.stats() for c in self.caches]
             used = sum(x["bytes_used"] for x in s)
             reserved = cfg.n_layers * self.n_slots * CompressedKVCache.bytes_per_slot(cfg.n_kv_heads, cfg.max_len, per_sequence_bases=self.caches[0].per_sequence_bases)
+        elif self.kv == "fp4":
+            used = sum(c.stats()["bytes_used"] for c in self.caches)
+            reserved = cfg.n_layers * self.n_slots * FP4KVCache.bytes_per_slot(cfg.n_kv_heads, cfg.max_len)
         else:
             used = bf16
             reserved = cfg.n_layers * self.n_slots * cfg.n_kv_heads * cfg.max_len * 2 * D * 2

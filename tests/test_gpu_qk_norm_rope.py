@@ -54,13 +54,15 @@ def test_a_weight_for_each_head():
 
 
 def test_without_weights_it_is_the_rotation_in_separate_operations():
-    """Bit for bit x1 cos - x2 sin, x2 cos + x1 sin with each product rounded, as the decode loop's own function computes it."""
+    """Bit for bit x1 cos - x2 sin, x2 cos + x1 sin with each product and sum rounded: what a decode loop of torch operations computes."""
     from gaac_amd import qk_norm_rope
-    from gaac_amd.serving import _rope
     require_gpu()
+    def separate(x, c, s):
+        a, b, c, s = x[..., :64].float(), x[..., 64:].float(), c[:, None], s[:, None]
+        return torch.cat([a * c - b * s, b * c + a * s], -1).to(x.dtype)
     for dtype in TYPES:
         q, k, _, pos, cos, sin = make(300, 5, 2, 128, 128, dtype, False)
-        for x, got in zip((q, k), qk_norm_rope(q, k, pos, cos, sin)): assert torch.equal(got, _rope(x, cos[pos], sin[pos]))
+        for x, got in zip((q, k), qk_norm_rope(q, k, pos, cos, sin)): assert torch.equal(got, separate(x, cos[pos], sin[pos]))
 
 
 @pytest.mark.parametrize("layout", ["head-major", "odd offset", "every other channel", "expanded"])
