@@ -17,7 +17,8 @@ namespace {
 constexpr int NT = 512, SEG = NT * 8, BINS = 2048, MAX_V = 1 << 20, MAX_SEGS = MAX_V / SEG;      // a segment is a block's: 8 elements a thread
 constexpr int BLOCKS = 512;
 constexpr int ROOM = 8192;      // elements of a row that are looked at one by one, at most
-static_assert(MAX_SEGS <= NT);
+constexpr int SORTED = 2 * NT;      // and of these so many by sorting them
+static_assert(MAX_SEGS <= NT && SORTED <= BINS);
 typedef unsigned long long u64;
 typedef unsigned u4 __attribute__((ext_vector_type(4)));
 
@@ -40,21 +41,35 @@ template <typename T> struct Row {
   __device__ __forceinline__ Row(const T* start, int V_) : shift((int)(reinterpret_cast<uintptr_t>(start) % 16 / sizeof(T))), V(V_) { base = start - shift; }
   __device__ __forceinline__ int segs() const { return (shift + V + SEG - 1) / SEG; }
   __device__ __forceinline__ int index(int seg, int i) const { return seg * SEG + threadIdx.x * 8 + i; }      // of element i of the thread, counted from base
-  __device__ __forceinline__ void load(int seg, float (&x)[8]) const {
+  struct Raw { T v[8]; };      // as they lie in memory: what is fetched ahead is not looked at
+  __device__ __forceinline__ Raw fetch(int seg) const {
     constexpr int G = 16 / sizeof(T);      // elements of a 16-byte load
+    Raw r;
 #pragma unroll
     for (int part = 0; part < 8 / G; ++part) {
       const int at = index(seg, part * G);
       if (at >= shift && at + G <= shift + V) {
         const u4 raw = *reinterpret_cast<const u4*>(base + at);
-        T v[G];
-        __builtin_memcpy(v, &raw, 16);
-#pragma unroll
-        for (int i = 0; i < G; ++i) x[part * G + i] = number(v[i]);
+        __builtin_memcpy(r.v + part * G, &raw, 16);
       } else {
 #pragma unroll
-        for (int i = 0; i < G; ++i) x[part * G + i] = at + i >= shift && at + i < shift + V ? number(base[at + i]) : -__builtin_inff();
+        for (int i = 0; i < G; ++i) r.v[part * G + i] = at + i >= shift && at + i < shift + V ? base[at + i] : (T)-__builtin_inff();
       }
+    }
+    return r;
+  }
+  static __device__ __forceinline__ void numbers(const Raw& r, float (&x)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = number(r.v[i]);
+  }
+  __device__ __forceinline__ void load(int seg, float (&x)[8]) const { numbers(fetch(seg), x); }
+  // f(seg, x) for every step-th segment of n from `first` on, the next one in flight meanwhile; r: the first
+  template <typename F> __device__ __forceinline__ void each_segment(int n, int first, int step, Raw r, F f) const {
+    for (int seg = first; seg < n; seg += step) {
+      float x[8];
+      numbers(r, x);
+      if (seg + step < n) r = fetch(seg + step);
+      f(seg, x);
     }
   }
 };
@@ -112,21 +127,29 @@ struct Shared {
   unsigned seg_ties[MAX_SEGS];
   u64 wave_mass[WAVES];
   unsigned wave_count[WAVES];
-  u64 total, before_mass;
-  unsigned total_count, before_count, found_count;
+  u64 before_mass;
+  unsigned before_count, found_count;
   int found, last;
 };
 
-// Inclusive prefix sums over the block of each thread's (count, mass); sh.total_count and sh.total are those of all.
-__device__ __forceinline__ void block_scan(Shared& sh, unsigned& count, u64& mass) {
-  const int l = threadIdx.x & 63, w = threadIdx.x >> 6;
+// Inclusive prefix sums over the block of each thread's (count, mass); returns those of all.
+struct Sums { unsigned count; u64 mass; };
+__device__ __forceinline__ Sums block_scan(Shared& sh, unsigned& count, u64& mass) {
+  const int w = threadIdx.x >> 6;
   mass = wave_scan(mass);
   count = wave_scan(count);
-  if (l == 63) { sh.wave_mass[w] = mass; sh.wave_count[w] = count; }
+  if ((threadIdx.x & 63) == 63) { sh.wave_mass[w] = mass; sh.wave_count[w] = count; }
   __syncthreads();
-  for (int i = 0; i < w; ++i) { mass += sh.wave_mass[i]; count += sh.wave_count[i]; }
-  if (threadIdx.x == NT - 1) { sh.total = mass; sh.total_count = count; }
+  Sums all{0, 0}, x[WAVES];
+#pragma unroll
+  for (int i = 0; i < WAVES; ++i) x[i] = {sh.wave_count[i], sh.wave_mass[i]};      // (all reads in flight together)
+#pragma unroll
+  for (int i = 0; i < WAVES; ++i) {
+    if (i == w) { count += all.count; mass += all.mass; }
+    all.count += x[i].count; all.mass += x[i].mass;
+  }
   __syncthreads();
+  return all;
 }
 
 struct Limit { unsigned key, ties; };      // the key of the last element kept, and how many of its equals are kept; key 0: all
@@ -143,14 +166,14 @@ __device__ __forceinline__ void clear_bins(Shared& sh) {
   __syncthreads();
 }
 constexpr int PER = BINS / NT;      // bins of a thread
-template <bool BY_MASS> __device__ void find_bin(Shared& sh, const unsigned (&counts)[PER], const u64 (&masses)[PER], unsigned before_count, u64 before_mass, unsigned want_count, u64 want_mass) {
+template <bool BY_MASS> __device__ unsigned find_bin(Shared& sh, const unsigned (&counts)[PER], const u64 (&masses)[PER], unsigned before_count, u64 before_mass, unsigned want_count, u64 want_mass) {
   unsigned count = 0;
   u64 mass = 0;
   for (int i = 0; i < PER; ++i) { count += counts[i]; mass += masses[i]; }
   const unsigned own_count = count;
   const u64 own_mass = mass;
   if (threadIdx.x == 0) sh.found = -1;
-  block_scan(sh, count, mass);
+  const unsigned all = block_scan(sh, count, mass).count;
   count += before_count - own_count; mass += before_mass - own_mass;      // before this thread's bins
   for (int i = 0; i < PER; ++i) {
     const unsigned c = count + counts[i];
@@ -161,17 +184,29 @@ template <bool BY_MASS> __device__ void find_bin(Shared& sh, const unsigned (&co
     count = c; mass = m;
   }
   __syncthreads();
+  return all;
 }
 
 // The first element in the order at which the running count reaches want_count (BY_MASS false) or the running sum of weights reaches want_mass (true), among
 // the elements with key above `from.key` and from.ties of its equals.  each(f) calls f(x) for the thread's share of the elements.
+// bin0: the bin of max - x where it falls, if that is known.
 template <bool BY_MASS, typename Each>
-__device__ Limit find_limit(Shared& sh, Each each, const Weights& weight, const Bins& bin_of, Limit from, unsigned want_count, u64 want_mass) {
+__device__ Limit find_limit(Shared& sh, Each each, const Weights& weight, const Bins& bin_of, Limit from, unsigned want_count, u64 want_mass, int bin0 = -1) {
   unsigned lo = 0, hi = 0xffffffffu, before_count = 0;
   u64 before_mass = 0;
-  int bin0 = -1;
   const float top = weight.top;
-  for (int level = 0;; ++level) {
+  const auto bounds = [&] {      // of the bin's keys, with room for the roundings of its index
+    lo = 0; hi = key_of(top);
+    if (__builtin_isfinite(top) && bin0 < BINS - 1) {
+      const double a = (double)top - (bin0 + 1) / (double)bin_of.scale * (1 + 1e-6), b = (double)top - bin0 / (double)bin_of.scale * (1 - 1e-6);
+      if (a > -3e38) lo = key_of((float)a + 0.f) - 2;
+      if (b > -3e38) hi = min(key_of((float)b + 0.f) + 2, hi);
+    }
+    lo = max(lo, from.key); hi = max(hi, lo);
+  };
+  int level = 0;
+  if (bin0 >= 0) { bounds(); level = 1; }
+  for (;; ++level) {
     // level 0: bins of top - x; then bins of 2^s keys in [lo, hi]
     const int s = level == 0 ? 0 : max(0, 32 - __builtin_clz((hi - lo) | 1) - 11);
     clear_bins(sh);
@@ -181,8 +216,8 @@ __device__ Limit find_limit(Shared& sh, Each each, const Weights& weight, const 
       const int b0 = bin_of(x);
       if (level > 0 && b0 != bin0) return;
       const int b = level == 0 ? b0 : (int)((hi - k) >> s);
-      atomicAdd(&sh.count[b], 1u);
-      if constexpr (BY_MASS) if (k != from.key) { const u64 m = fixed(weight(x)); if (m) atomicAdd(&sh.mass[b], m); }
+      if constexpr (!BY_MASS) atomicAdd(&sh.count[b], 1u);
+      else if (k != from.key) { const u64 m = fixed(weight(x)); if (m) atomicAdd(&sh.mass[b], m); }
     });
     __syncthreads();
     if constexpr (BY_MASS) {      // the equals of the limit that is there already: only the first of them are kept
@@ -202,13 +237,7 @@ __device__ Limit find_limit(Shared& sh, Each each, const Weights& weight, const 
     before_count = sh.before_count; before_mass = sh.before_mass;
     if (level == 0) {
       bin0 = f;
-      lo = 0; hi = key_of(top);
-      if (__builtin_isfinite(top) && f < BINS - 1) {      // bounds of the bin's keys, with room for the roundings of its index
-        const double a = (double)top - (f + 1) / (double)bin_of.scale * (1 + 1e-6), b = (double)top - f / (double)bin_of.scale * (1 - 1e-6);
-        if (a > -3e38) lo = key_of((float)a + 0.f) - 2;
-        if (b > -3e38) hi = min(key_of((float)b + 0.f) + 2, hi);
-      }
-      lo = max(lo, from.key); hi = max(hi, lo);
+      bounds();
     } else {
       hi -= (unsigned)f << s;
       lo = max(lo, hi - ((1u << s) - 1));
@@ -283,6 +312,7 @@ __device__ __forceinline__ u64 block_best(Shared& sh, u64 best) {
   if ((threadIdx.x & 63) == 63) sh.wave_mass[threadIdx.x >> 6] = best;
   __syncthreads();
   best = 0;
+#pragma unroll
   for (int i = 0; i < WAVES; ++i) best = larger(best, sh.wave_mass[i]);
   __syncthreads();
   return best;
@@ -311,14 +341,12 @@ template <typename Each> __device__ Limit full_limit(Shared& sh, Each each, cons
     u64 mass = 0;
     unsigned count = 0;
     each([&](float x) { if (key_of(x) > limit.key) mass += fixed(weight(x)); });
-    block_scan(sh, count, mass);
-    const u64 total = sh.total + (limit.key ? limit.ties * fixed(weight(value_of(limit.key))) : 0);
-    __syncthreads();
+    const u64 total = block_scan(sh, count, mass).mass + (limit.key ? limit.ties * fixed(weight(value_of(limit.key))) : 0);
     limit = find_limit<true>(sh, each, weight, bins, limit, 0, share_of(set.p, total));
   }
   return limit;
 }
-template <typename T> __device__ __forceinline__ u64 kept_mass(const float (&x)[8], const Weights& weight, const Settings& set, unsigned above, unsigned& ties) {
+__device__ __forceinline__ u64 kept_mass(const float (&x)[8], const Weights& weight, const Settings& set, unsigned above, unsigned& ties) {
   u64 mass = 0;
   for (int i = 0; i < 8; ++i) {
     const unsigned key = key_of(x[i]);
@@ -330,42 +358,58 @@ template <typename T> __device__ __forceinline__ u64 kept_mass(const float (&x)[
   return mass;
 }
 
-// The limit among n candidates (key << 32 | index): all elements of the order up to the limit but those of `certain` weight, of which none is a candidate.
-__device__ Limit candidate_limit(Shared& sh, const u64* cand, int n, const Settings& set, const Weights& weight, const Bins& bins, u64 want) {
-  if (n <= NT) {      // by rank: a thread counts what comes before its candidate, which puts it in its place in the order
-    const u64 e = threadIdx.x < n ? get(cand + threadIdx.x) ^ 0xffffffffu : 0;      // descends in the order
-    sh.mass[threadIdx.x] = e;
-    __syncthreads();
-    int rank = 0;
-    if (threadIdx.x < n) {
-#pragma unroll 8
-      for (int i = 0; i < n; ++i) rank += sh.mass[i] > e;
+// The limit among n candidates (key << 32 | index): all elements of the order up to the limit but those of `certain` weight, of which none is a candidate.  mine: the thread's of the first
+// SORTED; values: room
+// for them in LDS; bin: the one that they are all in, without a k.
+__device__ Limit candidate_limit(Shared& sh, const u64 (&mine)[2], const u64* cand, int n, float* values, const Settings& set, const Weights& weight, const Bins& bins, u64 want, int bin) {
+  if (n <= SORTED) {      // put in order: a bitonic sort in LDS
+    int N = 2;
+    while (N < n) N *= 2;
+    for (int j = 0; j < 2; ++j) {
+      const int i = threadIdx.x + j * NT;
+      if (i < N) sh.mass[i] = i < n ? mine[j] ^ 0xffffffffu : 0;      // descends in the order; none: last
     }
     __syncthreads();
-    if (threadIdx.x < n) sh.mass[rank] = e;
+    for (int size = 2; size <= N; size *= 2)
+      for (int stride = size / 2; stride > 0; stride /= 2) {
+        const int i = 2 * threadIdx.x - (threadIdx.x & (stride - 1));
+        if (threadIdx.x < N / 2) {
+          const u64 x = sh.mass[i], y = sh.mass[i + stride];
+          if ((x < y) == ((i & size) == 0)) { sh.mass[i] = y; sh.mass[i + stride] = x; }
+        }
+        // up to a stride of 64 a wave stays in its 128 places
+        if (max(stride, stride > 1 ? stride / 2 : size) > 64) __syncthreads(); else asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      }
     __syncthreads();
-    const unsigned key = threadIdx.x < n ? (unsigned)(sh.mass[threadIdx.x] >> 32) : 0;
-    const int k = set.k > 0 ? min(set.k, n) : n;
-    u64 mass = 0;
+    const int i0 = 2 * threadIdx.x, k = set.k > 0 ? min(set.k, n) : n;      // a thread: places i0 and i0 + 1
+    unsigned key[2];
+    for (int i = 0; i < 2; ++i) key[i] = i0 + i < n ? (unsigned)(sh.mass[i0 + i] >> 32) : 0;
     int keep = k;
     if (set.p < 1) {
-      if (threadIdx.x < k) mass = fixed(weight(value_of(key)));
-      const u64 own = mass;
+      u64 m[2], mass;
+      for (int i = 0; i < 2; ++i) m[i] = i0 + i < k ? fixed(weight(value_of(key[i]))) : 0;
+      mass = m[0] + m[1];
       unsigned none = 0;
-      block_scan(sh, none, mass);
-      const u64 target = set.k > 0 ? share_of(set.p, sh.total) : want;
+      const u64 all = block_scan(sh, none, mass).mass, target = set.k > 0 ? share_of(set.p, all) : want;
       if (threadIdx.x == 0) sh.found = k;
       __syncthreads();
-      if (threadIdx.x < k && mass - own < target && mass >= target) sh.found = threadIdx.x + 1;
+      mass -= m[0] + m[1];
+      for (int i = 0; i < 2; ++i) {
+        if (i0 + i < k && mass < target && mass + m[i] >= target) sh.found = i0 + i + 1;
+        mass += m[i];
+      }
       __syncthreads();
       keep = sh.found;
     }
     const unsigned last = (unsigned)(sh.mass[keep - 1] >> 32);
-    const unsigned ties = __syncthreads_count(threadIdx.x < keep && key == last);
-    return Limit{last, ties};
+    unsigned ties = (i0 < keep && key[0] == last) + (i0 + 1 < keep && key[1] == last);
+    u64 none = 0;
+    return Limit{last, block_scan(sh, ties, none).count};
   }
-  const auto each = [&](auto f) { for (int i = threadIdx.x; i < n; i += NT) f(value_of((unsigned)(get(cand + i) >> 32))); };
-  return set.k > 0 ? full_limit(sh, each, set, weight, bins) : find_limit<true>(sh, each, weight, bins, Limit{0, 0}, 0, want);
+#pragma unroll 4
+  for (int i = threadIdx.x; i < n; i += NT) values[i] = value_of((unsigned)(get(cand + i) >> 32));      // (each thread reads its own)
+  const auto each = [&](auto f) { for (int i = threadIdx.x; i < n; i += NT) f(values[i]); };
+  return set.k > 0 ? full_limit(sh, each, set, weight, bins) : find_limit<true>(sh, each, weight, bins, Limit{0, 0}, 0, want, bin);
 }
 
 // The token: sh.seg_mass and sh.seg_ties hold, by segments, the kept sums above limit.key and the number of its equals.
@@ -380,8 +424,7 @@ template <typename T> __device__ void draw(Shared& sh, const Args& a, int b, flo
   const unsigned before = ties - own_ties;
   const u64 own = s < segs ? sh.seg_mass[s] + tie_mass * (before >= limit.ties ? 0u : min(own_ties, limit.ties - before)) : 0;
   mass = own;
-  block_scan(sh, none, mass);
-  const u64 total = sh.total;
+  const u64 total = block_scan(sh, none, mass).mass;
   const double want = (double)u * (double)total;
   const u64 target = want > 0 ? (want < (double)total ? min((u64)want, total - 1) : total - 1) : 0;      // the first running sum above it
   if (mass - own <= target && target < mass) { sh.found = s; sh.before_mass = mass - own; sh.before_count = before; }
@@ -425,17 +468,18 @@ __device__ __forceinline__ bool last_of_row(Shared& sh, const Work& work) {
 }
 
 // The bin where the limit falls, in sh.found (-1: there are fewer than k): by count where there is a k, otherwise by sum, and then what is wanted of that bin's.
-__device__ __forceinline__ u64 find_cut(Shared& sh, const Settings& set, const unsigned (&counts)[PER], const u64 (&masses)[PER]) {
+// up_to: with a k, the elements up to that bin.
+__device__ __forceinline__ u64 find_cut(Shared& sh, const Settings& set, const unsigned (&counts)[PER], const u64 (&masses)[PER], unsigned& up_to) {
+  up_to = 0;
   if (set.k > 0) {
-    find_bin<false>(sh, counts, masses, 0, 0, (unsigned)set.k, 0);
+    const unsigned all = find_bin<false>(sh, counts, masses, 0, 0, (unsigned)set.k, 0);
+    up_to = sh.found < 0 ? all : sh.before_count + sh.found_count;
     return 0;
   }
   u64 m = 0;
   unsigned c = 0;
   for (int i = 0; i < PER; ++i) m += masses[i];
-  block_scan(sh, c, m);
-  const u64 want = share_of(set.p, sh.total);
-  __syncthreads();
+  const u64 want = share_of(set.p, block_scan(sh, c, m).mass);
   find_bin<true>(sh, counts, masses, 0, 0, 0, want);
   return want - sh.before_mass;
 }
@@ -446,13 +490,22 @@ template <typename T> __global__ __launch_bounds__(NT) void k_sample_max(Args a)
   const int b = blockIdx.y;
   const Row<T> row(static_cast<const T*>(a.logits) + b * a.stride, a.V);
   const Work work(a, b);
+  const auto first = row.fetch(blockIdx.x);
   for (int i = blockIdx.x * NT + threadIdx.x; i < BINS; i += gridDim.x * NT) { work.mass[i] = 0; work.count[i] = 0; }
   if (blockIdx.x == 0 && threadIdx.x == 0) *work.ticket = *work.n = 0;
-  for (int seg = blockIdx.x; seg < a.segs; seg += gridDim.x) {
-    float x[8];
-    row.load(seg, x);
+  row.each_segment(a.segs, blockIdx.x, gridDim.x, first, [&](int seg, const float (&x)[8]) {
     const u64 best = block_best(sh, segment_best(row, seg, x));
     if (threadIdx.x == 0) { work.best[seg] = best; work.seg_mass[seg] = 0; }
+  });
+}
+
+__device__ __forceinline__ void add_to_bins(Shared& sh, const Settings& set, const Weights& weight, const Bins& bins, const float (&x)[8]) {
+  for (int i = 0; i < 8; ++i) {
+    if (x[i] == -__builtin_inff()) continue;
+    const int bin = bins(x[i]);
+    if (set.k > 0) { atomicAdd(&sh.count[bin], 1u); continue; }
+    const u64 m = fixed(weight(x[i]));
+    if (m) atomicAdd(&sh.mass[bin], m);
   }
 }
 
@@ -470,24 +523,14 @@ template <typename T> __global__ __launch_bounds__(NT) void k_sample_bins(Args a
   const Work work(a, b);
   const Settings set(a, b);
   const float u = a.u[b];      // (fetched with the first loads)
-  float x[8];
-  row.load(blockIdx.x, x);
+  const auto first = row.fetch(blockIdx.x);
   const u64 best = block_best(sh, threadIdx.x < a.segs ? work.best[threadIdx.x] : 0);
   if (easy(a, b, row, set, best, blockIdx.x == 0)) return;
   const Weights weight{value_of((unsigned)(best >> 32)), 1.0 / (double)set.t};
   if (set.cut()) {
     const Bins bins(weight.top, set.t);
     clear_bins(sh);
-    for (int seg = blockIdx.x; seg < a.segs; seg += gridDim.x) {
-      if (seg != (int)blockIdx.x) row.load(seg, x);
-      for (int i = 0; i < 8; ++i) {
-        if (x[i] == -__builtin_inff()) continue;
-        const int bin = bins(x[i]);
-        if (set.k > 0) { atomicAdd(&sh.count[bin], 1u); continue; }
-        const u64 m = fixed(weight(x[i]));
-        if (m) atomicAdd(&sh.mass[bin], m);
-      }
-    }
+    row.each_segment(a.segs, blockIdx.x, gridDim.x, first, [&](int, const float (&x)[8]) { add_to_bins(sh, set, weight, bins, x); });
     __syncthreads();
     for (int i = threadIdx.x; i < BINS; i += NT) {
       if (sh.count[i]) atomicAdd(&work.count[i], sh.count[i]);
@@ -495,12 +538,11 @@ template <typename T> __global__ __launch_bounds__(NT) void k_sample_bins(Args a
     }
     return;
   }
-  for (int seg = blockIdx.x; seg < a.segs; seg += gridDim.x) {
-    if (seg != (int)blockIdx.x) row.load(seg, x);
+  row.each_segment(a.segs, blockIdx.x, gridDim.x, first, [&](int seg, const float (&x)[8]) {
     unsigned ties = 0;
-    const u64 mass = wave_scan(kept_mass<T>(x, weight, set, 0, ties));
+    const u64 mass = wave_scan(kept_mass(x, weight, set, 0, ties));
     if (l == 63 && mass) atomicAdd(&work.seg_mass[seg], mass);
-  }
+  });
   if (last_of_row(sh, work)) draw_kept(sh, a, b, u, row, set, weight, work);
 }
 
@@ -508,14 +550,14 @@ template <typename T> __global__ __launch_bounds__(NT) void k_sample_bins(Args a
 // row's last block finds the limit among the candidates and draws.
 template <typename T> __global__ __launch_bounds__(NT) void k_sample_draw(Args a) {
   __shared__ Shared sh;
+  __shared__ float values[ROOM];
   const int b = blockIdx.y, l = threadIdx.x & 63;
   const Row<T> row(static_cast<const T*>(a.logits) + b * a.stride, a.V);
   const Settings set(a, b);
   if (!set.cut() || set.greedy()) return;
   const Work work(a, b);
   const float u = a.u[b];
-  float x[8];
-  row.load(blockIdx.x, x);
+  const auto first = row.fetch(blockIdx.x);
   unsigned counts[PER];
   u64 masses[PER];
   for (int i = 0; i < PER; ++i) {
@@ -526,12 +568,11 @@ template <typename T> __global__ __launch_bounds__(NT) void k_sample_draw(Args a
   if (easy(a, b, row, set, best, false)) return;
   const Weights weight{value_of((unsigned)(best >> 32)), 1.0 / (double)set.t};
   const Bins bins(weight.top, set.t);
-  const u64 want = find_cut(sh, set, counts, masses);
+  unsigned up_to_k;
+  const u64 want = find_cut(sh, set, counts, masses, up_to_k);
   const int f = sh.found < 0 ? BINS - 1 : sh.found;      // fewer than k: all of them
-  const unsigned up_to_k = set.k > 0 ? (sh.found < 0 ? sh.total_count : sh.before_count + sh.found_count) : 0;
   const bool few = up_to_k <= ROOM;
-  for (int seg = blockIdx.x; seg < a.segs && few; seg += gridDim.x) {
-    if (seg != (int)blockIdx.x) row.load(seg, x);
+  row.each_segment(few ? a.segs : 0, blockIdx.x, gridDim.x, first, [&](int seg, const float (&x)[8]) {
     u64 mass = 0;
     unsigned mine = 0, take = 0;
     for (int i = 0; i < 8; ++i) {
@@ -544,31 +585,34 @@ template <typename T> __global__ __launch_bounds__(NT) void k_sample_draw(Args a
       mass = wave_scan(mass);
       if (l == 63 && mass) atomicAdd(&work.seg_mass[seg], mass);
     }
-    if (__ballot(mine > 0) == 0) continue;
+    if (__ballot(mine > 0) == 0) return;
     const unsigned run = wave_scan(mine);
     unsigned at = 0;
     if (l == 63) at = atomicAdd(work.n, run);
     at = (unsigned)__builtin_amdgcn_readlane((int)at, 63) + run - mine;
     for (int i = 0; i < 8; ++i)
       if (take >> i & 1) { if (at < ROOM) put(work.candidates + at, (u64)key_of(x[i]) << 32 | (unsigned)row.index(seg, i)); ++at; }
-  }
+  });
   if (!last_of_row(sh, work)) return;
   const int segs = row.segs();
+  const u64 seg_mass = threadIdx.x < segs ? get(work.seg_mass + threadIdx.x) : 0, mine[2] = {get(work.candidates + threadIdx.x), get(work.candidates + NT + threadIdx.x)};      // (some of it unset: how many there are comes with it)
   const unsigned n = few ? get(work.n) : up_to_k;
   Limit limit;
   if (n <= ROOM) {
-    if (threadIdx.x < segs) { sh.seg_mass[threadIdx.x] = get(work.seg_mass + threadIdx.x); sh.seg_ties[threadIdx.x] = 0; }
-    limit = candidate_limit(sh, work.candidates, (int)n, set, weight, bins, want);
+    if (threadIdx.x < segs) { sh.seg_mass[threadIdx.x] = seg_mass; sh.seg_ties[threadIdx.x] = 0; }
+    limit = candidate_limit(sh, mine, work.candidates, (int)n, values, set, weight, bins, want, f);
     __syncthreads();
-    for (int i = threadIdx.x; i < (int)n; i += NT) {
-      const u64 c = get(work.candidates + i);
+    const auto keep = [&](u64 c) {
       const unsigned key = (unsigned)(c >> 32);
-      if (key < limit.key) continue;
+      if (key < limit.key) return;
       const int s = (unsigned)c / SEG;
-      if (key == limit.key) { atomicAdd(&sh.seg_ties[s], 1u); continue; }
+      if (key == limit.key) { atomicAdd(&sh.seg_ties[s], 1u); return; }
       const double e = weight(value_of(key));
       if (!(e < set.min_p)) atomicAdd(&sh.seg_mass[s], fixed(e));
-    }
+    };
+    for (int j = 0; j < 2; ++j) if (threadIdx.x + j * NT < n) keep(mine[j]);
+#pragma unroll 4
+    for (int i = threadIdx.x + SORTED; i < (int)n; i += NT) keep(get(work.candidates + i));
   } else {
     limit = full_limit(sh, [&](auto f) {
       for (int s = 0; s < segs; ++s) {
@@ -578,12 +622,12 @@ template <typename T> __global__ __launch_bounds__(NT) void k_sample_draw(Args a
       }
     }, set, weight, bins);
     for (int s = 0; s < segs; ++s) {
+      float x[8];
       row.load(s, x);
       unsigned ties = 0;
-      u64 sum = kept_mass<T>(x, weight, set, limit.key, ties);
-      block_scan(sh, ties, sum);
-      if (threadIdx.x == 0) { sh.seg_mass[s] = sh.total; sh.seg_ties[s] = sh.total_count; }
-      __syncthreads();
+      u64 sum = kept_mass(x, weight, set, limit.key, ties);
+      const Sums all = block_scan(sh, ties, sum);
+      if (threadIdx.x == 0) { sh.seg_mass[s] = all.mass; sh.seg_ties[s] = all.count; }
     }
   }
   __syncthreads();
@@ -594,6 +638,7 @@ template <typename T> __global__ __launch_bounds__(NT) void k_sample_draw(Args a
 template <typename T> __global__ __launch_bounds__(NT) void k_sample_short(Args a) {
   __shared__ Shared sh;
   __shared__ u64 cand[SEG];
+  __shared__ float values[SEG];
   __shared__ int n;
   const int b = blockIdx.y;
   const Row<T> row(static_cast<const T*>(a.logits) + b * a.stride, a.V);
@@ -609,18 +654,13 @@ template <typename T> __global__ __launch_bounds__(NT) void k_sample_short(Args 
   if (set.cut()) {
     const Bins bins(weight.top, set.t);
     clear_bins(sh);
-    for (int i = 0; i < 8; ++i) {
-      if (x[i] == -__builtin_inff()) continue;
-      const int bin = bins(x[i]);
-      if (set.k > 0) { atomicAdd(&sh.count[bin], 1u); continue; }
-      const u64 m = fixed(weight(x[i]));
-      if (m) atomicAdd(&sh.mass[bin], m);
-    }
+    add_to_bins(sh, set, weight, bins, x);
     __syncthreads();
     unsigned counts[PER];
     u64 masses[PER];
     for (int i = 0; i < PER; ++i) { counts[i] = sh.count[threadIdx.x * PER + i]; masses[i] = sh.mass[threadIdx.x * PER + i]; }
-    const u64 want = find_cut(sh, set, counts, masses);
+    unsigned up_to_k;
+    const u64 want = find_cut(sh, set, counts, masses, up_to_k);
     const int f = sh.found < 0 ? BINS - 1 : sh.found;
     for (int i = 0; i < 8; ++i) {
       if (x[i] == -__builtin_inff()) continue;
@@ -628,12 +668,13 @@ template <typename T> __global__ __launch_bounds__(NT) void k_sample_short(Args 
       if (set.k > 0 ? bin <= f : bin == f) cand[atomicAdd(&n, 1)] = (u64)key_of(x[i]) << 32 | (unsigned)row.index(0, i);
     }
     __syncthreads();
-    limit = candidate_limit(sh, cand, n, set, weight, bins, want);
+    const u64 mine[2] = {cand[threadIdx.x], cand[NT + threadIdx.x]};
+    limit = candidate_limit(sh, mine, cand, n, values, set, weight, bins, want, f);
   }
   unsigned ties = 0;
-  u64 mass = kept_mass<T>(x, weight, set, limit.key, ties);
-  block_scan(sh, ties, mass);
-  if (threadIdx.x == 0) { sh.seg_mass[0] = sh.total; sh.seg_ties[0] = sh.total_count; }
+  u64 mass = kept_mass(x, weight, set, limit.key, ties);
+  const Sums all = block_scan(sh, ties, mass);
+  if (threadIdx.x == 0) { sh.seg_mass[0] = all.mass; sh.seg_ties[0] = all.count; }
   __syncthreads();
   draw(sh, a, b, u, row, set, weight, limit);
 }
