@@ -74,34 +74,40 @@ template <typename T> struct Row {
   }
 };
 
-// exp(y), y <= 0, as a multiple of 2^-43: y = n ln 2 + r, the series of exp to r^11 (|r| <= 0.35: what is left is below 1e-14), and the sum with 2^9, whose
-// last bit is 2^-43, rounds to it.
-__device__ __forceinline__ double exp64(double y) {
-  if (!(y > -31.0)) return 0.0;
-  const double n = __builtin_rint(y * 1.4426950408889634);
-  const double r = __builtin_fma(n, -5.5459262969660605e-09, __builtin_fma(n, -0.693147175014019, y));      // ln 2 = 27 bits of it and the rest
-  double e = 1.0 / 39916800;
-  e = __builtin_fma(e, r, 1.0 / 3628800);
-  e = __builtin_fma(e, r, 1.0 / 362880);
-  e = __builtin_fma(e, r, 1.0 / 40320);
-  e = __builtin_fma(e, r, 1.0 / 5040);
-  e = __builtin_fma(e, r, 1.0 / 720);
-  e = __builtin_fma(e, r, 1.0 / 120);
-  e = __builtin_fma(e, r, 1.0 / 24);
-  e = __builtin_fma(e, r, 1.0 / 6);
-  e = __builtin_fma(e, r, 0.5);
-  e = __builtin_fma(e, r, 1.0);
-  e = __builtin_fma(e, r, 1.0);
-  return __builtin_bit_cast(double, __builtin_bit_cast(u64, e) + ((u64)(long long)n << 52));
+// exp(y), y <= 0: y = n ln 2 / 64 + r, 2^(n / 64) from a table of the 64 roots in LDS and the exponent, times the series of exp to r^5 (|r| <= 0.0055: what is left
+// is below 1e-16).  15 operations in 64 bits; the series to r^11 without a table took 24 (64 mixed rows of 128256: 68 us, with the table 60).
+constexpr int ROOTS = 64;
+__device__ __forceinline__ void fill_roots(double* table) {      // by the first wave; 2^(j / 64) = exp(j ln 2 / 64) by its series
+  if (threadIdx.x < ROOTS) {
+    const double x = threadIdx.x * (0.6931471805599453 / ROOTS);
+    double e = 1;
+#pragma unroll
+    for (int k = 17; k > 0; --k) e = __builtin_fma(e, x * (1.0 / k), 1.0);
+    table[threadIdx.x] = e;
+  }
 }
+__device__ __forceinline__ double exp64(double y, const double* table) {
+  if (!(y > -31.0)) return 0.0;
+  const double n = __builtin_rint(y * 92.33248261689366);
+  const double r = __builtin_fma(n, -2.8447437476627285e-11, __builtin_fma(n, -0.010830424667801708, y));
+  const int i = (int)n;
+  double q = __builtin_fma(r, 1.0 / 120, 1.0 / 24);
+  q = __builtin_fma(q, r, 1.0 / 6);
+  q = __builtin_fma(q, r, 0.5);
+  q = __builtin_fma(q, r, 1.0);
+  const double t = table[i & (ROOTS - 1)];
+  return __builtin_bit_cast(double, __builtin_bit_cast(u64, __builtin_fma(t * q, r, t)) + ((u64)(long long)(i >> 6) << 52));
+}
+// As a multiple of 2^-43: the sum with 2^9, whose last bit that is, rounds to it.
 __device__ __forceinline__ u64 fixed(double w) { return __builtin_bit_cast(u64, w + 512.0) - __builtin_bit_cast(u64, 512.0); }
 
 struct Weights {      // of a row
   float top;
   double inv_t;
+  const double* roots;
   __device__ __forceinline__ double operator()(float x) const {
     if (x == top) return 1.0;
-    return x == -__builtin_inff() ? 0.0 : exp64(((double)x - (double)top) * inv_t);
+    return x == -__builtin_inff() ? 0.0 : exp64(((double)x - (double)top) * inv_t, roots);
   }
 };
 
@@ -123,6 +129,7 @@ constexpr int WAVES = NT / 64;
 struct Shared {
   u64 mass[BINS];           // of bins; candidates in order
   unsigned count[BINS];
+  double roots[ROOTS];
   u64 seg_mass[MAX_SEGS];
   unsigned seg_ties[MAX_SEGS];
   u64 wave_mass[WAVES];
@@ -524,9 +531,10 @@ template <typename T> __global__ __launch_bounds__(NT) void k_sample_bins(Args a
   const Settings set(a, b);
   const float u = a.u[b];      // (fetched with the first loads)
   const auto first = row.fetch(blockIdx.x);
+  fill_roots(sh.roots);
   const u64 best = block_best(sh, threadIdx.x < a.segs ? work.best[threadIdx.x] : 0);
   if (easy(a, b, row, set, best, blockIdx.x == 0)) return;
-  const Weights weight{value_of((unsigned)(best >> 32)), 1.0 / (double)set.t};
+  const Weights weight{value_of((unsigned)(best >> 32)), 1.0 / (double)set.t, sh.roots};
   if (set.cut()) {
     const Bins bins(weight.top, set.t);
     clear_bins(sh);
@@ -558,6 +566,7 @@ template <typename T> __global__ __launch_bounds__(NT) void k_sample_draw(Args a
   const Work work(a, b);
   const float u = a.u[b];
   const auto first = row.fetch(blockIdx.x);
+  fill_roots(sh.roots);
   unsigned counts[PER];
   u64 masses[PER];
   for (int i = 0; i < PER; ++i) {
@@ -566,7 +575,7 @@ template <typename T> __global__ __launch_bounds__(NT) void k_sample_draw(Args a
   }
   const u64 best = block_best(sh, threadIdx.x < a.segs ? work.best[threadIdx.x] : 0);
   if (easy(a, b, row, set, best, false)) return;
-  const Weights weight{value_of((unsigned)(best >> 32)), 1.0 / (double)set.t};
+  const Weights weight{value_of((unsigned)(best >> 32)), 1.0 / (double)set.t, sh.roots};
   const Bins bins(weight.top, set.t);
   unsigned up_to_k;
   const u64 want = find_cut(sh, set, counts, masses, up_to_k);
@@ -646,10 +655,11 @@ template <typename T> __global__ __launch_bounds__(NT) void k_sample_short(Args 
   const float u = a.u[b];      // (fetched with the first loads)
   float x[8];
   row.load(0, x);
+  fill_roots(sh.roots);
   if (threadIdx.x == 0) n = 0;
   const u64 best = block_best(sh, segment_best(row, 0, x));
   if (easy(a, b, row, set, best, true)) return;
-  const Weights weight{value_of((unsigned)(best >> 32)), 1.0 / (double)set.t};
+  const Weights weight{value_of((unsigned)(best >> 32)), 1.0 / (double)set.t, sh.roots};
   Limit limit{0, 0};
   if (set.cut()) {
     const Bins bins(weight.top, set.t);
