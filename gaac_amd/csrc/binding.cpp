@@ -528,7 +528,7 @@ PyObject* draw(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return whole_call(n, 7, [&]() -> PyObject* {
     const at::Tensor &x = here(a[0]), &u = here(a[1]);
     const int type = float_type(x);
-    if (x.dim() != 2 || x.size(0) == 0 || x.size(0) > 65535 || x.size(1) == 0 || x.size(1) > (1l << 20) - 16 || (x.size(1) > 1 && x.stride(1) != 1)) throw Otherwise{};
+    if (x.dim() != 2 || x.size(0) == 0 || x.size(0) >= 1l << 31 || x.size(1) == 0 || x.size(1) > (1l << 20) - 16 || (x.size(1) > 1 && x.stride(1) != 1)) throw Otherwise{};
     const long B = x.size(0), V = x.size(1);
     if (u.dim() != 1 || u.size(0) != B || u.scalar_type() != at::kFloat || !u.is_contiguous()) throw Otherwise{};
     const auto rows = [&](PyObject* o, at::ScalarType t) -> void* {
@@ -547,7 +547,7 @@ PyObject* draw(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const long top_k = THPVariable_CheckExact(a[3]) ? 0 : std::max(0l, std::min(number(a[3]), V));
     const float temperature = real(a[2]), top_p = real(a[4]), min_p = real(a[5]);
     void* stream = stream_of(a[6]);
-    const long work_bytes = B * (16 * ((V + 7 + 4095) / 4096) + 90128);      // work_bytes in sampling.py
+    const long segments = (V + 7 + 4095) / 4096, work_bytes = segments == 1 ? 0 : std::min(B, 1024l) * (16 * segments + 90128);      // work_bytes in sampling.py
     at::Tensor out = bytes(x, {B}, at::kLong), work = bytes(x, {work_bytes});
     must("gaac_sample", without_gil([&] {
       return p_gaac_sample(type, x.data_ptr(), B > 1 ? x.stride(0) : 0, static_cast<int>(B), static_cast<int>(V), static_cast<float*>(u.data_ptr()), t, temperature, k, static_cast<int>(top_k), p, top_p, m, min_p,

@@ -365,9 +365,8 @@ __device__ __forceinline__ u64 kept_mass(const float (&x)[8], const Weights& wei
   return mass;
 }
 
-// The limit among n candidates (key << 32 | index): all elements of the order up to the limit but those of `certain` weight, of which none is a candidate.  mine: the thread's of the first
-// SORTED; values: room
-// for them in LDS; bin: the one that they are all in, without a k.
+// The limit among n candidates (key << 32 | index): all elements of the order up to the limit, with a k, or all of the bin that it falls in, without; `want` is then
+// what is wanted of their sum.  mine: the thread's of the first SORTED; values: room for all of them in LDS.
 __device__ Limit candidate_limit(Shared& sh, const u64 (&mine)[2], const u64* cand, int n, float* values, const Settings& set, const Weights& weight, const Bins& bins, u64 want, int bin) {
   if (n <= SORTED) {      // put in order: a bitonic sort in LDS
     int N = 2;
@@ -689,31 +688,41 @@ template <typename T> __global__ __launch_bounds__(NT) void k_sample_short(Args 
   draw(sh, a, b, u, row, set, weight, limit);
 }
 
-template <typename T> int launch(const Args& a, int B, bool cut, hipStream_t stream) {
-  // two blocks a CU: each starts with the row's maxima or bins, which costs as much as several segments (64 rows of 128256: 49.7 us, 60.7 with 256 blocks, 56.4 with 1024)
-  const dim3 grid(min(a.segs, max(BLOCKS / B, 1)), B);
-  if (a.segs == 1) {
-    k_sample_short<T><<<grid, NT, 0, stream>>>(a);
-    return gaac::launch_status("gaac_sample");
+constexpr int ROWS = 1024, SHORT_ROWS = 65535;      // rows of a launch, at most: there is work memory for so many
+int segments(int V) { return (V + 7 + SEG - 1) / SEG; }      // whatever the rows' alignment
+long work_needed(int B, int V) { return segments(V) == 1 ? 0 : min(B, ROWS) * Work::bytes(segments(V)); }
+
+template <typename T> int launch(Args a, int B, bool cut, hipStream_t stream) {
+  const int rows = a.segs == 1 ? SHORT_ROWS : ROWS;
+  for (int b = 0; b < B; b += rows) {
+    const int n = min(B - b, rows);
+    // two blocks a CU: each starts with the row's maxima or bins, which costs as much as several segments (64 rows of 128256: 49.7 us, 60.7 with 256 blocks, 56.4 with 1024)
+    const dim3 grid(min(a.segs, max(BLOCKS / n, 1)), n);
+    if (a.segs == 1) {
+      k_sample_short<T><<<grid, NT, 0, stream>>>(a);
+    } else {
+      k_sample_max<T><<<grid, NT, 0, stream>>>(a);
+      k_sample_bins<T><<<grid, NT, 0, stream>>>(a);
+      if (cut) k_sample_draw<T><<<grid, NT, 0, stream>>>(a);
+    }
+    a.logits = static_cast<const T*>(a.logits) + n * a.stride;
+    a.u += n; a.out += n;
+    for (Setting* s : {&a.temperature, &a.top_p, &a.min_p}) if (s->rows) s->rows += n;
+    if (a.top_k_rows) a.top_k_rows += n;
   }
-  k_sample_max<T><<<grid, NT, 0, stream>>>(a);
-  k_sample_bins<T><<<grid, NT, 0, stream>>>(a);
-  if (cut) k_sample_draw<T><<<grid, NT, 0, stream>>>(a);
   return gaac::launch_status("gaac_sample");
 }
-
-int segments(int V) { return (V + 7 + SEG - 1) / SEG; }      // whatever the rows' alignment
 
 }  // namespace
 
 extern "C" int gaac_sample(int type, const void* logits, long row_stride, int B, int V, const float* u, const float* temperature_rows, float temperature, const int* top_k_rows, int top_k,
                            const float* top_p_rows, float top_p, const float* min_p_rows, float min_p, void* work, long work_bytes, int64_t* out, void* stream) {
-  GAAC_REQUIRE(logits != nullptr && u != nullptr && out != nullptr && work != nullptr, "gaac_sample: null pointer");
+  GAAC_REQUIRE(logits != nullptr && u != nullptr && out != nullptr, "gaac_sample: null pointer");
   GAAC_REQUIRE(type >= 0 && type <= 2, "gaac_sample: type must be 0 (bf16), 1 (fp16) or 2 (fp32)");
-  GAAC_REQUIRE(B > 0 && B <= 65535 && V > 0 && V <= MAX_V - 16 && row_stride >= 0, "gaac_sample: bad sizes (%d rows of %d logits, at most 65535 of %d)", B, V, MAX_V - 16);
+  GAAC_REQUIRE(B > 0 && V > 0 && V <= MAX_V - 16 && row_stride >= 0, "gaac_sample: bad sizes (%d rows of %d logits, at most %d)", B, V, MAX_V - 16);
   GAAC_REQUIRE(reinterpret_cast<uintptr_t>(logits) % (type == 2 ? 4 : 2) == 0, "gaac_sample: logits are not aligned to their type");
   const int segs = segments(V);
-  GAAC_REQUIRE(reinterpret_cast<uintptr_t>(work) % 8 == 0 && work_bytes >= B * Work::bytes(segs), "gaac_sample: %ld bytes of work memory, aligned to 8, are too few", work_bytes);
+  GAAC_REQUIRE(reinterpret_cast<uintptr_t>(work) % 8 == 0 && work_bytes >= work_needed(B, V) && (work != nullptr || segs == 1), "gaac_sample: %ld bytes of work memory, aligned to 8, are too few", work_bytes);
   const Args a{logits, row_stride, V, segs, u, {temperature_rows, temperature}, {top_p_rows, top_p}, {min_p_rows, min_p}, top_k_rows, top_k, (long*)out, (uint8_t*)work};
   const bool cut = top_k_rows != nullptr || top_p_rows != nullptr || (top_k > 0 && top_k < V) || top_p < 1;
   if (type == 0) return launch<__bf16>(a, B, cut, (hipStream_t)stream);

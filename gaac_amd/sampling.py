@@ -4,12 +4,14 @@ import torch
 from . import _lib
 from .rope import TYPES
 
-MAX_VOCAB, MAX_ROWS = (1 << 20) - 16, 65535
+MAX_VOCAB = (1 << 20) - 16
 
 
 def work_bytes(B: int, V: int) -> int:
-    """Scratch of a call: per row two words for each segment of 4096 logits, 2048 bins of 12 bytes, 8192 candidates, two counters."""
-    return B * (16 * -(-(V + 7) // 4096) + 12 * 2048 + 8 * 8192 + 16)
+    """Scratch of a call: none for rows of one segment of 4096 logits, otherwise for each of up to 1024 rows at a time two words for each segment, 2048 bins of 12 bytes, 8192
+    candidates, two counters."""
+    segments = -(-(V + 7) // 4096)
+    return 0 if segments == 1 else min(B, 1024) * (16 * segments + 12 * 2048 + 8 * 8192 + 16)
 
 
 def _setting(name: str, x, B: int, dtype, like: torch.Tensor):
@@ -29,13 +31,12 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_
 
     A temperature that is not positive: the first maximum.  A token whose logit is -inf or NaN never comes; -1 for a row that has nothing else.  An infinite
     maximum: evenly among the tokens that have it.  u outside [0, 1) counts as the nearest number inside, NaN as 0.  Sums are exact to 2^-43 of the largest
-    weight and do not depend on their order.  At most three launches, no wait."""
+    weight and do not depend on their order.  One launch for vocabularies up to 4089, otherwise at most three for every 1024 rows; no wait."""
     out = (_lib._calls or _lib.calls()).draw(logits, u, temperature, top_k, top_p, min_p, _lib.stream)
     if out is not None: return out
     if logits.dim() != 2 or logits.dtype not in TYPES or not 1 <= logits.shape[1] <= MAX_VOCAB:
         raise RuntimeError(f"sample expects logits bf16, fp16 or fp32 [B, V], V up to {MAX_VOCAB}, got {logits.dtype} {list(logits.shape)}")
     B, V = logits.shape
-    if B > MAX_ROWS: raise RuntimeError(f"sample takes {MAX_ROWS} rows at a time, got {B}")
     if u.dtype != torch.float32 or tuple(u.shape) != (B,): raise RuntimeError(f"sample expects u fp32 [{B}], got {u.dtype} {list(u.shape)}")
     (t_rows, t), (k_rows, k), (p_rows, p), (m_rows, m) = (_setting(name, x, B, dtype, logits) for name, x, dtype in (
         ("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32), ("min_p", min_p, torch.float32)))

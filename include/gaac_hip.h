@@ -267,7 +267,7 @@ int gaac_qk_norm_rope(int type, const void* q, const void* k, long q_token_strid
 
 /* One token per row of logits [B, V] (type as above, rows row_stride elements apart): out int64 [B].  Each setting comes per row (device, [B]) or, where
  * that is NULL, as one number.  u in [0, 1).  The definition is stated in gaac_amd/csrc/sample.hip.  work: scratch of this call, 8-byte aligned, need not be set to
- * anything: B * (16 * ceil((V + 7) / 4096) + 90128) bytes. */
+ * anything: min(B, 1024) * (16 * ceil((V + 7) / 4096) + 90128) bytes, or none where V + 7 <= 4096. */
 int gaac_sample(int type, const void* logits, long row_stride, int B, int V, const float* u, const float* temperature_rows, float temperature, const int* top_k_rows,
                 int top_k, const float* top_p_rows, float top_p, const float* min_p_rows, float min_p, void* work, long work_bytes, int64_t* out, void* stream);
 

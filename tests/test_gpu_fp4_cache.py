@@ -383,3 +383,46 @@ def test_stats_and_sizes():
     c.prefill(0, rows(70, 4), rows(70, 4)); c.prefill(2, rows(5, 4), rows(5, 4))
     s = c.stats()
     assert s["tokens"] == 75 and s["bytes_used"] == 75 * 4 * 136 and s["bf16_bytes"] == 75 * 4 * 512 and abs(s["ratio"] - 512 / 136) < 1e-12
+
+
+def test_a_saved_cache_is_read_as_before(tmp_path):
+    require_gpu()
+    n_kv, G = 2, 4
+    c = cache(2, n_kv, 3000)
+    k, v = rows(2500, n_kv, 1), rows(2500, n_kv, 2)
+    c.prefill(1, k, v)
+    q = torch.randn(1, n_kv * G, D, generator=torch.Generator().manual_seed(3)).to(torch.bfloat16).cuda()
+    slots = torch.ones(1, dtype=torch.int32, device="cuda")
+    want = c.attention(q, slots, D ** -0.5)
+    torch.save(c, tmp_path / "cache.pt")
+    d = torch.load(tmp_path / "cache.pt", weights_only=False)
+    assert torch.equal(d.attention(q, slots, D ** -0.5), want)
+    d.append(slots, k[:1], v[:1])
+    assert d.lens.tolist() == [0, 2501] and c.lens.tolist() == [0, 2500]
+
+
+def test_more_captured_calls_than_there_are_counters_for(monkeypatch):
+    """Calls captured behind the last set of counters, or of more rows than slots, take the launch of their own that adds up the splits."""
+    from gaac_amd import fp4_cache
+    require_gpu()
+    monkeypatch.setattr(fp4_cache, "CAPTURES", 2)
+    n_kv, G, B = 2, 4, 5
+    c = cache(3, n_kv, 600)
+    k, v = rows(600, n_kv, 1), rows(600, n_kv, 2)
+    for i, L in enumerate((600, 33, 257)): c.prefill(i, k[:L], v[:L])
+    q = torch.randn(B, n_kv * G, D, generator=torch.Generator().manual_seed(3)).to(torch.bfloat16).cuda()
+    few, many = torch.tensor([2, 0, 1], dtype=torch.int32, device="cuda"), torch.tensor([0, 0, 2, -1, 1], dtype=torch.int32, device="cuda")
+    want = [c.attention(q[:3], few, D ** -0.5, nsplit=4), c.attention(q, many, D ** -0.5, nsplit=4)]
+    graphs = []
+    for i in range(5):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g): out = c.attention(q, many, D ** -0.5, nsplit=4) if i == 1 else c.attention(q[:3], few, D ** -0.5, nsplit=4)
+        graphs.append((g, out, want[i == 1]))
+    assert c._captured == 2
+    for _ in range(3):
+        for g, out, ref in graphs:
+            out.zero_()
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, ref)
+            assert torch.equal(c.attention(q, many, D ** -0.5, nsplit=4), want[1])

@@ -147,3 +147,31 @@ def test_many_rows():
     x, u = logits(700, 900, torch.float16)
     s = dict(temperature=1.1, top_p=0.8)
     check(x, u, sample(x.cuda(), u.cuda(), **s), **s)
+
+
+@pytest.mark.parametrize("B,V", [(70000, 5), (1025, 4090), (2300, 4200)])
+def test_more_rows_than_a_launch_takes(B, V):
+    """Settings, random numbers and tokens of the rows behind the first launches' are their own; a few rows are drawn by the definition, and all rows alike in one call and in pieces."""
+    from gaac_amd import sample
+    require_gpu()
+    g = torch.Generator(device="cuda").manual_seed(5)
+    x = (torch.randn(B, V, generator=g, device="cuda") * 3).to(torch.bfloat16)
+    u = torch.rand(B, generator=g, device="cuda")
+    i = torch.arange(B, device="cuda")
+    s = dict(temperature=torch.where(i % 3 == 0, 0.0, 0.5 + (i % 5) * 0.3), top_k=(i % 7).int(), top_p=torch.where(i % 2 == 0, 1.0, 0.8), min_p=torch.where(i % 11 == 0, 0.1, 0.0))
+    got = sample(x, u, **s)
+    pieces = [sample(x[a:a + 500], u[a:a + 500], **{k: v[a:a + 500] for k, v in s.items()}) for a in range(0, B, 500)]
+    assert torch.equal(got, torch.cat(pieces))
+    at = torch.tensor([0, 1, 2, 1023, 1024, B - 2, B - 1]) if B < 70000 else torch.tensor([0, 65534, 65535, 65536, B - 1])
+    check(x[at.cuda()].cpu(), u[at.cuda()], got[at.cuda()], **{k: v[at.cuda()] for k, v in s.items()})
+
+
+def test_sums_that_fill_the_bins_and_more_candidates_than_there_is_room_for():
+    """All elements within one bin: more of them than are looked at one by one (8192) or sorted (1024)."""
+    from gaac_amd import sample
+    require_gpu()
+    for V in (900, 1100, 5000, 8192, 8300, 20000, 70000):
+        x = 3 + torch.rand(2, V, generator=torch.Generator().manual_seed(V)) * 0.02
+        u = torch.tensor([0.3, 0.95])
+        for s in (dict(top_p=0.5), dict(top_k=V // 2), dict(top_k=V - 3, top_p=0.9), dict(top_p=0.7, min_p=0.99), dict(top_k=700, top_p=0.3)):
+            for dtype in TYPES: check(x.to(dtype), u, sample(x.to(dtype).cuda(), u.cuda(), **s), **s)

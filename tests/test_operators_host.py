@@ -68,7 +68,6 @@ def test_samples_that_are_refused():
     x, u = torch.zeros(4, 100), torch.zeros(4)
     for bad in (x.double(), x[0], x[:, :0], torch.zeros(1).expand(2, 1 << 20)):
         with pytest.raises(RuntimeError, match="sample expects logits"): sample(bad, u)
-    with pytest.raises(RuntimeError, match="65535 rows at a time"): sample(torch.zeros(1, 2).expand(65536, 2), torch.zeros(65536))
     for bad in (u.double(), u[:3], u[:, None]):
         with pytest.raises(RuntimeError, match="sample expects u"): sample(x, bad)
     for name, bad in (("temperature", u.double()), ("temperature", u[:3]), ("top_k", u), ("top_k", torch.zeros(4, dtype=torch.int64)), ("top_p", u[:, None]), ("min_p", u.half())):
@@ -98,8 +97,9 @@ def test_samples_that_are_refused():
     ("gaac_sample", [0, 16, 100, 0, 100, 16, None, 1.0, None, 0, None, 1.0, None, 0.0, 16, 1 << 30, 16, None], "bad sizes"),
     ("gaac_sample", [0, 16, 100, 1, 1 << 20, 16, None, 1.0, None, 0, None, 1.0, None, 0.0, 16, 1 << 30, 16, None], "bad sizes"),
     ("gaac_sample", [0, 17, 100, 1, 100, 16, None, 1.0, None, 0, None, 1.0, None, 0.0, 16, 1 << 30, 16, None], "not aligned"),
-    ("gaac_sample", [0, 16, 100, 2, 100, 16, None, 1.0, None, 0, None, 1.0, None, 0.0, 16, 2 * (16 + 90128) - 1, 16, None], "work memory"),
-    ("gaac_sample", [0, 16, 100, 1, 100, 16, None, 1.0, None, 0, None, 1.0, None, 0.0, 20, 1 << 20, 16, None], "work memory"),
+    ("gaac_sample", [0, 16, 5000, 2, 5000, 16, None, 1.0, None, 0, None, 1.0, None, 0.0, 16, 2 * (32 + 90128) - 1, 16, None], "work memory"),
+    ("gaac_sample", [0, 16, 5000, 1, 5000, 16, None, 1.0, None, 0, None, 1.0, None, 0.0, 20, 1 << 20, 16, None], "work memory"),
+    ("gaac_sample", [0, 16, 5000, 1, 5000, 16, None, 1.0, None, 0, None, 1.0, None, 0.0, None, 1 << 20, 16, None], "work memory"),
 ])
 def test_the_library_refuses_before_it_launches(name, args, message):
     with pytest.raises(RuntimeError, match=f"{name} failed .*{message}"): _lib.call(name, *args)
