@@ -147,4 +147,10 @@ def on_device(*tensors):
     return _HERE if dev.index == torch._C._cuda_getDevice() else torch.cuda.device(dev)
 
 
+def no_backward(what: str, *tensors):
+    """Raises where a gradient would be lost without a word: these kernels have no backward pass."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad(), or with tensors that need no gradient")
+
+
 _HERE = contextlib.nullcontext()

@@ -9,6 +9,7 @@
 #include <dlfcn.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/ops/empty.h>
+#include <c10/core/GradMode.h>
 #include <c10/core/impl/DeviceGuardImplInterface.h>
 #include <algorithm>
 #include <exception>
@@ -435,6 +436,7 @@ PyObject* fp4_attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
     Refs get;
     const Fp4Cache c(get, a[0]);
     const at::Tensor &q = here(a[1]), &slots = here(a[2]);
+    if (c10::GradMode::is_enabled() && q.requires_grad()) throw Otherwise{};
     const long nsplit = number(a[4]), cap = number(get(a[0], n_cap));
     if (!is_rows(q, 3) || !q.is_contiguous() || reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 != 0 || q.size(0) == 0 || !is_slots(slots, q.size(0)) || nsplit < 1 || nsplit > 1 << 20) throw Otherwise{};
     const long B = q.size(0), n_q = q.size(1);
@@ -490,6 +492,7 @@ PyObject* norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return whole_call(n, 10, [&]() -> PyObject* {
     const at::Tensor &q = here(a[0]), &k = here(a[1]), &pos = here(a[2]), &cos = here(a[3]), &sin = here(a[4]);
     const int type = float_type(q);
+    if (c10::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || (a[5] != Py_None && tensor(a[5]).requires_grad()) || (a[6] != Py_None && tensor(a[6]).requires_grad()))) throw Otherwise{};
     if (q.dim() != 3 || k.dim() != 3 || q.scalar_type() != k.scalar_type() || q.size(0) != k.size(0) || q.size(2) != k.size(2) || q.size(0) == 0 || q.size(1) == 0 || k.size(1) == 0) throw Otherwise{};
     const long N = q.size(0), n_q = q.size(1), n_k = k.size(1), D = q.size(2);
     if ((D != 64 && D != 128 && D != 256) || N >= 1l << 28 || n_q >= 1 << 20 || n_k >= 1 << 20) throw Otherwise{};

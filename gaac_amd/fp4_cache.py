@@ -129,6 +129,7 @@ class FP4KVCache:
         B, n_q, _ = q.shape
         if n_q % self.n_kv or not 1 <= n_q // self.n_kv <= GMAX: raise RuntimeError(f"GQA group size must be 1..{GMAX}")
         if slots.dtype != torch.int32 or slots.dim() != 1 or slots.shape[0] != B: raise RuntimeError("attention expects slots int32 [B]")
+        _lib.no_backward("attention", q)
         if nsplit < 1: raise RuntimeError(f"attention expects at least one split, got {nsplit}")
         with _lib.on_device(self.data, q, slots):
             out = torch.empty(B, n_q, D, dtype=q.dtype, device=q.device)

@@ -26,7 +26,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, cos:
       of the first R channels the pairs (p, p + R/2), or (2p, 2p + 1) if interleaved, become (y1 cos - y2 sin, y2 cos + y1 sin); the rest stays y
 
     with row positions[token] (int64 or int32 [N]) of cos, sin (fp32 [max_pos, R/2], R a multiple of 16).  A token whose position the tables do not have becomes NaN.
-    In 32 bits, rounded once.  One launch, no wait."""
+    In 32 bits, rounded once.  One launch, no wait, no backward pass."""
     out = (_lib._calls or _lib.calls()).norm_rope(q, k, positions, cos, sin, q_weight, k_weight, eps, interleaved, _lib.stream)
     if out is not None: return out
     if q.dim() != 3 or k.dim() != 3 or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2] or q.dtype != k.dtype or q.dtype not in TYPES:
@@ -41,6 +41,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, cos:
     if q_weight is not None:
         for w, heads in ((q_weight, n_q), (k_weight, n_k)):
             if w.dtype != q.dtype or tuple(w.shape) not in ((D,), (heads, D)): raise RuntimeError(f"qk_norm_rope expects weights {q.dtype} [{D}] or [{heads}, {D}], got {w.dtype} {list(w.shape)}")
+    _lib.no_backward("qk_norm_rope", q, k, q_weight, k_weight)
     with _lib.on_device(q, k, positions, cos, sin, q_weight, k_weight):
         q_out, k_out = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, k))
         if N == 0: return q_out, k_out

@@ -103,3 +103,14 @@ def test_samples_that_are_refused():
 ])
 def test_the_library_refuses_before_it_launches(name, args, message):
     with pytest.raises(RuntimeError, match=f"{name} failed .*{message}"): _lib.call(name, *args)
+
+
+def test_gradients_are_not_lost_without_a_word():
+    x, pos, cos, w = torch.zeros(5, 2, 128, dtype=BF), torch.zeros(5, dtype=torch.int64), torch.zeros(10, 64), torch.ones(128, dtype=BF)
+    need = lambda t: t.clone().requires_grad_()
+    c = FP4KVCache(2, 2, 64, device="cpu")
+    calls = (lambda t: qk_norm_rope(t(x), x, pos, cos, cos), lambda t: qk_norm_rope(x, t(x), pos, cos, cos, w, w), lambda t: qk_norm_rope(x, x, pos, cos, cos, t(w), w), lambda t: qk_norm_rope(x, x, pos, cos, cos, w, t(w)),
+             lambda t: c.attention(t(x), torch.zeros(5, dtype=torch.int32), 1.0))
+    for call in calls:
+        with pytest.raises(RuntimeError, match="no backward pass"): call(need)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="no CPU path"): call(need)
