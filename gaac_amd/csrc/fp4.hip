@@ -115,12 +115,16 @@ __global__ __launch_bounds__(256) void k_fp4_load(const uint8_t* cache, int L, i
   if (tile * TT >= L) return;
   const uint8_t* in = cache + ((long)head * tiles + tile) * TILE;
   if (blockIdx.z == 0) {
-    const unsigned exps = *reinterpret_cast<const uint16_t*>(in + KS_AT + 2 * l);
-    for (int s = 0; s < 2; ++s) {
-      const u4 w = *reinterpret_cast<const u4*>(in + 1024 * s + 16 * l);
-      const int t = tile * TT + 16 * s + m;
-      if (t < L)
-        for (int i = 0; i < 4; ++i) *reinterpret_cast<u4*>(k + head * k_hs + t * k_rs + 32 * g + 8 * i) = decode_unit(w[i], scale_of(exps >> 8 * s & 255));
+    // (not in the order that a lane's 16 bytes have: a token's row is written as a whole by 16 lanes, and the dwords come out of the same lines)
+    unsigned w[8], e[8];
+    for (int i = 0; i < 8; ++i) {      // token 4 i + g, unit m
+      const int t = 4 * i + g, lane = 16 * (m >> 2) + (t & 15);
+      w[i] = *reinterpret_cast<const unsigned*>(in + 1024 * (t >> 4) + 16 * lane + 4 * (m & 3));
+      e[i] = in[KS_AT + 2 * lane + (t >> 4)];
+    }
+    for (int i = 0; i < 8; ++i) {
+      const int t = tile * TT + 4 * i + g;
+      if (t < L) *reinterpret_cast<u4*>(k + head * k_hs + t * k_rs + 8 * m) = decode_unit(w[i], scale_of(e[i]));
     }
   } else {
     const u2 exps = *reinterpret_cast<const u2*>(in + VS_AT + 32 * (m >> 2) + 8 * g);
