@@ -366,8 +366,8 @@ PyObject* page_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return THPVariable_Wrap(out);
   });
 }
-// The calls of the 4-bit cache, of qk_norm_rope and of sample, the same way.  Their tensors have to be on the current device.  Host us a call, Python / here: append
-// 7.8 / 4.6, attention 11.0 / 6.0, qk_norm_rope 15.9 / 5.4, sample 26 / 14 (three launches).
+// The calls of the 4-bit cache, of qk_norm_rope and of sample, the same way.  Their tensors have to be on the current device.  Host us a call, Python / here: prefill
+// 9.0 / 3.3, append 8.1 / 3.6, attention 8.2 / 5.1 (with splits 12.2 / 7.5), qk_norm_rope 16.4 / 5.9, sample 9.7 / 5.0 (of three launches 14.5 / 9.8).
 const at::Tensor& here(PyObject* o) {
   const at::Tensor& t = tensor(o);
   if (t.device() != c10::impl::getDeviceGuardImpl(c10::DeviceType::CUDA)->getDevice()) throw Otherwise{};

@@ -63,7 +63,9 @@ __device__ __forceinline__ u4 decode_unit(unsigned w, float scale) {
 
 // ---------------------------------------------------------------------------------------------------- prompt
 // A wave encodes K (blockIdx.z = 0) or V of one tile; four tiles a block.  Bound by HBM: 8 KB read and 2.1 KB written per tile and kind.  A lane
-// loads 64 bytes in a row of two tokens (K) or 16 of eight (V: whole 256-byte rows by 16 lanes); a store is 1 KB in a row.  Rows of the last tile behind the prompt become zero bytes.
+// loads 64 bytes in a row of two tokens (K) or 16 of eight (V: whole 256-byte rows by 16 lanes); a store is 1 KB in a row.  All 8 loads of a lane are in flight
+// before the first is used.  32768 tokens x 8 heads: 36.8 us, 4.6 TB/s read and written, a large copy's rate (K's rows loaded whole by 16 lanes and turned through LDS:
+// 36.3); 777 x 8: 3.4, a launch being 1.6.  Rows of the last tile behind the prompt become zero bytes.
 __global__ __launch_bounds__(256) void k_fp4_store(const uint16_t* k, const uint16_t* v, long k_hs, long k_rs, long v_hs, long v_rs, int L, int tiles, uint8_t* cache, int* len) {
   if (len != nullptr && blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0 && threadIdx.x == 0) *len = L;
   const int tile = blockIdx.x * 4 + (threadIdx.x >> 6), l = threadIdx.x & 63, m = l & 15, g = l >> 4, head = blockIdx.y;
@@ -110,6 +112,8 @@ __global__ __launch_bounds__(256) void k_fp4_store(const uint16_t* k, const uint
   }
 }
 
+// The way back, by the same waves.  Bound by HBM: 2.1 KB read and 8 KB written per tile and kind, rows of 256 bytes written by 16 lanes (32768 tokens x 8 heads:
+// 36.1 us, 4.7 TB/s; K with 64 bytes of a row a lane, as the encoder reads it: 48.5).
 __global__ __launch_bounds__(256) void k_fp4_load(const uint8_t* cache, int L, int tiles, uint16_t* k, uint16_t* v, long k_hs, long k_rs, long v_hs, long v_rs) {
   const int tile = blockIdx.x * 4 + (threadIdx.x >> 6), l = threadIdx.x & 63, m = l & 15, g = l >> 4, head = blockIdx.y;
   if (tile * TT >= L) return;
@@ -140,7 +144,8 @@ __global__ __launch_bounds__(256) void k_fp4_load(const uint8_t* cache, int L, i
 
 // ---------------------------------------------------------------------------------------------------- one token
 // A block per batch row, a thread per unit (K or V, head, 8 channels); a block of channels is four threads next to each other.  The row's length is
-// raised once all of the block have read it.
+// raised once all of the block have read it.  Bound by the launch and one load after the other (slot, length, element): 2.6 us from 4 rows x 8 heads to 32, of which
+// an empty launch takes 1.6.
 __global__ __launch_bounds__(256) void k_fp4_append(const int* slots, int n_slots, int n_kv, const uint16_t* k, const uint16_t* v, long k_bs, long k_hs, long v_bs, long v_hs, int* lens,
                                                     int tiles, int cap, uint8_t* cache, int* errors) {
   const int b = blockIdx.x, slot = slots[b];
@@ -148,8 +153,9 @@ __global__ __launch_bounds__(256) void k_fp4_append(const int* slots, int n_slot
   bool again = false;      // a slot that an earlier row of the batch names: two tokens for one place
   for (int i = threadIdx.x; i < b; i += 256) again |= slots[i] == slot;
   const int len = slot < n_slots ? lens[slot] : 0;
-  if (__syncthreads_or(again) || slot >= n_slots || len >= cap) {
-    if (threadIdx.x == 0) atomicOr(errors, slot >= n_slots ? 4 : len >= cap ? 1 : 2);
+  const bool full = (unsigned)len >= (unsigned)cap;      // (or below 0)
+  if (__syncthreads_or(again) || slot >= n_slots || full) {
+    if (threadIdx.x == 0) atomicOr(errors, slot >= n_slots ? 4 : full ? 1 : 2);
     return;
   }
   const int t = len & (TT - 1), s = t >> 4, m = t & 15, g = (t >> 2) & 3, i = t & 3;
@@ -174,7 +180,7 @@ __global__ __launch_bounds__(256) void k_fp4_append(const int* slots, int n_slot
 struct Share { int row, len, slot, first, end, index, count; };      // row < 0: nothing for this split
 
 __device__ __forceinline__ int row_slot(const int* slots, int b) { return slots[b]; }
-__device__ __forceinline__ int row_len(const int* lens, int n_slots, int cap, int slot) { return slot >= 0 && slot < n_slots ? min(lens[slot], cap) : 0; }
+__device__ __forceinline__ int row_len(const int* lens, int n_slots, int cap, int slot) { return slot >= 0 && slot < n_slots ? max(min(lens[slot], cap), 0) : 0; }      // (lens is the caller's to write)
 // Sums over the wave in the vector unit (rows of 16 by shifts, then across rows), not through LDS: a lane exchange there takes ten times as long.
 template <int CTRL, int ROWS> __device__ __forceinline__ int moved(int x) { return __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, false); }
 __device__ __forceinline__ int wave_scan(int x) {      // inclusive
@@ -360,7 +366,7 @@ __device__ __forceinline__ float lane(float x, int i) { return bits(__builtin_am
 constexpr int LINE = 32;      // tickets are a cache line apart: all blocks draw theirs at about the same time
 
 // Adds up the `count` splits from p0 on of the G heads of a (row, kv head), in their order, by the whole block: two waves a head, a lane a channel.  All loads of the
-// first 32 splits are in flight together (64K tokens x 8 heads, 32 splits: 1.6 us, against 3.8 in three dependent rounds).
+// first 32 splits are in flight together (64K tokens x 8 heads, 32 splits: 2.3 us, against 3.8 in three dependent rounds).
 __device__ void merge(const float* part, long acc_at, int p0, int count, int n_kv, int kvh, int G, uint16_t* out) {
   constexpr int AHEAD = 32, STEP = 8;
   const int l = threadIdx.x & 63;
@@ -378,7 +384,7 @@ __device__ void merge(const float* part, long acc_at, int p0, int count, int n_k
       for (int j = 0; j < AHEAD; j += STEP)
         if (j < n) {
 #pragma unroll
-          for (int i = j; i < j + STEP; ++i) x[i] = get(acc + (unsigned)(min(i, n - 1) * (int)step * DIM));
+          for (int i = j; i < j + STEP; ++i) x[i] = get(acc + (unsigned)min(i, n - 1) * (unsigned)step * DIM);
         }
       const u64 ms = l < n ? get(reinterpret_cast<const u64*>(part) + at + (i0 + l) * step) : 0xff800000ull;
       float m = bits((unsigned)ms), t = m;
@@ -403,6 +409,11 @@ __device__ void merge(const float* part, long acc_at, int p0, int count, int n_k
   }
 }
 
+// Decode attention.  Bound by the read of the cache where rows are long: 16 rows of 4096..65536 tokens x 8 heads 101 us, 606 MB, 6.0 TB/s, the rate of a plain read of
+// that size being 6.1; by the launch, the plan and the merge where the cache is short: 1 row of 65536 x 8 heads, 18.1 us, has its 71 MB by 15.4 (2.6 of
+// them launch and plan: 5.6 TB/s for the rest), leaves the partials until 16.9 and adds them up in 2.3.  A wave has whole tiles, so what it needs comes in 6 loads of whole lines
+// and no lane waits for another; one tile is in flight while another is worked on: 16 waves a CU, 68 KB of loads in flight on each.  Four waves a SIMD
+// need 128 registers at most: it has 123.
 // One block = eight waves = one split of one (row, kv head).  One split a row (P == B): the output is written here; otherwise a row with several splits leaves
 // partials, and the block that draws the last of the (row, kv head)'s tickets adds them up and puts the tickets back (tickets NULL: k_fp4_merge does it).
 __global__ __launch_bounds__(64 * NW, 4) void k_fp4_attn(const uint8_t* cache, const int* lens, const int* slots, int n_slots, int tiles, int cap, const uint16_t* q, int B, int n_kv, int G,
@@ -536,7 +547,7 @@ int gaac_fp4_append(const int* slots, int B, int n_slots, int n_kv, const void* 
 int gaac_fp4_attn(const uint8_t* cache, const int* lens, const int* slots, int n_slots, int tiles, int cap, const void* q, int B, int n_q, int n_kv, float scale, int nsplit, float* partials, unsigned* tickets, void* out,
                   void* stream) {
   GAAC_REQUIRE(cache != nullptr && lens != nullptr && slots != nullptr && q != nullptr && out != nullptr, "gaac_fp4_attn: null pointer");
-  GAAC_REQUIRE(B > 0 && n_slots > 0 && n_kv > 0 && n_q >= n_kv && n_q % n_kv == 0 && n_q / n_kv <= 16, "gaac_fp4_attn: GQA group size must be 1..16 (n_q %d, n_kv %d)", n_q, n_kv);
+  GAAC_REQUIRE(B > 0 && n_slots > 0 && n_kv > 0 && n_kv <= 65535 && n_q >= n_kv && n_q % n_kv == 0 && n_q / n_kv <= 16, "gaac_fp4_attn: GQA group size must be 1..16 (n_q %d, n_kv %d)", n_q, n_kv);
   GAAC_REQUIRE(tiles > 0 && cap > 0 && cap <= (long)tiles * TT && nsplit > 0 && (long)B * nsplit * n_kv < 1l << 31 && (long)B * n_q < 1l << 31, "gaac_fp4_attn: bad sizes (B %d, capacity %d in %d tiles, %d splits)", B,
                cap, tiles, nsplit);
   GAAC_REQUIRE(nsplit == 1 || (partials != nullptr && reinterpret_cast<uintptr_t>(partials) % 8 == 0), "gaac_fp4_attn: more than one split needs partials, 8-byte aligned");

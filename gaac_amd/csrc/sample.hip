@@ -6,7 +6,13 @@
 // Which token comes is a whole number, so a sum that is off in its last bits is an error: weights are computed in 64 bits and held as multiples of 2^-43
 // in 64-bit integers (2^20 of them fit), whose sums are exact in any order.
 // What is kept is a prefix of the order, so it is found as a key (the bits of x, in order) and the number of its equals that are kept: counts and sums by bins
-// of (max - x), then by ever finer bins of the key within the bin where the limit falls.
+// of (max - x), then the elements of the bin where the limit falls, in order: up to 1024 of them sorted in LDS, up to 8192 by ever finer bins of their keys, more by
+// such bins over the row.  Three launches: the row's maximum; bins; and the limits, the sums of segments and the token by the last of the row's blocks to
+// arrive.  A row of one segment takes one launch, bins and candidates in LDS.
+//
+// What bounds it: for few rows the chain of launches and of dependent steps in the last block (4 rows of 128256 in bf16, 1 MB: 22.6 us; kernels 4.2, 4.5 and 15.8,
+// launch 1.6 of each); for many the weights in 64 bits, computed twice for each element that can be kept, and atomic additions to bins (64
+// mixed rows of 128256 in fp32, 33 MB: 61.6 us; kernels 8.2, 20.7 and 34.6; the read alone 5.5).
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include "gaac_capi.h"
@@ -75,7 +81,7 @@ template <typename T> struct Row {
 };
 
 // exp(y), y <= 0: y = n ln 2 / 64 + r, 2^(n / 64) from a table of the 64 roots in LDS and the exponent, times the series of exp to r^5 (|r| <= 0.0055: what is left
-// is below 1e-16).  15 operations in 64 bits; the series to r^11 without a table took 24 (64 mixed rows of 128256: 68 us, with the table 60).
+// is below 1e-16).  15 operations in 64 bits; the series to r^11 without a table took 24 (64 mixed rows of 128256: 68 us, with the table 61.6).
 constexpr int ROOTS = 64;
 __device__ __forceinline__ void fill_roots(double* table) {      // by the first wave; 2^(j / 64) = exp(j ln 2 / 64) by its series
   if (threadIdx.x < ROOTS) {
@@ -696,7 +702,7 @@ template <typename T> int launch(Args a, int B, bool cut, hipStream_t stream) {
   const int rows = a.segs == 1 ? SHORT_ROWS : ROWS;
   for (int b = 0; b < B; b += rows) {
     const int n = min(B - b, rows);
-    // two blocks a CU: each starts with the row's maxima or bins, which costs as much as several segments (64 rows of 128256: 49.7 us, 60.7 with 256 blocks, 56.4 with 1024)
+    // two blocks a CU: each starts with the row's maxima or bins, which costs as much as several segments (64 rows of 128256 by top-p: 48.5 us, 57.8 with 256 blocks, 54.1 with 1024)
     const dim3 grid(min(a.segs, max(BLOCKS / n, 1)), n);
     if (a.segs == 1) {
       k_sample_short<T><<<grid, NT, 0, stream>>>(a);

@@ -147,6 +147,24 @@ def test_rows_that_cannot_be_added_are_left_out_and_reported():
         assert torch.equal(c.data, want.data)
 
 
+def test_lengths_that_a_caller_set_wrongly():
+    """lens is a tensor of the caller's to write (to drop tokens): below 0 counts as an empty slot that takes no token, above the capacity as a full one."""
+    require_gpu()
+    n_kv, L = 2, 64
+    k, v = rows(L, n_kv, 1), rows(L, n_kv, 2)
+    slots = torch.tensor([0, 1, 2], dtype=torch.int32, device="cuda")
+    q = torch.randn(3, 4, D, generator=torch.Generator().manual_seed(3)).to(torch.bfloat16).cuda()
+    for nsplit in (1, 3):
+        c = cache(3, n_kv, L)
+        for s in range(3): c.prefill(s, k, v)
+        held = c.decompress(1)
+        c.lens.copy_(torch.tensor([-40, 64, 2 ** 31 - 1], dtype=torch.int32))
+        check(c.attention(q, slots, D ** -0.5, nsplit=nsplit), q, [None, held, held], D ** -0.5)
+        before = c.data.clone()
+        c.append(slots, k[:3], v[:3])
+        assert int(c.overflow) == 1 and torch.equal(c.data, before) and c.lens.tolist() == [-40, 64, 2 ** 31 - 1]
+
+
 # ---------------------------------------------------------------------------------------------------- attention
 HEADS = [(8, 4), (4, 6), (1, 16), (16, 1), (2, 5), (3, 13)]
 
