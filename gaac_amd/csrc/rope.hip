@@ -1,7 +1,8 @@
 // Norms of queries and keys for each head and their rotation, in one pass over both.
 //   y = x * rsqrt(mean(x^2) + eps) * w over the head's D channels (no weights: y = x), then for each pair p < R/2 of the first R channels
 //   (y1 cos - y2 sin, y2 cos + y1 sin), the pair being (p, p + R/2), or (2p, 2p + 1) if interleaved; cos and sin are row `position` of tables.
-// Bound by HBM for a prompt (each element read once and written once), by the launch for a decode step.  A lane holds 16 channels of a head, two runs of 8 that
+// Bound by HBM for a prompt (each element read once and written once: 16384 tokens x 40 heads of 128 channels in bf16, 344 MB, 67 us, 5.1 TB/s, where a large copy
+// makes 4.7), by the launch for a decode step (4 tokens x 40 heads: 3.3 us, of which an empty launch takes 1.6; 777 x 28: 5.3).  A lane holds 16 channels of a head, two runs of 8 that
 // make whole pairs, so nothing but the sum of squares goes between lanes: D / 16 lanes a head, 16-byte loads.  A wave keeps to one token and goes through
 // its heads, the lane's cos and sin staying in registers.  Arithmetic in 32 bits, one rounding at the end; products are not fused into the sums of the
 // rotation, so that without weights a result is bit for bit what separate multiplications and additions in 32 bits give.
@@ -131,7 +132,9 @@ extern "C" int gaac_qk_norm_rope(int type, const void* q, const void* k, long q_
   GAAC_REQUIRE(all % 16 == 0 && (q_token_stride | q_head_stride | k_token_stride | k_head_stride | q_weight_stride | k_weight_stride) % (type == 2 ? 4 : 8) == 0, "gaac_qk_norm_rope: rows must be 16-byte aligned");
   const int groups = (n_q + n_k + 1024 / D - 1) / (1024 / D);      // of the 64 / (D/16) heads that a wave takes at a time
   Args a{q, k, q_weight, k_weight, positions, q_out, k_out, cos, sin, q_token_stride, q_head_stride, k_token_stride, k_head_stride, q_weight_stride, k_weight_stride, N, n_q, n_k, R, max_pos, groups, positions64 != 0, eps};
-  if (N * groups > 8192) a.parts = 1;
+  // A wave for each group of heads until the chip is full twice over, then one that goes through a token's groups and reads cos and sin once (40 heads of 128 channels, us,
+  // split / not: 4 tokens 2.8 / 5.2, 777 5.6 / 7.8, 2400 11.2 / 11.5, 4096 16.1 / 15.6, 16384 67.1 / 65.5).
+  if (N * groups > 16384) a.parts = 1;
   const bool norm = q_weight != nullptr;
   if (type == 0) launch<__bf16>(a, D, interleaved != 0, norm, (hipStream_t)stream);
   else if (type == 1) launch<_Float16>(a, D, interleaved != 0, norm, (hipStream_t)stream);
