@@ -24,8 +24,9 @@ constexpr int NT = 512, SEG = NT * 8, BINS = 2048, MAX_V = 1 << 20, MAX_SEGS = M
 constexpr int BLOCKS = 512;
 constexpr int ROOM = 8192;      // elements of a row that are looked at one by one, at most
 constexpr int SORTED = 2 * NT;      // and of these so many by sorting them
-static_assert(MAX_SEGS <= NT && SORTED <= BINS);
+static_assert(MAX_SEGS <= NT && 2 * SORTED <= BINS);
 typedef unsigned long long u64;
+template <int N> struct Number { static constexpr int value = N; };
 typedef unsigned u4 __attribute__((ext_vector_type(4)));
 
 // Order of floats as that of unsigned numbers; -0 and NaN have been taken away.
@@ -125,6 +126,7 @@ template <typename U> __device__ __forceinline__ U wave_scan(U x) {
   x += moved<0x142, 0xa>(x); x += moved<0x143, 0xc>(x);
   return x;
 }
+__device__ __forceinline__ u64 lane(u64 x, int i) { return (u64)(unsigned)__builtin_amdgcn_readlane((int)(x >> 32), i) << 32 | (unsigned)__builtin_amdgcn_readlane((int)x, i); }
 __device__ __forceinline__ u64 larger(u64 a, u64 b) { return a > b ? a : b; }
 __device__ __forceinline__ u64 wave_max(u64 x) {      // in lane 63
   x = larger(x, moved<0x111, 0xf>(x)); x = larger(x, moved<0x112, 0xf>(x)); x = larger(x, moved<0x114, 0xf>(x)); x = larger(x, moved<0x118, 0xf>(x));
@@ -371,52 +373,98 @@ __device__ __forceinline__ u64 kept_mass(const float (&x)[8], const Weights& wei
   return mass;
 }
 
+// x of the lane whose number differs in bit S: within rows of 16 lanes by data parallel moves (4: all three low bits turned, then the lower two back), across them by swaps
+// of rows and halves.
+template <int S> __device__ __forceinline__ unsigned across(unsigned x) {
+  const auto dpp = [](unsigned v, auto ctrl) { return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, decltype(ctrl)::value, 0xf, 0xf, false); };
+  if constexpr (S == 1) return dpp(x, Number<0xb1>{});
+  else if constexpr (S == 2) return dpp(x, Number<0x4e>{});
+  else if constexpr (S == 4) return dpp(dpp(x, Number<0x141>{}), Number<0x1b>{});
+  else if constexpr (S == 8) return dpp(x, Number<0x128>{});
+  else if constexpr (S == 16) { const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false); return threadIdx.x & 16 ? r[0] : r[1]; }
+  else { const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false); return threadIdx.x & 32 ? r[0] : r[1]; }
+}
+// The steps of stride S, S / 2 .. 1 of a bitonic merge of `size` places (i: the thread's), which descend where i & size is 0.
+template <int S> __device__ __forceinline__ void merge_in_wave(u64& x, int i, int size) {
+  const u64 y = (u64)across<S>((unsigned)(x >> 32)) << 32 | across<S>((unsigned)x);
+  if ((y > x) == (((i & S) == 0) == ((i & size) == 0))) x = y;
+  if constexpr (S > 1) merge_in_wave<S / 2>(x, i, size);
+}
+template <int SIZE> __device__ __forceinline__ void sort_in_wave(u64& x, int i) {
+  if constexpr (SIZE > 2) sort_in_wave<SIZE / 2>(x, i);
+  merge_in_wave<SIZE / 2>(x, i, SIZE);
+}
+// Puts up to SORTED numbers in descending order, x[j] being place threadIdx.x + j * NT; also where the result points to, in LDS.  A bitonic sort in registers: strides below
+// 64 within a wave, 64 to 256 through LDS, two buffers in turn so that a step takes one barrier, 512 within a thread.
+__device__ const u64* put_in_order(Shared& sh, u64 (&x)[2], int n) {
+  const int t = threadIdx.x;
+  const bool two = n > NT;
+  u64* buffer = sh.mass;
+  if (t - t % 64 < n) sort_in_wave<64>(x[0], t);
+  if (two) sort_in_wave<64>(x[1], t + NT);
+  for (int size = 128; size < 2 * n && size <= SORTED; size *= 2) {
+    int s = size / 2;
+    if (s == NT) {
+      if (x[0] < x[1]) { const u64 y = x[0]; x[0] = x[1]; x[1] = y; }
+      s /= 2;
+    }
+    for (; s >= 64; s /= 2) {
+      buffer[t] = x[0];
+      if (two) buffer[t + NT] = x[1];
+      __syncthreads();
+      for (int j = 0; j < 2; ++j) {
+        if (j == 1 && !two) break;
+        const int i = t + j * NT;
+        const u64 y = buffer[i ^ s];
+        if ((y > x[j]) == (((i & s) == 0) == ((i & size) == 0))) x[j] = y;
+      }
+      buffer = buffer == sh.mass ? sh.mass + SORTED : sh.mass;
+    }
+    merge_in_wave<32>(x[0], t, size);
+    if (two) merge_in_wave<32>(x[1], t + NT, size);
+  }
+  buffer[t] = x[0];
+  if (two) buffer[t + NT] = x[1];
+  __syncthreads();
+  return buffer;
+}
+
 // The limit among n candidates (key << 32 | index): all elements of the order up to the limit, with a k, or all of the bin that it falls in, without; `want` is then
 // what is wanted of their sum.  mine: the thread's of the first SORTED; values: room for all of them in LDS.
 __device__ Limit candidate_limit(Shared& sh, const u64 (&mine)[2], const u64* cand, int n, float* values, const Settings& set, const Weights& weight, const Bins& bins, u64 want, int bin) {
-  if (n <= SORTED) {      // put in order: a bitonic sort in LDS
-    int N = 2;
-    while (N < n) N *= 2;
-    for (int j = 0; j < 2; ++j) {
-      const int i = threadIdx.x + j * NT;
-      if (i < N) sh.mass[i] = i < n ? mine[j] ^ 0xffffffffu : 0;      // descends in the order; none: last
-    }
-    __syncthreads();
-    for (int size = 2; size <= N; size *= 2)
-      for (int stride = size / 2; stride > 0; stride /= 2) {
-        const int i = 2 * threadIdx.x - (threadIdx.x & (stride - 1));
-        if (threadIdx.x < N / 2) {
-          const u64 x = sh.mass[i], y = sh.mass[i + stride];
-          if ((x < y) == ((i & size) == 0)) { sh.mass[i] = y; sh.mass[i + stride] = x; }
-        }
-        // up to a stride of 64 a wave stays in its 128 places
-        if (max(stride, stride > 1 ? stride / 2 : size) > 64) __syncthreads(); else asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      }
-    __syncthreads();
-    const int i0 = 2 * threadIdx.x, k = set.k > 0 ? min(set.k, n) : n;      // a thread: places i0 and i0 + 1
-    unsigned key[2];
-    for (int i = 0; i < 2; ++i) key[i] = i0 + i < n ? (unsigned)(sh.mass[i0 + i] >> 32) : 0;
+  if (n <= SORTED) {
+    u64 x[2];      // places threadIdx.x and NT + threadIdx.x; descends in the order, none: last
+    for (int j = 0; j < 2; ++j) x[j] = (int)threadIdx.x + j * NT < n ? mine[j] ^ 0xffffffffu : 0;
+    const u64* sorted = put_in_order(sh, x, n);
+    const bool two = n > NT;
+    const int k = set.k > 0 ? min(set.k, n) : n;
     int keep = k;
     if (set.p < 1) {
-      u64 m[2], mass;
-      for (int i = 0; i < 2; ++i) m[i] = i0 + i < k ? fixed(weight(value_of(key[i]))) : 0;
-      mass = m[0] + m[1];
+      u64 m[2] = {0, 0}, mass[2], all = 0;
       unsigned none = 0;
-      const u64 all = block_scan(sh, none, mass).mass, target = set.k > 0 ? share_of(set.p, all) : want;
+      for (int j = 0; j < 2; ++j) {
+        if (j == 1 && !two) break;
+        if ((int)threadIdx.x + j * NT < k) m[j] = fixed(weight(value_of((unsigned)(x[j] >> 32))));
+        mass[j] = m[j];
+        const u64 sum = block_scan(sh, none, mass[j]).mass;
+        mass[j] += all;
+        all += sum;
+      }
+      const u64 target = set.k > 0 ? share_of(set.p, all) : want;
       if (threadIdx.x == 0) sh.found = k;
       __syncthreads();
-      mass -= m[0] + m[1];
-      for (int i = 0; i < 2; ++i) {
-        if (i0 + i < k && mass < target && mass + m[i] >= target) sh.found = i0 + i + 1;
-        mass += m[i];
-      }
+      for (int j = 0; j < 2; ++j)
+        if ((j == 0 || two) && mass[j] - m[j] < target && mass[j] >= target) sh.found = threadIdx.x + j * NT + 1;      // (with m 0: no place)
       __syncthreads();
       keep = sh.found;
     }
-    const unsigned last = (unsigned)(sh.mass[keep - 1] >> 32);
-    unsigned ties = (i0 < keep && key[0] == last) + (i0 + 1 < keep && key[1] == last);
-    u64 none = 0;
-    return Limit{last, block_scan(sh, ties, none).count};
+    const unsigned last = (unsigned)(sorted[keep - 1] >> 32);
+    for (int j = 0; j < 2; ++j) {      // the first of the last one's equals
+      const int i = threadIdx.x + j * NT;
+      if (i < n && (unsigned)(x[j] >> 32) == last && (i == 0 || (unsigned)(sorted[i - 1] >> 32) != last)) sh.before_count = i;
+    }
+    __syncthreads();
+    return Limit{last, keep - sh.before_count};
   }
 #pragma unroll 4
   for (int i = threadIdx.x; i < n; i += NT) values[i] = value_of((unsigned)(get(cand + i) >> 32));      // (each thread reads its own)
@@ -426,37 +474,61 @@ __device__ Limit candidate_limit(Shared& sh, const u64 (&mine)[2], const u64* ca
 
 // The token: sh.seg_mass and sh.seg_ties hold, by segments, the kept sums above limit.key and the number of its equals.
 template <typename T> __device__ void draw(Shared& sh, const Args& a, int b, float u, const Row<T>& row, const Settings& set, const Weights& weight, Limit limit) {
-  const int segs = row.segs(), s = threadIdx.x;
+  constexpr int EACH = (MAX_SEGS + 63) / 64;      // segments of a lane: each wave looks for the token's by itself, without a barrier
+  const int segs = row.segs(), l = threadIdx.x & 63;
   const double tie_weight = limit.key ? weight(value_of(limit.key)) : 0.0;
   const u64 tie_mass = tie_weight < set.min_p ? 0 : fixed(tie_weight);
-  const unsigned own_ties = s < segs ? sh.seg_ties[s] : 0;
-  unsigned ties = own_ties, none = 0;
-  u64 mass = 0;
-  block_scan(sh, ties, mass);
-  const unsigned before = ties - own_ties;
-  const u64 own = s < segs ? sh.seg_mass[s] + tie_mass * (before >= limit.ties ? 0u : min(own_ties, limit.ties - before)) : 0;
-  mass = own;
-  const u64 total = block_scan(sh, none, mass).mass;
+  unsigned own_ties[EACH], ties = 0, lane_ties = 0;
+  u64 own[EACH], mass = 0, lane_mass = 0;
+  for (int i = 0; i < EACH; ++i) {
+    const int s = l * EACH + i;
+    own_ties[i] = s < segs ? sh.seg_ties[s] : 0;
+    own[i] = s < segs ? sh.seg_mass[s] : 0;
+    lane_ties += own_ties[i];
+  }
+  ties = wave_scan(lane_ties) - lane_ties;      // before the lane's, then before the segment found
+  for (int i = 0; i < EACH; ++i) {
+    own[i] += tie_mass * (ties >= limit.ties ? 0u : min(own_ties[i], limit.ties - ties));
+    ties += own_ties[i];
+    lane_mass += own[i];
+  }
+  ties -= lane_ties;
+  mass = wave_scan(lane_mass);
+  const u64 total = lane(mass, 63);
+  mass -= lane_mass;
   const double want = (double)u * (double)total;
   const u64 target = want > 0 ? (want < (double)total ? min((u64)want, total - 1) : total - 1) : 0;      // the first running sum above it
-  if (mass - own <= target && target < mass) { sh.found = s; sh.before_mass = mass - own; sh.before_count = before; }
-  __syncthreads();
-  const int seg = sh.found;
-  const u64 before_mass = sh.before_mass;
-  const unsigned before_ties = sh.before_count;
+  const bool here = mass <= target && target < mass + lane_mass;
+  int at = 0;
+  unsigned in_segment = 0;
+  bool passed = false;
+  for (int i = 0; i < EACH; ++i) {
+    if (passed) continue;
+    passed = target < mass + own[i];
+    if (passed) { at = l * EACH + i; in_segment = own_ties[i]; }
+    else { mass += own[i]; ties += own_ties[i]; }
+  }
+  const int src = __builtin_ctzll(__ballot(here));
+  const int seg = __builtin_amdgcn_readlane(at, src);
+  const u64 before_mass = lane(mass, src);
+  const unsigned before_ties = __builtin_amdgcn_readlane(ties, src);
+  const bool all_ties = before_ties + (unsigned)__builtin_amdgcn_readlane(in_segment, src) <= limit.ties;
   float x[8];
   row.load(seg, x);
-  unsigned t = 0;
-  for (int i = 0; i < 8; ++i) t += key_of(x[i]) == limit.key;
-  const unsigned own_t = t;
-  mass = 0;
-  block_scan(sh, t, mass);
-  unsigned seen = before_ties + t - own_t;
+  unsigned seen = before_ties, none = 0;
+  if (!all_ties) {
+    unsigned t = 0;
+    for (int i = 0; i < 8; ++i) t += key_of(x[i]) == limit.key;
+    seen -= t;
+    u64 no_mass = 0;
+    block_scan(sh, t, no_mass);
+    seen += t;
+  }
   u64 e[8], sum = 0;
   for (int i = 0; i < 8; ++i) {
     const unsigned key = key_of(x[i]);
     e[i] = 0;
-    if (key == limit.key) { if (seen++ < limit.ties) e[i] = tie_mass; }
+    if (key == limit.key) { if (all_ties || seen++ < limit.ties) e[i] = tie_mass; }
     else if (key > limit.key) { const double y = weight(x[i]); if (!(y < set.min_p)) e[i] = fixed(y); }
     sum += e[i];
   }
