@@ -279,6 +279,11 @@ __device__ __forceinline__ u64 share_of(float p, u64 total) {      // the least 
   return m > 0 ? m : 1;
 }
 
+__device__ __forceinline__ u64 share_of_draw(float u, u64 total) {      // the token's is the first running sum above it
+  const double want = (double)u * (double)total;
+  return want > 0 ? (want < (double)total ? min((u64)want, total - 1) : total - 1) : 0;
+}
+
 struct Setting { const float* rows; float all; __device__ float operator()(int b) const { return rows ? rows[b] : all; } };
 struct Args {
   const void* logits;
@@ -390,9 +395,10 @@ template <int S> __device__ __forceinline__ void merge_in_wave(u64& x, int i, in
   if ((y > x) == (((i & S) == 0) == ((i & size) == 0))) x = y;
   if constexpr (S > 1) merge_in_wave<S / 2>(x, i, size);
 }
-template <int SIZE> __device__ __forceinline__ void sort_in_wave(u64& x, int i) {
-  if constexpr (SIZE > 2) sort_in_wave<SIZE / 2>(x, i);
-  merge_in_wave<SIZE / 2>(x, i, SIZE);
+// The n numbers of a wave, those of lanes from n on being 0, in descending order where i & the number of lanes is 0.
+template <int SIZE> __device__ __forceinline__ void sort_in_wave(u64& x, int i, int n = 64) {
+  if constexpr (SIZE > 2) sort_in_wave<SIZE / 2>(x, i, n);
+  if (n > SIZE / 2) merge_in_wave<SIZE / 2>(x, i, SIZE);
 }
 // Puts up to SORTED numbers in descending order, x[j] being place threadIdx.x + j * NT; also where the result points to, in LDS.  A bitonic sort in registers: strides below
 // 64 within a wave, 64 to 256 through LDS, two buffers in turn so that a step takes one barrier, 512 within a thread.
@@ -429,9 +435,43 @@ __device__ const u64* put_in_order(Shared& sh, u64 (&x)[2], int n) {
   return buffer;
 }
 
+// Up to 64 candidates (key << 32 | index; what is wanted of them as in candidate_limit), a lane each, by a wave without a barrier: x in order, the weight, its multiple of
+// 2^-43, and how many are kept before min-p.
+struct Few { u64 x, m; double w; int keep; };
+__device__ __forceinline__ Few order_few(u64 candidate, int n, const Settings& set, const Weights& weight, u64 want) {
+  const int l = threadIdx.x & 63, k = set.k > 0 ? min(set.k, n) : n;
+  Few r{l < n ? candidate ^ 0xffffffffu : 0, 0, 0, k};
+  sort_in_wave<64>(r.x, l, n);
+  if (l < k) r.w = weight(value_of((unsigned)(r.x >> 32)));
+  r.m = fixed(r.w);
+  if (set.p < 1) {
+    const u64 sum = wave_scan(r.m), target = set.k > 0 ? share_of(set.p, lane(sum, 63)) : want;
+    const u64 here = __ballot(sum - r.m < target && sum >= target);
+    if (here) r.keep = __builtin_ctzll(here) + 1;
+  }
+  return r;
+}
+// With a k, everything that may be kept is a candidate: the token of a row with up to 64 of them, by the first wave.  Index (below 2^20) and sum (up to 2^43) of a candidate are one
+// number, which puts them in the order of the vocabulary.
+__device__ __forceinline__ void draw_few(long* out, int shift, float u, u64 candidate, int n, const Settings& set, const Weights& weight) {
+  constexpr u64 MASS = ((u64)1 << 44) - 1;
+  if (threadIdx.x >= 64) return;
+  const int l = threadIdx.x;
+  const Few c = order_few(candidate, n, set, weight, 0);
+  u64 y = l < c.keep && !(c.w < set.min_p) && c.m > 0 ? (c.x & 0xfffff) << 44 | c.m : 0;      // (x has the index inverted)
+  sort_in_wave<64>(y, l, n);
+  const u64 m = y & MASS, sum = wave_scan(m), total = lane(sum, 63), target = share_of_draw(u, total);
+  if (sum - m <= target && target < sum) *out = (long)(~(unsigned)(y >> 44) & 0xfffff) - shift;
+}
+
 // The limit among n candidates (key << 32 | index): all elements of the order up to the limit, with a k, or all of the bin that it falls in, without; `want` is then
-// what is wanted of their sum.  mine: the thread's of the first SORTED; values: room for all of them in LDS.
-__device__ Limit candidate_limit(Shared& sh, const u64 (&mine)[2], const u64* cand, int n, float* values, const Settings& set, const Weights& weight, const Bins& bins, u64 want, int bin) {
+// what is wanted of their sum.  first: the lane's of the first 64; mine: the thread's of the first SORTED; values: room for all of them in LDS.
+__device__ Limit candidate_limit(Shared& sh, u64 first, const u64 (&mine)[2], const u64* cand, int n, float* values, const Settings& set, const Weights& weight, const Bins& bins, u64 want, int bin) {
+  if (n <= 64) {      // each wave by itself
+    const Few c = order_few(first, n, set, weight, want);
+    const unsigned key = (unsigned)(c.x >> 32), last = (unsigned)__builtin_amdgcn_readlane((int)key, c.keep - 1);
+    return Limit{last, (unsigned)__builtin_popcountll(__ballot((int)(threadIdx.x & 63) < c.keep && key == last))};
+  }
   if (n <= SORTED) {
     u64 x[2];      // places threadIdx.x and NT + threadIdx.x; descends in the order, none: last
     for (int j = 0; j < 2; ++j) x[j] = (int)threadIdx.x + j * NT < n ? mine[j] ^ 0xffffffffu : 0;
@@ -496,8 +536,7 @@ template <typename T> __device__ void draw(Shared& sh, const Args& a, int b, flo
   mass = wave_scan(lane_mass);
   const u64 total = lane(mass, 63);
   mass -= lane_mass;
-  const double want = (double)u * (double)total;
-  const u64 target = want > 0 ? (want < (double)total ? min((u64)want, total - 1) : total - 1) : 0;      // the first running sum above it
+  const u64 target = share_of_draw(u, total);
   const bool here = mass <= target && target < mass + lane_mass;
   int at = 0;
   unsigned in_segment = 0;
@@ -682,11 +721,16 @@ template <typename T> __global__ __launch_bounds__(NT) void k_sample_draw(Args a
   if (!last_of_row(sh, work)) return;
   const int segs = row.segs();
   const u64 seg_mass = threadIdx.x < segs ? get(work.seg_mass + threadIdx.x) : 0, mine[2] = {get(work.candidates + threadIdx.x), get(work.candidates + NT + threadIdx.x)};      // (some of it unset: how many there are comes with it)
+  const u64 first_few = get(work.candidates + l);
   const unsigned n = few ? get(work.n) : up_to_k;
+  if (set.k > 0 && n <= 64) {
+    draw_few(a.out + b, row.shift, u, first_few, (int)n, set, weight);
+    return;
+  }
   Limit limit;
   if (n <= ROOM) {
     if (threadIdx.x < segs) { sh.seg_mass[threadIdx.x] = seg_mass; sh.seg_ties[threadIdx.x] = 0; }
-    limit = candidate_limit(sh, mine, work.candidates, (int)n, values, set, weight, bins, want, f);
+    limit = candidate_limit(sh, first_few, mine, work.candidates, (int)n, values, set, weight, bins, want, f);
     __syncthreads();
     const auto keep = [&](u64 c) {
       const unsigned key = (unsigned)(c >> 32);
@@ -726,7 +770,7 @@ template <typename T> __global__ __launch_bounds__(NT) void k_sample_short(Args 
   __shared__ u64 cand[SEG];
   __shared__ float values[SEG];
   __shared__ int n;
-  const int b = blockIdx.y;
+  const int b = blockIdx.y, l = threadIdx.x & 63;
   const Row<T> row(static_cast<const T*>(a.logits) + b * a.stride, a.V);
   const Settings set(a, b);
   const float u = a.u[b];      // (fetched with the first loads)
@@ -755,8 +799,12 @@ template <typename T> __global__ __launch_bounds__(NT) void k_sample_short(Args 
       if (set.k > 0 ? bin <= f : bin == f) cand[atomicAdd(&n, 1)] = (u64)key_of(x[i]) << 32 | (unsigned)row.index(0, i);
     }
     __syncthreads();
+    if (set.k > 0 && n <= 64) {
+      draw_few(a.out + b, row.shift, u, cand[l], n, set, weight);
+      return;
+    }
     const u64 mine[2] = {cand[threadIdx.x], cand[NT + threadIdx.x]};
-    limit = candidate_limit(sh, mine, cand, n, values, set, weight, bins, want, f);
+    limit = candidate_limit(sh, cand[l], mine, cand, n, values, set, weight, bins, want, f);
   }
   unsigned ties = 0;
   u64 mass = kept_mass(x, weight, set, limit.key, ties);

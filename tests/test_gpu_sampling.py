@@ -175,3 +175,28 @@ def test_sums_that_fill_the_bins_and_more_candidates_than_there_is_room_for():
         u = torch.tensor([0.3, 0.95])
         for s in (dict(top_p=0.5), dict(top_k=V // 2), dict(top_k=V - 3, top_p=0.9), dict(top_p=0.7, min_p=0.99), dict(top_k=700, top_p=0.3)):
             for dtype in TYPES: check(x.to(dtype), u, sample(x.to(dtype).cuda(), u.cuda(), **s), **s)
+
+
+@pytest.mark.parametrize("kind", ["model", "few values", "flat"])
+@pytest.mark.parametrize("k", [1, 2, 3, 31, 32, 33, 63, 64, 65, 127, 128, 129, 255, 256, 257, 511, 512, 513, 1000, 1024, 1025, 2048, 8192, 8193])
+def test_as_many_candidates_as_are_put_in_order_at_a_time(k, kind):
+    """A wave's, a block's and two for each thread; rows of one segment and of several; equal numbers on both sides of the limit."""
+    from gaac_amd import sample
+    require_gpu()
+    for V in (4000, 9001):
+        for i, s in enumerate((dict(top_k=k), dict(top_k=k, top_p=0.8, temperature=3.0), dict(top_k=k, top_p=0.97, min_p=0.05, temperature=1.5))):
+            x, u = logits(3, V, torch.float32, 7 * k + i, kind)
+            check(x, u, sample(x.cuda(), u.cuda(), **s), **s)
+
+
+def test_every_token_of_a_short_list_comes():
+    """Random numbers all along a row's running sum: of lists of up to 64 and of more, at the ends of the vocabulary as well."""
+    from gaac_amd import sample
+    require_gpu()
+    for V, k in ((4000, 40), (20000, 64), (20000, 90), (1048560, 64)):
+        x = torch.full((1, V), -math.inf)
+        at = torch.cat([torch.tensor([0, 1, V - 2, V - 1]), torch.randperm(V - 4, generator=torch.Generator().manual_seed(k))[:k + 20] + 2])
+        x[0, at] = torch.randn(len(at), generator=torch.Generator().manual_seed(V)) * 0.5
+        u = (torch.arange(97) + 0.5) / 97
+        rows, s = x.cuda().expand(97, V), dict(top_k=k)
+        check(x.expand(97, V), u, sample(rows, u.cuda(), **s), **s)
