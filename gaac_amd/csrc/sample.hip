@@ -81,41 +81,39 @@ template <typename T> struct Row {
   }
 };
 
-// exp(y), y <= 0: y = n ln 2 / 64 + r, 2^(n / 64) from a table of the 64 roots in LDS and the exponent, times the series of exp to r^5 (|r| <= 0.0055: what is left
-// is below 1e-16).  15 operations in 64 bits; the series to r^11 without a table took 24 (64 mixed rows of 128256: 68 us, with the table 61.6).
-constexpr int ROOTS = 64;
-__device__ __forceinline__ void fill_roots(double* table) {      // by the first wave; 2^(j / 64) = exp(j ln 2 / 64) by its series
+// exp(y), y <= 0, from z = y * 256 / ln 2: the whole part n of z by a table of the 256 roots of 2 in LDS and the exponent, times the series of exp to r^4 of the rest,
+// r = (z - n) ln 2 / 256 (|r| <= 0.0014: what is left is below 1e-16).  z's own rounding is one of 2^-53 of y, and below -31 all is less than half of 2^-43.
+constexpr int ROOTS = 256;
+constexpr double LN2 = 0.6931471805599453, STEP = LN2 / ROOTS;
+__device__ __forceinline__ void fill_roots(double* table) {      // 2^(j / 256) = exp(j ln 2 / 256) by its series
   if (threadIdx.x < ROOTS) {
-    const double x = threadIdx.x * (0.6931471805599453 / ROOTS);
+    const double x = threadIdx.x * STEP;
     double e = 1;
 #pragma unroll
     for (int k = 17; k > 0; --k) e = __builtin_fma(e, x * (1.0 / k), 1.0);
     table[threadIdx.x] = e;
   }
 }
-__device__ __forceinline__ double exp64(double y, const double* table) {
-  if (!(y > -31.0)) return 0.0;
-  const double n = __builtin_rint(y * 92.33248261689366);
-  const double r = __builtin_fma(n, -2.8447437476627285e-11, __builtin_fma(n, -0.010830424667801708, y));
+__device__ __forceinline__ double exp_of(double z, const double* table) {
+  z = __builtin_fmax(z, -31.0 / STEP);      // (also where it is NaN)
+  const double n = __builtin_rint(z), f = z - n;
   const int i = (int)n;
-  double q = __builtin_fma(r, 1.0 / 120, 1.0 / 24);
-  q = __builtin_fma(q, r, 1.0 / 6);
-  q = __builtin_fma(q, r, 0.5);
-  q = __builtin_fma(q, r, 1.0);
-  const double t = table[i & (ROOTS - 1)];
-  return __builtin_bit_cast(double, __builtin_bit_cast(u64, __builtin_fma(t * q, r, t)) + ((u64)(long long)(i >> 6) << 52));
+  double q = __builtin_fma(f, STEP * STEP * STEP * STEP / 24, STEP * STEP * STEP / 6);
+  q = __builtin_fma(q, f, STEP * STEP / 2);
+  q = __builtin_fma(q, f, STEP);
+  const double t = table[i & (ROOTS - 1)], e = __builtin_fma(t * q, f, t);
+  const u64 bits = __builtin_bit_cast(u64, e);
+  return __builtin_bit_cast(double, (u64)((unsigned)(bits >> 32) + ((unsigned)(i & -ROOTS) << 12)) << 32 | (unsigned)bits);      // + i / 256 in the exponent
 }
 // As a multiple of 2^-43: the sum with 2^9, whose last bit that is, rounds to it.
 __device__ __forceinline__ u64 fixed(double w) { return __builtin_bit_cast(u64, w + 512.0) - __builtin_bit_cast(u64, 512.0); }
 
 struct Weights {      // of a row
   float top;
-  double inv_t;
+  double scale;      // 1 / (T STEP)
   const double* roots;
-  __device__ __forceinline__ double operator()(float x) const {
-    if (x == top) return 1.0;
-    return x == -__builtin_inff() ? 0.0 : exp64(((double)x - (double)top) * inv_t, roots);
-  }
+  __device__ __forceinline__ Weights(float top_, float t, const double* r) : top(top_), scale(1.0 / (double)t * (1.0 / STEP)), roots(r) {}
+  __device__ __forceinline__ double operator()(float x) const { return x == top ? 1.0 : exp_of(((double)x - (double)top) * scale, roots); }      // (-inf: less than half of 2^-43)
 };
 
 // Inclusive sums over the wave in the vector unit: shifts within rows of 16 lanes, then the last lane of a row to the next ones.
@@ -624,9 +622,11 @@ template <typename T> __global__ __launch_bounds__(NT) void k_sample_max(Args a)
 
 __device__ __forceinline__ void add_to_bins(Shared& sh, const Settings& set, const Weights& weight, const Bins& bins, const float (&x)[8]) {
   for (int i = 0; i < 8; ++i) {
-    if (x[i] == -__builtin_inff()) continue;
     const int bin = bins(x[i]);
-    if (set.k > 0) { atomicAdd(&sh.count[bin], 1u); continue; }
+    if (set.k > 0) {
+      if (x[i] != -__builtin_inff()) atomicAdd(&sh.count[bin], 1u);
+      continue;
+    }
     const u64 m = fixed(weight(x[i]));
     if (m) atomicAdd(&sh.mass[bin], m);
   }
@@ -650,7 +650,7 @@ template <typename T> __global__ __launch_bounds__(NT) void k_sample_bins(Args a
   fill_roots(sh.roots);
   const u64 best = block_best(sh, threadIdx.x < a.segs ? work.best[threadIdx.x] : 0);
   if (easy(a, b, row, set, best, blockIdx.x == 0)) return;
-  const Weights weight{value_of((unsigned)(best >> 32)), 1.0 / (double)set.t, sh.roots};
+  const Weights weight(value_of((unsigned)(best >> 32)), set.t, sh.roots);
   if (set.cut()) {
     const Bins bins(weight.top, set.t);
     clear_bins(sh);
@@ -691,7 +691,7 @@ template <typename T> __global__ __launch_bounds__(NT) void k_sample_draw(Args a
   }
   const u64 best = block_best(sh, threadIdx.x < a.segs ? work.best[threadIdx.x] : 0);
   if (easy(a, b, row, set, best, false)) return;
-  const Weights weight{value_of((unsigned)(best >> 32)), 1.0 / (double)set.t, sh.roots};
+  const Weights weight(value_of((unsigned)(best >> 32)), set.t, sh.roots);
   const Bins bins(weight.top, set.t);
   unsigned up_to_k;
   const u64 want = find_cut(sh, set, counts, masses, up_to_k);
@@ -780,7 +780,7 @@ template <typename T> __global__ __launch_bounds__(NT) void k_sample_short(Args 
   if (threadIdx.x == 0) n = 0;
   const u64 best = block_best(sh, segment_best(row, 0, x));
   if (easy(a, b, row, set, best, true)) return;
-  const Weights weight{value_of((unsigned)(best >> 32)), 1.0 / (double)set.t, sh.roots};
+  const Weights weight(value_of((unsigned)(best >> 32)), set.t, sh.roots);
   Limit limit{0, 0};
   if (set.cut()) {
     const Bins bins(weight.top, set.t);
