@@ -6,13 +6,13 @@
 // Which token comes is a whole number, so a sum that is off in its last bits is an error: weights are computed in 64 bits and held as multiples of 2^-43
 // in 64-bit integers (2^20 of them fit), whose sums are exact in any order.
 // What is kept is a prefix of the order, so it is found as a key (the bits of x, in order) and the number of its equals that are kept: counts and sums by bins
-// of (max - x), then the elements of the bin where the limit falls, in order: up to 1024 of them sorted in LDS, up to 8192 by ever finer bins of their keys, more by
-// such bins over the row.  Three launches: the row's maximum; bins; and the limits, the sums of segments and the token by the last of the row's blocks to
+// of (max - x), then the elements of the bin where the limit falls (with a k: all up to it), in order: up to 64 of them sorted by a wave, up to 1024 by the block, up to 8192
+// by ever finer bins of their keys, more by such bins over the row.  Three launches: the row's maximum; bins; and the limits, the sums of segments and the token by the last of the row's blocks to
 // arrive.  A row of one segment takes one launch, bins and candidates in LDS.
 //
-// What bounds it: for few rows the chain of launches and of dependent steps in the last block (4 rows of 128256 in bf16, 1 MB: 22.6 us; kernels 4.2, 4.5 and 15.8,
+// What bounds it: for few rows the chain of launches and of dependent steps in the last block (4 rows of 128256 in bf16, 1 MB, top-k 50: 16.6 us; kernels 3.0, 4.9 and 9.7,
 // launch 1.6 of each); for many the weights in 64 bits, computed twice for each element that can be kept, and atomic additions to bins (64
-// mixed rows of 128256 in fp32, 33 MB: 61.6 us; kernels 8.2, 20.7 and 34.6; the read alone 5.5).
+// mixed rows of 128256 in fp32, 33 MB: 52.3 us; kernels 7.0, 17.2 and 28.2; the read alone 5.5).
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include "gaac_capi.h"
@@ -83,6 +83,7 @@ template <typename T> struct Row {
 
 // exp(y), y <= 0, from z = y * 256 / ln 2: the whole part n of z by a table of the 256 roots of 2 in LDS and the exponent, times the series of exp to r^4 of the rest,
 // r = (z - n) ln 2 / 256 (|r| <= 0.0014: what is left is below 1e-16).  z's own rounding is one of 2^-53 of y, and below -31 all is less than half of 2^-43.
+// (64 roots, a series to r^5 and r in two steps: 64 mixed rows of 128256 56.3 us, so 52.3; the series to r^11 without a table some 7 more.)
 constexpr int ROOTS = 256;
 constexpr double LN2 = 0.6931471805599453, STEP = LN2 / ROOTS;
 __device__ __forceinline__ void fill_roots(double* table) {      // 2^(j / 256) = exp(j ln 2 / 256) by its series
@@ -399,7 +400,8 @@ template <int SIZE> __device__ __forceinline__ void sort_in_wave(u64& x, int i, 
   if (n > SIZE / 2) merge_in_wave<SIZE / 2>(x, i, SIZE);
 }
 // Puts up to SORTED numbers in descending order, x[j] being place threadIdx.x + j * NT; also where the result points to, in LDS.  A bitonic sort in registers: strides below
-// 64 within a wave, 64 to 256 through LDS, two buffers in turn so that a step takes one barrier, 512 within a thread.
+// 64 within a wave, 64 to 256 through LDS, two buffers in turn so that a step takes one barrier, 512 within a thread (53
+// numbers 2.0 us and 335 4.0, with all steps through LDS 4.3 and 7.5).
 __device__ const u64* put_in_order(Shared& sh, u64 (&x)[2], int n) {
   const int t = threadIdx.x;
   const bool two = n > NT;
@@ -450,7 +452,7 @@ __device__ __forceinline__ Few order_few(u64 candidate, int n, const Settings& s
   return r;
 }
 // With a k, everything that may be kept is a candidate: the token of a row with up to 64 of them, by the first wave.  Index (below 2^20) and sum (up to 2^43) of a candidate are one
-// number, which puts them in the order of the vocabulary.
+// number, which puts them in the order of the vocabulary (4 rows of 128256, k 50: 16.6 us; by the sums of segments and a second look at the token's 19.3).
 __device__ __forceinline__ void draw_few(long* out, int shift, float u, u64 candidate, int n, const Settings& set, const Weights& weight) {
   constexpr u64 MASS = ((u64)1 << 44) - 1;
   if (threadIdx.x >= 64) return;
@@ -822,7 +824,7 @@ template <typename T> int launch(Args a, int B, bool cut, hipStream_t stream) {
   const int rows = a.segs == 1 ? SHORT_ROWS : ROWS;
   for (int b = 0; b < B; b += rows) {
     const int n = min(B - b, rows);
-    // two blocks a CU: each starts with the row's maxima or bins, which costs as much as several segments (64 rows of 128256 by top-p: 48.5 us, 57.8 with 256 blocks, 54.1 with 1024)
+    // two blocks a CU: each starts with the row's maxima or bins, which costs as much as several segments (64 rows of 128256 by top-p: 42.2 us, 51.1 with 256 blocks, 48.2 with 1024)
     const dim3 grid(min(a.segs, max(BLOCKS / n, 1)), n);
     if (a.segs == 1) {
       k_sample_short<T><<<grid, NT, 0, stream>>>(a);
