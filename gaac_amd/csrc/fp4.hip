@@ -18,7 +18,7 @@
 
 namespace {
 
-constexpr int NW = 8;      // waves of an attention block: two blocks on a CU
+constexpr int NW = 8;      // waves of an attention block: two blocks on a CU (and dwords of a lane's part of a query)
 constexpr int DIM = 128, TT = 32, TILE = 4352, V_AT = 2048, KS_AT = 4096, VS_AT = 4224;
 
 typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
@@ -231,6 +231,8 @@ __device__ __forceinline__ void empty_row(const int* slots, int n_slots, int row
   for (int i = threadIdx.x; i < G * DIM; i += 64 * NW) out[((long)row * n_kv + kvh) * G * DIM + i] = slots[row] >= n_slots ? 0x7fc0 : 0;
 }
 
+__device__ __forceinline__ float bits(unsigned x) { return __builtin_bit_cast(float, x); }
+
 struct Tile { u4 k[2], v[2]; unsigned ks; u2 vs; };
 
 __device__ __forceinline__ Tile load_tile(const uint8_t* t, unsigned l) {
@@ -249,33 +251,44 @@ __device__ __forceinline__ Tile load_tile(const uint8_t* t, unsigned l) {
 // and 64 + 16 g .. of head n (the operand's order); hi_exp and lo_exp are exponent bytes, 255 (NaN) where q is not finite.
 struct Query { i8 hi, lo; unsigned hi_exp, lo_exp; };
 
-__device__ __forceinline__ Query load_query(const uint16_t* q, bool there, int g, bool negative) {
-  u4 x[4];
+// The maximum needs all of a head's channels, the conversion of the lane's eight dwords is shared out over the block's eight waves, one each (`halves`: in LDS; one barrier): by each wave
+// for itself it took more instructions than two tiles (1000 tokens x 8 heads 7.3 us, so 6.5; 32 rows of 300..6000 24.1, 23.2; 65536 x 8 18.0,
+// 17.2).
+struct RawQuery { u4 x[4]; u2 own; };
+__device__ __forceinline__ RawQuery load_query(const uint16_t* q, bool there, int g, int w) {
+  RawQuery r;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) x[i] = there ? *reinterpret_cast<const u4*>(q + 64 * (i >> 1) + 16 * g + 8 * (i & 1)) : u4{0, 0, 0, 0};
+  for (int i = 0; i < 4; ++i) r.x[i] = there ? *reinterpret_cast<const u4*>(q + 64 * (i >> 1) + 16 * g + 8 * (i & 1)) : u4{0, 0, 0, 0};
+  r.own = there ? *reinterpret_cast<const u2*>(q + 64 * (w >> 2) + 16 * g + 4 * (w & 3)) : u2{0, 0};
+  return r;
+}
+__device__ __forceinline__ Query convert_query(const RawQuery& raw, int w, bool negative, u2 (*halves)[64]) {
+  const int l = threadIdx.x & 63;
+  const u4 (&x)[4] = raw.x;
+  const u2 own = raw.own;
   unsigned a = pk_max(pk_max(unit_max(x[0]), unit_max(x[1])), pk_max(unit_max(x[2]), unit_max(x[3])));
   a = pk_max(a, __shfl_xor(a, 16));
   a = pk_max(a, __shfl_xor(a, 32));
   a = max(a & 0xffffu, a >> 16);
   const unsigned e = (unsigned)max((int)(a >> 7) - 7, 5);
-  const float down = __builtin_bit_cast(float, (254 - e) << 23) * (negative ? -1.f : 1.f);      // +-2^-E
+  const float down = bits((254 - e) << 23) * (negative ? -1.f : 1.f);      // +-2^-E
+  int hi = 0, lo = 0;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const float a0 = bits(own[k] << 16) * down, a1 = bits(own[k] & 0xffff0000u) * down;
+    const int h = __builtin_amdgcn_cvt_pk_fp8_f32(a0, a1, 0, false);
+    const float l0 = (a0 - __builtin_amdgcn_cvt_f32_fp8(h, 0)) * 16.f, l1 = (a1 - __builtin_amdgcn_cvt_f32_fp8(h, 1)) * 16.f;
+    const int o = __builtin_amdgcn_cvt_pk_fp8_f32(l0, l1, 0, false);
+    hi |= (h & 0xffff) << 16 * k; lo |= (o & 0xffff) << 16 * k;
+  }
+  halves[w][l] = u2{(unsigned)hi, (unsigned)lo};
+  __syncthreads();
   Query r;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      int hi = 0, lo = 0;
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const unsigned w = x[i][2 * j + k];
-        const float a0 = __builtin_bit_cast(float, w << 16) * down, a1 = __builtin_bit_cast(float, w & 0xffff0000u) * down;
-        const int h = __builtin_amdgcn_cvt_pk_fp8_f32(a0, a1, 0, false);
-        const float l0 = (a0 - __builtin_amdgcn_cvt_f32_fp8(h, 0)) * 16.f, l1 = (a1 - __builtin_amdgcn_cvt_f32_fp8(h, 1)) * 16.f;
-        const int o = __builtin_amdgcn_cvt_pk_fp8_f32(l0, l1, 0, false);
-        hi |= (h & 0xffff) << 16 * k; lo |= (o & 0xffff) << 16 * k;
-      }
-      r.hi[2 * i + j] = hi; r.lo[2 * i + j] = lo;
-    }
+  for (int c = 0; c < 8; ++c) {
+    const u2 v = halves[c][l];
+    r.hi[c] = (int)v[0]; r.lo[c] = (int)v[1];
+  }
   r.hi_exp = a >= 0x7f80u ? 255 : e; r.lo_exp = a >= 0x7f80u ? 255 : e - 4;
   return r;
 }
@@ -360,7 +373,6 @@ typedef unsigned long long u64;
 template <typename T> __device__ __forceinline__ void put(T* p, T v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 template <typename T> __device__ __forceinline__ T get(const T* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 __device__ __forceinline__ void stores_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
-__device__ __forceinline__ float bits(unsigned x) { return __builtin_bit_cast(float, x); }
 __device__ __forceinline__ float lane(float x, int i) { return bits(__builtin_amdgcn_readlane(__builtin_bit_cast(int, x), i)); }
 
 constexpr int LINE = 32;      // tickets are a cache line apart: all blocks draw theirs at about the same time
@@ -410,10 +422,10 @@ __device__ void merge(const float* part, long acc_at, int p0, int count, int n_k
 }
 
 // Decode attention.  Bound by the read of the cache where rows are long: 16 rows of 4096..65536 tokens x 8 heads 101 us, 606 MB, 6.0 TB/s, the rate of a plain read of
-// that size being 6.1; by the launch, the plan and the merge where the cache is short: 1 row of 65536 x 8 heads, 18.1 us, has its 71 MB by 15.4 (2.6 of
-// them launch and plan: 5.6 TB/s for the rest), leaves the partials until 16.9 and adds them up in 2.3.  A wave has whole tiles, so what it needs comes in 6 loads of whole lines
-// and no lane waits for another; one tile is in flight while another is worked on: 16 waves a CU, 68 KB of loads in flight on each.  Four waves a SIMD
-// need 128 registers at most: it has 123.
+// that size being 6.1; by the launch, the plan and the merge where the cache is short: 1 row of 65536 x 8 heads, 17.2 us, has its 71 MB after about 14 (2 to 2.6 of
+// them launch and plan), leaves the partials within 1.5 and adds them up in 2.3; by instructions on few CUs (a tile a SIMD 0.35 us).  A wave has whole tiles, so what it needs comes in 6 loads
+// of whole lines and no lane waits for another; one tile is in flight while another is worked on: 16 waves a CU, 68 KB of loads in flight on each.  Two tiles in
+// flight by 8 waves a CU take the same 101 us there, but 1 us more on shorter rows, whose first tiles wait for the second ones.  Four waves a SIMD need 128 registers at most: it has 124.
 // One block = eight waves = one split of one (row, kv head).  One split a row (P == B): the output is written here; otherwise a row with several splits leaves
 // partials, and the block that draws the last of the (row, kv head)'s tickets adds them up and puts the tickets back (tickets NULL: k_fp4_merge does it).
 __global__ __launch_bounds__(64 * NW, 4) void k_fp4_attn(const uint8_t* cache, const int* lens, const int* slots, int n_slots, int tiles, int cap, const uint16_t* q, int B, int n_kv, int G,
@@ -440,8 +452,11 @@ __global__ __launch_bounds__(64 * NW, 4) void k_fp4_attn(const uint8_t* cache, c
   // one tile in flight while another is worked on; behind the end the last one is read again and left alone
   const auto tile = [&](int t) { return load_tile(base + (long)min(t, end - 1) * TILE, l); };
   int t = first + w;
+  const RawQuery raw = load_query(q + q0 + n * DIM, n < G, g, w);
+  asm volatile("" ::: "memory");      // (the query first: the tile is still on its way while it is converted)
   Tile x = tile(t);
-  const Query qr = load_query(q + q0 + n * DIM, n < G, g, scale < 0);
+  __shared__ u2 halves[NW][64];
+  const Query qr = convert_query(raw, w, scale < 0, halves);
   const float scale2 = fabsf(scale) * 1.44269504f;
   Running r;
   r.max2 = -__builtin_inff(); r.sum = 0;
@@ -554,7 +569,7 @@ int gaac_fp4_attn(const uint8_t* cache, const int* lens, const int* slots, int n
   GAAC_REQUIRE(aligned16(q) && aligned16(cache), "gaac_fp4_attn: q must be 16-byte aligned");
   const int G = n_q / n_kv, P = B * nsplit;
   const int lds = 4 * (NW * G * OROW + 2 * NW * 16);
-  if (lds > 64 * 1024) {
+  if (lds > 60 * 1024) {      // (with the 4 KB that the kernel has by itself more than the 64 that need no asking)
     const hipError_t e = hipFuncSetAttribute((const void*)k_fp4_attn, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     if (e != hipSuccess) { gaac::fail("gaac_fp4_attn: %s", hipGetErrorString(e)); return (int)e; }
   }

@@ -166,7 +166,7 @@ def test_lengths_that_a_caller_set_wrongly():
 
 
 # ---------------------------------------------------------------------------------------------------- attention
-HEADS = [(8, 4), (4, 6), (1, 16), (16, 1), (2, 5), (3, 13)]
+HEADS = [(8, 4), (4, 6), (1, 16), (16, 1), (2, 5), (3, 13), (1, 14), (1, 15)]
 
 
 @pytest.mark.parametrize("n_kv,G", HEADS)
