@@ -26,17 +26,22 @@ CAPTURES = 64                   # captured calls of attention that get counters 
 
 
 @functools.lru_cache(maxsize=1024)
-def choose_nsplit(B: int, n_kv: int, S: int) -> int:
-    """Splits for each of B rows, S tokens in the longest, which the launch then shares out by length (csrc/fp4.hip).  Measured, 8 kv heads, 4 query heads each, us:
-      * up to 1500 tokens none (1000 tokens: 7.3, against 8.0 with 8 splits and 9.1 with 32; 1500: 8.4, with 16 the same);
-      * one block per CU (64K tokens: 18.3 with 32 splits, 20.7 with 16, 21.6 with 64; 8 rows of 7000..8192: 17.7 with 4, 21.6 with 2, 19.0 with 8; 16 rows of
-        4096..65536: 101 with 2, 185 with 1), of at least 128 tokens (2000: 8.6 with 16, 9.2 with 32; 16000: 10.6 with 32);
-      * heads that fill half of the chip by themselves: none, since a split's start and merge cost more than even shares save (32 rows of 300..6000: 24.4, against
-        26.8 with 2; 24 of 2000..16000: 52.6 and 52.6; 64 of 2000..16000: 107 and 114), but not where a single row may take as long as all (from 32768 tokens)."""
+def choose_nsplit(B: int, n_kv: int, S: int, G: int = 4) -> int:
+    """Splits for each of B rows, S tokens in the longest, G query heads a kv head, which the launch then shares out by length (csrc/fp4.hip).  Measured, 8 kv heads and G 4 unless noted, us:
+      * up to 1500 tokens none (1000 tokens: 6.5, against 7.2 with 8 splits; 1500: 7.5, with 16 the same);
+      * heads that fill half of the chip by themselves: none, since a split's start and merge cost more than even shares save (32 rows of 300..6000: 23.1, against
+        25.7 with 2; 24 of 2000..16000: 52.6 and 52.6; 64 of 2000..16000: 107 and 114), but not where a single row may take as long as all (from 32768 tokens);
+      * otherwise one block per CU (8 rows of 7000..8192: 16.9 with 4, 20.8 with 2, 18.2 with 8), two for long rows, whose tiles are worth more loads in flight (16 rows of 4096..65536: 101.9
+        with 4, 109 with 2; 8 of 32768: 48.9 with 8, 47.7 with 4);
+      * but of few heads no more splits than their merge by one block is worth: 16 (16384 tokens: 9.9, with 32 10.8; 4096: 8.1 and 9.8), from 24576 tokens 32 (65536: 17.5, with 16 19.4; 32768 x
+        1: 10.5, with 16 12.5, with 256 23; G 16 18, 18 and 71), and for G up to 4 64 from 65536 (131072 x 1: 16.1, with 32 18.5), 128 from 262144 (20.5, with 64 21.0; 10^6 x 1: 36.5,
+        with 64 52, with 256 41), for more heads to merge from four times these lengths (G 16, 131072 x 1: 26, with 64 29; 262144: 34, with 32 37; 10^6: 62, with 64 65)."""
     H = B * n_kv
     if S <= 1500: return 1
-    if H <= 128: return max(1, min(256 // H, S // 128))
-    return 1 if S < 32768 else 2
+    if H > 128: return 1 if S < 32768 else 2
+    s = S if G <= 4 else S // 4
+    few = 16 if S < 24576 else 32 if s < 65536 else 64 if s < 262144 else 128 if s < 1 << 21 else 256
+    return max(1, min((512 if H * S >= 1 << 22 else 256) // H, S // 128, few))
 
 
 def _rows(x: torch.Tensor) -> torch.Tensor:
@@ -119,10 +124,11 @@ class FP4KVCache:
     def attention(self, q: torch.Tensor, slots: torch.Tensor, scale: float, max_len: int | None = None, nsplit: int | None = None) -> torch.Tensor:
         """Decode-step read: bf16 [B, n_q, D] queries, row b over everything slot slots[b] holds; returns bf16 [B, n_q, D].  A row whose slot is -1 or empty is 0, one
         whose slot does not exist NaN.  max_len, the longest row if the caller knows it, only picks the split count when nsplit is not given."""
-        if nsplit is None: nsplit = choose_nsplit(max(len(q), 1), self.n_kv, min(int(max_len), self.cap) if max_len else self.cap)
+        shape = q.shape
+        if nsplit is None: nsplit = choose_nsplit(shape[0] or 1, self.n_kv, min(int(max_len), self.cap) if max_len else self.cap, shape[1] // self.n_kv) if len(shape) == 3 else 1
         if nsplit == 1: out = (_lib._calls or _lib.calls()).fp4_attend(self, q, slots, scale, 1, None, _lib.stream)
         elif nsplit > 1 and q.device == self.data.device and q.device.index == torch._C._cuda_getDevice():
-            out = (_lib._calls or _lib.calls()).fp4_attend(self, q, slots, scale, nsplit, self._counters(len(q) * self.n_kv), _lib.stream)
+            out = (_lib._calls or _lib.calls()).fp4_attend(self, q, slots, scale, nsplit, self._counters(shape[0] * self.n_kv if shape else 0), _lib.stream)
         else: out = None
         if out is not None: return out
         if q.dtype != torch.bfloat16 or q.dim() != 3 or q.shape[2] != D: raise RuntimeError(f"attention expects q bf16 [B, n_q, {D}], got {q.dtype} {list(q.shape)}")

@@ -11,7 +11,8 @@ BF = torch.bfloat16
 
 def test_sizes_of_the_cache():
     assert FP4KVCache.bytes_per_slot(8, 65536) == 8 * 2048 * 4352 + 4 and FP4KVCache.bytes_per_slot(1, 1) == 4352 + 4
-    assert [choose_nsplit(*x) for x in ((1, 8, 65536), (1, 8, 100), (1, 8, 2000), (16, 8, 65536), (32, 8, 6000), (300, 8, 65536), (1, 1, 10 ** 6))] == [32, 1, 15, 2, 1, 2, 256]
+    assert [choose_nsplit(*x) for x in ((1, 8, 65536), (1, 8, 100), (1, 8, 2000), (16, 8, 65536), (32, 8, 6000), (300, 8, 65536), (1, 1, 10 ** 6))] == [32, 1, 15, 4, 1, 2, 128]
+    assert [choose_nsplit(1, 1, S, G) for S in (8192, 32768, 131072, 10 ** 6) for G in (1, 4, 16)] == [16, 16, 16, 32, 32, 32, 64, 64, 32, 128, 128, 64]
     for bad in ((0, 8, 64), (1, 0, 64), (1, 8, 0)):
         with pytest.raises(RuntimeError, match="at least 1"): FP4KVCache(*bad, device="cpu")
 
