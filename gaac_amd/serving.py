@@ -308,7 +308,8 @@ class DecodeRunner:
     def start_decode(self, first_tokens: torch.Tensor, use_graph: bool = True, nsplit: int | None = None, sampling: dict | None = None):
         """first_tokens int64 [B]: the token each of slots 0..B-1 decodes next.  With use_graph the step (all layers, cache appends,
         attention, sampling, feeding the token back) is captured once and replayed.  sampling: arguments of sample() (temperature, top_k, top_p, min_p; numbers
-        or tensors [B]), decode() then takes the random numbers; None: the likeliest token."""
+        or tensors [B]), decode() then takes the random numbers; None: the likeliest token.  A row whose logits are all NaN or -inf has no token to draw: decode() returns
+        -1 for it, and the row goes on with token 0."""
         B, dev = first_tokens.shape[0], first_tokens.device
         self.B = B
         self.tok = first_tokens.clone()
@@ -316,7 +317,7 @@ class DecodeRunner:
         self.dlens = self.lens[:B].clone()
         self.nsplit = nsplit or (None if self.kv == "fp4" else choose_nsplit(B, self.cfg.n_kv_heads, self.cfg.max_len))      # (the 4-bit cache chooses by itself)
         self.sampling, self.u = sampling, torch.zeros(B, dtype=torch.float32, device=dev)
-        self.logits = None
+        self.logits = self.chosen = None
         self.graph = None
         if not use_graph: return
         side = torch.cuda.Stream(); side.wait_stream(torch.cuda.current_stream())
@@ -338,7 +339,12 @@ class DecodeRunner:
 
     def _one(self):
         self.logits = self._step(self.tok, self.slots, self.dlens, self.nsplit)
-        self.tok.copy_(self.logits.argmax(-1) if self.sampling is None else sample(self.logits, self.u, **self.sampling))
+        if self.sampling is None:
+            self.tok.copy_(self.logits.argmax(-1))
+            self.chosen = self.tok
+        else:
+            self.chosen = sample(self.logits, self.u, **self.sampling)
+            torch.clamp(self.chosen, min=0, out=self.tok)      # -1, a row without a token: the next step reads the embedding of token 0, not what lies before the table
 
     @torch.no_grad()
     def decode(self, n_steps: int, forced: torch.Tensor | None = None, keep_logits: bool = False, u: torch.Tensor | None = None):
@@ -352,7 +358,7 @@ class DecodeRunner:
             if u is not None: self.u.copy_(u[i])
             if self.graph is not None: self.graph.replay()
             else: self._one()
-            out.append(self.tok.clone())
+            out.append(self.chosen.clone())
             if keep_logits: logits.append(self.logits.float().clone())
             if forced is not None: self.tok.copy_(forced[i])
             self.steps += 1
