@@ -269,9 +269,10 @@ class DecodeRunner:
     # ---------------------------------------------------------------- prefill
     @torch.no_grad()
     def prefill(self, slot: int, tokens: torch.Tensor) -> torch.Tensor:
-        """tokens int64 [L] on the device: causal attention over the prompt's own K/V per layer, then the K/V go into `slot`.
+        """tokens int64 [L] on the device, up to cfg.max_len: causal attention over the prompt's own K/V per layer, then the K/V go into `slot`.
         Returns the logits of the last position [vocab] (fp32)."""
         cfg, L = self.cfg, tokens.shape[0]
+        if L > cfg.max_len: raise RuntimeError(f"prompt has {L} tokens, the model's positions end at {cfg.max_len}")
         pos = torch.arange(L, device=tokens.device)
         x = self.w.embed.index_select(0, tokens)
         cu = torch.tensor([0, L], dtype=torch.int32, device=tokens.device)
@@ -315,6 +316,7 @@ class DecodeRunner:
         self.tok = first_tokens.clone()
         self.slots = torch.arange(B, dtype=torch.int32, device=dev)
         self.dlens = self.lens[:B].clone()
+        self.longest = max(self.dlens.tolist(), default=0)      # tokens of the longest row, known to the host
         self.nsplit = nsplit or (None if self.kv == "fp4" else choose_nsplit(B, self.cfg.n_kv_heads, self.cfg.max_len))      # (the 4-bit cache chooses by itself)
         self.sampling, self.u = sampling, torch.zeros(B, dtype=torch.float32, device=dev)
         self.logits = self.chosen = None
@@ -350,11 +352,16 @@ class DecodeRunner:
     def decode(self, n_steps: int, forced: torch.Tensor | None = None, keep_logits: bool = False, u: torch.Tensor | None = None):
         """Runs n_steps steps (with sampling: u fp32 [n_steps, B] in [0, 1), a random number for every token); returns the generated tokens [n_steps, B] (device).  forced int64 [n_steps, B]: teacher forcing: the
         token every row consumes at step i+1 is forced[i] instead of the one it generated (the returned tokens are still the model's
-        own choices).  keep_logits: also returns the logits of every step [n_steps, B, vocab] (fp32)."""
+        own choices).  keep_logits: also returns the logits of every step [n_steps, B, vocab] (fp32).  Refused where a row would come to hold more than cfg.max_len
+        tokens: there is no position for them, and no room."""
         if (u is None) != (self.sampling is None) or u is not None and tuple(u.shape) != (n_steps, self.B):
             raise RuntimeError(f"decode expects u fp32 [{n_steps}, {self.B}] where start_decode was given sampling, and nothing otherwise")
+        if self.longest + n_steps > self.cfg.max_len:
+            self.longest = max(self.dlens.tolist(), default=0)      # (the caller may have taken tokens back)
+            if self.longest + n_steps > self.cfg.max_len: raise RuntimeError(f"decode of {n_steps} steps: the longest row holds {self.longest} tokens, the model's positions end at {self.cfg.max_len}")
         out, logits = [], []
         for i in range(n_steps):
+            self.longest += 1
             if u is not None: self.u.copy_(u[i])
             if self.graph is not None: self.graph.replay()
             else: self._one()

@@ -1,4 +1,4 @@
-"""The decode loop at its limits: rows without a token."""
+"""The decode loop at its limits: rows without a token, rows that are full."""
 import pytest
 import torch
 
@@ -30,3 +30,20 @@ def test_rows_without_a_token(kv, use_graph):
     w.final_norm.fill_(1.0)
     out = run.decode(4, u=torch.full((4, 3), 0.5, device="cuda"))
     assert ((out >= 0) & (out < cfg.vocab)).all() and torch.equal(out[-1], run.tok)
+
+
+@pytest.mark.parametrize("kv", ["fp4", "gaac", "bf16"])
+@pytest.mark.parametrize("use_graph", [False, True])
+def test_rows_up_to_the_last_position(kv, use_graph):
+    """max_len is no whole number of tiles: the last steps that fit are finite, one more is refused and leaves everything as it was."""
+    cfg, w, run, first = setup(kv, max_len=75, lens=(70, 37, 64))
+    settings = dict(temperature=0.8, top_k=20)
+    run.start_decode(first, use_graph=use_graph, sampling=settings)
+    u = torch.full((6, 3), 0.5, device="cuda")
+    with pytest.raises(RuntimeError, match="the longest row holds 70 tokens, the model's positions end at 75"): run.decode(6, u=u)
+    out, logits = run.decode(5, keep_logits=True, u=u[:5])
+    assert (out >= 0).all() and logits.isfinite().all() and run.lens.tolist() == [75, 42, 69]
+    with pytest.raises(RuntimeError, match="holds 75 tokens"): run.decode(1, u=u[:1])
+    assert run.lens.tolist() == [75, 42, 69]
+    if kv != "bf16":
+        for c in run.caches: assert c.decompress(0)[0].shape[0] == 75

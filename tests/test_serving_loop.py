@@ -39,3 +39,21 @@ def test_likeliest_and_forced_tokens_are_fed_as_they_are(monkeypatch):
     assert run.decode(2).tolist() == [[9, 4], [9, 4]] and [t.tolist() for t in given] == [[5, 6], [9, 4]]
     assert run.decode(2, forced=torch.tensor([[1, 2], [3, 8]])).tolist() == [[9, 4], [9, 4]] and [t.tolist() for t in given[2:]] == [[9, 4], [1, 2]]
     assert run.tok.tolist() == [3, 8]
+
+
+def test_rows_do_not_grow_past_the_models_positions(monkeypatch):
+    """Refused before anything runs: a step behind the last position would be one of NaN, over tokens that the caches left out."""
+    run, given = runner(monkeypatch, torch.zeros(2, CFG.vocab))
+    run.lens.copy_(torch.tensor([10, 60]))
+    run.start_decode(torch.tensor([5, 6]), use_graph=False)
+    with pytest.raises(RuntimeError, match="decode of 5 steps: the longest row holds 60 tokens, the model's positions end at 64"): run.decode(5)
+    assert not given and run.lens.tolist() == [10, 60]
+    run.decode(3)
+    with pytest.raises(RuntimeError, match="holds 63 tokens"): run.decode(2)
+    run.decode(1)
+    assert run.lens.tolist() == [14, 64] and len(given) == 4
+    with pytest.raises(RuntimeError, match="holds 64 tokens"): run.decode(1)
+    run.dlens.copy_(torch.tensor([14, 20]))      # tokens taken back
+    run.decode(40)
+    assert run.lens.tolist() == [54, 60]
+    with pytest.raises(RuntimeError, match="prompt has 65 tokens"): run.prefill(0, torch.zeros(65, dtype=torch.int64))
