@@ -194,6 +194,15 @@ class Weights:
         return 2 * (n + sum(t.numel() for l in self.layers for t in l.values()))
 
 
+def _norm_rope_host(x: torch.Tensor, weight: torch.Tensor | None, cos: torch.Tensor, sin: torch.Tensor, eps: float) -> torch.Tensor:
+    """qk_norm_rope's definition for one of its tensors on the host, where a prompt into an uncompressed cache needs no kernel: x [N, heads, D]; cos, sin [N, D/2]."""
+    y = x.float()
+    if weight is not None: y = y * torch.rsqrt(y.square().mean(-1, keepdim=True) + eps) * weight.float()
+    y1, y2 = y[..., :D // 2], y[..., D // 2:]
+    c, s = cos[:, None, :], sin[:, None, :]
+    return torch.cat([y1 * c - y2 * s, y2 * c + y1 * s], -1).to(x.dtype)
+
+
 class _Bf16Cache:
     """Uncompressed cache of one layer: K/V [n_slots*n_kv, cap, D] bf16; batch row b of a decode step uses slot b."""
     def __init__(self, n_slots: int, n_kv: int, cap: int, device):
@@ -257,7 +266,10 @@ class DecodeRunner:
         h = F.rms_norm(x, (cfg.hidden,), layer["norm1"], cfg.rms_eps)
         qkv = F.linear(h, layer["qkv"]).view(x.shape[0], cfg.n_heads + 2 * cfg.n_kv_heads, D)
         q, k, v = qkv[:, :cfg.n_heads], qkv[:, cfg.n_heads:cfg.n_heads + cfg.n_kv_heads], qkv[:, cfg.n_heads + cfg.n_kv_heads:]
-        q, k = qk_norm_rope(q, k, pos, self.w.cos, self.w.sin, layer.get("q_norm"), layer.get("k_norm"), cfg.rms_eps)
+        if x.is_cuda: q, k = qk_norm_rope(q, k, pos, self.w.cos, self.w.sin, layer.get("q_norm"), layer.get("k_norm"), cfg.rms_eps)
+        else:
+            cos, sin = self.w.cos.index_select(0, pos), self.w.sin.index_select(0, pos)
+            q, k = _norm_rope_host(q, layer.get("q_norm"), cos, sin, cfg.rms_eps), _norm_rope_host(k, layer.get("k_norm"), cos, sin, cfg.rms_eps)
         return q, k, v if self.kv == "fp4" else v.contiguous()      # (the 4-bit cache reads v where the projection left it)
 
     def _mlp(self, layer, x):

@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+import operators_ref as R
 from gaac_amd import serving
 from gaac_amd.serving import DecodeRunner, ModelConfig, Weights
 
@@ -57,3 +58,25 @@ def test_rows_do_not_grow_past_the_models_positions(monkeypatch):
     run.decode(40)
     assert run.lens.tolist() == [54, 60]
     with pytest.raises(RuntimeError, match="prompt has 65 tokens"): run.prefill(0, torch.zeros(65, dtype=torch.int64))
+
+
+@pytest.mark.parametrize("qk_norm", [False, True])
+def test_a_prompt_on_the_host(qk_norm):
+    """prefill() into an uncompressed cache takes no kernel and runs on the CPU: queries and keys by their definition, keys and values into the cache."""
+    cfg = ModelConfig(hidden=128, n_layers=2, n_heads=4, n_kv_heads=2, ffn=128, vocab=50, max_len=64, qk_norm=qk_norm)
+    w = Weights(cfg, "cpu", seed=3)
+    if qk_norm:
+        g = torch.Generator().manual_seed(4)
+        for l in w.layers: l.update(q_norm=(torch.rand(128, generator=g) + 0.5).to(torch.bfloat16), k_norm=(torch.rand(128, generator=g) + 0.5).to(torch.bfloat16))
+    run = DecodeRunner(w, n_slots=2, kv="bf16")
+    seen = []
+    for attn in run.attn: attn.register_forward_hook(lambda m, args, out: seen.append(args))
+    tokens = torch.randint(0, cfg.vocab, (37,), generator=torch.Generator().manual_seed(5))
+    assert run.prefill(1, tokens).isfinite().all() and run.lens.tolist() == [0, 37]
+    x = torch.nn.functional.rms_norm(w.embed.index_select(0, tokens), (cfg.hidden,), w.layers[0]["norm1"], cfg.rms_eps)
+    qkv = torch.nn.functional.linear(x, w.layers[0]["qkv"]).view(37, -1, 128)
+    for got, heads, name in ((seen[0][0], qkv[:, :4], "q_norm"), (seen[0][1], qkv[:, 4:6], "k_norm")):
+        ref, tol = R.norm_rope(heads, w.layers[0].get(name), w.cos[:37], w.sin[:37], False, cfg.rms_eps)
+        assert got.dtype == torch.bfloat16 and ((got.double() - ref).abs() <= tol).all()
+    for layer, (q, k, v) in enumerate(seen):
+        assert torch.equal(run.caches[layer].k[2:4, :37].transpose(0, 1), k) and torch.equal(run.caches[layer].v[2:4, :37].transpose(0, 1), v)
