@@ -10,9 +10,11 @@ Slot s owns cache heads [s*n_kv, (s+1)*n_kv); a head is a row of tiles of 32 tok
 append and attention take the batch's slot map and the slots' lengths from device memory and never return to the host, so a decode step can be captured in a
 HIP graph.  Calls on one cache must be ordered on one stream where one of them writes; attention may run on several streams at
 once, and in several graphs: its scratch is the call's own, and the counters by which the splits of a row find the last of them are one set for each stream and one
-for each captured call (CAPTURES of them; calls captured after these, or of more rows than the cache has slots, take a launch more instead)."""
+for each captured call.  A call that is not captured makes its stream's set, and sees to it that READY sets lie ready for captured calls of as many rows; a captured call that finds
+none, or after CAPTURES of them, takes a launch more instead.  128 bytes a row and kv head of a call, beside its partials: scratch of the calls, not of the slots."""
 from __future__ import annotations
 import functools
+import threading
 import torch
 from . import _lib
 from .codec import D
@@ -23,6 +25,9 @@ ROW_BYTES = D // 2 + D // 32    # bytes of a token and head of K or of V: codes 
 TILE_BYTES = 2 * T * ROW_BYTES
 LINE = 32                       # words from one counter of attention to the next
 CAPTURES = 64                   # captured calls of attention that get counters of their own
+READY = 16                      # sets of counters that calls outside of captures keep ready for calls inside, which cannot make any
+
+_LOCK = threading.Lock()        # over the sets that lie ready
 
 
 @functools.lru_cache(maxsize=1024)
@@ -69,24 +74,50 @@ class FP4KVCache:
         self.lens = torch.zeros(n_slots, dtype=torch.int32, device=device)          # tokens per slot
         # set by append instead of writing: bit 0 = a slot was full, bit 1 = a slot twice in a batch, bit 2 = no such slot
         self.overflow = torch.zeros(1, dtype=torch.int32, device=device)
-        self._tickets = {}      # stream -> counters, zero between launches
-        self._spare = torch.zeros(CAPTURES, self.H * LINE, dtype=torch.int32, device=device)      # of captured calls: one row each
-        self._captured = 0
+        self._no_counters()
+
+    def _no_counters(self):
+        self._tickets = {}                                           # stream -> counters, zero between launches
+        self._ready, self._ready_words, self._given = [], 0, []      # the same for captured calls: sets that lie ready and their size, sets that a captured call has
+
+    def __getstate__(self):      # counters belong to streams and graphs of this process
+        return {k: v for k, v in self.__dict__.items() if k not in ("_tickets", "_ready", "_ready_words", "_given")}
+
+    def __setstate__(self, state):
+        self.__dict__.update({k: v for k, v in state.items() if k not in ("_tickets", "_spare", "_captured")})      # (what caches saved earlier hold)
+        self._no_counters()
+
+    @property
+    def _captured(self) -> int:
+        return len(self._given)
 
     def _counters(self, n: int) -> torch.Tensor | None:
         """Counters of an attention launch, n of them: launches on one stream are in order and share theirs; a captured call may be replayed beside any other."""
+        words = n * LINE
         if torch._C._cuda_isCurrentStreamCapturing():
-            if n > self.H or self._captured == CAPTURES: return None
-            self._captured += 1
-            return self._spare[self._captured - 1]
+            with _LOCK:
+                if not self._ready or words > self._ready_words: return None
+                self._given.append(self._ready.pop())
+                return self._given[-1]
         stream = _lib.stream()
         have = self._tickets.get(stream)
-        if have is None or have.numel() < n * LINE: have = self._tickets[stream] = torch.zeros(max(n, self.H) * LINE, dtype=torch.int32, device=self.data.device)
+        if have is None or have.numel() < words: have = self._tickets[stream] = torch.zeros(words, dtype=torch.int32, device=self.data.device)
+        if words > self._ready_words or len(self._ready) < READY: self._make_ready(words)
         return have
+
+    def _make_ready(self, words: int):
+        with _LOCK:
+            if words > self._ready_words: self._ready, self._ready_words = [], words
+            missing = min(READY, CAPTURES - len(self._given)) - len(self._ready)
+            if missing < 1: return
+            side = torch.cuda.Stream(self.data.device)      # zero before this call returns, whatever the current stream still has to do: a graph may run on any
+            with torch.cuda.stream(side): made = torch.zeros(missing, self._ready_words, dtype=torch.int32, device=self.data.device)
+            side.synchronize()
+            self._ready.extend(made.unbind(0))
 
     @staticmethod
     def bytes_per_slot(n_kv: int, capacity: int) -> int:
-        """Device bytes one slot occupies: its tiles and its length."""
+        """Device bytes one slot occupies: its tiles and its length, which is all that a cache holds for its slots."""
         return n_kv * -(-capacity // T) * TILE_BYTES + 4
 
     def _check(self, what: str, k: torch.Tensor, v: torch.Tensor):

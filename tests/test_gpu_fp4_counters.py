@@ -1,0 +1,87 @@
+"""Counters of attention over the 4-bit cache: what they take, and captured calls that find some or none."""
+import pytest
+import torch
+
+from gpu_util import require_gpu
+
+pytestmark = pytest.mark.gpu
+D = 128
+
+
+def setup(lens=(600, 33, 257), n_kv=2, G=4, cap=600):
+    from gaac_amd import FP4KVCache
+    require_gpu()
+    c = FP4KVCache(len(lens), n_kv, cap)
+    g = torch.Generator().manual_seed(1)
+    for i, L in enumerate(lens): c.prefill(i, *(torch.randn(L, n_kv, D, generator=g).to(torch.bfloat16).cuda() for _ in range(2)))
+    q = torch.randn(len(lens), n_kv * G, D, generator=g).to(torch.bfloat16).cuda()
+    return c, q, torch.arange(len(lens), dtype=torch.int32, device="cuda")
+
+
+def capture(f):
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g): out = f()
+    return g, out
+
+
+def replayed(g, out, want):
+    for _ in range(3):
+        out.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+
+
+def test_counters_are_of_the_calls_and_not_of_the_slots():
+    """A cache of many slots that small batches attend over keeps counters for these batches."""
+    from gaac_amd import FP4KVCache
+    require_gpu()
+    c = FP4KVCache(200, 8, 64)
+    q, slots = torch.ones(2, 32, D, dtype=torch.bfloat16, device="cuda"), torch.tensor([7, 150], dtype=torch.int32, device="cuda")
+    for _ in range(3): c.attention(q, slots, 0.1, nsplit=2)
+    held = sum(t.untyped_storage().nbytes() for t in c._tickets.values()) + sum({t.untyped_storage().data_ptr(): t.untyped_storage().nbytes() for t in c._ready}.values())
+    assert held <= (1 + 16) * 2 * 8 * 128 and c._captured == 0
+    c.attention(q, slots, 0.1)
+    assert FP4KVCache(2, 2, 64).attention(q[:, :4], slots - 150, 0.1).shape == (2, 4, D)      # no splits: none
+
+
+def test_a_call_captured_before_any_other():
+    """No call outside of a capture has made counters: the splits are added up by a launch of their own."""
+    c, q, slots = setup()
+    g, out = capture(lambda: c.attention(q, slots, D ** -0.5, nsplit=4))
+    assert c._captured == 0
+    replayed(g, out, c.attention(q, slots, D ** -0.5, nsplit=4))
+
+
+def test_captured_calls_of_more_rows_and_of_fewer():
+    """Counters grow with the rows of the calls outside; captured calls that have some keep theirs."""
+    c, q, slots = setup()
+    one = (q[:1].contiguous(), slots[:1].contiguous())
+    want = c.attention(*one, D ** -0.5, nsplit=4)
+    graphs = [(*capture(lambda: c.attention(*one, D ** -0.5, nsplit=4)), want)]
+    all_rows = lambda: c.attention(q, slots, D ** -0.5, nsplit=4)
+    g, out = capture(all_rows)      # more rows than any call before
+    assert c._captured == 1
+    want = all_rows()
+    graphs += [(g, out, want), (*capture(all_rows), want)]
+    assert c._captured == 2
+    for _ in range(3):
+        for x in graphs: replayed(*x)
+        assert torch.equal(all_rows(), want)
+
+
+def test_a_busy_stream_does_not_keep_a_graph_from_its_counters():
+    """Counters made by a call on a stream that has much to do are zero for a graph on another stream at once."""
+    c, q, slots = setup()
+    call = lambda: c.attention(q, slots, D ** -0.5, nsplit=4)
+    want = call()
+    c._no_counters()
+    torch.cuda.synchronize()
+    busy = torch.cuda.Stream()
+    with torch.cuda.stream(busy):
+        torch.cuda._sleep(20_000_000)
+        late = call()
+    assert len(c._ready) == 16 and all(int(s.cpu().abs().max()) == 0 for s in c._ready)
+    torch.cuda.synchronize()
+    assert torch.equal(late, want)
+    replayed(*capture(call), want)
