@@ -105,6 +105,12 @@ class FP4KVCache:
         if words > self._ready_words or len(self._ready) < READY: self._make_ready(words)
         return have
 
+    def _unused(self, counters: torch.Tensor | None):
+        """Counters of a captured call that was not made after all."""
+        with _LOCK:
+            for i, s in enumerate(self._given):
+                if s is counters: self._ready.append(self._given.pop(i)); break
+
     def _make_ready(self, words: int):
         with _LOCK:
             if words > self._ready_words: self._ready, self._ready_words = [], words
@@ -157,11 +163,22 @@ class FP4KVCache:
         whose slot does not exist NaN.  max_len, the longest row if the caller knows it, only picks the split count when nsplit is not given."""
         shape = q.shape
         if nsplit is None: nsplit = choose_nsplit(shape[0] or 1, self.n_kv, min(int(max_len), self.cap) if max_len else self.cap, shape[1] // self.n_kv) if len(shape) == 3 else 1
+        tickets = out = None
         if nsplit == 1: out = (_lib._calls or _lib.calls()).fp4_attend(self, q, slots, scale, 1, None, _lib.stream)
-        elif nsplit > 1 and q.device == self.data.device and q.device.index == torch._C._cuda_getDevice():
-            out = (_lib._calls or _lib.calls()).fp4_attend(self, q, slots, scale, nsplit, self._counters(shape[0] * self.n_kv if shape else 0), _lib.stream)
-        else: out = None
+        elif nsplit > 1 and q.is_cuda and q.device == self.data.device and q.device.index == torch._C._cuda_getDevice():
+            tickets = self._counters(shape[0] * self.n_kv if shape else 0)
+            try: out = (_lib._calls or _lib.calls()).fp4_attend(self, q, slots, scale, nsplit, tickets, _lib.stream)
+            except BaseException:
+                self._unused(tickets)
+                raise
         if out is not None: return out
+        try: return self._attention(q, slots, scale, nsplit, tickets)
+        except BaseException:
+            self._unused(tickets)
+            raise
+
+    def _attention(self, q, slots, scale, nsplit, tickets) -> torch.Tensor:
+        """attention, where the binding does not make the call.  tickets: the call's counters, if it has some already."""
         if q.dtype != torch.bfloat16 or q.dim() != 3 or q.shape[2] != D: raise RuntimeError(f"attention expects q bf16 [B, n_q, {D}], got {q.dtype} {list(q.shape)}")
         B, n_q, _ = q.shape
         if n_q % self.n_kv or not 1 <= n_q // self.n_kv <= GMAX: raise RuntimeError(f"GQA group size must be 1..{GMAX}")
@@ -171,7 +188,10 @@ class FP4KVCache:
         with _lib.on_device(self.data, q, slots):
             out = torch.empty(B, n_q, D, dtype=q.dtype, device=q.device)
             if B == 0: return out
-            partials, tickets = (torch.empty(B * nsplit * n_q * (D + 2), dtype=torch.float32, device=q.device), self._counters(B * self.n_kv)) if nsplit > 1 else (None, None)
+            partials = None
+            if nsplit > 1:
+                partials = torch.empty(B * nsplit * n_q * (D + 2), dtype=torch.float32, device=q.device)
+                if tickets is None: tickets = self._counters(B * self.n_kv)
             q = q if q.is_contiguous() and q.data_ptr() % 16 == 0 else q.clone(memory_format=torch.contiguous_format)
             _lib.call("gaac_fp4_attn", self.data, self.lens, slots.contiguous(), self.n_slots, self.tiles, self.cap, q, B, n_q, self.n_kv, float(scale), int(nsplit), partials,
                       tickets, out, _lib.stream)

@@ -40,3 +40,10 @@ def test_saved_caches_have_no_counters():
     old = FP4KVCache.__new__(FP4KVCache)
     old.__setstate__(dict(n_slots=2, n_kv=4, tiles=2, cap=64, H=8, data=c.data, lens=c.lens, overflow=c.overflow, _tickets={0: c.lens}, _spare=torch.ones(64, 256, dtype=torch.int32), _captured=3))
     assert old._tickets == {} and old._captured == 0 and not hasattr(old, "_spare") and old.cap == 64
+
+
+def test_attention_on_the_host_is_refused_by_name_with_splits_too():
+    import pytest
+    c = FP4KVCache(2, 4, 4096, device="cpu")
+    for nsplit in (1, 3):
+        with pytest.raises(RuntimeError, match="no CPU path"): c.attention(torch.zeros(1, 4, 128, dtype=torch.bfloat16), torch.zeros(1, dtype=torch.int32), 1.0, nsplit=nsplit)

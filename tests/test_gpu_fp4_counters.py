@@ -85,3 +85,51 @@ def test_a_busy_stream_does_not_keep_a_graph_from_its_counters():
     torch.cuda.synchronize()
     assert torch.equal(late, want)
     replayed(*capture(call), want)
+
+
+def test_a_captured_call_takes_one_set(monkeypatch):
+    """Also where the binding leaves the call to Python (strided or misaligned queries, slots with gaps, a whole number as scale), and none where it is refused."""
+    from gaac_amd import _lib
+    c, q, slots = setup()
+    x = torch.zeros(3, 16, D, dtype=torch.bfloat16, device="cuda")
+    x[:, ::2] = q
+    odd = torch.zeros(q.numel() + 1, dtype=torch.bfloat16, device="cuda")[1:].view(q.shape)
+    odd.copy_(q)
+    gaps = torch.stack([slots, slots + 5], 1)[:, 0]
+    calls = [lambda: c.attention(q, slots, D ** -0.5, nsplit=4), lambda: c.attention(x[:, ::2], slots, D ** -0.5, nsplit=4), lambda: c.attention(odd, slots, D ** -0.5, nsplit=4),
+             lambda: c.attention(q, gaps, D ** -0.5, nsplit=4), lambda: c.attention(q, slots, 1, nsplit=4)]
+    want = [f() for f in calls]
+    for w in want[1:4]: assert torch.equal(w, want[0])
+    for python in (False, True):
+        if python: monkeypatch.setattr(_lib, "_calls", _lib._CtypesCalls())
+        for f, w in zip(calls, want):
+            before = c._captured
+            g, out = capture(f)
+            assert c._captured == before + 1
+            replayed(g, out, w)
+        before = c._captured
+        def refused():
+            with pytest.raises(RuntimeError, match="GQA group size"): c.attention(q[:, :3], slots, D ** -0.5, nsplit=4)
+            with pytest.raises(RuntimeError, match="slots int32"): c.attention(q, slots[:2], D ** -0.5, nsplit=4)
+            return q.clone()
+        capture(refused)
+        assert c._captured == before and len({s.data_ptr() for s in c._ready + c._given}) == len(c._ready + c._given)
+
+
+def test_threads_that_capture_at_once_get_sets_of_their_own():
+    """The sets are taken one by one: many threads that take counters as captured calls do never hold the same."""
+    import threading
+    c, q, slots = setup()
+    c.attention(q, slots, D ** -0.5, nsplit=4)
+    start, took = threading.Barrier(8), []
+    real = torch._C._cuda_isCurrentStreamCapturing
+    torch._C._cuda_isCurrentStreamCapturing = lambda: True
+    try:
+        def take():
+            start.wait()
+            for _ in range(2): took.append(c._counters(6))
+        threads = [threading.Thread(target=take) for _ in range(8)]
+        for t in threads: t.start()
+        for t in threads: t.join()
+    finally: torch._C._cuda_isCurrentStreamCapturing = real
+    assert len({t.data_ptr() for t in took}) == 16 and c._captured == 16 and c._ready == []
