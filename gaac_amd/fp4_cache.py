@@ -11,8 +11,9 @@ append and attention take the batch's slot map and the slots' lengths from devic
 HIP graph.  Calls on one cache must be ordered on one stream where one of them writes; attention may run on several streams at
 once, and in several graphs: its scratch is the call's own, and the counters by which the splits of a row find the last of them are one set for each stream and one
 for each captured call.  A call that is not captured makes its stream's set, and sees to it that READY sets lie ready for captured calls of as many rows; a captured call that finds
-none, or after CAPTURES of them, takes a launch more instead.  128 bytes a row and kv head of a call, beside its partials: scratch of the calls, not of the slots."""
+none, or after CAPTURES of them, takes a launch more instead; captured_counters and give_back return the sets of graphs that are dropped.  128 bytes a row and kv head of a call, beside its partials: scratch of the calls, not of the slots."""
 from __future__ import annotations
+import contextlib
 import functools
 import threading
 import torch
@@ -79,9 +80,10 @@ class FP4KVCache:
     def _no_counters(self):
         self._tickets = {}                                           # stream -> counters, zero between launches
         self._ready, self._ready_words, self._given = [], 0, []      # the same for captured calls: sets that lie ready and their size, sets that a captured call has
+        self._noted = {}                                             # thread -> the sets that calls inside its captured_counters() have taken
 
     def __getstate__(self):      # counters belong to streams and graphs of this process
-        return {k: v for k, v in self.__dict__.items() if k not in ("_tickets", "_ready", "_ready_words", "_given")}
+        return {k: v for k, v in self.__dict__.items() if k not in ("_tickets", "_ready", "_ready_words", "_given", "_noted")}
 
     def __setstate__(self, state):
         self.__dict__.update({k: v for k, v in state.items() if k not in ("_tickets", "_spare", "_captured")})      # (what caches saved earlier hold)
@@ -97,19 +99,42 @@ class FP4KVCache:
         if torch._C._cuda_isCurrentStreamCapturing():
             with _LOCK:
                 if not self._ready or words > self._ready_words: return None
-                self._given.append(self._ready.pop())
-                return self._given[-1]
+                have = self._ready.pop()
+                self._given.append(have)
+                noted = self._noted.get(threading.get_ident())
+                if noted is not None: noted.append(have)
+                return have
         stream = _lib.stream()
         have = self._tickets.get(stream)
         if have is None or have.numel() < words: have = self._tickets[stream] = torch.zeros(words, dtype=torch.int32, device=self.data.device)
         if words > self._ready_words or len(self._ready) < READY: self._make_ready(words)
         return have
 
+    @contextlib.contextmanager
+    def captured_counters(self):
+        """The sets of counters that attention() takes inside, in a list: for a capture whose graph will be dropped, and give_back then."""
+        me = threading.get_ident()
+        if me in self._noted: raise RuntimeError("captured_counters within captured_counters")
+        self._noted[me] = taken = []
+        try: yield taken
+        finally: del self._noted[me]
+
+    def give_back(self, counters: list):
+        """Counters of captured calls whose graph has run for the last time, the GPU being done with it: later captures take them again."""
+        with _LOCK:
+            for c in counters:
+                at = next((i for i, s in enumerate(self._given) if s is c), None)
+                if at is None: raise RuntimeError("give_back expects counters that captured calls of this cache hold")
+                self._given.pop(at)
+                if c.numel() >= self._ready_words: self._ready.append(c)      # (smaller ones are no longer handed out)
+
     def _unused(self, counters: torch.Tensor | None):
         """Counters of a captured call that was not made after all."""
-        with _LOCK:
-            for i, s in enumerate(self._given):
-                if s is counters: self._ready.append(self._given.pop(i)); break
+        with _LOCK: held = any(s is counters for s in self._given)
+        if not held: return
+        self.give_back([counters])
+        noted = self._noted.get(threading.get_ident(), [])
+        noted[:] = [s for s in noted if s is not counters]
 
     def _make_ready(self, words: int):
         with _LOCK:

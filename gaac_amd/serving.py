@@ -18,6 +18,7 @@ library's own BF16 decode kernel; the KV backend of a layer is CompressedKVCache
 (`Attention.fp4`: 4 bits, 3.76 times smaller than BF16, not lossless) or an uncompressed BF16 cache (`Attention.bf16`), the baseline.  A step takes the likeliest
 token or, with start_decode(sampling=...), one drawn by sample() from given random numbers."""
 from __future__ import annotations
+import contextlib
 from dataclasses import dataclass
 import torch
 import torch.nn.functional as F
@@ -258,6 +259,7 @@ class DecodeRunner:
         self.lens = torch.zeros(n_slots, dtype=torch.int32, device=dev)      # tokens held per slot
         self.steps = 0
         self.graph = None
+        self.counters = []      # (cache, counters of its captured calls) of the graph
         self.sampling = None
 
     # ---------------------------------------------------------------- layers
@@ -332,6 +334,10 @@ class DecodeRunner:
         self.nsplit = nsplit or (None if self.kv == "fp4" else choose_nsplit(B, self.cfg.n_kv_heads, self.cfg.max_len))      # (the 4-bit cache chooses by itself)
         self.sampling, self.u = sampling, torch.zeros(B, dtype=torch.float32, device=dev)
         self.logits = self.chosen = None
+        if self.counters:
+            torch.cuda.synchronize()      # the graph that goes has run for the last time
+            for c, counters in self.counters: c.give_back(counters)
+            self.counters = []
         self.graph = None
         if not use_graph: return
         side = torch.cuda.Stream(); side.wait_stream(torch.cuda.current_stream())
@@ -342,8 +348,10 @@ class DecodeRunner:
             self.dlens.copy_(keep); self.tok.copy_(first_tokens)
             torch.cuda.synchronize()
             g = torch.cuda.CUDAGraph()
-            with torch.cuda.graph(g, stream=side):
-                self._one()
+            with contextlib.ExitStack() as stack:
+                self.counters = [(c, stack.enter_context(c.captured_counters())) for c in self.caches if self.kv == "fp4"]
+                with torch.cuda.graph(g, stream=side):
+                    self._one()
             self.dlens.copy_(keep); self.tok.copy_(first_tokens)
         torch.cuda.current_stream().wait_stream(side)
         self.slots.copy_(torch.arange(B, dtype=torch.int32, device=dev))

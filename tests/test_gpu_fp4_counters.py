@@ -133,3 +133,48 @@ def test_threads_that_capture_at_once_get_sets_of_their_own():
         for t in threads: t.join()
     finally: torch._C._cuda_isCurrentStreamCapturing = real
     assert len({t.data_ptr() for t in took}) == 16 and c._captured == 16 and c._ready == []
+
+
+def test_counters_of_dropped_graphs_are_taken_again():
+    from gaac_amd import fp4_cache
+    c, q, slots = setup()
+    call = lambda: c.attention(q, slots, D ** -0.5, nsplit=4)
+    want = call()
+    kept = capture(call)
+    for i in range(fp4_cache.CAPTURES + 10):
+        with c.captured_counters() as counters: g, out = capture(call)
+        assert len(counters) == 1 and c._captured == 2
+        if i % 10 == 0:
+            replayed(g, out, want)
+            replayed(*kept, want)
+        torch.cuda.synchronize()
+        del g, out
+        c.give_back(counters)
+        assert c._captured == 1
+    with pytest.raises(RuntimeError, match="give_back expects counters"): c.give_back(counters)
+    with c.captured_counters() as counters:
+        call()      # not captured: none
+        capture(lambda: [pytest.raises(RuntimeError, c.attention, q, slots[:2], D ** -0.5, nsplit=4), q.clone()][1])      # refused: none
+    assert counters == [] and c._captured == 1
+    many = (q.repeat(4, 1, 1), slots.repeat(4))
+    with c.captured_counters() as counters: capture(call)
+    c.attention(*many, D ** -0.5, nsplit=2)      # larger sets are wanted from here on
+    c.give_back(counters)
+    assert all(s.numel() >= 12 * 2 * 32 for s in c._ready)
+
+
+def test_the_decode_loop_captures_anew_as_often_as_it_likes():
+    from gaac_amd import fp4_cache
+    from gaac_amd.serving import DecodeRunner, ModelConfig, Weights
+    dev = require_gpu()
+    cfg = ModelConfig(hidden=256, n_layers=2, n_heads=8, n_kv_heads=2, ffn=512, vocab=500, rope_theta=10000.0, max_len=2500)
+    run = DecodeRunner(Weights(cfg, dev, seed=1), n_slots=2, kv="fp4")
+    for i in range(2): run.prefill(i, torch.randint(0, cfg.vocab, (1900 + i,), generator=torch.Generator(device=dev).manual_seed(2 + i), device=dev))
+    for i in range(fp4_cache.CAPTURES + 3):
+        run.start_decode(torch.tensor([5, 6], device=dev))
+        assert [c._captured for c in run.caches] == [1, 1]      # with splits, and counters for them
+        if i % 20 == 0: run.decode(2)
+    held = run.lens.tolist()
+    graph = run.decode(3)
+    run.start_decode(torch.tensor([5, 6], device=dev), use_graph=False)
+    assert [c._captured for c in run.caches] == [0, 0] and held[1] == held[0] + 1 and graph.shape == (3, 2)
