@@ -42,6 +42,7 @@ _SIGNATURES = {
     "gaac_static_flags": [P, P],
     "gaac_fp4_store": [P, P] + [c_long] * 4 + [c_int] * 3 + [P] * 3,
     "gaac_fp4_load": [P] + [c_int] * 3 + [P, P] + [c_long] * 4 + [P],
+    "gaac_fp4_length": [P, c_int, P, P],
     "gaac_fp4_append": [P] + [c_int] * 3 + [P, P] + [c_long] * 4 + [P, c_int, c_int, P, P, P],
     "gaac_fp4_attn": [P, P, P, c_int, c_int, c_int, P, c_int, c_int, c_int, c_float, c_int, P, P, P, P],
     "gaac_qk_norm_rope": [c_int, P, P] + [c_long] * 5 + [c_int] * 4 + [P, P, c_long, c_long, c_float, P, c_int, P, P, c_int, c_int, P, P, P],

@@ -101,7 +101,7 @@ PyObject* invoke(const char* name, int (*fn)(A...), PyObject* const* args, Py_ss
   X(gaac_cache_append)                                                                                                                    \
   X(gaac_paged_store) X(gaac_paged_free) X(gaac_paged_release) X(gaac_paged_decode) X(gaac_paged_attn) X(gaac_bf16_attn)                  \
   X(gaac_attn_fused) X(gaac_attn_fused_static) X(gaac_static_init) X(gaac_static_reset) X(gaac_static_flags) X(gaac_attn_launch)    \
-  X(gaac_fp4_store) X(gaac_fp4_load) X(gaac_fp4_append) X(gaac_fp4_attn) X(gaac_qk_norm_rope) X(gaac_sample)
+  X(gaac_fp4_store) X(gaac_fp4_load) X(gaac_fp4_length) X(gaac_fp4_append) X(gaac_fp4_attn) X(gaac_qk_norm_rope) X(gaac_sample)
 #define X(name)                                            \
   decltype(&::name) p_##name = nullptr;                    \
   PyObject* py_##name(PyObject*, PyObject* const* args, Py_ssize_t n) { return invoke(#name, p_##name, args, n); }
@@ -465,7 +465,7 @@ PyObject* fp4_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
     void* stream = stream_of(a[2]);
     at::Tensor word = host_words(1);
     int* len = static_cast<int*>(word.data_ptr());
-    must("gaac_cache_check", without_gil([&] { return p_gaac_cache_check(nullptr, 0, c.lens + slot, nullptr, nullptr, 0, len, stream); }));
+    must("gaac_fp4_length", without_gil([&] { return p_gaac_fp4_length(c.lens + slot, static_cast<int>(c.tiles), len, stream); }));
     must("gaac_wait_words", without_gil([&] { return p_gaac_wait_words(len, 1, stream); }));
     const long L = *len, row = c.n_kv * DIM;
     const at::Tensor& like = tensor(get(a[0], n_data));

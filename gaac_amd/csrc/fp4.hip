@@ -13,6 +13,7 @@
 //   K's exponent byte of token 16 s + m, block g: 4096 + 2 l + s.  V's of token 16 s + 4 g + i, block b: 4224 + 32 b + 8 g + 4 s + i.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
+#include <limits.h>
 #include "gaac_capi.h"
 #include "../../include/gaac_hip.h"
 
@@ -141,6 +142,9 @@ __global__ __launch_bounds__(256) void k_fp4_load(const uint8_t* cache, int L, i
     }
   }
 }
+
+// A slot's length for the host, as the other kernels read it: the word is the caller's to write, and below 0 means "not there yet" to the host's wait.
+__global__ void k_fp4_length(const int* len, int cap, int* host) { __hip_atomic_store(host, max(min(*len, cap), 0), __ATOMIC_RELEASE, __HIP_MEMORY_SCOPE_SYSTEM); }
 
 // ---------------------------------------------------------------------------------------------------- one token
 // A block per batch row, a thread per unit (K or V, head, 8 channels); a block of channels is four threads next to each other.  The row's length is
@@ -555,6 +559,13 @@ int gaac_fp4_load(const uint8_t* cache, int L, int n_kv, int tiles, void* k, voi
   GAAC_REQUIRE(aligned16(k) && aligned16(v) && aligned16(cache) && (k_head_stride | k_row_stride | v_head_stride | v_row_stride) % 8 == 0, "gaac_fp4_load: rows must be 16-byte aligned");
   k_fp4_load<<<dim3((L + 4 * TT - 1) / (4 * TT), n_kv, 2), 256, 0, (hipStream_t)stream>>>(cache, L, tiles, (uint16_t*)k, (uint16_t*)v, k_head_stride, k_row_stride, v_head_stride, v_row_stride);
   return gaac::launch_status("gaac_fp4_load");
+}
+
+int gaac_fp4_length(const int* len, int tiles, int* host, void* stream) {
+  GAAC_REQUIRE(len != nullptr && host != nullptr && tiles > 0 && tiles <= INT_MAX / TT, "gaac_fp4_length: bad arguments (%d tiles)", tiles);
+  __atomic_store_n(host, -1, __ATOMIC_RELAXED);      // not there yet
+  k_fp4_length<<<1, 1, 0, (hipStream_t)stream>>>(len, tiles * TT, host);
+  return gaac::launch_status("gaac_fp4_length");
 }
 
 int gaac_fp4_append(const int* slots, int B, int n_slots, int n_kv, const void* k, const void* v, long k_batch_stride, long k_head_stride, long v_batch_stride, long v_head_stride, int* lens, int tiles, int cap,

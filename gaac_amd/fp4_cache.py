@@ -72,8 +72,8 @@ class FP4KVCache:
         self.cap = self.tiles * T
         self.H = n_slots * n_kv
         self.data = torch.zeros(self.H, self.tiles, TILE_BYTES, dtype=torch.uint8, device=device)
-        self.lens = torch.zeros(n_slots, dtype=torch.int32, device=device)          # tokens per slot
-        # set by append instead of writing: bit 0 = a slot was full, bit 1 = a slot twice in a batch, bit 2 = no such slot
+        self.lens = torch.zeros(n_slots, dtype=torch.int32, device=device)          # tokens per slot; the caller may set them: below 0 counts as 0, above cap as cap
+        # set by append instead of writing: bit 0 = a slot was full or its length below 0, bit 1 = a slot twice in a batch, bit 2 = no such slot
         self.overflow = torch.zeros(1, dtype=torch.int32, device=device)
         self._no_counters()
 
@@ -227,7 +227,7 @@ class FP4KVCache:
         """Raises if append had to leave a row out since the cache was made (waits for the stream).  used: the word, if the caller fetched it already."""
         hit = int(self.overflow) if used is None else used
         if hit:
-            raise RuntimeError("4-bit KV cache lost data:" + (" a sequence grew past the slot's token capacity;" if hit & 1 else "") +
+            raise RuntimeError("4-bit KV cache lost data:" + (" a sequence grew past the slot's token capacity, or its length was set below 0;" if hit & 1 else "") +
                                (" a slot stood twice in a batch;" if hit & 2 else "") + (" a batch named a slot that does not exist" if hit & 4 else ""))
 
     def decompress(self, slot: int) -> tuple[torch.Tensor, torch.Tensor]:
@@ -235,7 +235,7 @@ class FP4KVCache:
         both = (_lib._calls or _lib.calls()).fp4_read(self, slot, _lib.stream)
         if both is not None: return both
         if not 0 <= slot < self.n_slots: raise RuntimeError(f"decompress expects a slot in 0..{self.n_slots - 1}, got {slot}")
-        L = int(self.lens[slot])
+        L = max(0, min(int(self.lens[slot]), self.cap))
         k = torch.empty(L, self.n_kv, D, dtype=torch.bfloat16, device=self.data.device)
         v = torch.empty_like(k)
         if L:
@@ -245,6 +245,6 @@ class FP4KVCache:
 
     def stats(self) -> dict:
         """Occupancy (the keys of CompressedKVCache.stats): bytes_used counts codes and exponents of the tokens held."""
-        tokens = int(self.lens.sum())
+        tokens = int(self.lens.clamp(0, self.cap).sum())
         used, bf16 = tokens * self.n_kv * 2 * ROW_BYTES, tokens * self.n_kv * 2 * D * 2
         return dict(tokens=tokens, bytes_used=used, bf16_bytes=bf16, ratio=bf16 / max(1, used))

@@ -243,8 +243,11 @@ int gaac_fp4_store(const void* k, const void* v, long k_head_stride, long k_row_
 /* gaac_fp4_load: the values of a slot's first L tokens, bf16; cache: the slot's first tile. */
 int gaac_fp4_load(const uint8_t* cache, int L, int n_kv, int tiles, void* k, void* v, long k_head_stride, long k_row_stride, long v_head_stride,
                   long v_row_stride, void* stream);
+/* gaac_fp4_length: a slot's word of lens, below 0 as 0 and above its tiles' tokens as these, into host (pinned memory; set to -1 by the call and to the length when the
+ * stream has come that far: gaac_wait_words). */
+int gaac_fp4_length(const int* len, int tiles, int* host, void* stream);
 /* gaac_fp4_append: batch row b adds a token, k, v bf16 element (row b, head h, channel c) at x[b*batch_stride + h*head_stride + c], to slot slots[b] (below 0:
- * none).  A row that cannot be added is left out and sets a bit in errors: 1 = the slot holds cap tokens already, 2 = an earlier row of the batch names the
+ * none).  A row that cannot be added is left out and sets a bit in errors: 1 = the slot holds cap tokens already, or its length is below 0, 2 = an earlier row of the batch names the
  * same slot, 4 = there is no such slot. */
 int gaac_fp4_append(const int* slots, int B, int n_slots, int n_kv, const void* k, const void* v, long k_batch_stride, long k_head_stride, long v_batch_stride,
                     long v_head_stride, int* lens, int tiles, int cap, uint8_t* cache, int* errors, void* stream);

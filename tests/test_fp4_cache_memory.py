@@ -47,3 +47,16 @@ def test_attention_on_the_host_is_refused_by_name_with_splits_too():
     c = FP4KVCache(2, 4, 4096, device="cpu")
     for nsplit in (1, 3):
         with pytest.raises(RuntimeError, match="no CPU path"): c.attention(torch.zeros(1, 4, 128, dtype=torch.bfloat16), torch.zeros(1, dtype=torch.int32), 1.0, nsplit=nsplit)
+
+
+def test_stats_of_lengths_that_a_caller_set():
+    c = FP4KVCache(4, 2, 64, device="cpu")
+    c.lens.copy_(torch.tensor([-40, 64, 2 ** 31 - 1, 7], dtype=torch.int32))
+    assert c.stats()["tokens"] == 135 and c.stats()["bytes_used"] == 135 * 2 * 136
+
+
+def test_the_length_for_the_host_is_refused_without_its_words():
+    import pytest
+    from gaac_amd import _lib
+    for args in ((None, 2, 16, None), (16, 2, None, None), (16, 0, 16, None), (16, 1 << 26, 16, None)):
+        with pytest.raises(RuntimeError, match="gaac_fp4_length failed .*bad arguments"): _lib.call("gaac_fp4_length", *args)
