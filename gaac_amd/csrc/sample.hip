@@ -3,8 +3,9 @@
 //   least p times theirs; of these the ones with w >= min_p (the maximum has 1).  Token: the first i, by index, at which the running sum of the kept w
 //   exceeds u times their total.  T not positive: the first maximum.  Nothing but -inf (a NaN counts as one): -1.
 //
-// Which token comes is a whole number, so a sum that is off in its last bits is an error: weights are computed in 64 bits and held as multiples of 2^-43
-// in 64-bit integers (2^20 of them fit), whose sums are exact in any order.
+// Which token comes is a whole number, so it must not depend on the order in which a sum is taken: weights are computed in 64 bits and held as multiples of 2^-43 of the
+// largest in 64-bit integers (2^20 of them fit).  Their sums are exact; against the definition a weight is off by 2^-44 (and 0 below that), a sum over n tokens by n * 2^-44 at
+// most, 2^-24 for 2^20 of them, which is u's own last bit.  A share (p or u times a sum) is rounded to 53 bits, 2^-53 of it.
 // What is kept is a prefix of the order, so it is found as a key (the bits of x, in order) and the number of its equals that are kept: counts and sums by bins
 // of (max - x), then the elements of the bin where the limit falls (with a k: all up to it), in order: up to 64 of them sorted by a wave, up to 1024 by the block, up to 8192
 // by ever finer bins of their keys, more by such bins over the row.  Three launches: the row's maximum; bins; and the limits, the sums of segments and the token by the last of the row's blocks to

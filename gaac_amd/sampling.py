@@ -30,8 +30,9 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_
       token: the first i, in the order of the vocabulary, at which the running sum of the kept w exceeds u times their total
 
     A temperature that is not positive: the first maximum.  A token whose logit is -inf or NaN never comes; -1 for a row that has nothing else.  An infinite
-    maximum: evenly among the tokens that have it.  u outside [0, 1) counts as the nearest number inside, NaN as 0.  Sums are exact to 2^-43 of the largest
-    weight and do not depend on their order.  One launch for vocabularies up to 4089, otherwise at most three for every 1024 rows; no wait."""
+    maximum: evenly among the tokens that have it.  u outside [0, 1) counts as the nearest number inside, NaN as 0.  Weights are rounded to multiples of 2^-43
+    of the largest one, and what is rounded is added exactly: a sum over n tokens is off by at most n * 2^-44 of the largest weight (2^-24 for a vocabulary of 2^20), the same in
+    any order, and a token whose weight is below 2^-44 never comes.  One launch for vocabularies up to 4089, otherwise at most three for every 1024 rows; no wait."""
     out = (_lib._calls or _lib.calls()).draw(logits, u, temperature, top_k, top_p, min_p, _lib.stream)
     if out is not None: return out
     if logits.dim() != 2 or logits.dtype not in TYPES or not 1 <= logits.shape[1] <= MAX_VOCAB:
