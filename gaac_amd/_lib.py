@@ -4,6 +4,7 @@ missing, or a call is made without a GPU, the call raises."""
 from __future__ import annotations
 import contextlib, ctypes, os, warnings
 import torch
+from torch.autograd.forward_ad import unpack_dual
 
 _LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libgaac_hip.so")
 _lib = None
@@ -150,7 +151,8 @@ def on_device(*tensors):
 
 def no_backward(what: str, *tensors):
     """Raises where a gradient would be lost without a word: these kernels have no backward pass."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+    grad = torch.is_grad_enabled()
+    if any(t is not None and (grad and t.requires_grad or unpack_dual(t).tangent is not None) for t in tensors):
         raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad(), or with tensors that need no gradient")
 
 

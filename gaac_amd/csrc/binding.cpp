@@ -373,6 +373,7 @@ const at::Tensor& here(PyObject* o) {
   if (t.device() != c10::impl::getDeviceGuardImpl(c10::DeviceType::CUDA)->getDevice()) throw Otherwise{};
   return t;
 }
+bool loses_gradient(const at::Tensor& t) { return (c10::GradMode::is_enabled() && t.requires_grad()) || t._fw_grad(0).defined(); }
 // rows [n, heads, d] that a kernel reads through strides of whole 16 bytes
 void strides_of(const at::Tensor& t, long& row, long& head) {
   const long per = 16 / t.itemsize();
@@ -397,6 +398,7 @@ PyObject* fp4_prefill(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const Fp4Cache c(get, a[0]);
     const long slot = number(a[1]);
     const at::Tensor &k = here(a[2]), &v = here(a[3]);
+    if (loses_gradient(k) || loses_gradient(v)) throw Otherwise{};
     if (!is_rows(k, 3) || !is_rows(v, 3) || k.sizes() != v.sizes() || k.size(1) != c.n_kv || k.size(0) == 0 || k.size(0) > c.tiles * 32 || slot < 0 || slot >= c.n_slots) throw Otherwise{};
     long k_rs, k_hs, v_rs, v_hs;
     strides_of(k, k_rs, k_hs);
@@ -415,6 +417,7 @@ PyObject* fp4_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     Refs get;
     const Fp4Cache c(get, a[0]);
     const at::Tensor &slots = here(a[1]), &k = here(a[2]), &v = here(a[3]);
+    if (loses_gradient(k) || loses_gradient(v)) throw Otherwise{};
     if (!is_rows(k, 3) || !is_rows(v, 3) || k.sizes() != v.sizes() || k.size(1) != c.n_kv || k.size(0) == 0 || !is_slots(slots, k.size(0))) throw Otherwise{};
     long k_rs, k_hs, v_rs, v_hs;
     strides_of(k, k_rs, k_hs);
@@ -436,7 +439,7 @@ PyObject* fp4_attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
     Refs get;
     const Fp4Cache c(get, a[0]);
     const at::Tensor &q = here(a[1]), &slots = here(a[2]);
-    if (c10::GradMode::is_enabled() && q.requires_grad()) throw Otherwise{};
+    if (loses_gradient(q)) throw Otherwise{};
     const long nsplit = number(a[4]), cap = number(get(a[0], n_cap));
     if (!is_rows(q, 3) || !q.is_contiguous() || reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 != 0 || q.size(0) == 0 || !is_slots(slots, q.size(0)) || nsplit < 1 || nsplit > 1 << 20) throw Otherwise{};
     const long B = q.size(0), n_q = q.size(1);
@@ -492,7 +495,7 @@ PyObject* norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return whole_call(n, 10, [&]() -> PyObject* {
     const at::Tensor &q = here(a[0]), &k = here(a[1]), &pos = here(a[2]), &cos = here(a[3]), &sin = here(a[4]);
     const int type = float_type(q);
-    if (c10::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || (a[5] != Py_None && tensor(a[5]).requires_grad()) || (a[6] != Py_None && tensor(a[6]).requires_grad()))) throw Otherwise{};
+    if (loses_gradient(q) || loses_gradient(k) || loses_gradient(cos) || loses_gradient(sin) || (a[5] != Py_None && loses_gradient(tensor(a[5]))) || (a[6] != Py_None && loses_gradient(tensor(a[6])))) throw Otherwise{};
     if (q.dim() != 3 || k.dim() != 3 || q.scalar_type() != k.scalar_type() || q.size(0) != k.size(0) || q.size(2) != k.size(2) || q.size(0) == 0 || q.size(1) == 0 || k.size(1) == 0) throw Otherwise{};
     const long N = q.size(0), n_q = q.size(1), n_k = k.size(1), D = q.size(2);
     if ((D != 64 && D != 128 && D != 256) || N >= 1l << 28 || n_q >= 1 << 20 || n_k >= 1 << 20) throw Otherwise{};

@@ -11,7 +11,8 @@ append and attention take the batch's slot map and the slots' lengths from devic
 HIP graph.  Calls on one cache must be ordered on one stream where one of them writes; attention may run on several streams at
 once, and in several graphs: its scratch is the call's own, and the counters by which the splits of a row find the last of them are one set for each stream and one
 for each captured call.  A call that is not captured makes its stream's set, and sees to it that READY sets lie ready for captured calls of as many rows; a captured call that finds
-none, or after CAPTURES of them, takes a launch more instead; captured_counters and give_back return the sets of graphs that are dropped.  128 bytes a row and kv head of a call, beside its partials: scratch of the calls, not of the slots."""
+none, or after CAPTURES of them, takes a launch more instead; captured_counters and give_back return the sets of graphs that are dropped.  128 bytes a row and kv head of a call, beside its partials: scratch of the calls, not of the slots.
+No call has a backward pass: tensors whose gradient it would lose, in either mode of differentiation, are refused."""
 from __future__ import annotations
 import contextlib
 import functools
@@ -164,6 +165,7 @@ class FP4KVCache:
         L = k.shape[0]
         if not 0 <= slot < self.n_slots: raise RuntimeError(f"prefill expects a slot in 0..{self.n_slots - 1}, got {slot}")
         if L > self.cap: raise RuntimeError(f"prompt has {L} tokens, a slot holds {self.cap}")
+        _lib.no_backward("prefill", k, v)
         with _lib.on_device(self.data, k, v):
             k, v = _rows(k), _rows(v)
             (k_hs, k_rs), (v_hs, v_rs) = _strides(k), _strides(v)
@@ -176,6 +178,7 @@ class FP4KVCache:
         if (_lib._calls or _lib.calls()).fp4_append(self, slots, k, v, _lib.stream): return
         self._check("append", k, v)
         if slots.dtype != torch.int32 or slots.dim() != 1 or slots.shape[0] != k.shape[0]: raise RuntimeError("append expects slots int32 [B]")
+        _lib.no_backward("append", k, v)
         if k.shape[0] == 0: return
         with _lib.on_device(self.data, slots, k, v):
             k, v = _rows(k), _rows(v)

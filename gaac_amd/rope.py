@@ -41,7 +41,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, cos:
     if q_weight is not None:
         for w, heads in ((q_weight, n_q), (k_weight, n_k)):
             if w.dtype != q.dtype or tuple(w.shape) not in ((D,), (heads, D)): raise RuntimeError(f"qk_norm_rope expects weights {q.dtype} [{D}] or [{heads}, {D}], got {w.dtype} {list(w.shape)}")
-    _lib.no_backward("qk_norm_rope", q, k, q_weight, k_weight)
+    _lib.no_backward("qk_norm_rope", q, k, cos, sin, q_weight, k_weight)
     with _lib.on_device(q, k, positions, cos, sin, q_weight, k_weight):
         q_out, k_out = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, k))
         if N == 0: return q_out, k_out
