@@ -586,7 +586,9 @@ int gaac_fp4_attn(const uint8_t* cache, const int* lens, const int* slots, int n
                cap, tiles, nsplit);
   GAAC_REQUIRE(nsplit == 1 || (partials != nullptr && reinterpret_cast<uintptr_t>(partials) % 8 == 0), "gaac_fp4_attn: more than one split needs partials, 8-byte aligned");
   GAAC_REQUIRE(aligned16(q) && aligned16(cache), "gaac_fp4_attn: q must be 16-byte aligned");
-  const int G = n_q / n_kv, P = B * nsplit;
+  // The plan adds up the rows' tiles in 32 bits; a batch whose rows could come to more has blocks enough without splits.
+  const bool splits = nsplit > 1 && (long)B * tiles + (long)B * nsplit < 1l << 30;
+  const int G = n_q / n_kv, P = splits ? B * nsplit : B;
   const int lds = 4 * (NW * G * OROW + 2 * NW * 16);
   if (lds > 60 * 1024) {      // (with the 4 KB that the kernel has by itself more than the 64 that need no asking)
     const hipError_t e = hipFuncSetAttribute((const void*)k_fp4_attn, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
