@@ -158,8 +158,9 @@ __global__ __launch_bounds__(256) void k_fp4_append(const int* slots, int n_slot
   for (int i = threadIdx.x; i < b; i += 256) again |= slots[i] == slot;
   const int len = slot < n_slots ? lens[slot] : 0;
   const bool full = (unsigned)len >= (unsigned)cap;      // (or below 0)
-  if (__syncthreads_or(again) || slot >= n_slots || full) {
-    if (threadIdx.x == 0) atomicOr(errors, slot >= n_slots ? 4 : full ? 1 : 2);
+  const bool twice = __syncthreads_or(again);
+  if (twice || slot >= n_slots || full) {      // (of a slot named twice the length may be raised by now: what is reported does not go by it)
+    if (threadIdx.x == 0) atomicOr(errors, slot >= n_slots ? 4 : twice ? 2 : 1);
     return;
   }
   const int t = len & (TT - 1), s = t >> 4, m = t & 15, g = (t >> 2) & 3, i = t & 3;

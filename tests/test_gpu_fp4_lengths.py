@@ -51,3 +51,15 @@ def test_the_lengths_of_an_empty_cache_and_of_one_on_another_stream():
         c.prefill(1, x, x)
         k, v = c.decompress(1)
         assert torch.equal(k, x) and torch.equal(v, x)
+
+
+def test_a_slot_named_twice_is_reported_as_that():
+    """Whether it is full, has one place left or many: what the second row reports does not depend on when the first one has raised the length."""
+    require_gpu()
+    k = torch.ones(64, 1, D, dtype=torch.bfloat16, device="cuda")
+    for held, bits, length in ((64, 3, 64), (63, 2, 64), (10, 2, 11)):
+        for B in (2, 64):
+            c = FP4KVCache(1, 1, 64)
+            c.prefill(0, k[:held], k[:held])
+            c.append(torch.zeros(B, dtype=torch.int32, device="cuda"), k[:B], k[:B])
+            assert int(c.overflow) == bits and c.lens.tolist() == [length]
