@@ -498,7 +498,7 @@ PyObject* norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (loses_gradient(q) || loses_gradient(k) || loses_gradient(cos) || loses_gradient(sin) || (a[5] != Py_None && loses_gradient(tensor(a[5]))) || (a[6] != Py_None && loses_gradient(tensor(a[6])))) throw Otherwise{};
     if (q.dim() != 3 || k.dim() != 3 || q.scalar_type() != k.scalar_type() || q.size(0) != k.size(0) || q.size(2) != k.size(2) || q.size(0) == 0 || q.size(1) == 0 || k.size(1) == 0) throw Otherwise{};
     const long N = q.size(0), n_q = q.size(1), n_k = k.size(1), D = q.size(2);
-    if ((D != 64 && D != 128 && D != 256) || N >= 1l << 28 || n_q >= 1 << 20 || n_k >= 1 << 20) throw Otherwise{};
+    if ((D != 64 && D != 128 && D != 256) || N >= 1l << 26 || n_q >= 1 << 20 || n_k >= 1 << 20) throw Otherwise{};
     if (pos.dim() != 1 || pos.size(0) != N || !pos.is_contiguous() || (pos.scalar_type() != at::kLong && pos.scalar_type() != at::kInt)) throw Otherwise{};
     if (cos.scalar_type() != at::kFloat || sin.scalar_type() != at::kFloat || cos.dim() != 2 || cos.sizes() != sin.sizes() || cos.size(0) < 1 || cos.size(0) >= 1l << 31 || !cos.is_contiguous() || !sin.is_contiguous()) throw Otherwise{};
     const long R = 2 * cos.size(1);

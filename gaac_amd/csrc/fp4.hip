@@ -572,7 +572,7 @@ int gaac_fp4_length(const int* len, int tiles, int* host, void* stream) {
 int gaac_fp4_append(const int* slots, int B, int n_slots, int n_kv, const void* k, const void* v, long k_batch_stride, long k_head_stride, long v_batch_stride, long v_head_stride, int* lens, int tiles, int cap,
                     uint8_t* cache, int* errors, void* stream) {
   GAAC_REQUIRE(slots != nullptr && k != nullptr && v != nullptr && lens != nullptr && cache != nullptr && errors != nullptr, "gaac_fp4_append: null pointer");
-  GAAC_REQUIRE(B > 0 && n_slots > 0 && n_kv > 0 && n_kv < 1 << 24 && tiles > 0 && cap > 0 && cap <= (long)tiles * TT, "gaac_fp4_append: bad sizes (B %d, n_slots %d, n_kv %d, capacity %d in %d tiles)", B, n_slots,
+  GAAC_REQUIRE(B > 0 && B < 1 << 24 && n_slots > 0 && n_kv > 0 && n_kv < 1 << 24 && tiles > 0 && cap > 0 && cap <= (long)tiles * TT, "gaac_fp4_append: bad sizes (B %d, n_slots %d, n_kv %d, capacity %d in %d tiles)", B, n_slots,
                n_kv, cap, tiles);
   GAAC_REQUIRE(aligned16(k) && aligned16(v) && aligned16(cache) && (k_batch_stride | k_head_stride | v_batch_stride | v_head_stride) % 8 == 0, "gaac_fp4_append: rows must be 16-byte aligned");
   k_fp4_append<<<B, 256, 0, (hipStream_t)stream>>>(slots, n_slots, n_kv, (const uint16_t*)k, (const uint16_t*)v, k_batch_stride, k_head_stride, v_batch_stride, v_head_stride, lens, tiles, cap, cache, errors);
@@ -583,7 +583,7 @@ int gaac_fp4_attn(const uint8_t* cache, const int* lens, const int* slots, int n
                   void* stream) {
   GAAC_REQUIRE(cache != nullptr && lens != nullptr && slots != nullptr && q != nullptr && out != nullptr, "gaac_fp4_attn: null pointer");
   GAAC_REQUIRE(B > 0 && n_slots > 0 && n_kv > 0 && n_kv <= 65535 && n_q >= n_kv && n_q % n_kv == 0 && n_q / n_kv <= 16, "gaac_fp4_attn: GQA group size must be 1..16 (n_q %d, n_kv %d)", n_q, n_kv);
-  GAAC_REQUIRE(tiles > 0 && cap > 0 && cap <= (long)tiles * TT && nsplit > 0 && (long)B * nsplit * n_kv < 1l << 31 && (long)B * n_q < 1l << 31, "gaac_fp4_attn: bad sizes (B %d, capacity %d in %d tiles, %d splits)", B,
+  GAAC_REQUIRE(tiles > 0 && cap > 0 && cap <= (long)tiles * TT && nsplit > 0 && (long)B * nsplit * n_kv < (1l << 32) / (64 * NW) && (long)B * n_q < 1l << 31, "gaac_fp4_attn: bad sizes (B %d, capacity %d in %d tiles, %d splits)", B,
                cap, tiles, nsplit);
   GAAC_REQUIRE(nsplit == 1 || (partials != nullptr && reinterpret_cast<uintptr_t>(partials) % 8 == 0), "gaac_fp4_attn: more than one split needs partials, 8-byte aligned");
   GAAC_REQUIRE(aligned16(q) && aligned16(cache), "gaac_fp4_attn: q must be 16-byte aligned");

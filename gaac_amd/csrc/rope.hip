@@ -125,7 +125,7 @@ extern "C" int gaac_qk_norm_rope(int type, const void* q, const void* k, long q_
   GAAC_REQUIRE(q != nullptr && k != nullptr && positions != nullptr && cos != nullptr && sin != nullptr && q_out != nullptr && k_out != nullptr, "gaac_qk_norm_rope: null pointer");
   GAAC_REQUIRE(type >= 0 && type <= 2, "gaac_qk_norm_rope: type must be 0 (bf16), 1 (fp16) or 2 (fp32)");
   GAAC_REQUIRE((D == 64 || D == 128 || D == 256) && R > 0 && R <= D && R % 16 == 0, "gaac_qk_norm_rope: head_dim must be 64, 128 or 256, and a multiple of 16 channels of it rotated (%d of %d)", R, D);
-  GAAC_REQUIRE(N > 0 && n_q > 0 && n_k > 0 && max_pos > 0 && n_q < 1 << 20 && n_k < 1 << 20 && N < 1l << 28, "gaac_qk_norm_rope: bad sizes (%ld tokens, %d + %d heads, %d positions)", N, n_q, n_k, max_pos);
+  GAAC_REQUIRE(N > 0 && n_q > 0 && n_k > 0 && max_pos > 0 && n_q < 1 << 20 && n_k < 1 << 20 && N < 1l << 26, "gaac_qk_norm_rope: bad sizes (%ld tokens, %d + %d heads, %d positions)", N, n_q, n_k, max_pos);
   GAAC_REQUIRE((q_weight == nullptr) == (k_weight == nullptr), "gaac_qk_norm_rope: weights for both or for neither");
   const uintptr_t all = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(q_out) | reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(cos) |
                         reinterpret_cast<uintptr_t>(sin) | reinterpret_cast<uintptr_t>(q_weight) | reinterpret_cast<uintptr_t>(k_weight);
