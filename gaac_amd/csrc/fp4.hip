@@ -184,7 +184,6 @@ __global__ __launch_bounds__(256) void k_fp4_append(const int* slots, int n_slot
 // from the lengths on the device.
 struct Share { int row, len, slot, first, end, index, count; };      // row < 0: nothing for this split
 
-__device__ __forceinline__ int row_slot(const int* slots, int b) { return slots[b]; }
 __device__ __forceinline__ int row_len(const int* lens, int n_slots, int cap, int slot) { return slot >= 0 && slot < n_slots ? max(min(lens[slot], cap), 0) : 0; }      // (lens is the caller's to write)
 // Sums over the wave in the vector unit (rows of 16 by shifts, then across rows), not through LDS: a lane exchange there takes ten times as long.
 template <int CTRL, int ROWS> __device__ __forceinline__ int moved(int x) { return __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, false); }
