@@ -610,7 +610,7 @@ def bench_paged(a):
 def bench_serve(a):
     """Config 4: random-init bf16 Llama-3-8B-architecture decode (32 layers, hidden 4096, 32 / 8 heads, d=128, FFN 14336, theta 500000,
     vocab 128256), batch 4 at 32K-token random-token contexts, compressed cache vs uncompressed BF16 cache; greedy decode, the whole
-    step captured as one HIP graph."""
+    step captured as one HIP graph.  Beside them, as figures only, the 4-bit cache, greedy and with tokens drawn by sample()."""
     from gaac_amd.serving import ModelConfig, Weights, DecodeRunner
     dev = "cuda"
     B, ctx, steps = 4, 32768, max(16, min(a.steps, 64))
@@ -690,6 +690,21 @@ def bench_serve(a):
                              "logit_std": round(flogits["bf16"].std().item(), 4),
                              "noise_floor_max_abs_diff": round(dn.max().item(), 5), "noise_floor_mean_abs_diff": round(dn.mean().item(), 6),
                              "same_argmax_fraction": round((flogits["gaac"].argmax(-1) == flogits["bf16"].argmax(-1)).float().mean().item(), 4)}
+    for name, sampling in (("fp4", None), ("fp4_sampled", dict(temperature=0.7, top_k=50, top_p=0.9))):
+        run = DecodeRunner(w, n_slots=B, kv="fp4")
+        first = torch.stack([run.prefill(i, p).argmax() for i, p in enumerate(prompts)])
+        run.start_decode(first, use_graph=True, sampling=sampling)
+        u = None if sampling is None else torch.rand(8 + steps, B, generator=g, device=dev)
+        run.decode(8, u=None if u is None else u[:8]); torch.cuda.synchronize()
+        t0 = time.perf_counter()
+        run.decode(steps, u=None if u is None else u[8:])
+        torch.cuda.synchronize(); dt = time.perf_counter() - t0
+        st = run.kv_stats()
+        res[name] = {"tokens_per_s": round(B * steps / dt, 1), "ms_per_step": round(dt / steps * 1e3, 3), "kv_bytes_used": st["bytes_used"], "kv_bytes_reserved": st["bytes_reserved"],
+                     "kv_ratio_vs_bf16": round(st["ratio"], 4)}
+        if sampling: res[name]["sampling"] = sampling
+        del run
+        torch.cuda.empty_cache()
     res["same_tokens_fraction"] = round((toks["gaac"] == toks["bf16"]).float().mean().item(), 4)
     res["speedup"] = round(res["gaac"]["tokens_per_s"] / res["bf16"]["tokens_per_s"], 4)
     print(json.dumps(res))
