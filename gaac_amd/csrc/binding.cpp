@@ -367,7 +367,7 @@ PyObject* page_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 // The calls of the 4-bit cache, of qk_norm_rope and of sample, the same way.  Their tensors have to be on the current device.  Host us a call, Python / here: prefill
-// 9.0 / 3.3, append 8.1 / 3.6, attention 8.2 / 5.1 (with splits 12.2 / 7.5), qk_norm_rope 16.4 / 5.9, sample 9.7 / 5.0 (of three launches 14.5 / 9.8).
+// 9.9 / 3.3, append 8.8 / 3.6, attention 8.2 / 4.9 (with splits 11.1 / 7.1), qk_norm_rope 16.9 / 5.5, sample 9.0 / 4.7 (of three launches 14.0 / 9.8).
 const at::Tensor& here(PyObject* o) {
   const at::Tensor& t = tensor(o);
   if (t.device() != c10::impl::getDeviceGuardImpl(c10::DeviceType::CUDA)->getDevice()) throw Otherwise{};

@@ -257,7 +257,7 @@ struct Query { i8 hi, lo; unsigned hi_exp, lo_exp; };
 
 // The maximum needs all of a head's channels, the conversion of the lane's eight dwords is shared out over the block's eight waves, one each (`halves`: in LDS; one barrier): by each wave
 // for itself it took more instructions than two tiles (1000 tokens x 8 heads 7.3 us, so 6.5; 32 rows of 300..6000 24.1, 23.2; 65536 x 8 18.0,
-// 17.2).
+// 17.2; all with weights of one bf16 number).
 struct RawQuery { u4 x[4]; u2 own; };
 __device__ __forceinline__ RawQuery load_query(const uint16_t* q, bool there, int g, int w) {
   RawQuery r;
@@ -434,10 +434,10 @@ __device__ void merge(const float* part, long acc_at, int p0, int count, int n_k
 }
 
 // Decode attention.  Bound by the read of the cache where rows are long: 16 rows of 4096..65536 tokens x 8 heads 101 us, 606 MB, 6.0 TB/s, the rate of a plain read of
-// that size being 6.1; by the launch, the plan and the merge where the cache is short: 1 row of 65536 x 8 heads, 17.2 us, has its 71 MB after about 14 (2 to 2.6 of
-// them launch and plan), leaves the partials within 1.5 and adds them up in 2.3; by instructions on few CUs (a tile a SIMD 0.35 us).  A wave has whole tiles, so what it needs comes in 6 loads
+// that size being 6.1; by the launch, the plan and the merge where the cache is short: 1 row of 65536 x 8 heads, 17.1 us, has its 71 MB after about 14 (2 to 2.6 of
+// them launch and plan), leaves the partials within 1.5 and adds them up in 2.3; by instructions on few CUs (1000 x 8 heads, four tiles a wave, 7.1 us).  A wave has whole tiles, so what it needs comes in 6 loads
 // of whole lines and no lane waits for another; one tile is in flight while another is worked on: 16 waves a CU, 68 KB of loads in flight on each.  Two tiles in
-// flight by 8 waves a CU take the same 101 us there, but 1 us more on shorter rows, whose first tiles wait for the second ones.  Four waves a SIMD need 128 registers at most: it has 124.
+// flight by 8 waves a CU take the same 101 us there, but 1 us more on shorter rows, whose first tiles wait for the second ones.  Four waves a SIMD need 128 registers at most: it has 123.
 // One block = eight waves = one split of one (row, kv head).  One split a row (P == B): the output is written here; otherwise a row with several splits leaves
 // partials, and the block that draws the last of the (row, kv head)'s tickets adds them up and puts the tickets back (tickets NULL: k_fp4_merge does it).
 __global__ __launch_bounds__(64 * NW, 4) void k_fp4_attn(const uint8_t* cache, const int* lens, const int* slots, int n_slots, int tiles, int cap, const uint16_t* q, int B, int n_kv, int G,

@@ -35,14 +35,14 @@ _LOCK = threading.Lock()        # over the sets that lie ready
 @functools.lru_cache(maxsize=1024)
 def choose_nsplit(B: int, n_kv: int, S: int, G: int = 4) -> int:
     """Splits for each of B rows, S tokens in the longest, G query heads a kv head, which the launch then shares out by length (csrc/fp4.hip).  Measured, 8 kv heads and G 4 unless noted, us:
-      * up to 1500 tokens none (1000 tokens: 6.5, against 7.5 with 8 splits; 1500: 7.6, with 16 7.8);
-      * heads that fill half of the chip by themselves: none, since a split's start and merge cost more than even shares save (32 rows of 300..6000: 23.3, against
-        26.2 with 2; 24 of 2000..16000: 51.1 and 53.4; 64 of 2000..16000: 106 and 114), but not where a single row may take as long as all (from 32768 tokens);
-      * otherwise one block per CU (8 rows of 7000..8192: 16.8 with 4, 20.5 with 2, 17.5 with 8), two for long rows, whose tiles are worth more loads in flight (16 rows of 4096..65536: 101.8
-        with 4, 105.5 with 2; 8 of 32768: 48.9 with 8, 47.7 with 4);
-      * but of few heads no more splits than their merge by one block is worth: 16 (16384 tokens: 9.9, with 32 10.8; 4096: 8.1 and 9.8), from 24576 tokens 32 (65536: 17.5, with 16 19.4; 32768 x
-        1: 10.5, with 16 12.5, with 256 23; G 16 18, 18 and 71), and for G up to 4 64 from 65536 (131072 x 1: 16.1, with 32 18.5), 128 from 262144 (20.5, with 64 21.0; 10^6 x 1: 36.5,
-        with 64 52, with 256 41), for more heads to merge from four times these lengths (G 16, 131072 x 1: 26, with 64 29; 262144: 34, with 32 37; 10^6: 62, with 64 65)."""
+      * up to 1500 tokens none (1000 tokens: 7.0, against 7.8 with 7 splits; 8 rows of 1500: 8.8, with 4 9.5; but 1 row of 1500 alone 8.5, with 11 8.1);
+      * heads that fill half of the chip by themselves: none, since a split's start and merge cost more than even shares save (32 rows of 300..6000: 23.7, against
+        26.2 with 2; 24 of 2000..16000: 52.4 and 53.4; 64 of 2000..16000: 106 and 115), but not where a single row may take as long as all (from 32768 tokens);
+      * otherwise one block per CU (8 rows of 7000..8192: 17.8 with 4, 22.9 with 2, 18.0 with 8), two for long rows, whose tiles are worth more loads in flight (16 rows of 4096..65536: 101
+        with 4, 111 with 2; 8 of 32768: 50.8 with 8, 50.2 with 4);
+      * but of few heads no more splits than their merge by one block is worth: 16 (4096 tokens: 8.2, with 32 8.7; 16384: 10.7 and 10.1), from 24576 tokens 32 (65536: 18.2, with 16 21.8; 32768 x
+        1: 11.0, with 16 13.2, with 256 24; G 16 18.4, 19.1 and 73), and for G up to 4 64 from 65536 (131072 x 1: 16.1, with 32 19.8), 128 from 262144 (20.8, with 64 22.1; 10^6 x 1: 37.2,
+        with 64 57, with 256 40), for more heads to merge from four times these lengths (G 16, 131072 x 1: 27, with 64 29; 262144: 35, with 32 39; 10^6: 70, with 128 62)."""
     H = B * n_kv
     if S <= 1500: return 1
     if H > 128: return 1 if S < 32768 else 2
