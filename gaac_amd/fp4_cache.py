@@ -32,6 +32,11 @@ READY = 16                      # sets of counters that calls outside of capture
 _LOCK = threading.Lock()        # over the sets that lie ready
 
 
+@functools.lru_cache(maxsize=None)
+def _side_stream(device: torch.device) -> torch.cuda.Stream:
+    return torch.cuda.Stream(device)      # (one for all caches: the allocator keeps memory apart by streams)
+
+
 @functools.lru_cache(maxsize=1024)
 def choose_nsplit(B: int, n_kv: int, S: int, G: int = 4) -> int:
     """Splits for each of B rows, S tokens in the longest, G query heads a kv head, which the launch then shares out by length (csrc/fp4.hip).  Measured, 8 kv heads and G 4 unless noted, us:
@@ -142,7 +147,7 @@ class FP4KVCache:
             if words > self._ready_words: self._ready, self._ready_words = [], words
             missing = min(READY, CAPTURES - len(self._given)) - len(self._ready)
             if missing < 1: return
-            side = torch.cuda.Stream(self.data.device)      # zero before this call returns, whatever the current stream still has to do: a graph may run on any
+            side = _side_stream(self.data.device)      # zero before this call returns, whatever the current stream still has to do: a graph may run on any
             with torch.cuda.stream(side): made = torch.zeros(missing, self._ready_words, dtype=torch.int32, device=self.data.device)
             side.synchronize()
             self._ready.extend(made.unbind(0))

@@ -178,3 +178,15 @@ def test_the_decode_loop_captures_anew_as_often_as_it_likes():
     graph = run.decode(3)
     run.start_decode(torch.tensor([5, 6], device=dev), use_graph=False)
     assert [c._captured for c in run.caches] == [0, 0] and held[1] == held[0] + 1 and graph.shape == (3, 2)
+
+
+def test_counters_of_many_caches_come_from_one_stretch_of_memory():
+    """40 layers that each make their first counters reserve what these take, not a stretch of the allocator's for each."""
+    from gaac_amd import FP4KVCache
+    require_gpu()
+    caches = [FP4KVCache(1, 2, 64) for _ in range(40)]
+    q, slots = torch.ones(1, 8, D, dtype=torch.bfloat16, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    caches[0].attention(q, slots, 0.1, nsplit=2)
+    before = torch.cuda.memory_reserved()
+    for c in caches[1:]: c.attention(q, slots, 0.1, nsplit=2)
+    assert torch.cuda.memory_reserved() - before <= 4 << 20 and len({c._ready[0].data_ptr() for c in caches}) == 40
