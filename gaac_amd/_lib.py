@@ -48,6 +48,10 @@ _SIGNATURES = {
     "gaac_fp4_attn": [P, P, P, c_int, c_int, c_int, P, c_int, c_int, c_int, c_float, c_int, P, P, P, P],
     "gaac_qk_norm_rope": [c_int, P, P] + [c_long] * 5 + [c_int] * 4 + [P, P, c_long, c_long, c_float, P, c_int, P, P, c_int, c_int, P, P, P],
     "gaac_sample": [c_int, P, c_long, c_int, c_int, P, P, c_float, P, c_int, P, c_float, P, c_float, P, c_long, P, P],
+    "gaac_fp8_rows": [c_int, P, c_long, P, c_long, P, c_float, c_int, c_int, P, P, P, c_long, c_int, c_int, P],
+    "gaac_fp8_values": [P, P, c_long, c_int, c_int, c_int, c_int, P, c_long, P],
+    "gaac_fp8_product": [P, P, P, P, c_int, c_int, c_int, c_int, c_int, P, c_long, P],
+    "gaac_logprobs": [c_int, P, c_long, c_int, c_int, P, c_int, P, c_long, P, P, P, P, P, P],
     "gaac_attn_launch": [P] * 16 + [P, P, c_int, c_int, c_int, P, c_int, c_float, c_int, c_int, P, P, P, c_int, P, P, P, P, P],
 }
 

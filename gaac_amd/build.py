@@ -13,7 +13,7 @@ LIB = os.path.join(HERE, "libgaac_hip.so")
 LIB_W12 = os.path.join(HERE, "libgaac_hip_w12.so")            # measurement build -DGAAC_WAVES12: twelve-wave blocks, three waves per SIMD (see attn.hip); on demand only
 LIB_TIMING = os.path.join(HERE, "libgaac_hip_timing.so")      # same sources with -DGAAC_PHASE_TIMING (per-block phase time stamps); built on demand only
 BINDING = os.path.join(HERE, "_binding.so")
-SOURCES = ["codec.hip", "attn.hip", "cache.hip", "paged.hip", "fp4.hip", "rope.hip", "sample.hip"]
+SOURCES = ["codec.hip", "attn.hip", "cache.hip", "paged.hip", "fp4.hip", "rope.hip", "sample.hip", "fp8.hip", "logprobs.hip"]
 # bench.py's measurement aids (read probe, plain copy): their own library next to bench.py, not in the product library
 BENCH_SRC = os.path.join(os.path.dirname(HERE), "bench_kernels.hip")
 BENCH_LIB = os.path.join(os.path.dirname(HERE), "libgaac_bench.so")

@@ -1,0 +1,172 @@
+"""Rows and weights in 8 bits, and the steps of a model's layer on them: norm, projection, gated feed-forward block.
+
+128 consecutive elements of a row share a power of two 2^E, the smallest with max |x| <= 448 * 2^E, from -117 to 119; an element is held as the nearest e4m3 number (ties to the
+even code) times 2^E, 8.06 bits in all.  A block with a NaN or an infinity reads as NaN.  Weights are held the same way along their inputs.  The values are numbers of bf16, so reading
+them back rounds nothing; and since the matrix instruction takes powers of two as scales, a product is one sum in 32 bits.  Memory is laid out in the order of that
+instruction's operands (csrc/fp8.hip): rows and weights are for these functions, dequantize() has the values as a tensor.
+
+No call has a backward pass: tensors whose gradient it would lose, in either mode of differentiation, are refused.  No call waits for the GPU; all can be captured in a HIP graph."""
+from __future__ import annotations
+import torch
+from . import _lib
+from .rope import TYPES
+
+BLOCK = 128
+MAX_WIDTH = 65536           # elements of a row
+MAX_NORM_WIDTH = 32768
+MAX_ROWS = 1 << 20          # of a product
+
+
+def _memory(rows: int, K: int, device) -> tuple[torch.Tensor, torch.Tensor]:
+    """Data and exponents of rows (a multiple of 16)."""
+    nb = -(-K // BLOCK)
+    return torch.empty(rows * nb * BLOCK, dtype=torch.uint8, device=device), torch.empty(-(-nb // 4) * rows * 4, dtype=torch.uint8, device=device)
+
+
+def _padded(n: int) -> int:
+    return -(-n // 16) * 16
+
+
+def _row_stride(x: torch.Tensor) -> int:
+    return x.stride(0) if x.shape[0] > 1 else 0
+
+
+def _in_rows(x: torch.Tensor) -> torch.Tensor:
+    """x [M, K] as the kernels read it: elements next to each other, rows any stride apart."""
+    return x if x.shape[1] == 1 or x.stride(1) == 1 else x.contiguous()
+
+
+class FP8Rows:
+    """Rows [M, K] in 8 bits, from quantize_fp8, rms_norm_fp8 or fp8_gated."""
+    __slots__ = ("data", "exps", "shape")
+
+    def __init__(self, data: torch.Tensor, exps: torch.Tensor, shape: tuple[int, int]):
+        self.data, self.exps, self.shape = data, exps, shape
+
+    @property
+    def device(self):
+        return self.data.device
+
+    @property
+    def nbytes(self) -> int:
+        return self.data.numel() + self.exps.numel()
+
+    def dequantize(self) -> torch.Tensor:
+        """The values, bf16 [M, K]."""
+        return _values(self.data, self.exps, *self.shape, 1, 0)
+
+
+def _values(data, exps, M, K, step, first):
+    with _lib.on_device(data, exps):
+        out = torch.empty(M, K, dtype=torch.bfloat16, device=data.device)
+        if M: _lib.call("gaac_fp8_values", data, exps, _padded(M) * step, step, first, M, K, out, K, _lib.stream)
+        return out
+
+
+def _check_rows(what: str, x: torch.Tensor, most: int):
+    if x.dim() != 2 or x.dtype not in TYPES or not 1 <= x.shape[1] <= most:
+        raise RuntimeError(f"{what} expects rows bf16, fp16 or fp32 [M, K], K up to {most}, got {x.dtype} {list(x.shape)}")
+    if x.shape[0] > 1 << 24: raise RuntimeError(f"{what} takes up to 2^24 rows, got {x.shape[0]}")
+
+
+class FP8Weight:
+    """A weight [N, K] in 8 bits for fp8_linear, from bf16, fp16 or fp32; or with a second one of its shape, up, the pair of a gated block for fp8_gated (the first one is the gate).  Laid out once; the
+    tensors that it is made from are not kept."""
+    __slots__ = ("data", "exps", "N", "K", "gated")
+
+    def __init__(self, w: torch.Tensor, up: torch.Tensor | None = None):
+        for t in (w, up):
+            if t is None: continue
+            _check_rows("FP8Weight", t, MAX_WIDTH)
+            if not 1 <= t.shape[0] <= 1 << 22: raise RuntimeError(f"FP8Weight expects 1 to 2^22 rows, got {list(t.shape)}")
+        if up is not None and up.shape != w.shape: raise RuntimeError(f"FP8Weight expects gate and up of one shape, got {list(w.shape)} and {list(up.shape)}")
+        _lib.no_backward("FP8Weight", w, up)
+        (self.N, self.K), self.gated = w.shape, up is not None
+        parts = [w] if up is None else [w, up]
+        rows = _padded(self.N) * len(parts)
+        with _lib.on_device(*parts):
+            self.data, self.exps = _memory(rows, self.K, w.device)
+            for i, t in enumerate(parts):
+                t = _in_rows(t)
+                _lib.call("gaac_fp8_rows", TYPES[t.dtype], t, _row_stride(t), None, 0, None, 0.0, self.N, self.K, None, self.data, self.exps, rows, len(parts), i, _lib.stream)
+
+    @property
+    def device(self):
+        return self.data.device
+
+    @property
+    def nbytes(self) -> int:
+        return self.data.numel() + self.exps.numel()
+
+    def dequantize(self):
+        """The values, bf16 [N, K]; of a gated pair both."""
+        if self.gated: return tuple(_values(self.data, self.exps, self.N, self.K, 2, i) for i in range(2))
+        return _values(self.data, self.exps, self.N, self.K, 1, 0)
+
+
+def quantize_fp8(x: torch.Tensor) -> FP8Rows:
+    """x [M, K] (bf16, fp16 or fp32, K up to 65536, rows any stride apart) -> its rows in 8 bits.  One launch."""
+    _check_rows("quantize_fp8", x, MAX_WIDTH)
+    _lib.no_backward("quantize_fp8", x)
+    M, K = x.shape
+    with _lib.on_device(x):
+        data, exps = _memory(_padded(M), K, x.device)
+        x = _in_rows(x)
+        if M: _lib.call("gaac_fp8_rows", TYPES[x.dtype], x, _row_stride(x), None, 0, None, 0.0, M, K, None, data, exps, _padded(M), 1, 0, _lib.stream)
+        return FP8Rows(data, exps, (M, K))
+
+
+def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual: torch.Tensor | None = None):
+    """x [M, K] (bf16, fp16 or fp32, K up to 32768, rows any stride apart), weight [K] of its type -> FP8Rows of
+
+      y = h * rsqrt(mean(h^2) + eps) * weight,   h = x, or x + residual
+
+    with a residual [M, K] of x's type (FP8Rows, h): h in that type, a new contiguous tensor.  The norm is taken of the sum in 32 bits, before it is rounded for h; the sum of squares and y in 64 bits.  One launch."""
+    _check_rows("rms_norm_fp8", x, MAX_NORM_WIDTH)
+    M, K = x.shape
+    if weight.dtype != x.dtype or tuple(weight.shape) != (K,): raise RuntimeError(f"rms_norm_fp8 expects weight {x.dtype} [{K}], got {weight.dtype} {list(weight.shape)}")
+    if residual is not None and (residual.dtype != x.dtype or residual.shape != x.shape):
+        raise RuntimeError(f"rms_norm_fp8 expects residual {x.dtype} {list(x.shape)}, got {residual.dtype} {list(residual.shape)}")
+    _lib.no_backward("rms_norm_fp8", x, weight, residual)
+    with _lib.on_device(x, weight, residual):
+        data, exps = _memory(_padded(M), K, x.device)
+        rows = FP8Rows(data, exps, (M, K))
+        x, weight = _in_rows(x), weight.contiguous()
+        h = None
+        if residual is not None: residual, h = _in_rows(residual), torch.empty(M, K, dtype=x.dtype, device=x.device)
+        if M: _lib.call("gaac_fp8_rows", TYPES[x.dtype], x, _row_stride(x), residual, 0 if residual is None else _row_stride(residual), weight, float(eps), M, K, h, data, exps, _padded(M), 1, 0, _lib.stream)
+        return rows if h is None else (rows, h)
+
+
+def _operands(what: str, x, weight: FP8Weight, gated: bool, out_dtype):
+    if not isinstance(weight, FP8Weight) or weight.gated != gated:
+        raise RuntimeError(f"{what} expects an FP8Weight of {'a gate and an up projection' if gated else 'one weight'}" + (f", got {type(weight).__name__}" if not isinstance(weight, FP8Weight) else ""))
+    if out_dtype not in TYPES: raise RuntimeError(f"{what} makes bf16, fp16 or fp32, not {out_dtype}")
+    if not isinstance(x, FP8Rows):
+        _check_rows(what, x, MAX_WIDTH)
+        _lib.no_backward(what, x)
+    if x.shape[1] != weight.K or x.shape[0] > MAX_ROWS: raise RuntimeError(f"{what} expects up to 2^20 rows of the weight's {weight.K} inputs, got {list(x.shape)}")
+
+
+def _product(what, x, weight, gated, out_dtype):
+    _operands(what, x, weight, gated, out_dtype)
+    if not isinstance(x, FP8Rows): x = quantize_fp8(x)
+    M = x.shape[0]
+    with _lib.on_device(x.data, x.exps, weight.data, weight.exps):
+        out = torch.empty(M, weight.N, dtype=out_dtype, device=x.device)
+        if M: _lib.call("gaac_fp8_product", x.data, x.exps, weight.data, weight.exps, M, weight.N, weight.K, int(gated), TYPES[out_dtype], out, weight.N, _lib.stream)
+        return out
+
+
+def fp8_linear(x: torch.Tensor | FP8Rows, weight: FP8Weight, out_dtype: torch.dtype | None = None) -> torch.Tensor:
+    """x [M, K], rows in 8 bits or a tensor (bf16, fp16 or fp32) that is brought into 8 bits first -> x weight^T [M, N], of out_dtype, by default x's type, bf16 for rows in 8 bits.
+    Sums in 32 bits, in an order that depends on the sizes only, rounded once."""
+    return _product("fp8_linear", x, weight, False, out_dtype or (torch.bfloat16 if isinstance(x, FP8Rows) else x.dtype))
+
+
+def fp8_gated(x: torch.Tensor | FP8Rows, weight: FP8Weight, out_dtype: torch.dtype = torch.bfloat16, quantize: bool = False):
+    """x as for fp8_linear, weight FP8Weight(gate, up) -> silu(x gate^T) * (x up^T) [M, N], both sums in 32 bits, of out_dtype; with quantize the FP8Rows of that result in bf16, what
+    quantize_fp8 makes of it."""
+    if quantize and out_dtype != torch.bfloat16: raise RuntimeError(f"fp8_gated brings its result in bf16 into 8 bits, not {out_dtype}")
+    out = _product("fp8_gated", x, weight, True, out_dtype)
+    return quantize_fp8(out) if quantize else out

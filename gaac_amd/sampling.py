@@ -1,5 +1,6 @@
-"""Sampling of one token per row from logits, with given random numbers."""
+"""Sampling of one token per row from logits, with given random numbers; log probabilities of given tokens."""
 from __future__ import annotations
+from typing import NamedTuple
 import torch
 from . import _lib
 from .rope import TYPES
@@ -47,4 +48,46 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_
         work = torch.empty(work_bytes(B, V), dtype=torch.uint8, device=logits.device)
         if V > 1 and logits.stride(1) != 1 or B > 1 and logits.stride(0) < 0: logits = logits.contiguous()
         _lib.call("gaac_sample", TYPES[logits.dtype], logits, logits.stride(0) if B > 1 else 0, B, V, u.contiguous(), t_rows, float(t), k_rows, max(0, min(int(k), V)), p_rows, float(p), m_rows, float(m), work, work.numel(), out, _lib.stream)
+        return out
+
+
+MAX_TOP = 64
+
+
+class LogProbs(NamedTuple):
+    """What token_logprobs returns."""
+    logprob: torch.Tensor                       # fp32 [B]
+    rank: torch.Tensor                          # int64 [B]
+    entropy: torch.Tensor                       # fp32 [B]
+    top_logprobs: torch.Tensor | None = None    # fp32 [B, top]
+    top_tokens: torch.Tensor | None = None      # int64 [B, top]
+
+
+def logprobs_work_bytes(B: int, V: int, top: int) -> int:
+    """Scratch of a call: none for rows of one segment of 8192 logits, otherwise for each segment its sums and its `top` best tokens."""
+    segments = -(-V // 8192)
+    return 0 if segments == 1 else B * segments * (16 + 8 * top)
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> LogProbs:
+    """logits [B, V] (bf16, fp16 or fp32, rows any stride apart), tokens int64 [B] -> of each row, with log p_i = x_i - max - log(sum of exp(x - max)):
+
+      logprob   log p of the given token                     rank      tokens before it in the order of x descending, then index ascending (0: the likeliest)
+      entropy   -sum of p log p, in natural units            top_logprobs, top_tokens [B, top]      the first `top` (up to 64) of that order; None where top is 0
+
+    A NaN among the logits counts as -inf.  An infinite maximum: evenly among the tokens that have it.  A row with nothing but -inf: NaN for its log probabilities and entropy.  A token outside of the vocabulary:
+    NaN and rank -1.  Sums in 32 bits, in the same order each time.  One launch for vocabularies up to 8192, otherwise two; no wait, no backward pass."""
+    if logits.dim() != 2 or logits.dtype not in TYPES or not 1 <= logits.shape[1] <= MAX_VOCAB or logits.shape[0] > 1 << 23:
+        raise RuntimeError(f"token_logprobs expects logits bf16, fp16 or fp32 [B, V], V up to {MAX_VOCAB}, B up to 2^23, got {logits.dtype} {list(logits.shape)}")
+    B, V = logits.shape
+    if tokens.dtype != torch.int64 or tuple(tokens.shape) != (B,): raise RuntimeError(f"token_logprobs expects tokens int64 [{B}], got {tokens.dtype} {list(tokens.shape)}")
+    if not 0 <= top <= min(MAX_TOP, V): raise RuntimeError(f"token_logprobs gives 0 to {min(MAX_TOP, V)} alternatives of {V} logits, not {top}")
+    _lib.no_backward("token_logprobs", logits)
+    with _lib.on_device(logits, tokens):
+        new = lambda dtype, *shape: torch.empty(shape, dtype=dtype, device=logits.device)
+        out = LogProbs(new(torch.float32, B), new(torch.int64, B), new(torch.float32, B), *((new(torch.float32, B, top), new(torch.int64, B, top)) if top else (None, None)))
+        if B == 0: return out
+        work = new(torch.uint8, logprobs_work_bytes(B, V, top))
+        if V > 1 and logits.stride(1) != 1: logits = logits.contiguous()
+        _lib.call("gaac_logprobs", TYPES[logits.dtype], logits, logits.stride(0) if B > 1 else 0, B, V, tokens.contiguous(), top, work, work.numel(), *out, _lib.stream)
         return out

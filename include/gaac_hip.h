@@ -274,6 +274,28 @@ int gaac_qk_norm_rope(int type, const void* q, const void* k, long q_token_strid
 int gaac_sample(int type, const void* logits, long row_stride, int B, int V, const float* u, const float* temperature_rows, float temperature, const int* top_k_rows,
                 int top_k, const float* top_p_rows, float top_p, const float* min_p_rows, float min_p, void* work, long work_bytes, int64_t* out, void* stream);
 
+/* Rows in 8 bits (128 elements of a row share a power of two; tiles of 16 rows, the format is stated in gaac_amd/csrc/fp8.hip): data uint8 [padded_rows/16][ceil(K/128)][2048],
+ * exps uint8 [ceil(K/512)][padded_rows][4], padded_rows a multiple of 16 that holds the rows; rows behind the last and bytes of exps behind the last block need not be set.
+ * Rows of two tensors may alternate by tiles: this one has tiles tile_first, tile_first + tile_step, ...
+ * gaac_fp8_rows: rows x [M, K] (type as above, rows a stride in elements apart) into 8 bits; with a weight [K] after the root-mean-square norm x * rsqrt(mean(x^2) + eps) * weight
+ * (K up to 32768), and with a residual [M, K] of the sum of both, which is also written: sum [M, K], contiguous, not over the inputs. */
+int gaac_fp8_rows(int type, const void* x, long x_row_stride, const void* residual, long residual_row_stride, const void* weight, float eps, int M, int K,
+                  void* sum, void* data, void* exps, long padded_rows, int tile_step, int tile_first, void* stream);
+/* gaac_fp8_values: the values of such rows, bf16. */
+int gaac_fp8_values(const void* data, const void* exps, long padded_rows, int tile_step, int tile_first, int M, int K, void* out, long out_row_stride,
+                    void* stream);
+/* gaac_fp8_product: out [M, N] = x w^T, x M rows in 8 bits (padded to a multiple of 16), w N rows likewise; gated: w holds the rows of two weights of N rows, alternating by tiles, out = silu(x w0^T) *
+ * (x w1^T).  out of out_type, rows a stride in elements apart. */
+int gaac_fp8_product(const void* x, const void* x_exps, const void* w, const void* w_exps, int M, int N, int K, int gated, int out_type, void* out,
+                     long out_row_stride, void* stream);
+
+/* Of each row of logits [B, V] (type as above, rows row_stride elements apart): logprob [B] of the given token, rank [B] = tokens before it in the order of logits (ties: lower index
+ * first; -1 for a token outside of the vocabulary, whose logprob is NaN), entropy [B], and the `top` (up to 64) first of that order with their log probabilities, [B, top].  A NaN among
+ * the logits counts as -inf.  work: scratch of this call, 16-byte aligned, need not be set to anything: B * s * (16 + 8 * top) bytes, s = ceil(V / 8192), or none
+ * where s is 1. */
+int gaac_logprobs(int type, const void* logits, long row_stride, int B, int V, const int64_t* tokens, int top, void* work, long work_bytes, float* logprob,
+                  int64_t* rank, float* entropy, float* top_logprobs, int64_t* top_tokens, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
