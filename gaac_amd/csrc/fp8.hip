@@ -6,7 +6,8 @@
 //
 // 16 rows by one block are a tile, 2048 bytes in the order of the operands of the scaled 16x16x128 product, a lane's 16 bytes next to each other: row m, element
 // 32 g + 16 j + i of the block at byte 1024 j + 16 (16 g + m) + i.  (Which elements of a block a lane group has is free, as long as both operands agree: they share one power of
-// two.)  A row of tiles is the blocks one after the other.  The exponent bytes of four blocks are a dword, byte s that of block 4 q + s, dword [q][row]: the
+// two.)  The tiles of a block of K lie in a row, those of the next block
+// behind them: blocks of threads that go along K together read memory in one piece.  The exponent bytes of four blocks are a dword, byte s that of block 4 q + s, dword [q][row]: the
 // instruction picks the byte, so a dword serves four products.  Weights of a gated pair alternate: tile 2 t holds 16 rows of the gate, tile 2 t + 1 the same rows of the other.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -86,9 +87,28 @@ __device__ __forceinline__ unsigned max16(unsigned x) {
   x = max(x, rotated<0x128>(x)); x = max(x, rotated<0x124>(x)); x = max(x, rotated<0x122>(x)); x = max(x, rotated<0x121>(x));      // row_ror 8, 4, 2, 1
   return x;
 }
+// Sum over the wave, for all lanes, in the vector unit: rotations within 16 lanes, then halves swapped.
+template <int CTRL> __device__ __forceinline__ double rotated_sum(double x) {
+  const u2 v = __builtin_bit_cast(u2, x);
+  return x + __builtin_bit_cast(double, u2{rotated<CTRL>(v[0]), rotated<CTRL>(v[1])});
+}
 __device__ __forceinline__ double wave_sum(double x) {
-  for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o);
-  return x;
+  x = rotated_sum<0x128>(x); x = rotated_sum<0x124>(x); x = rotated_sum<0x122>(x); x = rotated_sum<0x121>(x);
+  u2 v = __builtin_bit_cast(u2, x);
+  u2 p = __builtin_bit_cast(u2, __builtin_amdgcn_permlane16_swap(v[0], v[0], false, false)), q = __builtin_bit_cast(u2, __builtin_amdgcn_permlane16_swap(v[1], v[1], false, false));
+  x = __builtin_bit_cast(double, u2{p[0], q[0]}) + __builtin_bit_cast(double, u2{p[1], q[1]});
+  v = __builtin_bit_cast(u2, x);
+  p = __builtin_bit_cast(u2, __builtin_amdgcn_permlane32_swap(v[0], v[0], false, false)); q = __builtin_bit_cast(u2, __builtin_amdgcn_permlane32_swap(v[1], v[1], false, false));
+  return __builtin_bit_cast(double, u2{p[0], q[0]}) + __builtin_bit_cast(double, u2{p[1], q[1]});
+}
+
+// y in 32 bits, rounded to an odd last bit where bits are lost: rounding once more, to 8 bits, then gives what rounding y itself would.  It matters only where the nearest number of 32 bits is a border between
+// two codes, which has 19 zeros at its end.
+__device__ __forceinline__ float to_odd(double y) {
+  const float f = (float)y;
+  const double d = y - (double)f;
+  const unsigned u = word(f);
+  return d == 0.0 || (u & 1u) || !(fabsf(f) < __builtin_inff()) ? f : bits((d > 0.0) == (f > 0.f) ? u + 1 : u - 1);
 }
 
 // ---------------------------------------------------------------------------------------------------- rows into 8 bits
@@ -102,65 +122,64 @@ struct RowsArgs {
   bool whole;
 };
 
-// `waves` waves a row, a lane CH runs of 8 elements of it, 16 lanes a block.  The sum of squares and the norm in 64 bits, which cost nothing beside the memory: a result next to the border
-// between two codes is then nearly always rounded as the formula says.
+// A block a row, of `waves` waves; a lane takes CH runs of 8 elements, 16 lanes a block of 128.  Bound by HBM: 16384 x 4096 in bf16 52 us (201 MB, 3.9 TB/s; a large copy makes 4.7 to 5.2), with norm and residual 113 (470 MB,
+// 4.2 TB/s); by launch and latency for a few rows (4 x 4096: 2.3, 3.6).  The sum of squares and the norm in 64 bits, which costs nothing beside the memory: a result next to the border between two
+// codes is rounded as the formula says.
 template <typename T, bool NORM, int CH>
 __global__ __launch_bounds__(1024) void k_fp8_rows(RowsArgs a) {
   __shared__ double sums[16];
-  const int l = threadIdx.x & 63, wave = threadIdx.x >> 6, part = wave % a.waves, row = blockIdx.x * ((blockDim.x >> 6) / a.waves) + wave / a.waves;
-  const bool there = row < a.M;
+  const int l = threadIdx.x & 63, part = threadIdx.x >> 6;
+  // A cache line of the result has pieces of 8 rows.  Blocks go to the XCDs in turns, each of which has its own L2: the rows of a tile are those of blocks that go to the same one (16384 x 4096: 62 us
+  // with rows in the blocks' order, 52 so).
+  const int turn = blockIdx.x & ~127u, in_turn = blockIdx.x & 127u, row = turn + 128 <= (int)gridDim.x ? turn + in_turn % 8 * 16 + in_turn / 8 : (int)blockIdx.x;
   const T* src = static_cast<const T*>(a.x) + row * a.x_rs;
+  const auto at = [&](int i) { return 8 * ((i * a.waves + part) * 64 + l); };
   float x[CH][8];
 #pragma unroll
-  for (int i = 0; i < CH; ++i) {
-    const int k = 8 * ((i * a.waves + part) * 64 + l);
-    load_some(src + k, there ? a.K - k : 0, a.whole, x[i]);
-  }
+  for (int i = 0; i < CH; ++i) load_some(src + at(i), a.K - at(i), a.whole, x[i]);
   if constexpr (NORM) {
     if (a.residual != nullptr) {
       const T* res = static_cast<const T*>(a.residual) + row * a.r_rs;
       T* out = static_cast<T*>(a.sum) + (long)row * a.K;
 #pragma unroll
       for (int i = 0; i < CH; ++i) {
-        const int k = 8 * ((i * a.waves + part) * 64 + l), n = there ? a.K - k : 0;
         float r[8];
-        load_some(res + k, n, a.whole, r);
+        load_some(res + at(i), a.K - at(i), a.whole, r);
         for (int j = 0; j < 8; ++j) x[i][j] += r[j];
-        store_some(out + k, n, a.whole, x[i]);
+        store_some(out + at(i), a.K - at(i), a.whole, x[i]);
       }
     }
+    float g[CH][8];      // (on their way while the sum is made)
+#pragma unroll
+    for (int i = 0; i < CH; ++i) load_some(static_cast<const T*>(a.weight) + at(i), a.K - at(i), a.whole, g[i]);
     double sum = 0;
 #pragma unroll
     for (int i = 0; i < CH; ++i)
       for (int j = 0; j < 8; ++j) sum = __builtin_fma((double)x[i][j], (double)x[i][j], sum);
     sum = wave_sum(sum);
     if (a.waves > 1) {
-      if (l == 0) sums[wave] = sum;
+      if (l == 0) sums[part] = sum;
       __syncthreads();
       sum = 0;
-      for (int i = 0; i < a.waves; ++i) sum += sums[wave - part + i];
+      for (int i = 0; i < a.waves; ++i) sum += sums[i];
     }
     const double r = 1.0 / __builtin_sqrt(sum / a.K + (double)a.eps);
-    const T* w = static_cast<const T*>(a.weight);
 #pragma unroll
     for (int i = 0; i < CH; ++i) {
-      const int k = 8 * ((i * a.waves + part) * 64 + l);
-      float g[8];
-      load_some(w + k, a.K - k, a.whole, g);
-      for (int j = 0; j < 8; ++j) x[i][j] = (float)((double)x[i][j] * r * (double)g[j]);
+      float y[8];
+      unsigned least = ~0u;
+      for (int j = 0; j < 8; ++j) { y[j] = (float)((double)x[i][j] * r * (double)g[i][j]); least = min(least, word(y[j]) & 0x7ffffu); }
+      if (least == 0) for (int j = 0; j < 8; ++j) y[j] = to_odd((double)x[i][j] * r * (double)g[i][j]);
+      for (int j = 0; j < 8; ++j) x[i][j] = at(i) + j < a.K ? y[j] : 0.f;      // (behind the row's end 0 * r may be a NaN)
     }
   }
-  if (!there) return;
   const long tile_row = (long)(row >> 4) * a.tile_step + a.tile_first;
 #pragma unroll
   for (int i = 0; i < CH; ++i) {
-    const int c = (i * a.waves + part) * 64 + l, kb = c >> 4, p = c & 15;
+    const int c = at(i) / 8, kb = c >> 4, p = c & 15;
     if (kb >= a.nb) continue;
-    if constexpr (NORM) {      // (behind the row's end 0 * r may be a NaN)
-      if (8 * c + 8 > a.K) for (int j = 0; j < 8; ++j) x[i][j] = 8 * c + j < a.K ? x[i][j] : 0.f;
-    }
     const unsigned e = exponent_byte(max16(magnitude8(x[i])));
-    *reinterpret_cast<u2*>(a.data + (tile_row * a.nb + kb) * TILE + 1024 * (p >> 1 & 1) + 16 * (16 * (p >> 2) + (row & 15)) + 8 * (p & 1)) = encode8(x[i], e);
+    *reinterpret_cast<u2*>(a.data + (kb * (a.pad >> 4) + tile_row) * TILE + 1024 * (p >> 1 & 1) + 16 * (16 * (p >> 2) + (row & 15)) + 8 * (p & 1)) = encode8(x[i], e);
     if (p == 0) a.exps[((kb >> 2) * a.pad + 16 * tile_row + (row & 15)) * 4 + (kb & 3)] = (uint8_t)e;
   }
 }
@@ -170,7 +189,7 @@ __global__ __launch_bounds__(256) void k_fp8_values(const uint8_t* data, const u
   const int p = threadIdx.x & 15, m = threadIdx.x >> 4, kb = blockIdx.x % nb;
   const long tile = blockIdx.x / nb, row = 16 * tile + m, tile_row = tile * tile_step + tile_first;
   if (row >= M) return;
-  const u2 w = *reinterpret_cast<const u2*>(data + (tile_row * nb + kb) * TILE + 1024 * (p >> 1 & 1) + 16 * (16 * (p >> 2) + m) + 8 * (p & 1));
+  const u2 w = *reinterpret_cast<const u2*>(data + (kb * (pad >> 4) + tile_row) * TILE + 1024 * (p >> 1 & 1) + 16 * (16 * (p >> 2) + m) + 8 * (p & 1));
   const unsigned e = exps[((kb >> 2) * pad + 16 * tile_row + m) * 4 + (kb & 3)];
   const float s = bits(e << 23);
   float x[8];
@@ -186,19 +205,20 @@ __global__ __launch_bounds__(256) void k_fp8_values(const uint8_t* data, const u
 
 // ---------------------------------------------------------------------------------------------------- products
 struct ProductArgs {
-  const void* x;             // rows in 8 bits, or as they come
+  const void* x;
   const unsigned* x_exps;
   const uint8_t* w;
   const unsigned* w_exps;
   void* out;
-  long x_rs, x_pad, w_pad, out_rs;
+  long x_pad, w_pad, out_rs;
   int M, N, K, nb, tiles;      // tiles: of 16 weight rows
   bool whole;                  // four outputs at a time
 };
 
 // One block of K of a tile of weights by one of rows, byte S of both exponent words.  The scaled product adds eight elements' products as whole multiples of 2^-13 of the largest one's power of
 // two, cutting what is below, and only these sums in 32 bits (found by trying: so does the product without scales).  That is an error of 1.5e-5 to 3e-5 of the output's size, a sixtieth of bf16's rounding and an
-// eighth of fp16's.  Outputs in 32 bits would show it: for them (EXACT) the codes go as bf16, scale included, which holds them exactly, into products that are added in 32 bits, at half the rate.
+// eighth of fp16's.  Outputs in 32 bits would show it, and so would what is rounded twice behind a sum (a gated block's inner result, where it crosses a border): for outputs in 32 bits, and where it costs nothing,
+// the codes go as bf16 (EXACT), scale included, which holds them exactly, into products that are added in 32 bits, at half the rate.
 template <int S> struct Byte { static constexpr int value = S; };
 template <bool EXACT> struct Operand;
 template <> struct Operand<false> {
@@ -242,54 +262,102 @@ template <typename O> __device__ __forceinline__ void put_some(O* p, f4 v, int n
   for (int i = 0; i < 4; ++i) if (i < n) p[i] = (O)v[i];
 }
 
+// Outputs col .. col + 3 of a row; of a gated pair from both sums.
+template <typename O, bool GATED> __device__ __forceinline__ void finish(const ProductArgs& a, int row, int col, f4 v, f4 up) {
+  if constexpr (GATED) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) v[k] = silu(v[k]) * up[k];
+  }
+  if (row < a.M && col < a.N) put_some(static_cast<O*>(a.out) + row * a.out_rs + col, v, a.N - col, a.whole);
+}
+
 // Few rows: the weights go by once.  A block has NT tiles of weights and MT of rows; its eight waves share the blocks of K out, four (a dword of exponents) at a time, and their sums meet in LDS, in
-// the waves' order.
-template <typename O, int MT, int NT, bool GATED>
-__global__ __launch_bounds__(512) void k_fp8_stream(ProductArgs a) {
+// the waves' order.  A wave holds the operands of AHEAD steps in registers, each set loaded again as soon as it is used: what bounds it is how many loads are on their way.
+template <typename O, int MT, int NT, int AHEAD, bool GATED>
+__global__ __launch_bounds__(512, 2) void k_fp8_stream(ProductArgs a) {
   static_assert(!GATED || NT % 2 == 0, "tiles of a gated pair alternate");
-  constexpr bool EXACT = sizeof(O) == 4;
-  __shared__ f4 part[8][MT * NT][64];
-  const int l = threadIdx.x & 63, wave = threadIdx.x >> 6, m = l & 15, g = l >> 4;
+  constexpr bool EXACT = sizeof(O) == 4 || MT == 1;
+  constexpr int WAVES = 8;
+  __shared__ f4 part[WAVES][MT * NT][64];
+  const int l = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), m = l & 15, g = l >> 4;
   const uint8_t *w[NT], *x[MT];
   const unsigned *we[NT], *xe[MT];
 #pragma unroll
   for (int i = 0; i < NT; ++i) {      // (a tile behind the last one is the last one again, and written by nobody)
     const long t = min((int)blockIdx.x * NT + i, a.tiles - 1);
-    w[i] = a.w + t * a.nb * TILE; we[i] = a.w_exps + 16 * t + m;
+    w[i] = a.w + t * TILE; we[i] = a.w_exps + 16 * t;
   }
 #pragma unroll
   for (int i = 0; i < MT; ++i) {
     const long t = min((int)blockIdx.y * MT + i, (a.M - 1) >> 4);
-    x[i] = static_cast<const uint8_t*>(a.x) + t * a.nb * TILE; xe[i] = a.x_exps + 16 * t + m;
+    x[i] = static_cast<const uint8_t*>(a.x) + t * TILE; xe[i] = a.x_exps + 16 * t;
   }
+  struct Set { u4 w[NT][2], x[MT][2]; } set[AHEAD];
+  unsigned ew[NT], ex[MT], next_w[NT], next_x[MT];
+  const auto load = [&](Set& s, int kb) {
+    const long at = min(kb, a.nb - 1);      // (behind the last block of K the last one again, which nobody uses)
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+      for (int h = 0; h < 2; ++h) s.w[i][h] = *reinterpret_cast<const u4*>(w[i] + at * a.w_pad * BLOCK + 1024 * h + 16 * l);
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+      for (int h = 0; h < 2; ++h) s.x[i][h] = *reinterpret_cast<const u4*>(x[i] + at * a.x_pad * BLOCK + 1024 * h + 16 * l);
+  };
+  const auto load_exps = [&](int q) {
+#pragma unroll
+    for (int i = 0; i < NT; ++i) next_w[i] = we[i][q * a.w_pad + m];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) next_x[i] = xe[i][q * a.x_pad + m];
+  };
+  const auto next_exps = [&] {
+#pragma unroll
+    for (int i = 0; i < NT; ++i) ew[i] = next_w[i];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) ex[i] = next_x[i];
+  };
   f4 acc[MT][NT] = {};
-  for (int q = wave; 4 * q < a.nb; q += 8) {
-    unsigned ew[NT], ex[MT];
+  const auto step = [&](auto byte) {
+    constexpr int S = decltype(byte)::value;
+    const Set& s = set[S % AHEAD];
+    Operand<EXACT> ow[NT];
 #pragma unroll
-    for (int i = 0; i < NT; ++i) ew[i] = we[i][q * a.w_pad];
+    for (int i = 0; i < NT; ++i) ow[i] = Operand<EXACT>::template of<S>(s.w[i][0], s.w[i][1], ew[i]);
 #pragma unroll
-    for (int i = 0; i < MT; ++i) ex[i] = xe[i][q * a.x_pad];
-    const auto step = [&](auto byte) {
-      constexpr int S = decltype(byte)::value;
-      const long at = (long)(4 * q + S) * TILE;
-      Operand<EXACT> ow[NT];
+    for (int j = 0; j < MT; ++j) {
+      const Operand<EXACT> ox = Operand<EXACT>::template of<S>(s.x[j][0], s.x[j][1], ex[j]);
 #pragma unroll
-      for (int i = 0; i < NT; ++i) ow[i] = operand<EXACT, S>(w[i] + at, l, ew[i]);
-#pragma unroll
-      for (int j = 0; j < MT; ++j) {
-        const Operand<EXACT> ox = operand<EXACT, S>(x[j] + at, l, ex[j]);
-#pragma unroll
-        for (int i = 0; i < NT; ++i) acc[j][i] = product<S>(ow[i], ox, acc[j][i]);
-      }
-    };
-    const int n = a.nb - 4 * q;
-    if (n >= 4) {
-      step(Byte<0>{}); step(Byte<1>{}); step(Byte<2>{}); step(Byte<3>{});
-    } else {
-      step(Byte<0>{});
-      if (n > 1) step(Byte<1>{});
-      if (n > 2) step(Byte<2>{});
+      for (int i = 0; i < NT; ++i) acc[j][i] = product<S>(ow[i], ox, acc[j][i]);
     }
+  };
+  const int quads = (a.nb + 3) / 4;
+  int q = wave;
+  if (q < quads) {
+    load_exps(q);
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) load(set[i], 4 * q + i);
+    __builtin_amdgcn_sched_barrier(0);
+    for (; q + WAVES < quads; q += WAVES) {
+      next_exps();
+      load_exps(q + WAVES);
+      const auto one = [&](auto byte) {
+        constexpr int S = decltype(byte)::value;
+        step(byte);
+        load(set[S % AHEAD], S + AHEAD < 4 ? 4 * q + S + AHEAD : 4 * (q + WAVES) + S + AHEAD - 4);
+        __builtin_amdgcn_sched_barrier(0);
+      };
+      one(Byte<0>{}); one(Byte<1>{}); one(Byte<2>{}); one(Byte<3>{});
+    }
+    next_exps();
+    const int n = a.nb - 4 * q;
+    step(Byte<0>{});
+    if constexpr (AHEAD == 2) load(set[0], 4 * q + 2);
+    __builtin_amdgcn_sched_barrier(0);
+    if (n > 1) step(Byte<1>{});
+    if constexpr (AHEAD == 2) load(set[1], 4 * q + 3);
+    __builtin_amdgcn_sched_barrier(0);
+    if (n > 2) step(Byte<2>{});
+    __builtin_amdgcn_sched_barrier(0);
+    if (n > 3) step(Byte<3>{});
   }
 #pragma unroll
   for (int j = 0; j < MT; ++j)
@@ -297,47 +365,256 @@ __global__ __launch_bounds__(512) void k_fp8_stream(ProductArgs a) {
     for (int i = 0; i < NT; ++i) part[wave][j * NT + i][l] = acc[j][i];
   __syncthreads();
   constexpr int EACH = GATED ? NT / 2 : NT;      // outputs of a tile of rows, by 16
-  for (int at = wave; at < MT * EACH; at += 8) {
+  for (int at = wave; at < MT * EACH; at += WAVES) {
     const int j = at / EACH, i = at % EACH;
     const auto sum = [&](int t) {
       f4 s = part[0][j * NT + t][l];
-      for (int k = 1; k < 8; ++k) s += part[k][j * NT + t][l];
+      for (int k = 1; k < WAVES; ++k) s += part[k][j * NT + t][l];
       return s;
     };
-    f4 v = sum(GATED ? 2 * i : i);
-    if constexpr (GATED) {
-      const f4 up = sum(2 * i + 1);
-      for (int k = 0; k < 4; ++k) v[k] = silu(v[k]) * up[k];
-    }
     const int row = 16 * ((int)blockIdx.y * MT + j) + m, col = 16 * ((int)blockIdx.x * EACH + i) + 4 * g;
-    if (row < a.M && col < a.N) put_some(static_cast<O*>(a.out) + row * a.out_rs + col, v, a.N - col, a.whole);
+    finish<O, GATED>(a, row, col, sum(GATED ? 2 * i : i), GATED ? sum(2 * i + 1) : f4{});
   }
 }
 
+// Many rows: tiles of both operands through LDS.  A block has WN x WM waves, a wave TN tiles of weights by TM of rows; a step is one block of K, whose tiles (whole kilobytes, in the
+// operands' order) go straight into LDS while the step before is computed, in two buffers by turns.
+typedef const __attribute__((address_space(1))) void* global_ptr;
+typedef __attribute__((address_space(3))) void* lds_ptr;
+
+template <typename O, int TN, int TM, int WN, int WM, int NBUF, bool GATED>
+__global__ __launch_bounds__(64 * WN * WM, TN * TM == 64 ? 1 : 2) void k_fp8_tiles(ProductArgs a, int blocks_n, int blocks_m) {
+  constexpr int W = WN * WM, TILES = WN * TN + WM * TM, LOADS = 2 * TILES / W, ROWS_W = 16 * WN * TN, ROWS = 16 * TILES;
+  static_assert(2 * TILES % W == 0 && ROWS_W % 64 == 0 && ROWS % 64 == 0 && TN % 2 == 0 && (NBUF == 2 || NBUF == 4), "every wave loads as many kilobytes; a wave loads the exponents of 64 rows of one operand; tiles of a gated pair alternate");
+  constexpr bool EXACT = sizeof(O) == 4;
+  __shared__ __attribute__((aligned(16))) uint8_t buf0[TILES * TILE];
+  __shared__ __attribute__((aligned(16))) uint8_t buf1[TILES * TILE];
+  __shared__ __attribute__((aligned(16))) uint8_t buf2[NBUF == 4 ? TILES * TILE : 16];
+  __shared__ __attribute__((aligned(16))) uint8_t buf3[NBUF == 4 ? TILES * TILE : 16];
+  __shared__ unsigned exps[2 * ROWS];
+  const auto buffer = [&](auto byte) -> uint8_t* {
+    constexpr int B = decltype(byte)::value % NBUF;
+    if constexpr (B == 0) return buf0; else if constexpr (B == 1) return buf1; else if constexpr (B == 2) return buf2; else return buf3;
+  };
+  const int l = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wn = wave % WN, wm = wave / WN, m = l & 15, g = l >> 4;
+  // Blocks that follow each other go to different XCDs: each XCD has a run of the tiles, in columns of 8 blocks of rows, so that what its L2 holds is used by all of its blocks.
+  const int total = blocks_n * blocks_m, xcd = blockIdx.x & 7, each = total / 8, over = total % 8;
+  const int id = xcd * each + min(xcd, over) + (int)(blockIdx.x >> 3);
+  const int group = id / (8 * blocks_n), in_group = id - group * 8 * blocks_n, high = min(8, blocks_m - 8 * group);
+  const int bm = 8 * group + in_group % high, bn = in_group / high;
+  const int last_x = (a.M - 1) >> 4;
+  const int last_q = (a.nb - 1) >> 2;
+  const uint8_t* src[LOADS];
+  long stride[LOADS];
+#pragma unroll
+  for (int i = 0; i < LOADS; ++i) {
+    const int c = wave * LOADS + i, t = c >> 1;
+    src[i] = (t < WN * TN ? a.w + (long)min(bn * WN * TN + t, a.tiles - 1) * TILE : static_cast<const uint8_t*>(a.x) + (long)min(bm * WM * TM + t - WN * TN, last_x) * TILE) + 1024 * (c & 1);
+    stride[i] = (t < WN * TN ? a.w_pad : a.x_pad) * BLOCK;
+  }
+  // (behind the last block of K the last one again, which nobody uses: no step is different from the others)
+  const auto fetch = [&](uint8_t* to, int kb) {
+    const long at = min(kb, a.nb - 1);
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const uint8_t* from = src[i] + at * stride[i];
+      asm("" : "+s"(from));
+      __builtin_amdgcn_global_load_lds((global_ptr)(from + 16u * l), (lds_ptr)(to + (wave * LOADS + i) * 1024), 16, 0, 0);
+    }
+  };
+  constexpr int PARTS = (ROWS / 64 + W - 1) / W;      // runs of 64 rows whose exponents a wave loads
+  const unsigned* exps_src[PARTS];
+  long exps_pad[PARTS];
+#pragma unroll
+  for (int i = 0; i < PARTS; ++i) {
+    const int r = 64 * (i * W + wave);
+    exps_pad[i] = r < ROWS_W ? a.w_pad : a.x_pad;
+    exps_src[i] = (r < ROWS_W ? a.w_exps : a.x_exps) + min((r < ROWS_W ? (long)bn * ROWS_W + r : (long)bm * (ROWS - ROWS_W) + r - ROWS_W) + l, exps_pad[i] - 1);
+  }
+  const auto fetch_exps = [&](int q) {
+#pragma unroll
+    for (int i = 0; i < PARTS; ++i)
+      if (ROWS % (64 * W) == 0 || 64 * (i * W + wave) < ROWS)
+        __builtin_amdgcn_global_load_lds((global_ptr)(exps_src[i] + min(q, last_q) * exps_pad[i]), (lds_ptr)(exps + (q & 1) * ROWS + 64 * (i * W + wave)), 4, 0, 0);
+  };
+  // A step's first operands are read while the last products of the step before run: the last TAIL tiles of weights go through the rows one row tile at a time, and each of these is then replaced by the next step's.
+  // Before that all of a buffer has been read, so the barrier stands there, once a step, and the buffer is filled again behind it.
+  constexpr int TAIL = 3, RING = 4;
+  static_assert(TN % RING == 0, "the slot of a step's first tile is free while the last TAIL are in use");
+  struct Raw { u4 a, b; };
+  const auto read = [&](const uint8_t* tile) { return Raw{*reinterpret_cast<const u4*>(tile + 16 * l), *reinterpret_cast<const u4*>(tile + 1024 + 16 * l)}; };
+  f4 acc[TM][TN] = {};
+  Raw w[RING], x[TM];
+  unsigned ew[TN], ex[TM], next_w[TN], next_x[TM];
+  const auto read_exps = [&](int q) {
+    const unsigned* e = exps + (q & 1) * ROWS;
+#pragma unroll
+    for (int i = 0; i < TN; ++i) next_w[i] = e[16 * (wn * TN + i) + m];
+#pragma unroll
+    for (int j = 0; j < TM; ++j) next_x[j] = e[ROWS_W + 16 * (wm * TM + j) + m];
+  };
+  // All of this wave's loads but those of the last NBUF - 2 steps are in LDS, all of its reads in registers; then the other waves' too.
+  const auto barrier = [&] {
+    constexpr int LATER = (NBUF - 2) * LOADS;
+    __builtin_amdgcn_s_waitcnt(0x0070 | (LATER & 15) | (LATER >> 4) << 14);
+    asm volatile("" ::: "memory"); __builtin_amdgcn_s_barrier(); asm volatile("" ::: "memory");
+  };
+  const int w_at = wn * TN * TILE, x_at = (WN * TN + wm * TM) * TILE;
+  // Keeps products where they stand between reads and barrier.
+  const auto pin = [&](f4& v) {
+    if constexpr (TN * TM == 64) asm volatile("" : "+a"(v)); else asm volatile("" : "+v"(v));
+  };
+  const auto step = [&](auto byte, int kb) {
+    constexpr int S = decltype(byte)::value;
+    uint8_t *now = buffer(Byte<S>{}), *then = buffer(Byte<S + 1>{});
+    Operand<EXACT> ox[TM];
+#pragma unroll
+    for (int j = 0; j < TM; ++j) ox[j] = Operand<EXACT>::template of<S>(x[j].a, x[j].b, ex[j]);
+#pragma unroll
+    for (int i = 0; i < TN - TAIL; ++i) {
+      w[(i + TAIL) % RING] = read(now + w_at + (i + TAIL) * TILE);
+      const Operand<EXACT> ow = Operand<EXACT>::template of<S>(w[i % RING].a, w[i % RING].b, ew[i]);
+#pragma unroll
+      for (int j = 0; j < TM; ++j) acc[j][i] = product<S>(ow, ox[j], acc[j][i]);
+#pragma unroll
+      for (int j = 0; j < TM; ++j) pin(acc[j][i]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    barrier();
+    if constexpr (S == 3) read_exps((kb >> 2) + 1);      // (before more is on its way into LDS: the compiler would wait for all of it)
+    fetch(now, kb + NBUF);
+    if constexpr (S == 0) fetch_exps((kb >> 2) + 1);
+    Operand<EXACT> ow[TAIL];
+#pragma unroll
+    for (int i = 0; i < TAIL; ++i) ow[i] = Operand<EXACT>::template of<S>(w[(TN - TAIL + i) % RING].a, w[(TN - TAIL + i) % RING].b, ew[TN - TAIL + i]);
+    w[0] = read(then + w_at);
+#pragma unroll
+    for (int j = 0; j < TM; ++j) {
+#pragma unroll
+      for (int i = 0; i < TAIL; ++i) acc[j][TN - TAIL + i] = product<S>(ow[i], ox[j], acc[j][TN - TAIL + i]);
+#pragma unroll
+      for (int i = 0; i < TAIL; ++i) pin(acc[j][TN - TAIL + i]);
+      x[j] = read(then + x_at + j * TILE);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int i = 1; i < TAIL; ++i) w[i] = read(then + w_at + i * TILE);
+  };
+  fetch_exps(0);
+  fetch(buf0, 0);
+  fetch(buf1, 1);
+  if constexpr (NBUF == 4) { fetch(buf2, 2); fetch(buf3, 3); }
+  __builtin_amdgcn_s_waitcnt(0x0070 | ((NBUF - 1) * LOADS & 15) | (NBUF - 1) * LOADS >> 4 << 14);
+  __syncthreads();
+  read_exps(0);
+#pragma unroll
+  for (int j = 0; j < TM; ++j) x[j] = read(buf0 + x_at + j * TILE);
+#pragma unroll
+  for (int i = 0; i < TAIL; ++i) w[i] = read(buf0 + w_at + i * TILE);
+  const auto next_exps = [&] {
+#pragma unroll
+    for (int i = 0; i < TN; ++i) ew[i] = next_w[i];
+#pragma unroll
+    for (int j = 0; j < TM; ++j) ex[j] = next_x[j];
+  };
+  int kb = 0;
+  for (; kb + 4 <= a.nb; kb += 4) {
+    next_exps();
+    step(Byte<0>{}, kb); step(Byte<1>{}, kb + 1); step(Byte<2>{}, kb + 2); step(Byte<3>{}, kb + 3);
+  }
+  if (kb < a.nb) {
+    next_exps();
+    step(Byte<0>{}, kb);
+    if (kb + 1 < a.nb) step(Byte<1>{}, kb + 1);
+    if (kb + 2 < a.nb) step(Byte<2>{}, kb + 2);
+  }
+#pragma unroll
+  for (int i = 0; i < TAIL; ++i) asm volatile("" : : "v"(w[i].a), "v"(w[i].b));
+  __builtin_amdgcn_s_waitcnt(0x0070);      // no load of this block is on its way into LDS that another one may have by then
+#pragma unroll
+  for (int j = 0; j < TM; ++j)
+#pragma unroll
+    for (int i = 0; i < TN; i += GATED ? 2 : 1)
+      finish<O, GATED>(a, 16 * ((bm * WM + wm) * TM + j) + m, 16 * (((bn * WN + wn) * TN + i) >> GATED) + 4 * g, acc[j][i], acc[j][GATED ? i + 1 : i]);
+}
+
+template <typename O, int TN, int TM, int WN, int WM, int NBUF> void launch_tiles(const ProductArgs& a, bool gated, hipStream_t s) {
+  const int n = (a.tiles + WN * TN - 1) / (WN * TN), m = (a.M + 16 * WM * TM - 1) / (16 * WM * TM);
+  if (gated) k_fp8_tiles<O, TN, TM, WN, WM, NBUF, true><<<n * m, 64 * WN * WM, 0, s>>>(a, n, m);
+  else k_fp8_tiles<O, TN, TM, WN, WM, NBUF, false><<<n * m, 64 * WN * WM, 0, s>>>(a, n, m);
+}
+template <typename O, int MT, int NT, int AHEAD> void launch_stream(const ProductArgs& a, bool gated, hipStream_t s) {
+  const dim3 grid((a.tiles + NT - 1) / NT, (a.M + 16 * MT - 1) / (16 * MT));
+  if constexpr (NT % 2 == 0) {
+    if (gated) return k_fp8_stream<O, MT, NT, AHEAD, true><<<grid, 512, 0, s>>>(a);
+  }
+  k_fp8_stream<O, MT, NT, AHEAD, false><<<grid, 512, 0, s>>>(a);
+}
+
+// Which form is taken: the one that should end first, its time being start + steps * (round * rounds + share * blocks / 256), rounds = blocks / 256 rounded up (a round: a block on each CU), steps the blocks of K
+// that a wave goes through.  The constants, in us, are fitted to the times of all forms over 102 sizes (1 to 4096 rows by 1024 to 28672 x 512 to 14336); over these the chosen form takes 2.5 % longer than the
+// best one in the mean (fp32: 0.7 %).  Up to 16 rows, and wherever a block has one tile of rows, the products are the exact ones for every type: the weights' way from memory hides them (4 x 4096 x 4096 4.8 us, 4.9 exact;
+// 4 x 28672 x 4096 21.8, 23.5).  Some of both sides, us, weights resident in turns (rows x N x K, outputs of 16 bits: stream of 1 x 1, 1 x 2, 2 x 2, 4 x 2 tiles | 64 x 64, 64 x 128, 128 x 128 with
+// four buffers, with two, 256 x 256 through LDS):
+//   4 x 4096 x 4096   4.9 5.5 5.8 6.7 | 9.7 13 17 21 42          48 x 4096 x 14336  28 23 16.6 22.9 | 31 47 51 87 142         64 x 28672 x 4096  71 69 41 33 | 26 22.5 24 32 48
+//   200 x 4096 x 4096  20 15 14 11.2 | 10.7 14 19 22 47          600 x 6144 x 4096  66 50 44 38 | 33 32 24 30 52              1024 x 28672 x 4096  1018 1018 524 328 | 215 221 159 146 115
+//   2048 x 4096 x 14336  1006 566 355 250 | 192 180 126 112 149  4096 x 4096 x 4096  314 227 195 148 | 124 125 87 71 63
+struct Form { int n, m, waves; float start, round, share; };      // tiles of weights and of rows a block, waves that share out K
+constexpr Form FORMS[9] = {{1, 1, 8, 1.61f, .33f, .34f}, {2, 1, 8, 1.71f, .51f, .31f}, {2, 2, 8, 1.82f, .5f, .65f}, {2, 4, 8, 2.32f, .61f, 1.03f},
+                           {4, 4, 1, 4.16f, .2f, .05f}, {8, 4, 1, 3.8f, .37f, .11f}, {8, 8, 1, 5.45f, .36f, .24f}, {8, 8, 1, 3.13f, .59f, .3f}, {16, 16, 1, 4.51f, 1.11f, .64f}};
+constexpr Form EXACT_FORMS[6] = {{1, 1, 8, 1.43f, .38f, .32f}, {2, 1, 8, .55f, .81f, .22f}, {2, 2, 8, 2.27f, .82f, .22f}, {2, 4, 8, .97f, .78f, 1.17f}, {4, 4, 1, 5.36f, .31f, .08f}, {8, 8, 1, 7.81f, .86f, .24f}};
+template <int COUNT> int form_of(const Form (&forms)[COUNT], const ProductArgs& a, bool gated) {
+  int best = -1;
+  float least = 0;
+  for (int i = 0; i < (a.M <= 16 ? 2 : COUNT); ++i) {
+    const Form& f = forms[i];
+    if (gated && f.n % 2 != 0) continue;
+    const long blocks = (long)((a.tiles + f.n - 1) / f.n) * ((a.M + 16 * f.m - 1) / (16 * f.m));
+    const int steps = f.waves == 1 ? a.nb : 4 * (((a.nb + 3) / 4 + f.waves - 1) / f.waves);
+    const float time = f.start + steps * (f.round * ((blocks + 255) / 256) + f.share * blocks / 256.f);
+    if (best < 0 || time < least) { best = i; least = time; }
+  }
+  return best;
+}
 template <typename O> void launch_product(const ProductArgs& a, bool gated, hipStream_t s) {
-  if (gated) {
-    const int most = (a.tiles + 1) / 2;
-    if (a.M <= 16) k_fp8_stream<O, 1, 2, true><<<dim3(most, 1), 512, 0, s>>>(a);
-    else k_fp8_stream<O, 4, 2, true><<<dim3(most, (a.M + 63) / 64), 512, 0, s>>>(a);
+  if constexpr (sizeof(O) == 4) {
+    switch (form_of(EXACT_FORMS, a, gated)) {
+      case 0: return launch_stream<O, 1, 1, 4>(a, gated, s);
+      case 1: return launch_stream<O, 1, 2, 4>(a, gated, s);
+      case 2: return launch_stream<O, 2, 2, 4>(a, gated, s);
+      case 3: return launch_stream<O, 4, 2, 2>(a, gated, s);
+      case 4: return launch_tiles<O, 4, 1, 1, 4, 4>(a, gated, s);
+      default: return launch_tiles<O, 4, 4, 2, 2, 2>(a, gated, s);
+    }
   } else {
-    if (a.M <= 16) k_fp8_stream<O, 1, 1, false><<<dim3(a.tiles, 1), 512, 0, s>>>(a);
-    else k_fp8_stream<O, 4, 2, false><<<dim3((a.tiles + 1) / 2, (a.M + 63) / 64), 512, 0, s>>>(a);
+    switch (form_of(FORMS, a, gated)) {
+      case 0: return launch_stream<O, 1, 1, 4>(a, gated, s);
+      case 1: return launch_stream<O, 1, 2, 4>(a, gated, s);
+      case 2: return launch_stream<O, 2, 2, 4>(a, gated, s);
+      case 3: return launch_stream<O, 4, 2, 2>(a, gated, s);
+      case 4: return launch_tiles<O, 4, 1, 1, 4, 4>(a, gated, s);
+      case 5: return launch_tiles<O, 4, 1, 2, 4, 4>(a, gated, s);
+      case 6: return launch_tiles<O, 4, 2, 2, 4, 4>(a, gated, s);
+      case 7: return launch_tiles<O, 4, 2, 2, 4, 2>(a, gated, s);
+      default: return launch_tiles<O, 8, 4, 2, 4, 2>(a, gated, s);
+    }
   }
 }
 
-template <typename T, int CH> void launch_rows(const RowsArgs& a, int block, hipStream_t s) {
-  const unsigned grid = (unsigned)((a.M + block / a.waves - 1) / (block / a.waves));
-  if constexpr (CH < 8) if (a.weight != nullptr) return k_fp8_rows<T, true, CH><<<grid, 64 * block, 0, s>>>(a);
-  k_fp8_rows<T, false, CH><<<grid, 64 * block, 0, s>>>(a);
+template <typename T, int CH> void launch_rows(const RowsArgs& a, hipStream_t s) {
+  if constexpr (CH < 8) {
+    if (a.weight != nullptr) return k_fp8_rows<T, true, CH><<<a.M, 64 * a.waves, 0, s>>>(a);
+  }
+  k_fp8_rows<T, false, CH><<<a.M, 64 * a.waves, 0, s>>>(a);
 }
+// One run a lane for few rows, where latency counts, two for many (us, one / two runs, with the norm: 4 x 4096 4.0 / 4.8, 300 x 4096 6.3 / 6.9, 777 x 5000 12.5 / 10.9, 16384 x 4096 125 / 113); more only where a block's 16 waves
+// would not do.  (The norm of 8 runs would not fit the registers.)
 template <typename T> void launch_rows(RowsArgs a, hipStream_t s) {
-  int ch = 1;
   const auto waves = [&](int n) { return (a.nb * 16 + 64 * n - 1) / (64 * n); };
-  const int most = a.weight != nullptr ? 4 : 8;      // (the norm of 8 runs would not fit the registers)
-  while (ch < most && (waves(ch) > 16 || (long)a.M * waves(ch) > 8192)) ch *= 2;
+  int ch = (long)a.M * waves(1) <= 4096 ? 1 : 2;
+  while (waves(ch) > 16) ch *= 2;
   a.waves = waves(ch);
-  const int block = (long)a.M * a.waves > 2048 ? 16 / a.waves * a.waves : a.waves;
-  if (ch == 1) launch_rows<T, 1>(a, block, s); else if (ch == 2) launch_rows<T, 2>(a, block, s); else if (ch == 4) launch_rows<T, 4>(a, block, s); else launch_rows<T, 8>(a, block, s);
+  if (ch == 1) launch_rows<T, 1>(a, s); else if (ch == 2) launch_rows<T, 2>(a, s); else if (ch == 4) launch_rows<T, 4>(a, s); else launch_rows<T, 8>(a, s);
 }
 
 uintptr_t address(const void* p) { return reinterpret_cast<uintptr_t>(p); }
@@ -380,7 +657,7 @@ extern "C" int gaac_fp8_product(const void* x, const void* x_exps, const void* w
   GAAC_REQUIRE((address(x) | address(w)) % 16 == 0 && (address(x_exps) | address(w_exps)) % 4 == 0, "gaac_fp8_product: data must be 16-byte aligned, exponents 4-byte");
   const int size = out_type == 2 ? 4 : 2, tiles = (N + 15) / 16 * (gated ? 2 : 1);
   const bool whole = address(out) % (4 * size) == 0 && out_row_stride % 4 == 0;
-  const ProductArgs a{x, static_cast<const unsigned*>(x_exps), static_cast<const uint8_t*>(w), static_cast<const unsigned*>(w_exps), out, 0, 16l * ((M + 15) / 16), 16l * tiles, out_row_stride, M, N, K, (K + BLOCK - 1) / BLOCK, tiles, whole};
+  const ProductArgs a{x, static_cast<const unsigned*>(x_exps), static_cast<const uint8_t*>(w), static_cast<const unsigned*>(w_exps), out, 16l * ((M + 15) / 16), 16l * tiles, out_row_stride, M, N, K, (K + BLOCK - 1) / BLOCK, tiles, whole};
   if (out_type == 0) launch_product<__bf16>(a, gated != 0, (hipStream_t)stream);
   else if (out_type == 1) launch_product<_Float16>(a, gated != 0, (hipStream_t)stream);
   else launch_product<float>(a, gated != 0, (hipStream_t)stream);

@@ -274,7 +274,7 @@ int gaac_qk_norm_rope(int type, const void* q, const void* k, long q_token_strid
 int gaac_sample(int type, const void* logits, long row_stride, int B, int V, const float* u, const float* temperature_rows, float temperature, const int* top_k_rows,
                 int top_k, const float* top_p_rows, float top_p, const float* min_p_rows, float min_p, void* work, long work_bytes, int64_t* out, void* stream);
 
-/* Rows in 8 bits (128 elements of a row share a power of two; tiles of 16 rows, the format is stated in gaac_amd/csrc/fp8.hip): data uint8 [padded_rows/16][ceil(K/128)][2048],
+/* Rows in 8 bits (128 elements of a row share a power of two; tiles of 16 rows, the format is stated in gaac_amd/csrc/fp8.hip): data uint8 [ceil(K/128)][padded_rows/16][2048],
  * exps uint8 [ceil(K/512)][padded_rows][4], padded_rows a multiple of 16 that holds the rows; rows behind the last and bytes of exps behind the last block need not be set.
  * Rows of two tensors may alternate by tiles: this one has tiles tile_first, tile_first + tile_step, ...
  * gaac_fp8_rows: rows x [M, K] (type as above, rows a stride in elements apart) into 8 bits; with a weight [K] after the root-mean-square norm x * rsqrt(mean(x^2) + eps) * weight
