@@ -563,7 +563,127 @@ PyObject* draw(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return THPVariable_Wrap(out);
   });
 }
-#define GAAC_WHOLE_CALLS(X) X(attend) X(token_append) X(prompt_store) X(page_encode) X(page_decode) X(fp4_prefill) X(fp4_append) X(fp4_attend) X(fp4_read) X(norm_rope) X(draw)
+// Rows in 8 bits, their products, and log probabilities, the same way.  Host us a call, Python / here: see the numbers at gaac_amd/fp8.py's calls.
+long blocks_of(long K) { return (K + 127) / 128; }
+long padded(long rows) { return (rows + 15) / 16 * 16; }
+at::ScalarType type_of(long code) {
+  if (code < 0 || code > 2) throw Otherwise{};
+  return code == 0 ? at::kBFloat16 : code == 1 ? at::kHalf : at::kFloat;
+}
+// [M, K] with elements next to each other -> its row stride
+long rows_of(const at::Tensor& t, long most) {
+  if (t.dim() != 2 || t.size(0) == 0 || t.size(0) > 1l << 24 || t.size(1) == 0 || t.size(1) > most || (t.size(1) > 1 && t.stride(1) != 1)) throw Otherwise{};
+  return t.size(0) > 1 ? t.stride(0) : 0;
+}
+struct Rows8 {
+  at::Tensor data, exps;
+  Rows8(const at::Tensor& like, long M, long K) : data(bytes(like, {padded(M) * blocks_of(K) * 128})), exps(bytes(like, {(blocks_of(K) + 3) / 4 * padded(M) * 4})) {}
+};
+
+// fp8_rows(x, weight or None, eps, residual or None, stream) -> (data, exps) or (data, exps, sum)
+PyObject* fp8_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return whole_call(n, 5, [&]() -> PyObject* {
+    const at::Tensor& x = here(a[0]);
+    const int type = float_type(x);
+    const bool norm = a[1] != Py_None, add = a[3] != Py_None;
+    const long x_rs = rows_of(x, norm ? 32768 : 65536), M = x.size(0), K = x.size(1);
+    if (loses_gradient(x)) throw Otherwise{};
+    void *w = nullptr, *r = nullptr, *h = nullptr;
+    long r_rs = 0;
+    float eps = 0;
+    at::Tensor sum;
+    if (norm) {
+      const at::Tensor& t = here(a[1]);
+      if (t.scalar_type() != x.scalar_type() || t.dim() != 1 || t.size(0) != K || !t.is_contiguous() || loses_gradient(t) || !PyFloat_CheckExact(a[2])) throw Otherwise{};
+      w = t.data_ptr(); eps = static_cast<float>(PyFloat_AS_DOUBLE(a[2]));
+    }
+    if (add) {
+      const at::Tensor& t = here(a[3]);
+      if (!norm || t.scalar_type() != x.scalar_type() || t.sizes() != x.sizes() || loses_gradient(t)) throw Otherwise{};
+      r_rs = rows_of(t, 32768); r = t.data_ptr();
+      sum = bytes(x, {M, K}, x.scalar_type()); h = sum.data_ptr();
+    }
+    void* stream = stream_of(a[4]);
+    const Rows8 out(x, M, K);
+    must("gaac_fp8_rows", without_gil([&] {
+      return p_gaac_fp8_rows(type, x.data_ptr(), x_rs, r, r_rs, w, eps, static_cast<int>(M), static_cast<int>(K), h, out.data.data_ptr(), out.exps.data_ptr(), padded(M), 1, 0, stream);
+    }));
+    if (add) return Py_BuildValue("(NNN)", THPVariable_Wrap(out.data), THPVariable_Wrap(out.exps), THPVariable_Wrap(sum));
+    return Py_BuildValue("(NN)", THPVariable_Wrap(out.data), THPVariable_Wrap(out.exps));
+  });
+}
+
+// fp8_multiply(x [M, K], or data of M rows; exps or None, M, weight's data, exps, N, K, gated, type, stream) -> [M, N]
+PyObject* fp8_multiply(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return whole_call(n, 10, [&]() -> PyObject* {
+    const at::Tensor &x = here(a[0]), &w = here(a[3]), &we = here(a[4]);
+    const long M = number(a[2]), N = number(a[5]), K = number(a[6]), type = number(a[8]);
+    const bool rows = a[1] != Py_None;
+    if (M <= 0 || M > 1 << 20) throw Otherwise{};
+    const int gated = PyObject_IsTrue(a[7]);
+    const at::ScalarType out_type = type_of(type);
+    long x_rs = 0;
+    if (!rows) {
+      x_rs = rows_of(x, 65536);
+      if (x.size(0) != M || x.size(1) != K || loses_gradient(x)) throw Otherwise{};
+    }
+    const int x_type = rows ? 0 : float_type(x);
+    void* stream = stream_of(a[9]);
+    at::Tensor data, exps;
+    if (rows) { data = x; exps = here(a[1]); }
+    else {
+      const Rows8 made(x, M, K);
+      data = made.data; exps = made.exps;
+      must("gaac_fp8_rows", without_gil([&] {
+        return p_gaac_fp8_rows(x_type, x.data_ptr(), x_rs, nullptr, 0, nullptr, 0.f, static_cast<int>(M), static_cast<int>(K), nullptr, data.data_ptr(), exps.data_ptr(), padded(M), 1, 0, stream);
+      }));
+    }
+    at::Tensor out = bytes(x, {M, N}, out_type);
+    must("gaac_fp8_product", without_gil([&] {
+      return p_gaac_fp8_product(data.data_ptr(), exps.data_ptr(), w.data_ptr(), we.data_ptr(), static_cast<int>(M), static_cast<int>(N), static_cast<int>(K), gated, static_cast<int>(type), out.data_ptr(), N, stream);
+    }));
+    return THPVariable_Wrap(out);
+  });
+}
+
+// fp8_values(data, exps, M, K, tile step, first tile, stream) -> bf16 [M, K]
+PyObject* fp8_values(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return whole_call(n, 7, [&]() -> PyObject* {
+    const at::Tensor &data = here(a[0]), &exps = here(a[1]);
+    const long M = number(a[2]), K = number(a[3]), step = number(a[4]), first = number(a[5]);
+    if (M <= 0) throw Otherwise{};
+    void* stream = stream_of(a[6]);
+    at::Tensor out = bytes(data, {M, K}, at::kBFloat16);
+    must("gaac_fp8_values", without_gil([&] {
+      return p_gaac_fp8_values(data.data_ptr(), exps.data_ptr(), padded(M) * step, static_cast<int>(step), static_cast<int>(first), static_cast<int>(M), static_cast<int>(K), out.data_ptr(), K, stream);
+    }));
+    return THPVariable_Wrap(out);
+  });
+}
+
+// logprobs(logits, tokens, top, stream) -> (logprob, rank, entropy, top_logprobs or None, top_tokens or None)
+PyObject* logprobs(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return whole_call(n, 4, [&]() -> PyObject* {
+    const at::Tensor &x = here(a[0]), &t = here(a[1]);
+    const int type = float_type(x);
+    const long top = number(a[2]);
+    if (x.dim() != 2 || x.size(0) == 0 || x.size(0) > 1l << 23 || x.size(1) == 0 || x.size(1) > (1l << 20) - 16 || (x.size(1) > 1 && x.stride(1) != 1) || loses_gradient(x)) throw Otherwise{};
+    const long B = x.size(0), V = x.size(1);
+    if (t.dim() != 1 || t.size(0) != B || t.scalar_type() != at::kLong || !t.is_contiguous() || top < 0 || top > std::min(64l, V)) throw Otherwise{};
+    void* stream = stream_of(a[3]);
+    const long segments = (V + 8191) / 8192, work_bytes = segments == 1 ? 0 : B * segments * (16 + 8 * top);      // logprobs_work_bytes in sampling.py
+    at::Tensor work = bytes(x, {work_bytes}), value = bytes(x, {B}, at::kFloat), rank = bytes(x, {B}, at::kLong), entropy = bytes(x, {B}, at::kFloat), top_values, top_tokens;
+    if (top > 0) { top_values = bytes(x, {B, top}, at::kFloat); top_tokens = bytes(x, {B, top}, at::kLong); }
+    must("gaac_logprobs", without_gil([&] {
+      return p_gaac_logprobs(type, x.data_ptr(), B > 1 ? x.stride(0) : 0, static_cast<int>(B), static_cast<int>(V), static_cast<int64_t*>(t.data_ptr()), static_cast<int>(top), work.data_ptr(), work_bytes,
+                             static_cast<float*>(value.data_ptr()), static_cast<int64_t*>(rank.data_ptr()), static_cast<float*>(entropy.data_ptr()), top > 0 ? static_cast<float*>(top_values.data_ptr()) : nullptr,
+                             top > 0 ? static_cast<int64_t*>(top_tokens.data_ptr()) : nullptr, stream);
+    }));
+    return Py_BuildValue("(NNNNN)", THPVariable_Wrap(value), THPVariable_Wrap(rank), THPVariable_Wrap(entropy), top > 0 ? THPVariable_Wrap(top_values) : Py_NewRef(Py_None),
+                         top > 0 ? THPVariable_Wrap(top_tokens) : Py_NewRef(Py_None));
+  });
+}
+#define GAAC_WHOLE_CALLS(X) X(attend) X(token_append) X(prompt_store) X(page_encode) X(page_decode) X(fp4_prefill) X(fp4_append) X(fp4_attend) X(fp4_read) X(norm_rope) X(draw) X(fp8_rows) X(fp8_multiply) X(fp8_values) X(logprobs)
 
 // bind(path): the entry points of the library at path (the product or one of its measurement builds); AttributeError names a missing one
 PyObject* bind(PyObject*, PyObject* path) {

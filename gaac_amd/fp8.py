@@ -57,6 +57,8 @@ class FP8Rows:
 
 
 def _values(data, exps, M, K, step, first):
+    out = (_lib._calls or _lib.calls()).fp8_values(data, exps, M, K, step, first, _lib.stream)
+    if out is not None: return out
     with _lib.on_device(data, exps):
         out = torch.empty(M, K, dtype=torch.bfloat16, device=data.device)
         if M: _lib.call("gaac_fp8_values", data, exps, _padded(M) * step, step, first, M, K, out, K, _lib.stream)
@@ -106,6 +108,8 @@ class FP8Weight:
 
 def quantize_fp8(x: torch.Tensor) -> FP8Rows:
     """x [M, K] (bf16, fp16 or fp32, K up to 65536, rows any stride apart) -> its rows in 8 bits.  One launch."""
+    out = (_lib._calls or _lib.calls()).fp8_rows(x, None, None, None, _lib.stream)
+    if out is not None: return FP8Rows(*out, tuple(x.shape))
     _check_rows("quantize_fp8", x, MAX_WIDTH)
     _lib.no_backward("quantize_fp8", x)
     M, K = x.shape
@@ -122,6 +126,8 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, resid
       y = h * rsqrt(mean(h^2) + eps) * weight,   h = x, or x + residual
 
     with a residual [M, K] of x's type (FP8Rows, h): h in that type, a new contiguous tensor.  The norm is taken of the sum in 32 bits, before it is rounded for h; the sum of squares and y in 64 bits.  One launch."""
+    out = (_lib._calls or _lib.calls()).fp8_rows(x, weight, eps, residual, _lib.stream) if weight is not None else None
+    if out is not None: return FP8Rows(out[0], out[1], tuple(x.shape)) if residual is None else (FP8Rows(out[0], out[1], tuple(x.shape)), out[2])
     _check_rows("rms_norm_fp8", x, MAX_NORM_WIDTH)
     M, K = x.shape
     if weight.dtype != x.dtype or tuple(weight.shape) != (K,): raise RuntimeError(f"rms_norm_fp8 expects weight {x.dtype} [{K}], got {weight.dtype} {list(weight.shape)}")
@@ -149,6 +155,11 @@ def _operands(what: str, x, weight: FP8Weight, gated: bool, out_dtype):
 
 
 def _product(what, x, weight, gated, out_dtype):
+    if isinstance(weight, FP8Weight) and weight.gated == gated and out_dtype in TYPES:
+        data, exps = (x.data, x.exps) if isinstance(x, FP8Rows) else (x, None)
+        if x.shape[-1] == weight.K:
+            out = (_lib._calls or _lib.calls()).fp8_multiply(data, exps, x.shape[0], weight.data, weight.exps, weight.N, weight.K, gated, TYPES[out_dtype], _lib.stream)
+            if out is not None: return out
     _operands(what, x, weight, gated, out_dtype)
     if not isinstance(x, FP8Rows): x = quantize_fp8(x)
     M = x.shape[0]

@@ -77,6 +77,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
 
     A NaN among the logits counts as -inf.  An infinite maximum: evenly among the tokens that have it.  A row with nothing but -inf: NaN for its log probabilities and entropy.  A token outside of the vocabulary:
     NaN and rank -1.  Sums in 32 bits, in the same order each time.  One launch for vocabularies up to 8192, otherwise two; no wait, no backward pass."""
+    out = (_lib._calls or _lib.calls()).logprobs(logits, tokens, top, _lib.stream)
+    if out is not None: return LogProbs(*out)
     if logits.dim() != 2 or logits.dtype not in TYPES or not 1 <= logits.shape[1] <= MAX_VOCAB or logits.shape[0] > 1 << 23:
         raise RuntimeError(f"token_logprobs expects logits bf16, fp16 or fp32 [B, V], V up to {MAX_VOCAB}, B up to 2^23, got {logits.dtype} {list(logits.shape)}")
     B, V = logits.shape
