@@ -12,11 +12,13 @@ built on it.
                                                          captured as a graph with padded rows at slot -1, the escape-capacity check
                                                          every 16 steps
 
-The model is a Llama-architecture stack (RMSNorm, rotary embedding, GQA, SwiGLU) on plain torch ops with random weights; queries and keys
+The model is a Llama-architecture stack (RMSNorm, rotary embedding, GQA, SwiGLU) with random weights, on plain torch ops, or with ModelConfig.weights = "fp8" on weights in 8 bits by rms_norm_fp8, fp8_linear
+and fp8_gated (8.06 bits a weight of the layers; the embedding and the head stay bf16); queries and keys
 are rotated, and with ModelConfig.qk_norm normalised for each head before, by qk_norm_rope.  Where the reference calls flash-attn (prefill, and the uncompressed decode path) this module uses torch's scaled_dot_product_attention and the
 library's own BF16 decode kernel; the KV backend of a layer is CompressedKVCache (`Attention.gaac`), FP4KVCache
 (`Attention.fp4`: 4 bits, 3.76 times smaller than BF16, not lossless) or an uncompressed BF16 cache (`Attention.bf16`), the baseline.  A step takes the likeliest
-token or, with start_decode(sampling=...), one drawn by sample() from given random numbers."""
+token or, with start_decode(sampling=...), one drawn by sample() from given random numbers; with start_decode(logprobs=n) it also says what that token was worth and which n were
+likelier, as prefill(logprobs=n) does of a prompt's tokens."""
 from __future__ import annotations
 import contextlib
 from dataclasses import dataclass
@@ -26,7 +28,8 @@ from .kv_cache import CompressedKVCache
 from .kernel import bf16_attention, choose_nsplit, AttnWorkspace
 from .fp4_cache import FP4KVCache
 from .rope import qk_norm_rope
-from .sampling import sample
+from .sampling import sample, token_logprobs, LogProbs
+from .fp8 import FP8Weight, fp8_gated, fp8_linear, rms_norm_fp8
 
 D = 128
 
@@ -169,11 +172,13 @@ class ModelConfig:
     rms_eps: float = 1e-5
     max_len: int = 32768 + 256
     qk_norm: bool = False       # RMSNorm of every query and key head before the rotation
+    weights: str = "bf16"       # of the layers' projections: "bf16" or "fp8"
 
 
 class Weights:
-    """Random-init BF16 weights of the stack (no checkpoint is read)."""
+    """Random-init weights of the stack (no checkpoint is read): BF16, with cfg.weights "fp8" those of the layers' projections brought into 8 bits, which needs a GPU."""
     def __init__(self, cfg: ModelConfig, device="cuda", seed: int = 0):
+        if cfg.weights not in ("bf16", "fp8"): raise RuntimeError(f"weights are bf16 or fp8, not {cfg.weights}")
         g = torch.Generator(device=device).manual_seed(seed)
         w = lambda *shape, std=0.02: (torch.randn(*shape, generator=g, device=device, dtype=torch.float32) * std).to(torch.bfloat16)
         self.cfg = cfg
@@ -181,9 +186,14 @@ class Weights:
         self.lm_head = w(cfg.vocab, cfg.hidden)
         self.final_norm = torch.ones(cfg.hidden, dtype=torch.bfloat16, device=device)
         qkv_out = (cfg.n_heads + 2 * cfg.n_kv_heads) * D
-        self.layers = [dict(norm1=torch.ones(cfg.hidden, dtype=torch.bfloat16, device=device), qkv=w(qkv_out, cfg.hidden),
-                            o=w(cfg.hidden, cfg.n_heads * D), norm2=torch.ones(cfg.hidden, dtype=torch.bfloat16, device=device),
-                            gate_up=w(2 * cfg.ffn, cfg.hidden), down=w(cfg.hidden, cfg.ffn)) for _ in range(cfg.n_layers)]
+        self.layers = []
+        for _ in range(cfg.n_layers):
+            layer = dict(norm1=torch.ones(cfg.hidden, dtype=torch.bfloat16, device=device), qkv=w(qkv_out, cfg.hidden),
+                         o=w(cfg.hidden, cfg.n_heads * D), norm2=torch.ones(cfg.hidden, dtype=torch.bfloat16, device=device),
+                         gate_up=w(2 * cfg.ffn, cfg.hidden), down=w(cfg.hidden, cfg.ffn))
+            if cfg.weights == "fp8":      # the same random weights, a layer at a time
+                layer.update(qkv=FP8Weight(layer["qkv"]), o=FP8Weight(layer["o"]), gate_up=FP8Weight(layer["gate_up"][:cfg.ffn], layer["gate_up"][cfg.ffn:]), down=FP8Weight(layer["down"]))
+            self.layers.append(layer)
         if cfg.qk_norm:
             for l in self.layers: l.update(q_norm=torch.ones(D, dtype=torch.bfloat16, device=device), k_norm=torch.ones(D, dtype=torch.bfloat16, device=device))
         half = torch.arange(0, D, 2, device=device, dtype=torch.float32) / D
@@ -192,7 +202,7 @@ class Weights:
 
     def nbytes(self) -> int:
         n = self.embed.numel() + self.lm_head.numel() + self.final_norm.numel()
-        return 2 * (n + sum(t.numel() for l in self.layers for t in l.values()))
+        return 2 * n + sum(t.nbytes for l in self.layers for t in l.values())
 
 
 def _norm_rope_host(x: torch.Tensor, weight: torch.Tensor | None, cos: torch.Tensor, sin: torch.Tensor, eps: float) -> torch.Tensor:
@@ -234,6 +244,10 @@ class _Bf16Cache:
         return tokens * self.n_kv * 2 * D * 2
 
 
+def _joined(parts: list[LogProbs], join) -> LogProbs:
+    return LogProbs(*(None if x[0] is None else join(x) for x in zip(*parts)))
+
+
 class DecodeRunner:
     """Prefill sequences into slots, then run greedy decode steps for slots 0..B-1, optionally as one captured HIP graph."""
     def __init__(self, weights: Weights, n_slots: int, kv: str = "gaac", bases: dict | None = None, ovf_bytes_per_tile: int = 128,
@@ -263,12 +277,11 @@ class DecodeRunner:
         self.sampling = None
 
     # ---------------------------------------------------------------- layers
-    def _qkv(self, layer, x, pos):
+    def _heads(self, layer, qkv, pos):
         cfg = self.cfg
-        h = F.rms_norm(x, (cfg.hidden,), layer["norm1"], cfg.rms_eps)
-        qkv = F.linear(h, layer["qkv"]).view(x.shape[0], cfg.n_heads + 2 * cfg.n_kv_heads, D)
+        qkv = qkv.view(qkv.shape[0], cfg.n_heads + 2 * cfg.n_kv_heads, D)
         q, k, v = qkv[:, :cfg.n_heads], qkv[:, cfg.n_heads:cfg.n_heads + cfg.n_kv_heads], qkv[:, cfg.n_heads + cfg.n_kv_heads:]
-        if x.is_cuda: q, k = qk_norm_rope(q, k, pos, self.w.cos, self.w.sin, layer.get("q_norm"), layer.get("k_norm"), cfg.rms_eps)
+        if qkv.is_cuda: q, k = qk_norm_rope(q, k, pos, self.w.cos, self.w.sin, layer.get("q_norm"), layer.get("k_norm"), cfg.rms_eps)
         else:
             cos, sin = self.w.cos.index_select(0, pos), self.w.sin.index_select(0, pos)
             q, k = _norm_rope_host(q, layer.get("q_norm"), cos, sin, cfg.rms_eps), _norm_rope_host(k, layer.get("k_norm"), cos, sin, cfg.rms_eps)
@@ -280,25 +293,45 @@ class DecodeRunner:
         gu = F.linear(h, layer["gate_up"])
         return x + F.linear(F.silu(gu[:, :cfg.ffn]) * gu[:, cfg.ffn:], layer["down"])
 
+    def _layers(self, x, pos):
+        """The stack on embeddings x [N, hidden]; the context says how the layers attend."""
+        cfg, n = self.cfg, x.shape[0]
+        if cfg.weights == "bf16":
+            for layer, attn in zip(self.w.layers, self.attn):
+                h = F.rms_norm(x, (cfg.hidden,), layer["norm1"], cfg.rms_eps)
+                o = attn(*self._heads(layer, F.linear(h, layer["qkv"]), pos))
+                x = self._mlp(layer, x + F.linear(o.reshape(n, cfg.n_heads * D), layer["o"]))
+            return x
+        out = None      # of the layer before: added to x by the norm that follows
+        for layer, attn in zip(self.w.layers, self.attn):
+            if out is None: h = rms_norm_fp8(x, layer["norm1"], cfg.rms_eps)
+            else: h, x = rms_norm_fp8(out, layer["norm1"], cfg.rms_eps, residual=x)
+            o = attn(*self._heads(layer, fp8_linear(h, layer["qkv"]), pos))
+            h, x = rms_norm_fp8(fp8_linear(o.reshape(n, cfg.n_heads * D), layer["o"]), layer["norm2"], cfg.rms_eps, residual=x)
+            out = fp8_linear(fp8_gated(h, layer["gate_up"]), layer["down"])
+        return x if out is None else x + out
+
     # ---------------------------------------------------------------- prefill
     @torch.no_grad()
-    def prefill(self, slot: int, tokens: torch.Tensor) -> torch.Tensor:
+    def prefill(self, slot: int, tokens: torch.Tensor, logprobs: int | None = None):
         """tokens int64 [L] on the device, up to cfg.max_len: causal attention over the prompt's own K/V per layer, then the K/V go into `slot`.
-        Returns the logits of the last position [vocab] (fp32)."""
+        Returns the logits of the last position [vocab] (fp32); with logprobs, a number of alternatives, also the LogProbs of tokens 1 .. L - 1, each from the position before it."""
         cfg, L = self.cfg, tokens.shape[0]
         if L > cfg.max_len: raise RuntimeError(f"prompt has {L} tokens, the model's positions end at {cfg.max_len}")
         pos = torch.arange(L, device=tokens.device)
         x = self.w.embed.index_select(0, tokens)
         cu = torch.tensor([0, L], dtype=torch.int32, device=tokens.device)
         set_context(True, cu, cu, L, L, prefill_spans=[(slot, 0, L)])
-        for layer, attn in zip(self.w.layers, self.attn):
-            q, k, v = self._qkv(layer, x, pos)
-            o = attn(q, k, v)
-            x = self._mlp(layer, x + F.linear(o.reshape(L, cfg.n_heads * D), layer["o"]))
+        x = self._layers(x, pos)
         reset_context()
         self.lens[slot] = L
-        x = F.rms_norm(x[-1:], (cfg.hidden,), self.w.final_norm, cfg.rms_eps)
-        return F.linear(x, self.w.lm_head)[0].float()
+        logits = self._logits(x[-1:])[0].float()
+        if logprobs is None: return logits
+        parts = [token_logprobs(self._logits(x[i:min(i + 1024, L - 1)]), tokens[i + 1:min(i + 1024, L - 1) + 1], top=logprobs) for i in range(0, max(L - 1, 1), 1024)]
+        return logits, _joined(parts, torch.cat)
+
+    def _logits(self, x):
+        return F.linear(F.rms_norm(x, (self.cfg.hidden,), self.w.final_norm, self.cfg.rms_eps), self.w.lm_head)
 
     # ---------------------------------------------------------------- decode
     def _step(self, tokens: torch.Tensor, slots: torch.Tensor, lens: torch.Tensor, nsplit: int) -> torch.Tensor:
@@ -309,22 +342,19 @@ class DecodeRunner:
         x = self.w.embed.index_select(0, tokens)
         # decode inputs of the step (model_runner.py:209-215): the slot map of the batch rows; lengths stay on the device
         set_context(False, max_seqlen_k=cfg.max_len, context_lens=lens, kv_slots=slots)
-        for layer, attn in zip(self.w.layers, self.attn):
-            attn.nsplit = nsplit
-            q, k, v = self._qkv(layer, x, pos)
-            o = attn(q, k, v)
-            x = self._mlp(layer, x + F.linear(o.reshape(x.shape[0], cfg.n_heads * D), layer["o"]))
+        for attn in self.attn: attn.nsplit = nsplit
+        x = self._layers(x, pos)
         reset_context()
         lens += (slots >= 0).to(lens.dtype)
-        x = F.rms_norm(x, (cfg.hidden,), self.w.final_norm, cfg.rms_eps)
-        return F.linear(x, self.w.lm_head)
+        return self._logits(x)
 
     @torch.no_grad()
-    def start_decode(self, first_tokens: torch.Tensor, use_graph: bool = True, nsplit: int | None = None, sampling: dict | None = None):
+    def start_decode(self, first_tokens: torch.Tensor, use_graph: bool = True, nsplit: int | None = None, sampling: dict | None = None,
+                     logprobs: int | None = None):
         """first_tokens int64 [B]: the token each of slots 0..B-1 decodes next.  With use_graph the step (all layers, cache appends,
         attention, sampling, feeding the token back) is captured once and replayed.  sampling: arguments of sample() (temperature, top_k, top_p, min_p; numbers
         or tensors [B]), decode() then takes the random numbers; None: the likeliest token.  A row whose logits are all NaN or -inf has no token to draw: decode() returns
-        -1 for it, and the row goes on with token 0."""
+        -1 for it, and the row goes on with token 0.  logprobs: a number of alternatives; decode() then also returns the LogProbs of the tokens."""
         B, dev = first_tokens.shape[0], first_tokens.device
         self.B = B
         self.tok = first_tokens.clone()
@@ -333,7 +363,8 @@ class DecodeRunner:
         self.longest = max(self.dlens.tolist(), default=0)      # tokens of the longest row, known to the host
         self.nsplit = nsplit or (None if self.kv == "fp4" else choose_nsplit(B, self.cfg.n_kv_heads, self.cfg.max_len))      # (the 4-bit cache chooses by itself)
         self.sampling, self.u = sampling, torch.zeros(B, dtype=torch.float32, device=dev)
-        self.logits = self.chosen = None
+        self.logits = self.chosen = self.worth = None
+        self.logprobs = logprobs
         if self.counters:
             torch.cuda.synchronize()      # the graph that goes has run for the last time
             for c, counters in self.counters: c.give_back(counters)
@@ -364,22 +395,24 @@ class DecodeRunner:
         if self.sampling is None:
             self.tok.copy_(self.logits.argmax(-1))
             self.chosen = self.tok
+            if self.logprobs is not None: self.worth = token_logprobs(self.logits, self.tok, top=self.logprobs)
         else:
             self.chosen = sample(self.logits, self.u, **self.sampling)
+            if self.logprobs is not None: self.worth = token_logprobs(self.logits, self.chosen, top=self.logprobs)
             torch.clamp(self.chosen, min=0, out=self.tok)      # -1, a row without a token: the next step reads the embedding of token 0, not what lies before the table
 
     @torch.no_grad()
     def decode(self, n_steps: int, forced: torch.Tensor | None = None, keep_logits: bool = False, u: torch.Tensor | None = None):
         """Runs n_steps steps (with sampling: u fp32 [n_steps, B] in [0, 1), a random number for every token); returns the generated tokens [n_steps, B] (device).  forced int64 [n_steps, B]: teacher forcing: the
         token every row consumes at step i+1 is forced[i] instead of the one it generated (the returned tokens are still the model's
-        own choices).  keep_logits: also returns the logits of every step [n_steps, B, vocab] (fp32).  Refused where a row would come to hold more than cfg.max_len
+        own choices).  keep_logits: also returns the logits of every step [n_steps, B, vocab] (fp32); with start_decode(logprobs=n) also, last, the tokens' LogProbs [n_steps, B, ..].  Refused where a row would come to hold more than cfg.max_len
         tokens: there is no position for them, and no room."""
         if (u is None) != (self.sampling is None) or u is not None and tuple(u.shape) != (n_steps, self.B):
             raise RuntimeError(f"decode expects u fp32 [{n_steps}, {self.B}] where start_decode was given sampling, and nothing otherwise")
         if self.longest + n_steps > self.cfg.max_len:
             self.longest = max(self.dlens.tolist(), default=0)      # (the caller may have taken tokens back)
             if self.longest + n_steps > self.cfg.max_len: raise RuntimeError(f"decode of {n_steps} steps: the longest row holds {self.longest} tokens, the model's positions end at {self.cfg.max_len}")
-        out, logits = [], []
+        out, logits, worth = [], [], []
         for i in range(n_steps):
             self.longest += 1
             if u is not None: self.u.copy_(u[i])
@@ -387,6 +420,7 @@ class DecodeRunner:
             else: self._one()
             out.append(self.chosen.clone())
             if keep_logits: logits.append(self.logits.float().clone())
+            if self.logprobs is not None: worth.append(LogProbs(*(None if x is None else x.clone() for x in self.worth)))
             if forced is not None: self.tok.copy_(forced[i])
             self.steps += 1
             if self.kv == "gaac" and self.steps % 16 == 0:      # every 16 steps a head finalizes at most one tile (model_runner.py:268-273)
@@ -395,7 +429,8 @@ class DecodeRunner:
             elif self.kv == "fp4" and self.steps % 16 == 0:
                 for c, n in zip(self.caches, torch.cat([c.overflow for c in self.caches]).tolist()): c.check_capacity(n)
         self.lens[:self.B] = self.dlens
-        return (torch.stack(out), torch.stack(logits)) if keep_logits else torch.stack(out)
+        result = [torch.stack(out)] + ([torch.stack(logits)] if keep_logits else []) + ([_joined(worth, torch.stack)] if self.logprobs is not None else [])
+        return result[0] if len(result) == 1 else tuple(result)
 
     # ---------------------------------------------------------------- accounting
     def kv_stats(self) -> dict:
