@@ -2,8 +2,8 @@
 //   p_i = exp(x_i - max) / S, S = sum of exp(x_i - max);  log p_i = (x_i - max) - log S;  entropy = log S - sum of exp(x_i - max) (x_i - max) / S
 // One read of the logits: a block takes a segment of 8192 of a row into registers, its maximum, and with it the sums of e^d and of d e^d; segments are joined with the factors
 // e^(max of one - max of all).  The order of tokens is x descending, then index ascending: as one 64-bit key, in which no two tokens are alike.  Each wave takes the
-// best key of every lane; the `top`-th best of these 64 is a bound that `top` tokens at least reach, the largest bound of the block's waves leaves little more than that
-// (alternatives lie far apart, most lanes have one), and these few are ranked by counting.
+// largest x of every lane, and of these 64 the n-th largest, n an eighth of `top`: the least of the block's eight is a bound that `top` tokens at least reach and few others (alternatives lie far apart, most lanes have
+// one), and these few are ranked by counting.  Where many reach it, as with tokens that are alike, the bound is one of keys: the larger of that, and of what `top` lanes of one wave reach.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include "gaac_capi.h"
@@ -11,7 +11,7 @@
 
 namespace {
 
-constexpr int THREADS = 512, WAVES = THREADS / 64, EACH = 16, SEGMENT = THREADS * EACH, MAX_TOP = 64, MAX_VOCAB = (1 << 20) - 16, MERGE = 256;
+constexpr int THREADS = 512, WAVES = THREADS / 64, EACH = 16, SEGMENT = THREADS * EACH, MAX_TOP = 64, MAX_VOCAB = (1 << 20) - 16;
 typedef unsigned long long u64;
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
@@ -21,38 +21,57 @@ __device__ __forceinline__ void load16(const __bf16* p, float* x) { const bf8 v 
 __device__ __forceinline__ void load16(const _Float16* p, float* x) { const h8 v = *reinterpret_cast<const h8*>(p); for (int i = 0; i < 8; ++i) x[i] = (float)v[i]; }
 __device__ __forceinline__ void load16(const float* p, float* x) { const f4 v = *reinterpret_cast<const f4*>(p); for (int i = 0; i < 4; ++i) x[i] = v[i]; }
 
-// e^d for d <= 0: the product with log2(e) in two parts, the second by the first two terms of its series (off by 2^-23 of itself, where one part alone would lose d's last bits).
+// e^d for -104 <= d <= 0: the product with log2(e) in two parts, the second by the first two terms of its series (off by 2^-22 of itself, where one part alone would lose d's last bits).
 __device__ __forceinline__ float exp_of(float d) {
-  const float t = d * 1.44269502f, r = __builtin_fmaf(d, 1.44269502f, -t) + d * 1.92596303e-8f;
+  const float t = d * 1.44269502f, r = __builtin_fmaf(d, 1.33497652e-8f, __builtin_fmaf(d, 1.44269502f, -t) * 0.693147181f);
   const float e = __builtin_amdgcn_exp2f(t);
-  return d > -104.f ? __builtin_fmaf(e, r * 0.693147181f, e) : 0.f;
+  return __builtin_fmaf(e, r, e);
 }
 __device__ __forceinline__ float cleaned(float x) { return x != x ? -__builtin_inff() : x; }      // NaN: a token that never comes
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) < __builtin_inff(); }
 __device__ __forceinline__ float distance(float x, float top) { return x == top ? 0.f : x - top; }      // (also where both are infinite)
 
 // The place in the order of tokens: larger is earlier.
-__device__ __forceinline__ u64 key_of(float x, int index) {
+__device__ __forceinline__ unsigned order_of(float x) {
   const unsigned b = __builtin_bit_cast(unsigned, x == 0.f ? 0.f : x);      // (-0 is 0)
-  return (u64)(b & 0x80000000u ? ~b : b | 0x80000000u) << 32 | (unsigned)~index;
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
+__device__ __forceinline__ u64 key_of(float x, int index) { return (u64)order_of(x) << 32 | (unsigned)~index; }
 __device__ __forceinline__ float value_of(u64 key) {
   const unsigned b = (unsigned)(key >> 32);
   return __builtin_bit_cast(float, b & 0x80000000u ? b & 0x7fffffffu : ~b);
 }
 __device__ __forceinline__ int index_of(u64 key) { return (int)~(unsigned)key; }
 
-__device__ __forceinline__ float wave_max(float x) { for (int o = 32; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor(x, o)); return x; }
-__device__ __forceinline__ float wave_sum(float x) { for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o); return x; }
-__device__ __forceinline__ int wave_sum(int x) { for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o); return x; }
+// Over the wave, for all lanes, in the vector unit: rotations within 16 lanes, then halves swapped.
+typedef unsigned u2 __attribute__((ext_vector_type(2)));
+template <int CTRL, typename T> __device__ __forceinline__ T rotated(T x) { return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, false)); }
+template <typename T, typename F> __device__ __forceinline__ T over_wave(T x, F f) {
+  x = f(x, rotated<0x128>(x)); x = f(x, rotated<0x124>(x)); x = f(x, rotated<0x122>(x)); x = f(x, rotated<0x121>(x));
+  unsigned w = __builtin_bit_cast(unsigned, x);
+  u2 p = __builtin_bit_cast(u2, __builtin_amdgcn_permlane16_swap(w, w, false, false));
+  x = f(__builtin_bit_cast(T, (unsigned)p[0]), __builtin_bit_cast(T, (unsigned)p[1]));
+  w = __builtin_bit_cast(unsigned, x);
+  p = __builtin_bit_cast(u2, __builtin_amdgcn_permlane32_swap(w, w, false, false));
+  return f(__builtin_bit_cast(T, (unsigned)p[0]), __builtin_bit_cast(T, (unsigned)p[1]));
+}
+__device__ __forceinline__ float wave_max(float x) { return over_wave(x, [](float a, float b) { return fmaxf(a, b); }); }
+__device__ __forceinline__ float wave_sum(float x) { return over_wave(x, [](float a, float b) { return a + b; }); }
+__device__ __forceinline__ int wave_sum(int x) { return over_wave(x, [](int a, int b) { return a + b; }); }
 
-// The n-th largest of the wave's 64 words; if there are equal ones, all of them count.
-__device__ __forceinline__ unsigned nth_of(unsigned x, int n) {
+// The n-th largest of the wave's 64 words, its BITS upper bits; if there are equal ones, all of them count.
+template <int BITS = 32> __device__ __forceinline__ unsigned nth_of(unsigned x, int n) {
   unsigned t = 0;
-  for (int b = 31; b >= 0; --b) {
+  for (int b = 31; b >= 32 - BITS; --b) {
     const unsigned trial = t | 1u << b;
     if (__popcll(__ballot(x >= trial)) >= n) t = trial;
   }
   return t;
+}
+__device__ __forceinline__ u64 nth_of(u64 x, int n) {
+  const unsigned high = (unsigned)(x >> 32), h = nth_of(high, n);
+  if (__popcll(__ballot(high >= h)) == n) return (u64)h << 32;
+  return (u64)h << 32 | nth_of(high == h ? (unsigned)x : 0u, n - __popcll(__ballot(high > h)));
 }
 
 struct Sums { float max, sum, weighted; int above; };      // above: tokens before the given one
@@ -71,15 +90,34 @@ __device__ __forceinline__ void write_top(const Out& o, long at, u64 key, const 
   o.top_tokens[at] = index_of(key);
 }
 
-// Work memory of a row and segment: its sums, and behind those of all rows its `top` best keys.
+// Places of c keys in their order, by counting: wave w compares with every WIDTH-th.  places: zeros.
+template <int WIDTH> __device__ __forceinline__ void count_places(const u64* keys, int c, int* places) {
+  const int l = threadIdx.x & 63;
+  for (int i = l; i < c; i += 64) {
+    const u64 k = keys[i];
+    int before = 0, j = threadIdx.x >> 6;
+    for (; j + 7 * WIDTH < c; j += 8 * WIDTH) {      // eight reads on their way
+#pragma unroll
+      for (int n = 0; n < 8; ++n) before += keys[j + n * WIDTH] > k;
+    }
+    for (; j < c; j += WIDTH) before += keys[j] > k;
+    if (WIDTH == 1) places[i] = before; else if (before > 0) atomicAdd(&places[i], before);
+  }
+}
+
+constexpr int most_found(int top) { return WAVES * EACH * top; }      // keys at or above a bound of keys: no wave has more than `top` lanes there, each with its EACH tokens
+
+// Work memory of a row and segment: its sums, and behind those of all rows its `top` best keys.  About 25 instructions a logit, fewer than its way from memory takes in 32 bits.
 template <typename T>
 __global__ __launch_bounds__(THREADS) void k_logprobs(const T* logits, long row_stride, int V, const int64_t* tokens, int top, int segments, Sums* sums, u64* best, Out out) {
   constexpr int PER = 16 / sizeof(T), RUNS = EACH / PER;
   __shared__ float red[3][WAVES];
   __shared__ int above_of[WAVES];
-  __shared__ u64 bound_of[WAVES];
-  extern __shared__ u64 found[];      // a wave has `top` lanes at most at or above its bound, each with its EACH tokens
+  __shared__ unsigned value_of_wave[WAVES];
+  __shared__ u64 key_of_wave[2 * WAVES];
   __shared__ int count;
+  extern __shared__ u64 found[];      // most_found keys, then as many places
+  int* places = reinterpret_cast<int*>(found + most_found(top));
   const int l = threadIdx.x & 63, wave = threadIdx.x >> 6, segment = blockIdx.x % segments, first = segment * SEGMENT, n = min(V - first, SEGMENT);
   const long row = blockIdx.x / segments;
   const T* src = logits + row * row_stride + first;
@@ -98,102 +136,165 @@ __global__ __launch_bounds__(THREADS) void k_logprobs(const T* logits, long row_
   const long given = tokens[row];
   const int token = given >= 0 && given < V ? (int)given : -1;
   const float mine = token >= 0 ? cleaned((float)logits[row * row_stride + token]) : 0.f;
+  const auto index = [&](int i) { return (int)((i / PER * THREADS + threadIdx.x) * PER + i % PER); };
   float m = -__builtin_inff();
 #pragma unroll
   for (int i = 0; i < EACH; ++i) { x[i] = cleaned(x[i]); m = fmaxf(m, x[i]); }
-  const auto index = [&](int i) { return (int)((i / PER * THREADS + threadIdx.x) * PER + i % PER); };
-  m = wave_max(m);
+  const float best_of_wave = wave_max(m);
+  const int share = (top + WAVES - 1) / WAVES;
+  if (top > 0) {
+    const unsigned bound = share == 1 ? order_of(best_of_wave) : nth_of<16>(order_of(m), share);
+    if (l == 0) value_of_wave[wave] = bound;
+  }
+  m = best_of_wave;
   if (l == 0) red[0][wave] = m;
   __syncthreads();
   for (int i = 0; i < WAVES; ++i) m = fmaxf(m, red[0][i]);
   float sum = 0, weighted = 0;
   int above = 0;
+  if (finite(m)) {
 #pragma unroll
-  for (int i = 0; i < EACH; ++i) {
-    const float d = distance(x[i], m), e = exp_of(d);
-    const bool alive = x[i] > -__builtin_inff();
-    sum += alive ? e : 0.f;
-    weighted += alive && e > 0.f ? e * d : 0.f;
-    const int at = first + index(i);
-    above += at < V && (x[i] > mine || (x[i] == mine && at < token));
+    for (int i = 0; i < EACH; ++i) {      // (what is masked: e^-104 is 0)
+      const float d = fmaxf(x[i] - m, -104.f), e = exp_of(d);
+      sum += e;
+      weighted = __builtin_fmaf(e, d, weighted);
+    }
+  } else if (m > 0.f) {
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) sum += x[i] == m ? 1.f : 0.f;
+  }
+  if (finite(mine)) {      // before the token whatever is not smaller, behind it what is larger; what is behind the row's end is -inf
+#pragma unroll
+    for (int r = 0; r < RUNS; ++r) {
+      const int at = first + (r * THREADS + threadIdx.x) * PER;
+      if (at > token || at + PER <= token) {
+        const float limit = at > token ? mine : mine == 0.f ? -1.40129846e-45f : __builtin_bit_cast(float, __builtin_bit_cast(int, mine) + (mine > 0.f ? -1 : 1));      // the next one below
+#pragma unroll
+        for (int i = 0; i < PER; ++i) above += x[r * PER + i] > limit;
+      } else {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) above += at + i < token ? x[r * PER + i] >= mine : x[r * PER + i] > mine;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) above += index(i) < n && (x[i] > mine || (x[i] == mine && first + index(i) < token));
   }
   sum = wave_sum(sum); weighted = wave_sum(weighted); above = wave_sum(above);
+  if (l == 0) { red[1][wave] = sum; red[2][wave] = weighted; above_of[wave] = above; }
   u64 bound = 0;
   if (top > 0) {
+    unsigned b = value_of_wave[0];
+    for (int i = 1; i < WAVES; ++i) b = min(b, value_of_wave[i]);
+    bound = (u64)max(b, order_of(-__builtin_inff())) << 32;      // (with its upper bits only it may lie below -inf, where no number is)
+    const float limit = value_of(bound);
+    int reach = 0;
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) reach += x[i] >= limit;
+    reach = wave_sum(reach);
+    if (l == 0 && reach > 0) atomicAdd(&count, reach);
+  }
+  __syncthreads();
+  Sums s{m, 0.f, 0.f, 0};
+  for (int i = 0; i < WAVES; ++i) { s.sum += red[1][i]; s.weighted += red[2][i]; s.above += above_of[i]; }
+  if (threadIdx.x == 0) {
+    if (segments == 1) write_row(out, row, token, V, mine, s); else sums[(long)row * segments + segment] = s;
+  }
+  if (top == 0) return;
+  const int reached = count;
+  __syncthreads();
+  if (threadIdx.x == 0) count = 0;
+  if (reached > 4 * top + 128 || reached > most_found(top)) {      // many alike
     u64 b = 0;
 #pragma unroll
     for (int i = 0; i < EACH; ++i) {
       const u64 k = index(i) < n ? key_of(x[i], first + index(i)) : 0;
       b = k > b ? k : b;
     }
-    const unsigned high = nth_of((unsigned)(b >> 32), top);
-    const int before = __popcll(__ballot((unsigned)(b >> 32) > high));
-    const unsigned low = nth_of((unsigned)(b >> 32) == high ? (unsigned)b : 0u, top - before);
-    bound = (u64)high << 32 | low;
+    const u64 all = nth_of(b, top), part = nth_of(b, share);
+    if (l == 0) { key_of_wave[wave] = all; key_of_wave[WAVES + wave] = part; }
+    __syncthreads();
+    bound = key_of_wave[WAVES];
+    for (int i = 1; i < WAVES; ++i) bound = min(bound, key_of_wave[WAVES + i]);
+    for (int i = 0; i < WAVES; ++i) bound = max(bound, key_of_wave[i]);
   }
-  if (l == 0) { red[1][wave] = sum; red[2][wave] = weighted; above_of[wave] = above; bound_of[wave] = bound; }
   __syncthreads();
-  Sums s{m, 0.f, 0.f, 0};
-  for (int i = 0; i < WAVES; ++i) { s.sum += red[1][i]; s.weighted += red[2][i]; s.above += above_of[i]; bound = bound_of[i] > bound ? bound_of[i] : bound; }
-  if (threadIdx.x == 0) {
-    if (segments == 1) write_row(out, row, token, V, mine, s); else sums[(long)row * segments + segment] = s;
-  }
-  if (top == 0) return;
+  const float limit = bound == 0 ? -__builtin_inff() : value_of(bound);      // (0: fewer than `top` lanes have a token)
 #pragma unroll
-  for (int i = 0; i < EACH; ++i) {
-    const u64 k = index(i) < n ? key_of(x[i], first + index(i)) : 0;
-    if (k != 0 && k >= bound) found[atomicAdd(&count, 1)] = k;
-  }
+  for (int i = 0; i < EACH; ++i)
+    if (x[i] >= limit && index(i) < n) {
+      const u64 k = key_of(x[i], first + index(i));
+      if (k >= bound) {
+        const int at = atomicAdd(&count, 1);
+        found[at] = k; places[at] = 0;
+      }
+    }
   __syncthreads();
   const int c = count;
+  count_places<WAVES>(found, c, places);
+  __syncthreads();
   u64* mine_best = best + ((long)row * segments + segment) * top;
   for (int i = threadIdx.x; i < c; i += THREADS) {
-    const u64 k = found[i];
-    int before = 0;
-    for (int j = 0; j < c; ++j) before += found[j] > k;
+    const int before = places[i];
     if (before < top) {
-      if (segments == 1) write_top(out, row * top + before, k, s); else mine_best[before] = k;
+      if (segments == 1) write_top(out, row * top + before, found[i], s); else mine_best[before] = found[i];
     }
   }
   if (segments > 1) for (int i = c + threadIdx.x; i < top; i += THREADS) mine_best[i] = 0;      // a last segment with fewer tokens
 }
 
-// Joins a row's segments.  Candidates are ranked by counting, behind a bound that leaves `top` of them at least.
+// Joins a row's segments, a wave a row.  Candidates at or above the `top`-th largest of the lanes' best, ranked by counting.
 template <typename T>
-__global__ __launch_bounds__(MERGE) void k_logprobs_merge(const T* logits, long row_stride, int V, const int64_t* tokens, int top, int segments, const Sums* sums, const u64* best, Out out) {
-  extern __shared__ u64 found[];
+__global__ __launch_bounds__(64) void k_logprobs_merge(const T* logits, long row_stride, int V, const int64_t* tokens, int top, int segments, const Sums* sums, const u64* best, Out out) {
+  extern __shared__ u64 found[];      // top * most keys, then as many places
   const long row = blockIdx.x;
+  const int l = threadIdx.x, c = segments * top, most = (c + 63) / 64;
   const Sums* mine = sums + row * segments;
+  const u64* keys = best + row * c;
   const long given = tokens[row];
   const int token = given >= 0 && given < V ? (int)given : -1;
-  Sums s{-__builtin_inff(), 0.f, 0.f, 0};
-  for (int i = 0; i < segments; ++i) s.max = fmaxf(s.max, mine[i].max);
-  for (int i = 0; i < segments; ++i) {
-    const Sums t = mine[i];
-    const float d = distance(t.max, s.max), e = t.max > -__builtin_inff() ? exp_of(d) : 0.f;
-    if (e > 0.f) { s.sum += e * t.sum; s.weighted += e * __builtin_fmaf(d, t.sum, t.weighted); }
-    s.above += t.above;
-  }
-  if (threadIdx.x == 0) write_row(out, row, token, V, token >= 0 ? cleaned((float)logits[row * row_stride + token]) : 0.f, s);
+  u64 b = 0;
+#pragma unroll 4
+  for (int i = l; i < c; i += 64) { const u64 k = keys[i]; b = k > b ? k : b; }
+  const Sums none{-__builtin_inff(), 0.f, 0.f, 0}, t0 = l < segments ? mine[l] : none, t1 = l + 64 < segments ? mine[l + 64] : none;      // (up to 128 segments)
+  const float x = token >= 0 ? cleaned((float)logits[row * row_stride + token]) : 0.f;
+  Sums s{wave_max(fmaxf(t0.max, t1.max)), 0.f, 0.f, t0.above + t1.above};
+  const auto add = [&](const Sums& t) {
+    const float d = fmaxf(distance(t.max, s.max), -104.f), e = exp_of(d);
+    if (t.max > -__builtin_inff()) { s.sum += e * t.sum; s.weighted += e * __builtin_fmaf(d, t.sum, t.weighted); }
+  };
+  add(t0); add(t1);
+  s.sum = wave_sum(s.sum); s.weighted = wave_sum(s.weighted); s.above = wave_sum(s.above);
+  if (l == 0) write_row(out, row, token, V, x, s);
   if (top == 0) return;
-  const int c = segments * top;
-  for (int i = threadIdx.x; i < c; i += MERGE) found[i] = best[row * c + i];
-  __syncthreads();
-  for (int i = threadIdx.x; i < c; i += MERGE) {
-    const u64 k = found[i];
-    if (k == 0) continue;
-    int before = 0;
-    for (int j = 0; j < c; ++j) before += found[j] > k;
-    if (before < top) write_top(out, row * top + before, k, s);
+  int* places = reinterpret_cast<int*>(found + top * most);
+  // Every segment's list is sorted: the least of their n-th keys, n = top / segments rounded up, is a bound that `top` keys at least reach.  Where many more do, also the `top`-th largest of the lanes' best.
+  const int nth = (top + segments - 1) / segments - 1;
+  u64 bound = min(l < segments ? keys[l * top + nth] : ~0ull, l + 64 < segments ? keys[(l + 64) * top + nth] : ~0ull);
+  for (int o = 32; o > 0; o >>= 1) bound = min(bound, (u64)__shfl_xor(bound, o));
+  int reached = 0;
+#pragma unroll 4
+  for (int i = l; i < c; i += 64) reached += keys[i] >= bound;
+  if (wave_sum(reached) > min(max(64, top + top / 2), top * most)) bound = max(bound, nth_of(b, top));
+  int held = 0;
+  for (int i0 = 0; i0 < c; i0 += 64) {
+    const u64 k = i0 + l < c ? keys[i0 + l] : 0;
+    const u64 here = __ballot(k != 0 && k >= bound);
+    if (k != 0 && k >= bound) found[held + __popcll(here & ((1ull << l) - 1))] = k;
+    held += __popcll(here);
   }
+  __syncthreads();
+  count_places<1>(found, held, places);
+  for (int i = l; i < held; i += 64)
+    if (places[i] < top) write_top(out, row * top + places[i], found[i], s);
 }
 
 template <typename T> void launch(const void* logits, long row_stride, int B, int V, const int64_t* tokens, int top, void* work, const Out& out, hipStream_t stream) {
   const int segments = (V + SEGMENT - 1) / SEGMENT;
   Sums* sums = static_cast<Sums*>(work);
   u64* best = reinterpret_cast<u64*>(sums + (long)B * segments);
-  k_logprobs<T><<<(unsigned)B * segments, THREADS, sizeof(u64) * WAVES * EACH * top, stream>>>(static_cast<const T*>(logits), row_stride, V, tokens, top, segments, sums, best, out);
-  if (segments > 1) k_logprobs_merge<T><<<B, MERGE, sizeof(u64) * segments * top, stream>>>(static_cast<const T*>(logits), row_stride, V, tokens, top, segments, sums, best, out);
+  k_logprobs<T><<<(unsigned)B * segments, THREADS, 12 * most_found(top), stream>>>(static_cast<const T*>(logits), row_stride, V, tokens, top, segments, sums, best, out);
+  if (segments > 1) k_logprobs_merge<T><<<B, 64, 12 * top * ((segments * top + 63) / 64), stream>>>(static_cast<const T*>(logits), row_stride, V, tokens, top, segments, sums, best, out);
 }
 
 }  // namespace
