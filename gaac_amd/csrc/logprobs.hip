@@ -105,6 +105,7 @@ template <int WIDTH> __device__ __forceinline__ void count_places(const u64* key
   }
 }
 
+constexpr int most_ranked(int top) { return 2 * top + 64; }
 constexpr int most_found(int top) { return WAVES * EACH * top; }      // keys at or above a bound of keys: no wave has more than `top` lanes there, each with its EACH tokens
 
 // Work memory of a row and segment: its sums, and behind those of all rows its `top` best keys.  About 25 instructions a logit, fewer than its way from memory takes in 32 bits.
@@ -122,11 +123,12 @@ __global__ __launch_bounds__(THREADS) void k_logprobs(const T* logits, long row_
   const long row = blockIdx.x / segments;
   const T* src = logits + row * row_stride + first;
   const bool aligned = reinterpret_cast<uintptr_t>(src) % 16 == 0;
+  const int slot = n < SEGMENT ? l * WAVES + wave : (int)threadIdx.x;      // (a short segment is spread over all waves: the bound below goes by the one that has the least)
   if (threadIdx.x == 0) count = 0;
   float x[EACH];
 #pragma unroll
   for (int r = 0; r < RUNS; ++r) {
-    const int at = (r * THREADS + threadIdx.x) * PER;
+    const int at = (r * THREADS + slot) * PER;
     if (aligned && at + PER <= n) load16(src + at, x + r * PER);
     else {
 #pragma unroll
@@ -136,7 +138,7 @@ __global__ __launch_bounds__(THREADS) void k_logprobs(const T* logits, long row_
   const long given = tokens[row];
   const int token = given >= 0 && given < V ? (int)given : -1;
   const float mine = token >= 0 ? cleaned((float)logits[row * row_stride + token]) : 0.f;
-  const auto index = [&](int i) { return (int)((i / PER * THREADS + threadIdx.x) * PER + i % PER); };
+  const auto index = [&](int i) { return (i / PER * THREADS + slot) * PER + i % PER; };
   float m = -__builtin_inff();
 #pragma unroll
   for (int i = 0; i < EACH; ++i) { x[i] = cleaned(x[i]); m = fmaxf(m, x[i]); }
@@ -166,7 +168,7 @@ __global__ __launch_bounds__(THREADS) void k_logprobs(const T* logits, long row_
   if (finite(mine)) {      // before the token whatever is not smaller, behind it what is larger; what is behind the row's end is -inf
 #pragma unroll
     for (int r = 0; r < RUNS; ++r) {
-      const int at = first + (r * THREADS + threadIdx.x) * PER;
+      const int at = first + (r * THREADS + slot) * PER;
       if (at > token || at + PER <= token) {
         const float limit = at > token ? mine : mine == 0.f ? -1.40129846e-45f : __builtin_bit_cast(float, __builtin_bit_cast(int, mine) + (mine > 0.f ? -1 : 1));      // the next one below
 #pragma unroll
@@ -243,19 +245,33 @@ __global__ __launch_bounds__(THREADS) void k_logprobs(const T* logits, long row_
   if (segments > 1) for (int i = c + threadIdx.x; i < top; i += THREADS) mine_best[i] = 0;      // a last segment with fewer tokens
 }
 
-// Joins a row's segments, a wave a row.  Candidates at or above the `top`-th largest of the lanes' best, ranked by counting.
+// A bound that at least n and at most `most` of c different keys in LDS reach (or all that are not 0, where they are fewer), by a wave: bit by bit the largest that n reach, until they are few enough.
+__device__ __forceinline__ u64 key_bound(const u64* keys, int c, int n, int most) {
+  u64 t = 0;
+  for (int b = 63; b >= 0; --b) {
+    const u64 trial = t | 1ull << b;
+    int reach = 0;
+#pragma unroll 4
+    for (int i = threadIdx.x & 63; i < c; i += 64) reach += keys[i] >= trial;
+    reach = wave_sum(reach);
+    if (reach >= n) t = trial;
+    if (reach >= n && reach <= most) break;
+  }
+  return t;
+}
+
+// Joins a row's segments, a wave a row.  Every segment's list is sorted: the least of their n-th keys, n = top / segments rounded up, is a bound that `top` keys at least reach.  Those that do are ranked by
+// counting; where they are many more (a short last segment, or likely tokens in one place), those that reach a bound found bit by bit.
 template <typename T>
 __global__ __launch_bounds__(64) void k_logprobs_merge(const T* logits, long row_stride, int V, const int64_t* tokens, int top, int segments, const Sums* sums, const u64* best, Out out) {
-  extern __shared__ u64 found[];      // top * most keys, then as many places
+  extern __shared__ u64 keys[];      // of all segments, then those that are ranked, then their places
   const long row = blockIdx.x;
-  const int l = threadIdx.x, c = segments * top, most = (c + 63) / 64;
+  const int l = threadIdx.x, c = segments * top, most = most_ranked(top);
   const Sums* mine = sums + row * segments;
-  const u64* keys = best + row * c;
   const long given = tokens[row];
   const int token = given >= 0 && given < V ? (int)given : -1;
-  u64 b = 0;
 #pragma unroll 4
-  for (int i = l; i < c; i += 64) { const u64 k = keys[i]; b = k > b ? k : b; }
+  for (int i = l; i < c; i += 64) keys[i] = best[row * c + i];
   const Sums none{-__builtin_inff(), 0.f, 0.f, 0}, t0 = l < segments ? mine[l] : none, t1 = l + 64 < segments ? mine[l + 64] : none;      // (up to 128 segments)
   const float x = token >= 0 ? cleaned((float)logits[row * row_stride + token]) : 0.f;
   Sums s{wave_max(fmaxf(t0.max, t1.max)), 0.f, 0.f, t0.above + t1.above};
@@ -267,15 +283,16 @@ __global__ __launch_bounds__(64) void k_logprobs_merge(const T* logits, long row
   s.sum = wave_sum(s.sum); s.weighted = wave_sum(s.weighted); s.above = wave_sum(s.above);
   if (l == 0) write_row(out, row, token, V, x, s);
   if (top == 0) return;
-  int* places = reinterpret_cast<int*>(found + top * most);
-  // Every segment's list is sorted: the least of their n-th keys, n = top / segments rounded up, is a bound that `top` keys at least reach.  Where many more do, also the `top`-th largest of the lanes' best.
+  __syncthreads();
+  u64* found = keys + c;
+  int* places = reinterpret_cast<int*>(found + most);
   const int nth = (top + segments - 1) / segments - 1;
   u64 bound = min(l < segments ? keys[l * top + nth] : ~0ull, l + 64 < segments ? keys[(l + 64) * top + nth] : ~0ull);
   for (int o = 32; o > 0; o >>= 1) bound = min(bound, (u64)__shfl_xor(bound, o));
   int reached = 0;
 #pragma unroll 4
   for (int i = l; i < c; i += 64) reached += keys[i] >= bound;
-  if (wave_sum(reached) > min(max(64, top + top / 2), top * most)) bound = max(bound, nth_of(b, top));
+  if (wave_sum(reached) > most) bound = key_bound(keys, c, top, most);
   int held = 0;
   for (int i0 = 0; i0 < c; i0 += 64) {
     const u64 k = i0 + l < c ? keys[i0 + l] : 0;
@@ -294,7 +311,7 @@ template <typename T> void launch(const void* logits, long row_stride, int B, in
   Sums* sums = static_cast<Sums*>(work);
   u64* best = reinterpret_cast<u64*>(sums + (long)B * segments);
   k_logprobs<T><<<(unsigned)B * segments, THREADS, 12 * most_found(top), stream>>>(static_cast<const T*>(logits), row_stride, V, tokens, top, segments, sums, best, out);
-  if (segments > 1) k_logprobs_merge<T><<<B, 64, 12 * top * ((segments * top + 63) / 64), stream>>>(static_cast<const T*>(logits), row_stride, V, tokens, top, segments, sums, best, out);
+  if (segments > 1) k_logprobs_merge<T><<<B, 64, 8 * segments * top + 12 * most_ranked(top), stream>>>(static_cast<const T*>(logits), row_stride, V, tokens, top, segments, sums, best, out);
 }
 
 }  // namespace
