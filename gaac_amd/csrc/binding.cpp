@@ -667,7 +667,7 @@ PyObject* logprobs(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const at::Tensor &x = here(a[0]), &t = here(a[1]);
     const int type = float_type(x);
     const long top = number(a[2]);
-    if (x.dim() != 2 || x.size(0) == 0 || x.size(0) > 1l << 23 || x.size(1) == 0 || x.size(1) > (1l << 20) - 16 || (x.size(1) > 1 && x.stride(1) != 1) || loses_gradient(x)) throw Otherwise{};
+    if (x.dim() != 2 || x.size(0) == 0 || x.size(1) == 0 || x.size(1) > (1l << 20) - 16 || x.size(0) > (1l << 22) / ((x.size(1) + 8191) / 8192) || (x.size(1) > 1 && x.stride(1) != 1) || loses_gradient(x)) throw Otherwise{};
     const long B = x.size(0), V = x.size(1);
     if (t.dim() != 1 || t.size(0) != B || t.scalar_type() != at::kLong || !t.is_contiguous() || top < 0 || top > std::min(64l, V)) throw Otherwise{};
     void* stream = stream_of(a[3]);

@@ -117,7 +117,7 @@ struct RowsArgs {
   void* sum;
   uint8_t *data, *exps;
   long x_rs, r_rs, pad;
-  int M, K, nb, waves, tile_step, tile_first;
+  int K, nb, waves, tile_step, tile_first, first;
   float eps;
   bool whole;
 };
@@ -131,7 +131,7 @@ __global__ __launch_bounds__(1024) void k_fp8_rows(RowsArgs a) {
   const int l = threadIdx.x & 63, part = threadIdx.x >> 6;
   // A cache line of the result has pieces of 8 rows.  Blocks go to the XCDs in turns, each of which has its own L2: the rows of a tile are those of blocks that go to the same one (16384 x 4096: 62 us
   // with rows in the blocks' order, 52 so).
-  const int turn = blockIdx.x & ~127u, in_turn = blockIdx.x & 127u, row = turn + 128 <= (int)gridDim.x ? turn + in_turn % 8 * 16 + in_turn / 8 : (int)blockIdx.x;
+  const int turn = blockIdx.x & ~127u, in_turn = blockIdx.x & 127u, row = (turn + 128 <= (int)gridDim.x ? turn + in_turn % 8 * 16 + in_turn / 8 : (int)blockIdx.x) + a.first;
   const T* src = static_cast<const T*>(a.x) + row * a.x_rs;
   const auto at = [&](int i) { return 8 * ((i * a.waves + part) * 64 + l); };
   float x[CH][8];
@@ -185,9 +185,9 @@ __global__ __launch_bounds__(1024) void k_fp8_rows(RowsArgs a) {
 }
 
 // The way back: a block of threads a tile, 16 lanes a row's 256 bytes.
-__global__ __launch_bounds__(256) void k_fp8_values(const uint8_t* data, const uint8_t* exps, long pad, int tile_step, int tile_first, int M, int K, int nb, __bf16* out, long out_rs, bool whole) {
+__global__ __launch_bounds__(256) void k_fp8_values(const uint8_t* data, const uint8_t* exps, long pad, int tile_step, int tile_first, long first, int M, int K, int nb, __bf16* out, long out_rs, bool whole) {
   const int p = threadIdx.x & 15, m = threadIdx.x >> 4, kb = blockIdx.x % nb;
-  const long tile = blockIdx.x / nb, row = 16 * tile + m, tile_row = tile * tile_step + tile_first;
+  const long tile = first + blockIdx.x / nb, row = 16 * tile + m, tile_row = tile * tile_step + tile_first;
   if (row >= M) return;
   const u2 w = *reinterpret_cast<const u2*>(data + (kb * (pad >> 4) + tile_row) * TILE + 1024 * (p >> 1 & 1) + 16 * (16 * (p >> 2) + m) + 8 * (p & 1));
   const unsigned e = exps[((kb >> 2) * pad + 16 * tile_row + m) * 4 + (kb & 3)];
@@ -413,15 +413,17 @@ __global__ __launch_bounds__(64 * WN * WM, TN * TM == 64 ? 1 : 2) void k_fp8_til
     stride[i] = (t < WN * TN ? a.w_pad : a.x_pad) * BLOCK;
   }
   // (behind the last block of K the last one again, which nobody uses: no step is different from the others)
-  const auto fetch = [&](uint8_t* to, int kb) {
-    const long at = min(kb, a.nb - 1);
+  int next = 0;
+  const auto fetch_part = [&](uint8_t* to, int from_i, int end_i) {
 #pragma unroll
-    for (int i = 0; i < LOADS; ++i) {
-      const uint8_t* from = src[i] + at * stride[i];
+    for (int i = from_i; i < end_i; ++i) {
+      const uint8_t* from = src[i];
       asm("" : "+s"(from));
       __builtin_amdgcn_global_load_lds((global_ptr)(from + 16u * l), (lds_ptr)(to + (wave * LOADS + i) * 1024), 16, 0, 0);
+      src[i] += next < a.nb - 1 ? stride[i] : 0;
     }
   };
+  const auto fetch = [&](uint8_t* to) { fetch_part(to, 0, LOADS); ++next; };
   constexpr int PARTS = (ROWS / 64 + W - 1) / W;      // runs of 64 rows whose exponents a wave loads
   const unsigned* exps_src[PARTS];
   long exps_pad[PARTS];
@@ -482,7 +484,6 @@ __global__ __launch_bounds__(64 * WN * WM, TN * TM == 64 ? 1 : 2) void k_fp8_til
     }
     barrier();
     if constexpr (S == 3) read_exps((kb >> 2) + 1);      // (before more is on its way into LDS: the compiler would wait for all of it)
-    fetch(now, kb + NBUF);
     if constexpr (S == 0) fetch_exps((kb >> 2) + 1);
     Operand<EXACT> ow[TAIL];
 #pragma unroll
@@ -495,15 +496,17 @@ __global__ __launch_bounds__(64 * WN * WM, TN * TM == 64 ? 1 : 2) void k_fp8_til
 #pragma unroll
       for (int i = 0; i < TAIL; ++i) pin(acc[j][TN - TAIL + i]);
       x[j] = read(then + x_at + j * TILE);
+      fetch_part(now, LOADS * j / TM, LOADS * (j + 1) / TM);
       __builtin_amdgcn_sched_barrier(0);
     }
+    ++next;
 #pragma unroll
     for (int i = 1; i < TAIL; ++i) w[i] = read(then + w_at + i * TILE);
   };
   fetch_exps(0);
-  fetch(buf0, 0);
-  fetch(buf1, 1);
-  if constexpr (NBUF == 4) { fetch(buf2, 2); fetch(buf3, 3); }
+  fetch(buf0);
+  fetch(buf1);
+  if constexpr (NBUF == 4) { fetch(buf2); fetch(buf3); }
   __builtin_amdgcn_s_waitcnt(0x0070 | ((NBUF - 1) * LOADS & 15) | (NBUF - 1) * LOADS >> 4 << 14);
   __syncthreads();
   read_exps(0);
@@ -552,24 +555,26 @@ template <typename O, int MT, int NT, int AHEAD> void launch_stream(const Produc
 }
 
 // Which form is taken: the one that should end first, its time being start + steps * (round * rounds + share * blocks / 256), rounds = blocks / 256 rounded up (a round: a block on each CU), steps the blocks of K
-// that a wave goes through.  The constants, in us, are fitted to the times of all forms over 102 sizes (1 to 4096 rows by 1024 to 28672 x 512 to 14336); over these the chosen form takes 2.5 % longer than the
-// best one in the mean (fp32: 0.7 %).  Up to 16 rows, and wherever a block has one tile of rows, the products are the exact ones for every type: the weights' way from memory hides them (4 x 4096 x 4096 4.8 us, 4.9 exact;
-// 4 x 28672 x 4096 21.8, 23.5).  Some of both sides, us, weights resident in turns (rows x N x K, outputs of 16 bits: stream of 1 x 1, 1 x 2, 2 x 2, 4 x 2 tiles | 64 x 64, 64 x 128, 128 x 128 with
-// four buffers, with two, 256 x 256 through LDS):
-//   4 x 4096 x 4096   4.9 5.5 5.8 6.7 | 9.7 13 17 21 42          48 x 4096 x 14336  28 23 16.6 22.9 | 31 47 51 87 142         64 x 28672 x 4096  71 69 41 33 | 26 22.5 24 32 48
-//   200 x 4096 x 4096  20 15 14 11.2 | 10.7 14 19 22 47          600 x 6144 x 4096  66 50 44 38 | 33 32 24 30 52              1024 x 28672 x 4096  1018 1018 524 328 | 215 221 159 146 115
-//   2048 x 4096 x 14336  1006 566 355 250 | 192 180 126 112 149  4096 x 4096 x 4096  314 227 195 148 | 124 125 87 71 63
+// that a wave goes through.  The constants, in us, are fitted to the times of all forms over 180 sizes (1 to 8192 rows by 1024 to 28672 x 512 to 14336); over these the chosen form takes 1.6 % longer than the
+// best one in the mean (fp32: 0.9 % over 77).  Up to 16 rows, and wherever a block has one tile of rows, the products are the exact ones for every type: the weights' way from memory hides most of them (8 x 4096 x 4096 4.9 us,
+// 4.8 without; 8 x 28672 x 4096 23.6, 21.8).  Some of both sides, us, weights resident in turns (rows x N x K, outputs of 16 bits: stream of 1 x 1, 1 x 2, 2 x 2, 4 x 2 tiles | 64 x 64,
+// 64 x 128, 128 x 128 with four buffers, with two, 256 x 256 through LDS):
+//   8 x 4096 x 4096  4.9 5.6             8 x 28672 x 4096  23.9 23.6                                 48 x 4096 x 14336  28 25 16.9 23 | 32 48 51 95 142
+//   64 x 28672 x 4096  71 70 41 33 | 27 23.0 25 34 48            200 x 4096 x 4096  21 21 15 12 | 10.4 13 17 25 45             777 x 6144 x 4096  - - 56 49 | 41 41 37 35 51
+//   1024 x 28672 x 4096  - - 520 328 | 213 212 151 149 113       2048 x 4096 x 14336  | 190 174 120 116 158                    8192 x 8192 x 8192  | 810 753 581 511 403
 struct Form { int n, m, waves; float start, round, share; };      // tiles of weights and of rows a block, waves that share out K
-constexpr Form FORMS[9] = {{1, 1, 8, 1.61f, .33f, .34f}, {2, 1, 8, 1.71f, .51f, .31f}, {2, 2, 8, 1.82f, .5f, .65f}, {2, 4, 8, 2.32f, .61f, 1.03f},
-                           {4, 4, 1, 4.16f, .2f, .05f}, {8, 4, 1, 3.8f, .37f, .11f}, {8, 8, 1, 5.45f, .36f, .24f}, {8, 8, 1, 3.13f, .59f, .3f}, {16, 16, 1, 4.51f, 1.11f, .64f}};
-constexpr Form EXACT_FORMS[6] = {{1, 1, 8, 1.43f, .38f, .32f}, {2, 1, 8, .55f, .81f, .22f}, {2, 2, 8, 2.27f, .82f, .22f}, {2, 4, 8, .97f, .78f, 1.17f}, {4, 4, 1, 5.36f, .31f, .08f}, {8, 8, 1, 7.81f, .86f, .24f}};
+constexpr Form FORMS[9] = {{1, 1, 8, 1.f, .34f, .38f}, {2, 1, 8, 1.79f, .51f, .31f}, {2, 2, 8, 1.79f, .5f, .64f}, {2, 4, 8, 2.01f, .63f, .98f},
+                           {4, 4, 1, 4.05f, .28f, 0.f}, {8, 4, 1, 3.86f, .37f, .07f}, {8, 8, 1, 4.92f, .36f, .22f}, {8, 8, 1, 3.14f, .59f, .21f}, {16, 16, 1, 5.99f, 1.06f, .65f}};
+constexpr Form EXACT_FORMS[6] = {{1, 1, 8, .92f, .38f, .33f}, {2, 1, 8, .82f, .84f, .26f}, {2, 2, 8, .29f, .93f, .59f}, {2, 4, 8, .9f, .67f, 1.63f}, {4, 4, 1, 8.93f, .27f, .05f}, {8, 8, 1, 8.44f, .69f, .1f}};
+// (Forms whose launch would have more than 65535 blocks in y or 2^32 threads in x are left out; the fourth never has.)
 template <int COUNT> int form_of(const Form (&forms)[COUNT], const ProductArgs& a, bool gated) {
   int best = -1;
   float least = 0;
   for (int i = 0; i < (a.M <= 16 ? 2 : COUNT); ++i) {
     const Form& f = forms[i];
     if (gated && f.n % 2 != 0) continue;
-    const long blocks = (long)((a.tiles + f.n - 1) / f.n) * ((a.M + 16 * f.m - 1) / (16 * f.m));
+    const long high = (a.M + 16 * f.m - 1) / (16 * f.m), blocks = (a.tiles + f.n - 1) / f.n * high;
+    if (f.waves == 1 ? blocks >= 1 << 22 : high > 65535) continue;
     const int steps = f.waves == 1 ? a.nb : 4 * (((a.nb + 3) / 4 + f.waves - 1) / f.waves);
     const float time = f.start + steps * (f.round * ((blocks + 255) / 256) + f.share * blocks / 256.f);
     if (best < 0 || time < least) { best = i; least = time; }
@@ -601,20 +606,24 @@ template <typename O> void launch_product(const ProductArgs& a, bool gated, hipS
   }
 }
 
-template <typename T, int CH> void launch_rows(const RowsArgs& a, hipStream_t s) {
-  if constexpr (CH < 8) {
-    if (a.weight != nullptr) return k_fp8_rows<T, true, CH><<<a.M, 64 * a.waves, 0, s>>>(a);
+constexpr int MOST_ROWS = 1 << 20;      // of one launch, of up to 1024 threads a row: a launch has less than 2^32
+template <typename T, int CH> void launch_rows(RowsArgs a, int M, hipStream_t s) {
+  for (a.first = 0; a.first < M; a.first += MOST_ROWS) {
+    const int n = M - a.first < MOST_ROWS ? M - a.first : MOST_ROWS;
+    if constexpr (CH < 8) {
+      if (a.weight != nullptr) { k_fp8_rows<T, true, CH><<<n, 64 * a.waves, 0, s>>>(a); continue; }
+    }
+    k_fp8_rows<T, false, CH><<<n, 64 * a.waves, 0, s>>>(a);
   }
-  k_fp8_rows<T, false, CH><<<a.M, 64 * a.waves, 0, s>>>(a);
 }
 // One run a lane for few rows, where latency counts, two for many (us, one / two runs, with the norm: 4 x 4096 4.0 / 4.8, 300 x 4096 6.3 / 6.9, 777 x 5000 12.5 / 10.9, 16384 x 4096 125 / 113); more only where a block's 16 waves
 // would not do.  (The norm of 8 runs would not fit the registers.)
-template <typename T> void launch_rows(RowsArgs a, hipStream_t s) {
+template <typename T> void launch_rows(RowsArgs a, int M, hipStream_t s) {
   const auto waves = [&](int n) { return (a.nb * 16 + 64 * n - 1) / (64 * n); };
-  int ch = (long)a.M * waves(1) <= 4096 ? 1 : 2;
+  int ch = (long)M * waves(1) <= 4096 ? 1 : 2;
   while (waves(ch) > 16) ch *= 2;
   a.waves = waves(ch);
-  if (ch == 1) launch_rows<T, 1>(a, s); else if (ch == 2) launch_rows<T, 2>(a, s); else if (ch == 4) launch_rows<T, 4>(a, s); else launch_rows<T, 8>(a, s);
+  if (ch == 1) launch_rows<T, 1>(a, M, s); else if (ch == 2) launch_rows<T, 2>(a, M, s); else if (ch == 4) launch_rows<T, 4>(a, M, s); else launch_rows<T, 8>(a, M, s);
 }
 
 uintptr_t address(const void* p) { return reinterpret_cast<uintptr_t>(p); }
@@ -632,10 +641,10 @@ extern "C" int gaac_fp8_rows(int type, const void* x, long x_row_stride, const v
   GAAC_REQUIRE(address(data) % 16 == 0 && address(exps) % 4 == 0, "gaac_fp8_rows: data must be 16-byte aligned, exponents 4-byte");
   const int per = type == 2 ? 4 : 8;
   const bool whole = (address(x) | address(residual) | address(weight) | address(sum)) % 16 == 0 && (x_row_stride | residual_row_stride | K) % per == 0 && K % 8 == 0;
-  const RowsArgs a{x, residual, weight, sum, static_cast<uint8_t*>(data), static_cast<uint8_t*>(exps), x_row_stride, residual_row_stride, padded_rows, M, K, (K + BLOCK - 1) / BLOCK, 1, tile_step, tile_first, eps, whole};
-  if (type == 0) launch_rows<__bf16>(a, (hipStream_t)stream);
-  else if (type == 1) launch_rows<_Float16>(a, (hipStream_t)stream);
-  else launch_rows<float>(a, (hipStream_t)stream);
+  const RowsArgs a{x, residual, weight, sum, static_cast<uint8_t*>(data), static_cast<uint8_t*>(exps), x_row_stride, residual_row_stride, padded_rows, K, (K + BLOCK - 1) / BLOCK, 1, tile_step, tile_first, 0, eps, whole};
+  if (type == 0) launch_rows<__bf16>(a, M, (hipStream_t)stream);
+  else if (type == 1) launch_rows<_Float16>(a, M, (hipStream_t)stream);
+  else launch_rows<float>(a, M, (hipStream_t)stream);
   return gaac::launch_status("gaac_fp8_rows");
 }
 
@@ -646,7 +655,10 @@ extern "C" int gaac_fp8_values(const void* data, const void* exps, long padded_r
   GAAC_REQUIRE(address(data) % 16 == 0 && address(exps) % 4 == 0, "gaac_fp8_values: data must be 16-byte aligned, exponents 4-byte");
   const int nb = (K + BLOCK - 1) / BLOCK;
   const bool whole = address(out) % 16 == 0 && out_row_stride % 8 == 0;
-  k_fp8_values<<<(unsigned)((M + 15) / 16) * nb, 256, 0, (hipStream_t)stream>>>(static_cast<const uint8_t*>(data), static_cast<const uint8_t*>(exps), padded_rows, tile_step, tile_first, M, K, nb, static_cast<__bf16*>(out), out_row_stride, whole);
+  const long tiles = (M + 15) / 16, most = (1 << 22) / nb;      // (a launch has less than 2^32 threads)
+  for (long first = 0; first < tiles; first += most)
+    k_fp8_values<<<(unsigned)((tiles - first < most ? tiles - first : most) * nb), 256, 0, (hipStream_t)stream>>>(static_cast<const uint8_t*>(data), static_cast<const uint8_t*>(exps), padded_rows, tile_step, tile_first, first, M, K,
+                                                                                                               nb, static_cast<__bf16*>(out), out_row_stride, whole);
   return gaac::launch_status("gaac_fp8_values");
 }
 

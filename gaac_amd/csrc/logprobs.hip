@@ -320,7 +320,7 @@ extern "C" int gaac_logprobs(int type, const void* logits, long row_stride, int 
                              float* top_logprobs, int64_t* top_tokens, void* stream) {
   GAAC_REQUIRE(logits != nullptr && tokens != nullptr && logprob != nullptr && rank != nullptr && entropy != nullptr, "gaac_logprobs: null pointer");
   GAAC_REQUIRE(type >= 0 && type <= 2, "gaac_logprobs: type must be 0 (bf16), 1 (fp16) or 2 (fp32)");
-  GAAC_REQUIRE(B > 0 && B <= 1 << 23 && V > 0 && V <= MAX_VOCAB, "gaac_logprobs: bad sizes (%d rows of %d logits, up to 2^23 of %d)", B, V, MAX_VOCAB);
+  GAAC_REQUIRE(B > 0 && V > 0 && V <= MAX_VOCAB && (long)B * ((V + SEGMENT - 1) / SEGMENT) <= 1 << 22, "gaac_logprobs: bad sizes (%d rows of %d logits, up to 2^22 segments of %d and rows of %d)", B, V, SEGMENT, MAX_VOCAB);
   GAAC_REQUIRE(top >= 0 && top <= MAX_TOP && top <= V && (top == 0 || (top_logprobs != nullptr && top_tokens != nullptr)), "gaac_logprobs: up to %d alternatives, no more than there are logits (%d of %d)", MAX_TOP, top, V);
   const long segments = (V + SEGMENT - 1) / SEGMENT, need = segments == 1 ? 0 : B * segments * (16 + 8l * top);
   GAAC_REQUIRE(need == 0 || (work != nullptr && reinterpret_cast<uintptr_t>(work) % 16 == 0 && work_bytes >= need), "gaac_logprobs: needs %ld bytes of work memory, 16-byte aligned", need);

@@ -157,7 +157,7 @@ def _operands(what: str, x, weight: FP8Weight, gated: bool, out_dtype):
 def _product(what, x, weight, gated, out_dtype):
     if isinstance(weight, FP8Weight) and weight.gated == gated and out_dtype in TYPES:
         data, exps = (x.data, x.exps) if isinstance(x, FP8Rows) else (x, None)
-        if x.shape[-1] == weight.K:
+        if len(x.shape) == 2 and x.shape[1] == weight.K:
             out = (_lib._calls or _lib.calls()).fp8_multiply(data, exps, x.shape[0], weight.data, weight.exps, weight.N, weight.K, gated, TYPES[out_dtype], _lib.stream)
             if out is not None: return out
     _operands(what, x, weight, gated, out_dtype)

@@ -79,8 +79,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> 
     NaN and rank -1.  Sums in 32 bits, in the same order each time.  One launch for vocabularies up to 8192, otherwise two; no wait, no backward pass."""
     out = (_lib._calls or _lib.calls()).logprobs(logits, tokens, top, _lib.stream)
     if out is not None: return LogProbs(*out)
-    if logits.dim() != 2 or logits.dtype not in TYPES or not 1 <= logits.shape[1] <= MAX_VOCAB or logits.shape[0] > 1 << 23:
-        raise RuntimeError(f"token_logprobs expects logits bf16, fp16 or fp32 [B, V], V up to {MAX_VOCAB}, B up to 2^23, got {logits.dtype} {list(logits.shape)}")
+    if logits.dim() != 2 or logits.dtype not in TYPES or not 1 <= logits.shape[1] <= MAX_VOCAB or logits.shape[0] * -(-logits.shape[1] // 8192) > 1 << 22:
+        raise RuntimeError(f"token_logprobs expects logits bf16, fp16 or fp32 [B, V], V up to {MAX_VOCAB}, up to 2^22 segments of 8192, got {logits.dtype} {list(logits.shape)}")
     B, V = logits.shape
     if tokens.dtype != torch.int64 or tuple(tokens.shape) != (B,): raise RuntimeError(f"token_logprobs expects tokens int64 [{B}], got {tokens.dtype} {list(tokens.shape)}")
     if not 0 <= top <= min(MAX_TOP, V): raise RuntimeError(f"token_logprobs gives 0 to {min(MAX_TOP, V)} alternatives of {V} logits, not {top}")

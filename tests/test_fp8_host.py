@@ -55,14 +55,15 @@ def test_products_that_are_refused():
         with pytest.raises(RuntimeError, match="in bf16 into 8 bits"): fp8_gated(x, pair, out_dtype=torch.float32, quantize=True)
         for call in (lambda: fp8_linear(x, w), lambda: fp8_gated(x, pair), lambda: fp8_gated(x, pair, quantize=True)):
             with pytest.raises(RuntimeError, match="no CPU path"): call()
-    with pytest.raises(RuntimeError, match="expects rows bf16"): fp8_linear(X.double(), w, out_dtype=torch.bfloat16)
+    for bad in (X.double(), X[0], X[None], X[0, 0]):
+        with pytest.raises(RuntimeError, match="expects rows bf16"): fp8_linear(bad, w, out_dtype=torch.bfloat16)
     with pytest.raises(RuntimeError, match="up to 2\\^20 rows"): fp8_linear(torch.zeros(1, 256).expand((1 << 20) + 1, 256), w)
     with pytest.raises(RuntimeError, match="no CPU path"): rows.dequantize()
 
 
 def test_logprobs_that_are_refused():
     x, t = torch.zeros(4, 100), torch.zeros(4, dtype=torch.int64)
-    for bad in (x.double(), x[0], x[:, :0], torch.zeros(1).expand(4, 1 << 20)):
+    for bad in (x.double(), x[0], x[:, :0], torch.zeros(1).expand(4, 1 << 20), torch.zeros(1).expand((1 << 22) + 1, 8), torch.zeros(1).expand((1 << 21) + 1, 8193)):
         with pytest.raises(RuntimeError, match="token_logprobs expects logits"): token_logprobs(bad, t)
     for bad in (t.int(), t[:3], t[:, None], t.float()):
         with pytest.raises(RuntimeError, match="token_logprobs expects tokens"): token_logprobs(x, bad)
@@ -105,6 +106,8 @@ def test_gradients_are_not_lost_without_a_word(name):
     ("gaac_fp8_product", [16, 16, 16, 16, 5, 64, 256, 0, 4, 16, 64, None], "type must be"),
     ("gaac_fp8_product", [16, 16, 24, 16, 5, 64, 256, 0, 0, 16, 64, None], "16-byte aligned"),
     ("gaac_logprobs", [0, 16, 100, 0, 100, 16, 0, None, 0, 16, 16, 16, None, None, None], "bad sizes"),
+    ("gaac_logprobs", [0, 16, 100, (1 << 22) + 1, 100, 16, 0, None, 0, 16, 16, 16, None, None, None], "bad sizes"),
+    ("gaac_logprobs", [0, 16, 8193, (1 << 21) + 1, 8193, 16, 0, 16, 1 << 40, 16, 16, 16, None, None, None], "bad sizes"),
     ("gaac_logprobs", [0, 16, 100, 4, 1 << 20, 16, 0, None, 0, 16, 16, 16, None, None, None], "bad sizes"),
     ("gaac_logprobs", [0, 16, 100, 4, 100, 16, 65, None, 0, 16, 16, 16, 16, 16, None], "alternatives"),
     ("gaac_logprobs", [0, 16, 100, 4, 100, 16, 5, None, 0, 16, 16, 16, None, 16, None], "alternatives"),
