@@ -556,16 +556,16 @@ template <typename O, int MT, int NT, int AHEAD> void launch_stream(const Produc
 
 // Which form is taken: the one that should end first, its time being start + steps * (round * rounds + share * blocks / 256), rounds = blocks / 256 rounded up (a round: a block on each CU), steps the blocks of K
 // that a wave goes through.  The constants, in us, are fitted to the times of all forms over 180 sizes (1 to 8192 rows by 1024 to 28672 x 512 to 14336); over these the chosen form takes 1.6 % longer than the
-// best one in the mean (fp32: 0.9 % over 77).  Up to 16 rows, and wherever a block has one tile of rows, the products are the exact ones for every type: the weights' way from memory hides most of them (8 x 4096 x 4096 4.9 us,
+// best one in the mean (fp32: 0.6 % over 77).  Up to 16 rows, and wherever a block has one tile of rows, the products are the exact ones for every type: the weights' way from memory hides most of them (8 x 4096 x 4096 4.9 us,
 // 4.8 without; 8 x 28672 x 4096 23.6, 21.8).  Some of both sides, us, weights resident in turns (rows x N x K, outputs of 16 bits: stream of 1 x 1, 1 x 2, 2 x 2, 4 x 2 tiles | 64 x 64,
 // 64 x 128, 128 x 128 with four buffers, with two, 256 x 256 through LDS):
 //   8 x 4096 x 4096  4.9 5.6             8 x 28672 x 4096  23.9 23.6                                 48 x 4096 x 14336  28 25 16.9 23 | 32 48 51 95 142
 //   64 x 28672 x 4096  71 70 41 33 | 27 23.0 25 34 48            200 x 4096 x 4096  21 21 15 12 | 10.4 13 17 25 45             777 x 6144 x 4096  - - 56 49 | 41 41 37 35 51
 //   1024 x 28672 x 4096  - - 520 328 | 213 212 151 149 113       2048 x 4096 x 14336  | 190 174 120 116 158                    8192 x 8192 x 8192  | 810 753 581 511 403
 struct Form { int n, m, waves; float start, round, share; };      // tiles of weights and of rows a block, waves that share out K
-constexpr Form FORMS[9] = {{1, 1, 8, 1.f, .34f, .38f}, {2, 1, 8, 1.79f, .51f, .31f}, {2, 2, 8, 1.79f, .5f, .64f}, {2, 4, 8, 2.01f, .63f, .98f},
-                           {4, 4, 1, 4.05f, .28f, 0.f}, {8, 4, 1, 3.86f, .37f, .07f}, {8, 8, 1, 4.92f, .36f, .22f}, {8, 8, 1, 3.14f, .59f, .21f}, {16, 16, 1, 5.99f, 1.06f, .65f}};
-constexpr Form EXACT_FORMS[6] = {{1, 1, 8, .92f, .38f, .33f}, {2, 1, 8, .82f, .84f, .26f}, {2, 2, 8, .29f, .93f, .59f}, {2, 4, 8, .9f, .67f, 1.63f}, {4, 4, 1, 8.93f, .27f, .05f}, {8, 8, 1, 8.44f, .69f, .1f}};
+constexpr Form FORMS[9] = {{1, 1, 8, .76f, .46f, .28f}, {2, 1, 8, 1.81f, .57f, .24f}, {2, 2, 8, 1.79f, .5f, .63f}, {2, 4, 8, 1.9f, .63f, 1.f},
+                           {4, 4, 1, 3.97f, .28f, 0.f}, {8, 4, 1, 3.84f, .37f, .07f}, {8, 8, 1, 4.86f, .36f, .22f}, {8, 8, 1, 3.14f, .59f, .2f}, {16, 16, 1, 5.49f, 1.06f, .66f}};
+constexpr Form EXACT_FORMS[6] = {{1, 1, 8, .92f, .38f, .33f}, {2, 1, 8, .71f, .84f, .24f}, {2, 2, 8, .14f, .94f, .61f}, {2, 4, 8, .3f, .78f, 1.5f}, {4, 4, 1, 8.81f, .25f, .06f}, {8, 8, 1, 8.3f, .67f, .13f}};
 // (Forms whose launch would have more than 65535 blocks in y or 2^32 threads in x are left out; the fourth never has.)
 template <int COUNT> int form_of(const Form (&forms)[COUNT], const ProductArgs& a, bool gated) {
   int best = -1;

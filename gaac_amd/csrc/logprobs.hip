@@ -261,7 +261,7 @@ __device__ __forceinline__ u64 key_bound(const u64* keys, int c, int n, int most
 }
 
 // Joins a row's segments, a wave a row.  Every segment's list is sorted: the least of their n-th keys, n = top / segments rounded up, is a bound that `top` keys at least reach.  Those that do are ranked by
-// counting; where they are many more (a short last segment, or likely tokens in one place), those that reach a bound found bit by bit.
+// counting; where they are many more (a short last segment, or likely tokens in one place), those that reach the `top`-th of the lanes' best keys, and where these are too many as well, a bound found bit by bit.
 template <typename T>
 __global__ __launch_bounds__(64) void k_logprobs_merge(const T* logits, long row_stride, int V, const int64_t* tokens, int top, int segments, const Sums* sums, const u64* best, Out out) {
   extern __shared__ u64 keys[];      // of all segments, then those that are ranked, then their places
@@ -289,10 +289,19 @@ __global__ __launch_bounds__(64) void k_logprobs_merge(const T* logits, long row
   const int nth = (top + segments - 1) / segments - 1;
   u64 bound = min(l < segments ? keys[l * top + nth] : ~0ull, l + 64 < segments ? keys[(l + 64) * top + nth] : ~0ull);
   for (int o = 32; o > 0; o >>= 1) bound = min(bound, (u64)__shfl_xor(bound, o));
-  int reached = 0;
+  const auto too_many = [&] {
+    int reached = 0;
 #pragma unroll 4
-  for (int i = l; i < c; i += 64) reached += keys[i] >= bound;
-  if (wave_sum(reached) > most) bound = key_bound(keys, c, top, most);
+    for (int i = l; i < c; i += 64) reached += keys[i] >= bound;
+    return wave_sum(reached) > most;
+  };
+  if (too_many()) {
+    u64 b = 0;
+#pragma unroll 4
+    for (int i = l; i < c; i += 64) b = max(b, keys[i]);
+    bound = max(bound, nth_of(b, top));
+    if (too_many()) bound = key_bound(keys, c, top, most);
+  }
   int held = 0;
   for (int i0 = 0; i0 < c; i0 += 64) {
     const u64 k = i0 + l < c ? keys[i0 + l] : 0;

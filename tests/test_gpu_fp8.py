@@ -142,6 +142,17 @@ def test_gated_blocks(M, N, K, dtype):
     same(rows.dequantize(), R.stored(out))
 
 
+# sizes at which the forms that the smaller ones do not reach are taken: blocks of 4 x 2 tiles, of 64 x 128, 128 x 128 and 256 x 256 outputs; each with rows, columns and inputs that end inside a tile, and exponents inside a dword
+@pytest.mark.parametrize("M,N,K", [(150, 2000, 2100), (40, 9000, 1100), (300, 4100, 1300), (1100, 3700, 900), (700, 4100, 1000), (3000, 2100, 129), (4097, 5000, 650), (4111, 4999, 140), (3300, 4200, 200)])
+@pytest.mark.parametrize("dtype", [BF, FP16, FP32])
+def test_larger_products(M, N, K, dtype):
+    x, a, b = rnd(M, K, seed=M, dtype=dtype), rnd(N, K, seed=N), rnd(N, K, seed=N + 1)
+    a, b = a * K ** -0.5, b * K ** -0.5
+    X = R.stored(x)
+    within(fp8_linear(x, FP8Weight(a)), *R.product(X, R.stored(a), dtype))
+    within(fp8_gated(x, FP8Weight(a, b), out_dtype=dtype), *R.gated(X, R.stored(a), R.stored(b), dtype))
+
+
 @pytest.mark.parametrize("M", [1, 16, 40, 300, 700])
 def test_a_row_that_is_not_finite_is_its_own_matter(M):
     x, w = rnd(M, 700, seed=8), rnd(600, 700, seed=9)
