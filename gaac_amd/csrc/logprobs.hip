@@ -21,12 +21,9 @@ __device__ __forceinline__ void load16(const __bf16* p, float* x) { const bf8 v 
 __device__ __forceinline__ void load16(const _Float16* p, float* x) { const h8 v = *reinterpret_cast<const h8*>(p); for (int i = 0; i < 8; ++i) x[i] = (float)v[i]; }
 __device__ __forceinline__ void load16(const float* p, float* x) { const f4 v = *reinterpret_cast<const f4*>(p); for (int i = 0; i < 4; ++i) x[i] = v[i]; }
 
-// e^d for -104 <= d <= 0: the product with log2(e) in two parts, the second by the first two terms of its series (off by 2^-22 of itself, where one part alone would lose d's last bits).
-__device__ __forceinline__ float exp_of(float d) {
-  const float t = d * 1.44269502f, r = __builtin_fmaf(d, 1.33497652e-8f, __builtin_fmaf(d, 1.44269502f, -t) * 0.693147181f);
-  const float e = __builtin_amdgcn_exp2f(t);
-  return __builtin_fmaf(e, r, e);
-}
+// e^d for -104 <= d <= 0.  The product is rounded to 24 bits: e^d is off by |d| 2^-24 of itself, as much as by the rounding of d, a difference of 32-bit numbers.  What is far below the maximum adds little to a sum
+// unless there are e^|d| of its kind, so |d| is 14 at most where it counts: 2^-20, less than a logarithm of that size is rounded by.  (The product in two parts: four more instructions a logit, 104 us instead of 97 for 777 x 128256 in fp32 with 5 alternatives.)
+__device__ __forceinline__ float exp_of(float d) { return __builtin_amdgcn_exp2f(d * 1.44269502f); }
 __device__ __forceinline__ float cleaned(float x) { return x != x ? -__builtin_inff() : x; }      // NaN: a token that never comes
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) < __builtin_inff(); }
 __device__ __forceinline__ float distance(float x, float top) { return x == top ? 0.f : x - top; }      // (also where both are infinite)
@@ -108,7 +105,9 @@ template <int WIDTH> __device__ __forceinline__ void count_places(const u64* key
 constexpr int most_ranked(int top) { return 2 * top + 64; }
 constexpr int most_found(int top) { return WAVES * EACH * top; }      // keys at or above a bound of keys: no wave has more than `top` lanes there, each with its EACH tokens
 
-// Work memory of a row and segment: its sums, and behind those of all rows its `top` best keys.  About 25 instructions a logit, fewer than its way from memory takes in 32 bits.
+// Work memory of a row and segment: its sums, and behind those of all rows its `top` best keys.  What bounds it is the blocks' way from load to store, four
+// blocks a CU at once: instructions and waits (without alternatives 777 x 128256 take 73 us in fp32, 65 in bf16; with 5 97 and 91).  What is the same for a wave is counted by the scalar unit (ballots), and the given token's
+// logit is waited for behind the maximum.  Blocks that take several segments and read the next one ahead need 83 registers, three blocks a CU: 148 instead of 97.
 template <typename T>
 __global__ __launch_bounds__(THREADS) void k_logprobs(const T* logits, long row_stride, int V, const int64_t* tokens, int top, int segments, Sums* sums, u64* best, Out out) {
   constexpr int PER = 16 / sizeof(T), RUNS = EACH / PER;
@@ -125,23 +124,35 @@ __global__ __launch_bounds__(THREADS) void k_logprobs(const T* logits, long row_
   const bool aligned = reinterpret_cast<uintptr_t>(src) % 16 == 0;
   const int slot = n < SEGMENT ? l * WAVES + wave : (int)threadIdx.x;      // (a short segment is spread over all waves: the bound below goes by the one that has the least)
   if (threadIdx.x == 0) count = 0;
-  float x[EACH];
-#pragma unroll
-  for (int r = 0; r < RUNS; ++r) {
-    const int at = (r * THREADS + slot) * PER;
-    if (aligned && at + PER <= n) load16(src + at, x + r * PER);
-    else {
-#pragma unroll
-      for (int i = 0; i < PER; ++i) x[r * PER + i] = at + i < n ? (float)src[at + i] : -__builtin_inff();
-    }
-  }
   const long given = tokens[row];
   const int token = given >= 0 && given < V ? (int)given : -1;
-  const float mine = token >= 0 ? cleaned((float)logits[row * row_stride + token]) : 0.f;
+  float x[EACH];
+  if (aligned && n == SEGMENT) {
+#pragma unroll
+    for (int r = 0; r < RUNS; ++r) load16(src + (r * THREADS + threadIdx.x) * PER, x + r * PER);
+  } else {
+#pragma unroll
+    for (int r = 0; r < RUNS; ++r) {
+      const int at = (r * THREADS + slot) * PER;
+      if (aligned && at + PER <= n) load16(src + at, x + r * PER);
+      else {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) x[r * PER + i] = at + i < n ? (float)src[at + i] : -__builtin_inff();
+      }
+    }
+  }
+  const T at_token = logits[row * row_stride + max(token, 0)];      // (read last, and waited for only after the maximum)
   const auto index = [&](int i) { return (i / PER * THREADS + slot) * PER + i % PER; };
   float m = -__builtin_inff();
+  bool odd = false;      // a NaN among them
 #pragma unroll
-  for (int i = 0; i < EACH; ++i) { x[i] = cleaned(x[i]); m = fmaxf(m, x[i]); }
+  for (int i = 0; i < EACH; i += 2) odd |= __builtin_isunordered(x[i], x[i + 1]);
+  if (__any(odd)) {
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) x[i] = cleaned(x[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) m = fmaxf(m, x[i]);
   const float best_of_wave = wave_max(m);
   const int share = (top + WAVES - 1) / WAVES;
   if (top > 0) {
@@ -165,24 +176,17 @@ __global__ __launch_bounds__(THREADS) void k_logprobs(const T* logits, long row_
 #pragma unroll
     for (int i = 0; i < EACH; ++i) sum += x[i] == m ? 1.f : 0.f;
   }
-  if (finite(mine)) {      // before the token whatever is not smaller, behind it what is larger; what is behind the row's end is -inf
+  const float mine = token >= 0 ? cleaned((float)at_token) : 0.f;
+  const auto below = [](float v) { return v == 0.f ? -1.40129846e-45f : __builtin_bit_cast(float, __builtin_bit_cast(int, v) + (v > 0.f ? -1 : 1)); };      // the next one below
+  if (finite(mine) && (token < first || token >= first + SEGMENT)) {      // before the token whatever is not smaller, behind it what is larger; what is behind the row's end is -inf
+    const float limit = token < first ? mine : below(mine);
 #pragma unroll
-    for (int r = 0; r < RUNS; ++r) {
-      const int at = first + (r * THREADS + slot) * PER;
-      if (at > token || at + PER <= token) {
-        const float limit = at > token ? mine : mine == 0.f ? -1.40129846e-45f : __builtin_bit_cast(float, __builtin_bit_cast(int, mine) + (mine > 0.f ? -1 : 1));      // the next one below
-#pragma unroll
-        for (int i = 0; i < PER; ++i) above += x[r * PER + i] > limit;
-      } else {
-#pragma unroll
-        for (int i = 0; i < PER; ++i) above += at + i < token ? x[r * PER + i] >= mine : x[r * PER + i] > mine;
-      }
-    }
+    for (int i = 0; i < EACH; ++i) above += __popcll(__ballot(x[i] > limit));
   } else {
 #pragma unroll
-    for (int i = 0; i < EACH; ++i) above += index(i) < n && (x[i] > mine || (x[i] == mine && first + index(i) < token));
+    for (int i = 0; i < EACH; ++i) above += __popcll(__ballot(index(i) < n && (x[i] > mine || (x[i] == mine && first + index(i) < token))));
   }
-  sum = wave_sum(sum); weighted = wave_sum(weighted); above = wave_sum(above);
+  sum = wave_sum(sum); weighted = wave_sum(weighted);
   if (l == 0) { red[1][wave] = sum; red[2][wave] = weighted; above_of[wave] = above; }
   u64 bound = 0;
   if (top > 0) {
@@ -192,8 +196,7 @@ __global__ __launch_bounds__(THREADS) void k_logprobs(const T* logits, long row_
     const float limit = value_of(bound);
     int reach = 0;
 #pragma unroll
-    for (int i = 0; i < EACH; ++i) reach += x[i] >= limit;
-    reach = wave_sum(reach);
+    for (int i = 0; i < EACH; ++i) reach += __popcll(__ballot(x[i] >= limit));
     if (l == 0 && reach > 0) atomicAdd(&count, reach);
   }
   __syncthreads();
