@@ -123,8 +123,9 @@ struct RowsArgs {
 };
 
 // A block a row, of `waves` waves; a lane takes CH runs of 8 elements, 16 lanes a block of 128.  Bound by HBM: 16384 x 4096 in bf16 52 us (201 MB, 3.9 TB/s; a large copy makes 4.7 to 5.2), with norm and residual 113 (470 MB,
-// 4.2 TB/s); by launch and latency for a few rows (4 x 4096: 2.3, 3.6).  The sum of squares and the norm in 64 bits, which costs nothing beside the memory: a result next to the border between two
-// codes is rounded as the formula says.
+// 4.2 TB/s); by launch and latency for a few rows (4 x 4096: 2.3, 3.6).  The sum of squares and the norm in 64 bits: a result next to the border between two
+// codes is rounded as the formula says.  With a residual that costs nothing beside the memory; without one the conversions show (8192 x 4096 35 us, 28 without the norm; 8192 x 14336 152, 88).  Pairs of 32-bit numbers took
+// longer (registers: 16384 x 4096 with residual 121, 118 in 64 bits then).
 template <typename T, bool NORM, int CH>
 __global__ __launch_bounds__(1024) void k_fp8_rows(RowsArgs a) {
   __shared__ double sums[16];
@@ -184,7 +185,7 @@ __global__ __launch_bounds__(1024) void k_fp8_rows(RowsArgs a) {
   }
 }
 
-// The way back: a block of threads a tile, 16 lanes a row's 256 bytes.
+// The way back: a block of threads a tile, 16 lanes a row's 256 bytes.  Bound by HBM: 16384 x 4096 37 us (201 MB, 5.4 TB/s).
 __global__ __launch_bounds__(256) void k_fp8_values(const uint8_t* data, const uint8_t* exps, long pad, int tile_step, int tile_first, long first, int M, int K, int nb, __bf16* out, long out_rs, bool whole) {
   const int p = threadIdx.x & 15, m = threadIdx.x >> 4, kb = blockIdx.x % nb;
   const long tile = first + blockIdx.x / nb, row = 16 * tile + m, tile_row = tile * tile_step + tile_first;
@@ -272,7 +273,8 @@ template <typename O, bool GATED> __device__ __forceinline__ void finish(const P
 }
 
 // Few rows: the weights go by once.  A block has NT tiles of weights and MT of rows; its eight waves share the blocks of K out, four (a dword of exponents) at a time, and their sums meet in LDS, in
-// the waves' order.  A wave holds the operands of AHEAD steps in registers, each set loaded again as soon as it is used: what bounds it is how many loads are on their way.
+// the waves' order.  A wave holds the operands of AHEAD steps in registers, each set loaded again as soon as it is used: what bounds it is how many loads are on their way
+// (a CU draws 145 GB/s from its L2 at most).  4 x 6144 x 4096 4.6 us (25.4 MB, 5.5 TB/s), 4 x 28672 x 4096 gated 20.4 (118 MB, 5.8), 48 x 4096 x 14336 13.4 (59 MB, 4.4), 200 x 4096 x 4096 in fp32 13.4 to 14 (480 TFLOP/s).
 template <typename O, int MT, int NT, int AHEAD, bool GATED>
 __global__ __launch_bounds__(512, 2) void k_fp8_stream(ProductArgs a) {
   static_assert(!GATED || NT % 2 == 0, "tiles of a gated pair alternate");
@@ -378,7 +380,9 @@ __global__ __launch_bounds__(512, 2) void k_fp8_stream(ProductArgs a) {
 }
 
 // Many rows: tiles of both operands through LDS.  A block has WN x WM waves, a wave TN tiles of weights by TM of rows; a step is one block of K, whose tiles (whole kilobytes, in the
-// operands' order) go straight into LDS while the step before is computed, in two buffers by turns.
+// operands' order) go straight into LDS while steps before are computed, in two or four buffers by turns.  256 x 256, two buffers: matrix unit and LDS share the time: a step is 2048 cycles of products on each SIMD's unit
+// and moves 256 KB (64 in, 192 out) at 128 bytes a cycle, as many; 8192 x 28672 x 4096 812 to 825 us (2330 to 2370 TFLOP/s; the matrix units busy for 55 % of the cycles), 8192 x 8192 x 8192 403 (2730; the library's product 338 to 386).  Smaller blocks
+// have four buffers, or two where two blocks share a CU: a step waits for HBM, 0.8 us with one step on its way, 0.45 with three (777 x 6144 x 4096 in 128 x 128 33 us, 1180 TFLOP/s: 336 blocks are two rounds).
 typedef const __attribute__((address_space(1))) void* global_ptr;
 typedef __attribute__((address_space(3))) void* lds_ptr;
 
