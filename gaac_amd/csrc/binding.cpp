@@ -564,7 +564,7 @@ PyObject* draw(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 // Rows in 8 bits, their products, and log probabilities, the same way.  Host us a call, Python / here: quantize_fp8 11.2 / 6.1, rms_norm_fp8 with a residual 14.6 / 7.0, dequantize 7.8 / 5.0, a product of rows in
-// 8 bits 8.5 / 5.2 and of a tensor 21.1 / 9.5 (two launches; its 8 bits in two allocations instead of one: 10.2), token_logprobs 15.5 / 7.0, with alternatives 19.4 / 8.8.
+// 8 bits 8.5 / 5.2 and of a tensor 21.1 / 9.5 (two launches; its 8 bits in two allocations instead of one: 10.2), token_logprobs 15.7 / 6.5, with alternatives 19.5 / 8.2.
 long blocks_of(long K) { return (K + 127) / 128; }
 long padded(long rows) { return (rows + 15) / 16 * 16; }
 at::ScalarType type_of(long code) {
@@ -676,10 +676,11 @@ PyObject* logprobs(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (t.dim() != 1 || t.size(0) != B || t.scalar_type() != at::kLong || !t.is_contiguous() || top < 0 || top > std::min(64l, V)) throw Otherwise{};
     void* stream = stream_of(a[3]);
     const long segments = (V + 8191) / 8192, work_bytes = segments == 1 ? 0 : B * segments * (16 + 8 * top);      // logprobs_work_bytes in sampling.py
-    at::Tensor work = bytes(x, {work_bytes}), value = bytes(x, {B}, at::kFloat), rank = bytes(x, {B}, at::kLong), entropy = bytes(x, {B}, at::kFloat), top_values, top_tokens;
+    at::Tensor work, value = bytes(x, {B}, at::kFloat), rank = bytes(x, {B}, at::kLong), entropy = bytes(x, {B}, at::kFloat), top_values, top_tokens;
+    if (work_bytes > 0) work = bytes(x, {work_bytes});
     if (top > 0) { top_values = bytes(x, {B, top}, at::kFloat); top_tokens = bytes(x, {B, top}, at::kLong); }
     must("gaac_logprobs", without_gil([&] {
-      return p_gaac_logprobs(type, x.data_ptr(), B > 1 ? x.stride(0) : 0, static_cast<int>(B), static_cast<int>(V), static_cast<int64_t*>(t.data_ptr()), static_cast<int>(top), work.data_ptr(), work_bytes,
+      return p_gaac_logprobs(type, x.data_ptr(), B > 1 ? x.stride(0) : 0, static_cast<int>(B), static_cast<int>(V), static_cast<int64_t*>(t.data_ptr()), static_cast<int>(top), work_bytes > 0 ? work.data_ptr() : nullptr, work_bytes,
                              static_cast<float*>(value.data_ptr()), static_cast<int64_t*>(rank.data_ptr()), static_cast<float*>(entropy.data_ptr()), top > 0 ? static_cast<float*>(top_values.data_ptr()) : nullptr,
                              top > 0 ? static_cast<int64_t*>(top_tokens.data_ptr()) : nullptr, stream);
     }));

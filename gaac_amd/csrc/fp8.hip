@@ -122,7 +122,7 @@ struct RowsArgs {
   bool whole;
 };
 
-// A block a row, of `waves` waves; a lane takes CH runs of 8 elements, 16 lanes a block of 128.  Bound by HBM: 16384 x 4096 in bf16 52 us (201 MB, 3.9 TB/s; a large copy makes 4.7 to 5.2), with norm and residual 113 (470 MB,
+// A block a row (for few rows without the norm: a part of a row), of `waves` waves; a lane takes CH runs of 8 elements, 16 lanes a block of 128.  Bound by HBM: 16384 x 4096 in bf16 52 us (201 MB, 3.9 TB/s; a large copy makes 4.7 to 5.2), with norm and residual 113 (470 MB,
 // 4.2 TB/s); by launch and latency for a few rows (4 x 4096: 2.3, 3.6).  The sum of squares and the norm in 64 bits: a result next to the border between two
 // codes is rounded as the formula says.  With a residual that costs nothing beside the memory; without one the conversions show (8192 x 4096 35 us, 28 without the norm; 8192 x 14336 152, 88).  Pairs of 32-bit numbers took
 // longer (registers: 16384 x 4096 with residual 121, 118 in 64 bits then).
@@ -134,7 +134,8 @@ __global__ __launch_bounds__(1024) void k_fp8_rows(RowsArgs a) {
   // with rows in the blocks' order, 52 so).
   const int turn = blockIdx.x & ~127u, in_turn = blockIdx.x & 127u, row = (turn + 128 <= (int)gridDim.x ? turn + in_turn % 8 * 16 + in_turn / 8 : (int)blockIdx.x) + a.first;
   const T* src = static_cast<const T*>(a.x) + row * a.x_rs;
-  const auto at = [&](int i) { return 8 * ((i * a.waves + part) * 64 + l); };
+  const int from = NORM ? part : (int)blockIdx.y * a.waves + part, all = NORM ? a.waves : (int)gridDim.y * a.waves;
+  const auto at = [&](int i) { return 8 * ((i * all + from) * 64 + l); };
   float x[CH][8];
 #pragma unroll
   for (int i = 0; i < CH; ++i) load_some(src + at(i), a.K - at(i), a.whole, x[i]);
@@ -610,24 +611,26 @@ template <typename O> void launch_product(const ProductArgs& a, bool gated, hipS
   }
 }
 
-constexpr int MOST_ROWS = 1 << 20;      // of one launch, of up to 1024 threads a row: a launch has less than 2^32
-template <typename T, int CH> void launch_rows(RowsArgs a, int M, hipStream_t s) {
+constexpr int MOST_ROWS = 1 << 20, PART = 4;      // of one launch, of up to 1024 threads a row: a launch has less than 2^32 in x | waves of a part of a row
+template <typename T, int CH> void launch_rows(RowsArgs a, int M, int parts, hipStream_t s) {
   for (a.first = 0; a.first < M; a.first += MOST_ROWS) {
     const int n = M - a.first < MOST_ROWS ? M - a.first : MOST_ROWS;
     if constexpr (CH < 8) {
       if (a.weight != nullptr) { k_fp8_rows<T, true, CH><<<n, 64 * a.waves, 0, s>>>(a); continue; }
     }
-    k_fp8_rows<T, false, CH><<<n, 64 * a.waves, 0, s>>>(a);
+    k_fp8_rows<T, false, CH><<<dim3(n, parts), 64 * a.waves, 0, s>>>(a);
   }
 }
 // One run a lane for few rows, where latency counts, two for many (us, one / two runs, with the norm: 4 x 4096 4.0 / 4.8, 300 x 4096 6.3 / 6.9, 777 x 5000 12.5 / 10.9, 16384 x 4096 125 / 113); more only where a block's 16 waves
-// would not do.  (The norm of 8 runs would not fit the registers.)
+// would not do.  (The norm of 8 runs would not fit the registers.)  Few rows without the norm in parts of up to four waves, a block each (us, a block a row / in parts: 4 x 14336 2.9 / 2.2, 48 x 14336 3.9 / 3.1); many rows
+// not: 2048 x 16384 25.9 / 30.0, as the parts of a row are then read far from each other.
 template <typename T> void launch_rows(RowsArgs a, int M, hipStream_t s) {
   const auto waves = [&](int n) { return (a.nb * 16 + 64 * n - 1) / (64 * n); };
-  int ch = (long)M * waves(1) <= 4096 ? 1 : 2;
-  while (waves(ch) > 16) ch *= 2;
-  a.waves = waves(ch);
-  if (ch == 1) launch_rows<T, 1>(a, M, s); else if (ch == 2) launch_rows<T, 2>(a, M, s); else if (ch == 4) launch_rows<T, 4>(a, M, s); else launch_rows<T, 8>(a, M, s);
+  int ch = (long)M * waves(1) <= 4096 ? 1 : 2, parts = 1;
+  if (ch == 1 && a.weight == nullptr) parts = (waves(1) + PART - 1) / PART;
+  while ((waves(ch) + parts - 1) / parts > 16) ch *= 2;
+  a.waves = (waves(ch) + parts - 1) / parts;
+  if (ch == 1) launch_rows<T, 1>(a, M, parts, s); else if (ch == 2) launch_rows<T, 2>(a, M, 1, s); else if (ch == 4) launch_rows<T, 4>(a, M, 1, s); else launch_rows<T, 8>(a, M, 1, s);
 }
 
 uintptr_t address(const void* p) { return reinterpret_cast<uintptr_t>(p); }
