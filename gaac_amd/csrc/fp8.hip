@@ -381,20 +381,21 @@ __global__ __launch_bounds__(512, 2) void k_fp8_stream(ProductArgs a) {
 }
 
 // Many rows: tiles of both operands through LDS.  A block has WN x WM waves, a wave TN tiles of weights by TM of rows; a step is one block of K, whose tiles (whole kilobytes, in the
-// operands' order) go straight into LDS while steps before are computed, in two or four buffers by turns.  256 x 256, two buffers: matrix unit and LDS share the time: a step is 2048 cycles of products on each SIMD's unit
+// operands' order) go straight into LDS while steps before are computed, in two to four buffers by turns.  256 x 256, two buffers: matrix unit and LDS share the time: a step is 2048 cycles of products on each SIMD's unit
 // and moves 256 KB (64 in, 192 out) at 128 bytes a cycle, as many; 8192 x 28672 x 4096 812 to 825 us (2330 to 2370 TFLOP/s; the matrix units busy for 55 % of the cycles), 8192 x 8192 x 8192 403 (2730; the library's product 338 to 386).  Smaller blocks
-// have four buffers, or two where two blocks share a CU: a step waits for HBM, 0.8 us with one step on its way, 0.45 with three (777 x 6144 x 4096 in 128 x 128 33 us, 1180 TFLOP/s: 336 blocks are two rounds).
+// have four buffers, or two where two blocks share a CU: a step waits for HBM, 0.8 us with one step on its way, 0.45 with three.  192 rows x 128 of weights, three buffers (their turns and those of the exponents' bytes meet again after
+// twelve steps): where it saves a round, 777 x 6144 x 4096 28.5 us (1370 TFLOP/s, 240 blocks; 37 with 336 of 128 x 128), 1536 x 4096 x 14336 84 (104).
 typedef const __attribute__((address_space(1))) void* global_ptr;
 typedef __attribute__((address_space(3))) void* lds_ptr;
 
 template <typename O, int TN, int TM, int WN, int WM, int NBUF, bool GATED>
 __global__ __launch_bounds__(64 * WN * WM, TN * TM == 64 ? 1 : 2) void k_fp8_tiles(ProductArgs a, int blocks_n, int blocks_m) {
   constexpr int W = WN * WM, TILES = WN * TN + WM * TM, LOADS = 2 * TILES / W, ROWS_W = 16 * WN * TN, ROWS = 16 * TILES;
-  static_assert(2 * TILES % W == 0 && ROWS_W % 64 == 0 && ROWS % 64 == 0 && TN % 2 == 0 && (NBUF == 2 || NBUF == 4), "every wave loads as many kilobytes; a wave loads the exponents of 64 rows of one operand; tiles of a gated pair alternate");
+  static_assert(2 * TILES % W == 0 && ROWS_W % 64 == 0 && ROWS % 64 == 0 && TN % 2 == 0 && NBUF >= 2 && NBUF <= 4, "every wave loads as many kilobytes; a wave loads the exponents of 64 rows of one operand; tiles of a gated pair alternate");
   constexpr bool EXACT = sizeof(O) == 4;
   __shared__ __attribute__((aligned(16))) uint8_t buf0[TILES * TILE];
   __shared__ __attribute__((aligned(16))) uint8_t buf1[TILES * TILE];
-  __shared__ __attribute__((aligned(16))) uint8_t buf2[NBUF == 4 ? TILES * TILE : 16];
+  __shared__ __attribute__((aligned(16))) uint8_t buf2[NBUF > 2 ? TILES * TILE : 16];
   __shared__ __attribute__((aligned(16))) uint8_t buf3[NBUF == 4 ? TILES * TILE : 16];
   __shared__ unsigned exps[2 * ROWS];
   const auto buffer = [&](auto byte) -> uint8_t* {
@@ -472,8 +473,8 @@ __global__ __launch_bounds__(64 * WN * WM, TN * TM == 64 ? 1 : 2) void k_fp8_til
     if constexpr (TN * TM == 64) asm volatile("" : "+a"(v)); else asm volatile("" : "+v"(v));
   };
   const auto step = [&](auto byte, int kb) {
-    constexpr int S = decltype(byte)::value;
-    uint8_t *now = buffer(Byte<S>{}), *then = buffer(Byte<S + 1>{});
+    constexpr int U = decltype(byte)::value, S = U % 4;
+    uint8_t *now = buffer(Byte<U>{}), *then = buffer(Byte<U + 1>{});
     Operand<EXACT> ox[TM];
 #pragma unroll
     for (int j = 0; j < TM; ++j) ox[j] = Operand<EXACT>::template of<S>(x[j].a, x[j].b, ex[j]);
@@ -511,7 +512,8 @@ __global__ __launch_bounds__(64 * WN * WM, TN * TM == 64 ? 1 : 2) void k_fp8_til
   fetch_exps(0);
   fetch(buf0);
   fetch(buf1);
-  if constexpr (NBUF == 4) { fetch(buf2); fetch(buf3); }
+  if constexpr (NBUF > 2) fetch(buf2);
+  if constexpr (NBUF == 4) fetch(buf3);
   __builtin_amdgcn_s_waitcnt(0x0070 | ((NBUF - 1) * LOADS & 15) | (NBUF - 1) * LOADS >> 4 << 14);
   __syncthreads();
   read_exps(0);
@@ -526,15 +528,53 @@ __global__ __launch_bounds__(64 * WN * WM, TN * TM == 64 ? 1 : 2) void k_fp8_til
     for (int j = 0; j < TM; ++j) ex[j] = next_x[j];
   };
   int kb = 0;
-  for (; kb + 4 <= a.nb; kb += 4) {
-    next_exps();
-    step(Byte<0>{}, kb); step(Byte<1>{}, kb + 1); step(Byte<2>{}, kb + 2); step(Byte<3>{}, kb + 3);
-  }
-  if (kb < a.nb) {
-    next_exps();
-    step(Byte<0>{}, kb);
-    if (kb + 1 < a.nb) step(Byte<1>{}, kb + 1);
-    if (kb + 2 < a.nb) step(Byte<2>{}, kb + 2);
+  if constexpr (NBUF == 3) {
+    for (; kb + 12 <= a.nb; kb += 12) {
+      next_exps();
+      step(Byte<0>{}, kb); step(Byte<1>{}, kb + 1); step(Byte<2>{}, kb + 2); step(Byte<3>{}, kb + 3);
+      next_exps();
+      step(Byte<4>{}, kb + 4); step(Byte<5>{}, kb + 5); step(Byte<6>{}, kb + 6); step(Byte<7>{}, kb + 7);
+      next_exps();
+      step(Byte<8>{}, kb + 8); step(Byte<9>{}, kb + 9); step(Byte<10>{}, kb + 10); step(Byte<11>{}, kb + 11);
+    }
+    const int left = a.nb - kb;
+    if (left >= 8) {
+      next_exps();
+      step(Byte<0>{}, kb); step(Byte<1>{}, kb + 1); step(Byte<2>{}, kb + 2); step(Byte<3>{}, kb + 3);
+      next_exps();
+      step(Byte<4>{}, kb + 4); step(Byte<5>{}, kb + 5); step(Byte<6>{}, kb + 6); step(Byte<7>{}, kb + 7);
+      if (left > 8) {
+        next_exps();
+        step(Byte<8>{}, kb + 8);
+        if (left > 9) step(Byte<9>{}, kb + 9);
+        if (left > 10) step(Byte<10>{}, kb + 10);
+      }
+    } else if (left > 0) {
+      next_exps();
+      step(Byte<0>{}, kb);
+      if (left > 1) step(Byte<1>{}, kb + 1);
+      if (left > 2) step(Byte<2>{}, kb + 2);
+      if (left > 3) {
+        step(Byte<3>{}, kb + 3);
+        if (left > 4) {
+          next_exps();
+          step(Byte<4>{}, kb + 4);
+          if (left > 5) step(Byte<5>{}, kb + 5);
+          if (left > 6) step(Byte<6>{}, kb + 6);
+        }
+      }
+    }
+  } else {
+    for (; kb + 4 <= a.nb; kb += 4) {
+      next_exps();
+      step(Byte<0>{}, kb); step(Byte<1>{}, kb + 1); step(Byte<2>{}, kb + 2); step(Byte<3>{}, kb + 3);
+    }
+    if (kb < a.nb) {
+      next_exps();
+      step(Byte<0>{}, kb);
+      if (kb + 1 < a.nb) step(Byte<1>{}, kb + 1);
+      if (kb + 2 < a.nb) step(Byte<2>{}, kb + 2);
+    }
   }
 #pragma unroll
   for (int i = 0; i < TAIL; ++i) asm volatile("" : : "v"(w[i].a), "v"(w[i].b));
@@ -561,15 +601,15 @@ template <typename O, int MT, int NT, int AHEAD> void launch_stream(const Produc
 
 // Which form is taken: the one that should end first, its time being start + steps * (round * rounds + share * blocks / 256), rounds = blocks / 256 rounded up (a round: a block on each CU), steps the blocks of K
 // that a wave goes through.  The constants, in us, are fitted to the times of all forms over 180 sizes (1 to 8192 rows by 1024 to 28672 x 512 to 14336); over these the chosen form takes 1.6 % longer than the
-// best one in the mean (fp32: 0.6 % over 77).  Up to 16 rows, and wherever a block has one tile of rows, the products are the exact ones for every type: the weights' way from memory hides most of them (8 x 4096 x 4096 4.9 us,
+// best one in the mean (fp32: 0.6 % over 77), and over 112 with the form of 192 rows 1.3 % (2.8 without it).  Up to 16 rows, and wherever a block has one tile of rows, the products are the exact ones for every type: the weights' way from memory hides most of them (8 x 4096 x 4096 4.9 us,
 // 4.8 without; 8 x 28672 x 4096 23.6, 21.8).  Some of both sides, us, weights resident in turns (rows x N x K, outputs of 16 bits: stream of 1 x 1, 1 x 2, 2 x 2, 4 x 2 tiles | 64 x 64,
-// 64 x 128, 128 x 128 with four buffers, with two, 256 x 256 through LDS):
+// 64 x 128, 128 x 128 with four buffers, with two, 256 x 256, 192 x 128 through LDS):
 //   8 x 4096 x 4096  4.9 5.6             8 x 28672 x 4096  23.9 23.6                                 48 x 4096 x 14336  28 25 16.9 23 | 32 48 51 95 142
-//   64 x 28672 x 4096  71 70 41 33 | 27 23.0 25 34 48            200 x 4096 x 4096  21 21 15 12 | 10.4 13 17 25 45             777 x 6144 x 4096  - - 56 49 | 41 41 37 35 51
+//   64 x 28672 x 4096  71 70 41 33 | 27 23.0 25 34 48            200 x 4096 x 4096  21 21 15 12 | 10.4 13 17 25 45             777 x 6144 x 4096  - - 56 49 | 41 41 37 35 51 28.5
 //   1024 x 28672 x 4096  - - 520 328 | 213 212 151 149 113       2048 x 4096 x 14336  | 190 174 120 116 158                    8192 x 8192 x 8192  | 810 753 581 511 403
 struct Form { int n, m, waves; float start, round, share; };      // tiles of weights and of rows a block, waves that share out K
-constexpr Form FORMS[9] = {{1, 1, 8, .76f, .46f, .28f}, {2, 1, 8, 1.81f, .57f, .24f}, {2, 2, 8, 1.79f, .5f, .63f}, {2, 4, 8, 1.9f, .63f, 1.f},
-                           {4, 4, 1, 3.97f, .28f, 0.f}, {8, 4, 1, 3.84f, .37f, .07f}, {8, 8, 1, 4.86f, .36f, .22f}, {8, 8, 1, 3.14f, .59f, .2f}, {16, 16, 1, 5.49f, 1.06f, .66f}};
+constexpr Form FORMS[10] = {{1, 1, 8, .76f, .46f, .28f}, {2, 1, 8, 1.81f, .57f, .24f}, {2, 2, 8, 1.79f, .5f, .63f}, {2, 4, 8, 1.9f, .63f, 1.f},
+                           {4, 4, 1, 3.97f, .28f, 0.f}, {8, 4, 1, 3.84f, .37f, .07f}, {8, 8, 1, 4.86f, .36f, .22f}, {8, 8, 1, 3.14f, .59f, .2f}, {16, 16, 1, 5.49f, 1.06f, .66f}, {8, 12, 1, 4.f, .44f, .4f}};
 constexpr Form EXACT_FORMS[6] = {{1, 1, 8, .92f, .38f, .33f}, {2, 1, 8, .71f, .84f, .24f}, {2, 2, 8, .14f, .94f, .61f}, {2, 4, 8, .3f, .78f, 1.5f}, {4, 4, 1, 8.81f, .25f, .06f}, {8, 8, 1, 8.3f, .67f, .13f}};
 // (Forms whose launch would have more than 65535 blocks in y or 2^32 threads in x are left out; the fourth never has.)
 template <int COUNT> int form_of(const Form (&forms)[COUNT], const ProductArgs& a, bool gated) {
@@ -606,7 +646,8 @@ template <typename O> void launch_product(const ProductArgs& a, bool gated, hipS
       case 5: return launch_tiles<O, 4, 1, 2, 4, 4>(a, gated, s);
       case 6: return launch_tiles<O, 4, 2, 2, 4, 4>(a, gated, s);
       case 7: return launch_tiles<O, 4, 2, 2, 4, 2>(a, gated, s);
-      default: return launch_tiles<O, 8, 4, 2, 4, 2>(a, gated, s);
+      case 8: return launch_tiles<O, 8, 4, 2, 4, 2>(a, gated, s);
+      default: return launch_tiles<O, 4, 3, 2, 4, 3>(a, gated, s);
     }
   }
 }

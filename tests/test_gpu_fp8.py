@@ -153,6 +153,17 @@ def test_larger_products(M, N, K, dtype):
     within(fp8_gated(x, FP8Weight(a, b), out_dtype=dtype), *R.gated(X, R.stored(a), R.stored(b), dtype))
 
 
+# blocks of 192 x 128 outputs go through K in turns of twelve blocks, and every number of blocks that is left has an end of its own
+@pytest.mark.parametrize("blocks", [2, 3, 4, 5, 6, 7, 8, 9, 10, 11, 12, 13, 19, 24])
+def test_every_end_of_the_inputs(blocks):
+    M, N, K = 770, 6100, 128 * blocks - 5
+    x, a = rnd(M, K, seed=blocks), rnd(N, K, seed=blocks + 1) * K ** -0.5
+    X, A = R.stored(x), R.stored(a)
+    within(fp8_linear(x, FP8Weight(a)), *R.product(X, A, BF))
+    gate, up = a[:3050], a[3050:]
+    within(fp8_gated(x, FP8Weight(gate, up)), *R.gated(X, R.stored(gate), R.stored(up), BF))
+
+
 @pytest.mark.parametrize("M", [1, 16, 40, 300, 700])
 def test_a_row_that_is_not_finite_is_its_own_matter(M):
     x, w = rnd(M, 700, seed=8), rnd(600, 700, seed=9)
