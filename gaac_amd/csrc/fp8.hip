@@ -275,7 +275,7 @@ template <typename O, bool GATED> __device__ __forceinline__ void finish(const P
 
 // Few rows: the weights go by once.  A block has NT tiles of weights and MT of rows; its eight waves share the blocks of K out, four (a dword of exponents) at a time, and their sums meet in LDS, in
 // the waves' order.  A wave holds the operands of AHEAD steps in registers, each set loaded again as soon as it is used: what bounds it is how many loads are on their way
-// (a CU draws 145 GB/s from its L2 at most).  4 x 6144 x 4096 4.6 us (25.4 MB, 5.5 TB/s), 4 x 28672 x 4096 gated 20.4 (118 MB, 5.8), 48 x 4096 x 14336 13.4 (59 MB, 4.4), 200 x 4096 x 4096 in fp32 13.4 to 14 (480 TFLOP/s).
+// (a CU draws 145 GB/s from its L2 at most).  4 x 6144 x 4096 4.6 us (25.4 MB, 5.5 TB/s), 4 x 28672 x 4096 gated 20.4 (118 MB, 5.8), 48 x 4096 x 14336 13.4 (59 MB, 4.4), 200 x 4096 x 4096 in fp32 13.4 to 14.6 (480 TFLOP/s).
 template <typename O, int MT, int NT, int AHEAD, bool GATED>
 __global__ __launch_bounds__(512, 2) void k_fp8_stream(ProductArgs a) {
   static_assert(!GATED || NT % 2 == 0, "tiles of a gated pair alternate");
