@@ -80,7 +80,7 @@ def gated(x, gate, up, dtype):
 def logprobs(logits, tokens, top):
     """(logprob, rank, entropy, top_logprobs, top_tokens, tolerance of a log probability of size p, of the entropy), fp64 / int64 on the CPU.
 
-    e^d is off by 2^-21 of itself; a sum passes 16 + 6 + 8 additions and one for each segment, 2^-24 each, at most 2^-18 for the segments of the tests; so the sum's logarithm is off by 2^-17; differences and
+    e^d is off by 1.2 |d| 2^-24 of itself, 2^-19 for |d| up to 26 (what lies farther below adds less than 2^-19 of the sum, even 2^18 times); a sum passes 16 + 6 + 8 additions and one for each segment, 2^-24 each, at most 2^-18 for the segments of the tests; so the sum's logarithm is off by 2^-17; differences and
     the result are rounded to 24 bits.  The entropy's second term is such a sum of e^d d, over the first."""
     x = logits.detach().double().cpu()
     x = torch.where(x.isnan(), -torch.inf, x)
