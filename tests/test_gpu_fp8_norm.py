@@ -1,0 +1,69 @@
+"""The norm before rows in 8 bits, code by code: results that 32 bits round to zero.
+
+The kernel has y in 64 bits, off by a few 2^-52 of itself, so its codes are the formula's wherever y is not that near to a border; rows here are equal to the definition, without a tolerance."""
+import pytest
+import torch
+
+import fp8_ref as R
+from gaac_amd import FP8Weight, _lib, fp8_linear, rms_norm_fp8
+from gpu_util import require_gpu
+
+pytestmark = pytest.mark.gpu
+BF, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
+
+
+@pytest.fixture(autouse=True, params=["binding", "ctypes"])
+def gpu(request, monkeypatch):
+    require_gpu()
+    if request.param == "ctypes": monkeypatch.setattr(_lib, "_calls", _lib._CtypesCalls())
+
+
+def rnd(*shape, seed=0, dtype=BF):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed)).to(dtype)
+
+
+def codes_of(x, w, eps, residual=None):
+    """rms_norm_fp8's values, fp64 on the CPU, and those of the definition: of the sum in 32 bits, where there is a residual."""
+    dev = lambda t: None if t is None else t.cuda()
+    out = rms_norm_fp8(dev(x), dev(w), eps, residual=dev(residual))
+    return (out if residual is None else out[0]).dequantize().double().cpu(), R.stored(R.norm(x if residual is None else x.float() + residual.float(), w, eps)[0])
+
+
+def same(a, b):
+    assert torch.equal(a.isnan(), b.isnan()), f"{int(a.isnan().sum())} NaN, {int(b.isnan().sum())} by the definition"
+    assert torch.equal(a.nan_to_num(0), b.nan_to_num(0)), f"{int((a != b).sum())} of {a.numel()} codes differ"
+
+
+@pytest.mark.parametrize("dtype", [BF, FP32])
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("M,K", [(1, 128), (3, 300), (17, 4096), (5, 5000), (2, 20000)])
+def test_results_that_32_bits_round_to_zero(M, K, residual, dtype):
+    """Elements of ordinary rows with h * weight from 1e-44 to 1e-60, of both signs: 0 in 8 bits, and what is beside them by the definition."""
+    x, w = rnd(M, K, seed=K, dtype=dtype), torch.rand(K, generator=torch.Generator().manual_seed(1)).to(dtype) + 0.5
+    r = rnd(M, K, seed=K + 1, dtype=dtype) if residual else None
+    at = torch.arange(5, K, 37)
+    w[at] = (10.0 ** -torch.linspace(24, 30, len(at)).double()).to(dtype)
+    x[:, at] = ((10.0 ** -torch.linspace(20, 30, len(at)).double()) * torch.where(torch.arange(len(at)) % 3 == 0, -1, 1)).to(dtype)
+    if residual: r[:, at] = 0
+    w[at[-1]] = -w[at[-1]]
+    got, want = codes_of(x, w, 1e-5, r)
+    same(got, want)
+    assert (got[:, at] == 0).all()
+    out = fp8_linear(rms_norm_fp8(x.cuda(), w.cuda(), 1e-5), FP8Weight(rnd(20, K, seed=3).cuda()))
+    assert out.isfinite().all()
+    # blocks with nothing else, in rows that have other blocks
+    if K > 128:
+        w[:128], x[:, :128] = 1e-25, 1e-25
+        if residual: r[:, :128] = 0
+        got, want = codes_of(x, w, 1e-5, r)
+        same(got, want)
+        assert (got[:, :128] == 0).all() and (got[:, 128:] != 0).any()
+
+
+def test_one_element_far_above_another():
+    for dtype in (BF, FP32):
+        x = torch.zeros(1, 128, dtype=dtype)
+        x[0, 3], x[0, 70] = 1e20, 1e-27
+        got, want = codes_of(x, torch.ones(128, dtype=dtype), 1e-6)
+        same(got, want)
+        assert got[0, 70] == 0 and got[0, 3] == 11      # sqrt(128) is 11.3
