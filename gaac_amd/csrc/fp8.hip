@@ -103,12 +103,12 @@ __device__ __forceinline__ double wave_sum(double x) {
 }
 
 // y in 32 bits, rounded to an odd last bit where bits are lost: rounding once more, to 8 bits, then gives what rounding y itself would.  It matters only where the nearest number of 32 bits is a border between
-// two codes, which has 19 zeros at its end.  The neighbour is taken by magnitude, so that 0 has one too, the smallest number of y's sign.
+// two codes, which has 19 zeros at its end.  The neighbour is taken by magnitude: what is rounded to 0 becomes the smallest number of y's sign, what is finite and rounded to infinity the largest.
 __device__ __forceinline__ float to_odd(double y) {
   const float f = (float)y;
-  const double d = fabs(y) - fabs((double)f);
+  const double d = fabs(y) - fabs((double)f);      // (NaN where y is infinite or NaN)
   const unsigned u = word(f);
-  return d == 0.0 || (u & 1u) || !(fabsf(f) < __builtin_inff()) ? f : bits(d > 0.0 ? u + 1 : u - 1);
+  return !(d < 0.0 || d > 0.0) || (u & 1u) ? f : bits(d > 0.0 ? u + 1 : u - 1);
 }
 
 // ---------------------------------------------------------------------------------------------------- rows into 8 bits

@@ -1,4 +1,4 @@
-"""The norm before rows in 8 bits, code by code: results that 32 bits round to zero.
+"""The norm before rows in 8 bits, code by code: results below and beyond what 32 bits hold.
 
 The kernel has y in 64 bits, off by a few 2^-52 of itself, so its codes are the formula's wherever y is not that near to a border; rows here are equal to the definition, without a tolerance."""
 import pytest
@@ -67,3 +67,16 @@ def test_one_element_far_above_another():
         got, want = codes_of(x, torch.ones(128, dtype=dtype), 1e-6)
         same(got, want)
         assert got[0, 70] == 0 and got[0, 3] == 11      # sqrt(128) is 11.3
+
+
+@pytest.mark.parametrize("dtype", [BF, FP32])
+def test_results_beyond_32_bits(dtype):
+    """A finite result beyond the largest number of 32 bits is held as 448 * 2^119, as every result beyond that is."""
+    x, w = rnd(6, 700, seed=4, dtype=dtype), torch.full((700,), 2.9e38, dtype=dtype)
+    w[300:] = 3.0
+    got, want = codes_of(x, w, 1e-5)
+    same(got, want)
+    assert got.isfinite().all() and got.abs().max() == 448 * 2.0 ** 119 and (got[:, :256].abs() == got.abs().max()).any(1).all()
+    x[2, 5], w[310] = torch.inf, torch.inf      # what is not finite stays so
+    got, want = codes_of(x, w, 1e-5)
+    assert got[[0, 1, 3, 4, 5], 256:384].isnan().all() and got[[0, 1, 3, 4, 5], :256].isfinite().all() and got[2, :128].isnan().all() and (got[2, 128:256] == 0).all()
