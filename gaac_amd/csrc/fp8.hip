@@ -124,7 +124,7 @@ struct RowsArgs {
 
 // A block a row (for few rows without the norm: a part of a row), of `waves` waves; a lane takes CH runs of 8 elements, 16 lanes a block of 128.  Bound by HBM: 16384 x 4096 in bf16 52 us (201 MB, 3.9 TB/s; a large copy makes 4.7 to 5.2), with norm and residual 113 (470 MB,
 // 4.2 TB/s); by launch and latency for a few rows (4 x 4096: 2.3, 3.6).  The sum of squares and the norm in 64 bits: a result next to the border between two
-// codes is rounded as the formula says.  With a residual that costs nothing beside the memory; without one the conversions show (8192 x 4096 35 us, 28 without the norm; 8192 x 14336 152, 88).  Pairs of 32-bit numbers took
+// codes is rounded as the formula says, of the sum of row and residual in 32 bits and of eps as a number of 32 bits.  With a residual that costs nothing beside the memory; without one the conversions show (8192 x 4096 35 us, 28 without the norm; 8192 x 14336 152, 88).  Pairs of 32-bit numbers took
 // longer (registers: 16384 x 4096 with residual 121, 118 in 64 bits then).
 template <typename T, bool NORM, int CH>
 __global__ __launch_bounds__(1024) void k_fp8_rows(RowsArgs a) {

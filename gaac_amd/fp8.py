@@ -125,7 +125,8 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, resid
 
       y = h * rsqrt(mean(h^2) + eps) * weight,   h = x, or x + residual
 
-    with a residual [M, K] of x's type (FP8Rows, h): h in that type, a new contiguous tensor.  The norm is taken of the sum in 32 bits, before it is rounded for h; the sum of squares and y in 64 bits.  One launch."""
+    with a residual [M, K] of x's type (FP8Rows, h): h in that type, a new contiguous tensor.  The norm is taken of the sum in 32 bits, before it is rounded for h; eps is rounded to 32 bits; the sum of squares and y are
+    in 64 bits, so the codes are those of y by the formula, unless y is within a few 2^-52 of a border between two codes.  One launch."""
     out = (_lib._calls or _lib.calls()).fp8_rows(x, weight, eps, residual, _lib.stream) if weight is not None else None
     if out is not None: return FP8Rows(out[0], out[1], tuple(x.shape)) if residual is None else (FP8Rows(out[0], out[1], tuple(x.shape)), out[2])
     _check_rows("rms_norm_fp8", x, MAX_NORM_WIDTH)

@@ -278,7 +278,7 @@ int gaac_sample(int type, const void* logits, long row_stride, int B, int V, con
  * exps uint8 [ceil(K/512)][padded_rows][4], padded_rows a multiple of 16 that holds the rows; rows behind the last and bytes of exps behind the last block need not be set.
  * Rows of two tensors may alternate by tiles: this one has tiles tile_first, tile_first + tile_step, ...
  * gaac_fp8_rows: rows x [M, K] (type as above, rows a stride in elements apart) into 8 bits; with a weight [K] after the root-mean-square norm x * rsqrt(mean(x^2) + eps) * weight
- * (K up to 32768), and with a residual [M, K] of the sum of both, which is also written: sum [M, K], contiguous, not over the inputs. */
+ * (K up to 32768; in 64 bits, of eps as it is handed over), and with a residual [M, K] of the sum of both, which is also written: sum [M, K], contiguous, not over the inputs. */
 int gaac_fp8_rows(int type, const void* x, long x_row_stride, const void* residual, long residual_row_stride, const void* weight, float eps, int M, int K,
                   void* sum, void* data, void* exps, long padded_rows, int tile_step, int tile_first, void* stream);
 /* gaac_fp8_values: the values of such rows, bf16. */

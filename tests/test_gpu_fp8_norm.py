@@ -1,4 +1,4 @@
-"""The norm before rows in 8 bits, code by code: results below and beyond what 32 bits hold.
+"""The norm before rows in 8 bits, code by code: results below and beyond what 32 bits hold, results next to a border between two codes.
 
 The kernel has y in 64 bits, off by a few 2^-52 of itself, so its codes are the formula's wherever y is not that near to a border; rows here are equal to the definition, without a tolerance."""
 import pytest
@@ -80,3 +80,43 @@ def test_results_beyond_32_bits(dtype):
     x[2, 5], w[310] = torch.inf, torch.inf      # what is not finite stays so
     got, want = codes_of(x, w, 1e-5)
     assert got[[0, 1, 3, 4, 5], 256:384].isnan().all() and got[[0, 1, 3, 4, 5], :256].isfinite().all() and got[2, :128].isnan().all() and (got[2, 128:256] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [BF, FP16, FP32])
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("M,K", [(1, 1), (4, 4096), (17, 129), (5, 5000), (700, 512), (3, 32768), (130, 14336), (2500, 1024)])
+def test_codes_are_the_formulas(M, K, residual, dtype):
+    x, w, r = rnd(M, K, seed=1, dtype=dtype), rnd(K, seed=2, dtype=dtype), rnd(M, K, seed=3, dtype=dtype) if residual else None
+    same(*codes_of(x, w, 1e-5, r))
+
+
+def next_to_borders(x, eps, seed):
+    """A weight fp32 [K] for a row x fp32 [1, K] with which every y lies next to a border between two codes, nearer than half a step of 32 bits: targets are the middles of the grid's values from 2^-6 to 448
+    in blocks whose largest element is 440, and in every third block 448 itself, the border between two powers of two."""
+    K = x.shape[1]
+    g = torch.Generator().manual_seed(seed)
+    middles = ((R.GRID[1:] + R.GRID[:-1]) / 2)[8:]
+    target = middles[torch.randint(0, len(middles), (K,), generator=g)]
+    target[::128] = 440.0
+    target[::384] = 448.0
+    h = x.double()
+    r = 1 / torch.sqrt((h * h).mean() + eps)
+    w = (target / (h[0] * r)).float()
+    off = (h[0] * r * w.double() - target) / target
+    assert (off.abs() > 2.0 ** -45).all() and (off.abs() < 2.0 ** -23).all()
+    return w
+
+
+@pytest.mark.parametrize("scale,eps", [(1.0, 1e-5), (1e-4, 0.1), (0.02, 1e-3), (1e-20, 1e-6)])
+@pytest.mark.parametrize("seed", range(3))
+def test_results_next_to_a_border(seed, scale, eps):
+    """What a norm in 32 bits, or one rounded to 32 bits before it is rounded to 8, would get wrong.  eps is a number of 32 bits."""
+    eps = torch.tensor(eps).double().item()
+    x = (torch.rand(1, 3000, generator=torch.Generator().manual_seed(seed)) + 0.5) * scale
+    w = next_to_borders(x, eps, seed + 10)
+    y, _ = R.norm(x, w, eps)
+    want = R.stored(y)
+    twice = R.stored(y.float())
+    assert (want != twice).sum() > 3000 / 8      # (the test can tell: rounded twice, these are other codes)
+    same(codes_of(x, w, eps)[0], want)
+    same(codes_of(x, w, eps, torch.zeros_like(x))[0], want)
