@@ -51,6 +51,7 @@ _SIGNATURES = {
     "gaac_fp8_rows": [c_int, P, c_long, P, c_long, P, c_float, c_int, c_int, P, P, P, c_long, c_int, c_int, P],
     "gaac_fp8_values": [P, P, c_long, c_int, c_int, c_int, c_int, P, c_long, P],
     "gaac_fp8_product": [P, P, P, P, c_int, c_int, c_int, c_int, c_int, P, c_long, P],
+    "gaac_fp8_product_form": [c_int] * 5 + [P],
     "gaac_logprobs": [c_int, P, c_long, c_int, c_int, P, c_int, P, c_long, P, P, P, P, P, P],
     "gaac_attn_launch": [P] * 16 + [P, P, c_int, c_int, c_int, P, c_int, c_float, c_int, c_int, P, P, P, c_int, P, P, P, P, P],
 }

@@ -102,7 +102,7 @@ PyObject* invoke(const char* name, int (*fn)(A...), PyObject* const* args, Py_ss
   X(gaac_paged_store) X(gaac_paged_free) X(gaac_paged_release) X(gaac_paged_decode) X(gaac_paged_attn) X(gaac_bf16_attn)                  \
   X(gaac_attn_fused) X(gaac_attn_fused_static) X(gaac_static_init) X(gaac_static_reset) X(gaac_static_flags) X(gaac_attn_launch)    \
   X(gaac_fp4_store) X(gaac_fp4_load) X(gaac_fp4_length) X(gaac_fp4_append) X(gaac_fp4_attn) X(gaac_qk_norm_rope) X(gaac_sample) \
-  X(gaac_fp8_rows) X(gaac_fp8_values) X(gaac_fp8_product) X(gaac_logprobs)
+  X(gaac_fp8_rows) X(gaac_fp8_values) X(gaac_fp8_product) X(gaac_fp8_product_form) X(gaac_logprobs)
 #define X(name)                                            \
   decltype(&::name) p_##name = nullptr;                    \
   PyObject* py_##name(PyObject*, PyObject* const* args, Py_ssize_t n) { return invoke(#name, p_##name, args, n); }

@@ -626,9 +626,10 @@ template <int COUNT> int form_of(const Form (&forms)[COUNT], const ProductArgs& 
   }
   return best;
 }
+int form_of(const ProductArgs& a, bool gated, bool exact) { return exact ? form_of(EXACT_FORMS, a, gated) : form_of(FORMS, a, gated); }
 template <typename O> void launch_product(const ProductArgs& a, bool gated, hipStream_t s) {
   if constexpr (sizeof(O) == 4) {
-    switch (form_of(EXACT_FORMS, a, gated)) {
+    switch (form_of(a, gated, true)) {
       case 0: return launch_stream<O, 1, 1, 4>(a, gated, s);
       case 1: return launch_stream<O, 1, 2, 4>(a, gated, s);
       case 2: return launch_stream<O, 2, 2, 4>(a, gated, s);
@@ -637,7 +638,7 @@ template <typename O> void launch_product(const ProductArgs& a, bool gated, hipS
       default: return launch_tiles<O, 4, 4, 2, 2, 2>(a, gated, s);
     }
   } else {
-    switch (form_of(FORMS, a, gated)) {
+    switch (form_of(a, gated, false)) {
       case 0: return launch_stream<O, 1, 1, 4>(a, gated, s);
       case 1: return launch_stream<O, 1, 2, 4>(a, gated, s);
       case 2: return launch_stream<O, 2, 2, 4>(a, gated, s);
@@ -722,4 +723,14 @@ extern "C" int gaac_fp8_product(const void* x, const void* x_exps, const void* w
   else if (out_type == 1) launch_product<_Float16>(a, gated != 0, (hipStream_t)stream);
   else launch_product<float>(a, gated != 0, (hipStream_t)stream);
   return gaac::launch_status("gaac_fp8_product");
+}
+
+extern "C" int gaac_fp8_product_form(int M, int N, int K, int gated, int out_type, int* form) {
+  GAAC_REQUIRE(form != nullptr, "gaac_fp8_product_form: null pointer");
+  GAAC_REQUIRE(out_type >= 0 && out_type <= 2, "gaac_fp8_product_form: type must be 0 (bf16), 1 (fp16) or 2 (fp32)");
+  GAAC_REQUIRE(M > 0 && M <= 1 << 20 && K > 0 && K <= MAX_K && N > 0 && N <= 1 << 22, "gaac_fp8_product_form: bad sizes (%d rows of %d by %d)", M, K, N);
+  ProductArgs a{};
+  a.M = M; a.N = N; a.K = K; a.nb = (K + BLOCK - 1) / BLOCK; a.tiles = (N + 15) / 16 * (gated ? 2 : 1);
+  *form = form_of(a, gated != 0, out_type == 2);
+  return 0;
 }

@@ -288,6 +288,8 @@ int gaac_fp8_values(const void* data, const void* exps, long padded_rows, int ti
  * (x w1^T).  out of out_type, rows a stride in elements apart. */
 int gaac_fp8_product(const void* x, const void* x_exps, const void* w, const void* w_exps, int M, int N, int K, int gated, int out_type, void* out,
                      long out_row_stride, void* stream);
+/* gaac_fp8_product_form: the number of the form that such a product takes (the rule and the forms are stated in gaac_amd/csrc/fp8.hip: 0 to 9, for outputs in 32 bits 0 to 5) into *form, on the host; launches nothing. */
+int gaac_fp8_product_form(int M, int N, int K, int gated, int out_type, int* form);
 
 /* Of each row of logits [B, V] (type as above, rows row_stride elements apart): logprob [B] of the given token, rank [B] = tokens before it in the order of logits (ties: lower index
  * first; -1 for a token outside of the vocabulary, whose logprob is NaN), entropy [B], and the `top` (up to 64) first of that order with their log probabilities, [B, top].  A NaN among
