@@ -81,7 +81,7 @@ def test_long_sums(M, N, K):
     for dtype in (BF, FP16, FP32): assert torch.equal(fp8_linear(rows, W, out_dtype=dtype), y.to(dtype))
 
 
-@pytest.mark.parametrize("wide,form,M,N,K", [(c[0], *c[2:]) for c in CASES if not c[1] and (c[0] or c[2] < 2)])
+@pytest.mark.parametrize("wide,form,M,N,K", [(c[0], *c[2:]) for c in CASES if not c[1] and (c[0] or c[2] < 2) and c[5] > 500])
 def test_exact_sums(wide, form, M, N, K):
     """Outputs in 32 bits, and those of 16 bits of up to 16 rows: in every block one element of both operands is 448, so that one product is 2^12 times its neighbours'.  The sum has all of these; the product of codes in 8 bits
     would cut them to multiples of 2^3."""
