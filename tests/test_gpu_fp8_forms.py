@@ -99,3 +99,15 @@ def test_exact_sums(wide, form, M, N, K):
         want = (y * scale).float().to(dtype)
         assert ((y[:4] - lost) * scale).float().to(dtype).ne(want[:4]).float().mean() > 0.8      # (the test can tell)
         assert torch.equal(fp8_linear(quantize_fp8(x * scale), held(w), out_dtype=dtype), want)
+
+
+@pytest.mark.parametrize("M", [1, 40])
+def test_silu_far_below_zero(M):
+    """Gates down to -80 by the formula; below -87, where 1 + e^-g leaves 32 bits, the result may be 0."""
+    gates = torch.tensor([-0.5, -1, -8, -40, -72, -80, -88, -96, -104, -160, -448, 448, 80], device="cuda")
+    G = FP8Weight(gates[:, None], torch.full((len(gates), 1), 2.0 ** 20, device="cuda"))
+    out = fp8_gated(torch.ones(M, 1, device="cuda"), G, out_dtype=FP32).double()
+    g = gates.double().expand(M, -1)
+    y = g * torch.sigmoid(g) * 2.0 ** 20
+    tol = (2.0 ** -20 + g.abs() * 2.0 ** -22) * y.abs() + torch.finfo(FP32).smallest_normal * 2.0 ** -23
+    assert ((out - y).abs() <= torch.where(g < -87, y.abs() * 1.01, tol)).all()
