@@ -111,3 +111,16 @@ def test_silu_far_below_zero(M):
     y = g * torch.sigmoid(g) * 2.0 ** 20
     tol = (2.0 ** -20 + g.abs() * 2.0 ** -22) * y.abs() + torch.finfo(FP32).smallest_normal * 2.0 ** -23
     assert ((out - y).abs() <= torch.where(g < -87, y.abs() * 1.01, tol)).all()
+
+
+def test_exact_sums_for_a_gated_block_in_bf16():
+    """A result in 32 bits, rounded by the caller: what rounding the formula's value gives, but for elements next to a border.  Off by 2^-19 of itself (|g| up to 8; sums in 32 bits lose less for all but elements near 0),
+    of borders 2^-8 apart, two sides: one element in 2^10, and as many again for what is near 0."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    normal = lambda *shape: torch.randn(*shape, generator=g, device="cuda")
+    M, N, K = 700, 2000, 1024
+    x, G = quantize_fp8(normal(M, K)), FP8Weight(normal(N, K) * K ** -0.5, normal(N, K) * K ** -0.5)
+    gate, up = (x.dequantize().double() @ w.double().T for w in G.dequantize())
+    assert gate.abs().max() < 8
+    want = (gate * torch.sigmoid(gate) * up).float().to(BF)
+    assert fp8_gated(x, G, out_dtype=FP32).to(BF).ne(want).float().mean() < 2.0 ** -9
