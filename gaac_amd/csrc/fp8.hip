@@ -601,7 +601,8 @@ template <typename O, int MT, int NT, int AHEAD> void launch_stream(const Produc
 
 // Which form is taken: the one that should end first, its time being start + steps * (round * rounds + share * blocks / 256), rounds = blocks / 256 rounded up (a round: a block on each CU), steps the blocks of K
 // that a wave goes through.  The constants, in us, are fitted to the times of all forms over 180 sizes (1 to 8192 rows by 1024 to 28672 x 512 to 14336); over these the chosen form takes 1.6 % longer than the
-// best one in the mean (fp32: 0.6 % over 77), and over 112 with the form of 192 rows 1.3 % (2.8 without it).  Up to 16 rows, and wherever a block has one tile of rows, the products are the exact ones for every type: the weights' way from memory hides most of them (8 x 4096 x 4096 4.9 us,
+// best one in the mean (fp32: 0.6 % over 77), and over 112 with the form of 192 rows 1.3 % (2.8 without it); at worst 48 % (100 x 2048 x 512, 3.7 us for 2.5).  Over sizes outside of the fit, drawn from 1 to 8192 rows, 512 to 28672 outputs and 256 to
+// 16384 inputs, 2.5 % in the mean and 23 % at worst (90 sizes; fp32 1.1 % and 19 %, gated 3.8 % and 41 %, 40 each); a tenth of them miss the best form by more than a tenth.  Up to 16 rows, and wherever a block has one tile of rows, the products are the exact ones for every type: the weights' way from memory hides most of them (8 x 4096 x 4096 4.9 us,
 // 4.8 without; 8 x 28672 x 4096 23.6, 21.8).  Some of both sides, us, weights resident in turns (rows x N x K, outputs of 16 bits: stream of 1 x 1, 1 x 2, 2 x 2, 4 x 2 tiles | 64 x 64,
 // 64 x 128, 128 x 128 with four buffers, with two, 256 x 256, 192 x 128 through LDS):
 //   8 x 4096 x 4096  4.9 5.6             8 x 28672 x 4096  23.9 23.6                                 48 x 4096 x 14336  28 25 16.9 23 | 32 48 51 95 142
