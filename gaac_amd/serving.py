@@ -28,7 +28,7 @@ from .kv_cache import CompressedKVCache
 from .kernel import bf16_attention, choose_nsplit, AttnWorkspace
 from .fp4_cache import FP4KVCache
 from .rope import qk_norm_rope
-from .sampling import sample, token_logprobs, LogProbs
+from .sampling import MAX_TOP, sample, token_logprobs, LogProbs
 from .fp8 import FP8Weight, fp8_gated, fp8_linear, rms_norm_fp8
 
 D = 128
@@ -311,6 +311,11 @@ class DecodeRunner:
             out = fp8_linear(fp8_gated(h, layer["gate_up"]), layer["down"])
         return x if out is None else x + out
 
+    def _check_logprobs(self, what: str, logprobs: int | None):
+        """Refused before a token is stored: token_logprobs would refuse it behind the step that made the logits."""
+        most = min(MAX_TOP, self.cfg.vocab)
+        if logprobs is not None and not 0 <= logprobs <= most: raise RuntimeError(f"{what} gives 0 to {most} alternatives, not {logprobs}")
+
     # ---------------------------------------------------------------- prefill
     @torch.no_grad()
     def prefill(self, slot: int, tokens: torch.Tensor, logprobs: int | None = None):
@@ -318,6 +323,7 @@ class DecodeRunner:
         Returns the logits of the last position [vocab] (fp32); with logprobs, a number of alternatives, also the LogProbs of tokens 1 .. L - 1, each from the position before it."""
         cfg, L = self.cfg, tokens.shape[0]
         if L > cfg.max_len: raise RuntimeError(f"prompt has {L} tokens, the model's positions end at {cfg.max_len}")
+        self._check_logprobs("prefill", logprobs)
         pos = torch.arange(L, device=tokens.device)
         x = self.w.embed.index_select(0, tokens)
         cu = torch.tensor([0, L], dtype=torch.int32, device=tokens.device)
@@ -355,6 +361,7 @@ class DecodeRunner:
         attention, sampling, feeding the token back) is captured once and replayed.  sampling: arguments of sample() (temperature, top_k, top_p, min_p; numbers
         or tensors [B]), decode() then takes the random numbers; None: the likeliest token.  A row whose logits are all NaN or -inf has no token to draw: decode() returns
         -1 for it, and the row goes on with token 0.  logprobs: a number of alternatives; decode() then also returns the LogProbs of the tokens."""
+        self._check_logprobs("start_decode", logprobs)
         B, dev = first_tokens.shape[0], first_tokens.device
         self.B = B
         self.tok = first_tokens.clone()
